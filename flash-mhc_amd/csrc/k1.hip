@@ -28,6 +28,7 @@
 #include "fmhc_common.h"
 #include "k1_premap.h"
 #include "k2_chain.h"
+#include "pack8.h"
 
 namespace fmhc {
 
@@ -628,11 +629,11 @@ struct BwdSlices {
   int n;    // slices of all parts
 };
 
-template <bool EPI, bool GI>
+template <bool EPI, bool GI, typename SRC>
 struct BwdFrag {
   u32x4 gv, pv;   // go / proj_out row of token tbase + col, d = 8 * grp .. + 8
   float inv[4];   // inv_rms of tokens tbase + 4 * grp + q
-  u32x4 xv[4];    // x of those tokens, k = kl .. kl + 8
+  typename SRC::Raw xv[4];  // x of those tokens, k = kl .. kl + 8
   u32x4 g3[EPI ? 4 : 1];  // EPI: the K3 output gradient of those tokens at the lane's c
   float hp[EPI ? 4 : 1];  // EPI: their h_pre of the lane's stream j
   u32x4 gi[GI ? 4 : 1];   // GI: x's incoming gradient at the lane's 8 k
@@ -660,8 +661,11 @@ struct BwdFrag {
 // operand takes the kernel to one wave per SIMD; it is still bound by HBM
 // (measured: +80 us at T=65536, C=1024 for the 512 MiB it reads, against
 // 260 us for the separate accumulation pass it replaces).
-template <bool DW, bool FULLK, bool EPI, bool GI, bool NT, int NBUF>
-__global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ x,
+//
+// SRC: x in bf16, or in 8 bits with scales xs (pack8.h; streams of C columns).
+// The codes become bf16 in registers, exactly, and everything after is the same.
+template <bool DW, bool FULLK, bool EPI, bool GI, bool NT, int NBUF, typename SRC>
+__global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __restrict__ x,
                                                    const uint16_t* __restrict__ W,
                                                    const uint16_t* __restrict__ go,
                                                    const uint16_t* __restrict__ proj,
@@ -671,7 +675,8 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
                                                    const uint16_t* __restrict__ go3,
                                                    const float* __restrict__ h_pre,
                                                    const uint16_t* __restrict__ gi,
-                                                   int64_t T, int nC, const BwdSlices sl, int64_t nruns, int C) {
+                                                   int64_t T, int nC, const BwdSlices sl, int64_t nruns, int C,
+                                                   const uint8_t* __restrict__ xs) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int col = lane & 15;  // A row (token) for the loads of go, B/D column
@@ -715,10 +720,13 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
   // VALU build: W[d][kl .. kl + 8) for d = 0..31 and the lane columns, and the token block's go rows.
   __shared__ u32x4 wvl[kValu ? 4 : 1][kValu ? 32 * 16 : 1];
   __shared__ u32x4 gvl[kValu ? 4 : 1][kValu ? 16 * 4 : 1];
-  // EPI: the lane's stream j and position c (k .. k + 7 stay in one stream:
+  // EPI, 8 bits: the lane's stream j and position c (k .. k + 7 stay in one stream:
   // C % 8 == 0, or the parts are the streams).
-  const int sj = EPI ? kl / C : 0;
-  const uint32_t c3bytes = EPI ? 2u * static_cast<uint32_t>(kl - sj * C) : 0u;
+  constexpr bool kStream = EPI || SRC::kPacked;
+  const int sj = kStream ? kl / C : 0;
+  const int cj = kStream ? kl - sj * C : 0;
+  const uint32_t c3bytes = 2u * static_cast<uint32_t>(cj);
+  const int ngroups = SRC::kPacked ? pack_groups(C) : 0;  // scales of a stream's row
   f32x4 dacc[DW ? 8 : 1][2];
 #pragma unroll
   for (int m = 0; m < (DW ? 8 : 1); ++m) dacc[m][0] = dacc[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -764,7 +772,7 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
   auto block_base = [&](int tb) { return (run + static_cast<int64_t>(tb) * nruns) * 16; };
   // Valid rows of the block starting at tbase (16 except in the last block).
   auto block_rows = [&](int64_t tbase) { return static_cast<int>(T - tbase < 16 ? T - tbase : 16); };
-  auto load = [&](BwdFrag<EPI, GI>& f, int tb) {
+  auto load = [&](BwdFrag<EPI, GI, SRC>& f, int tb) {
     const int64_t tbase = block_base(tb);
     const int last = block_rows(tbase) - 1;  // rows past the end re-read the last one
     const int rg = col < last ? col : last;
@@ -785,7 +793,10 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
       const int r0 = 4 * grp + q;
       const uint32_t r = static_cast<uint32_t>(r0 < last ? r0 : last);
       if (last != 15) f.inv[q] = *reinterpret_cast<const float*>(ib + 4u * r);
-      f.xv[q] = Lanes<8, NT>::raw(reinterpret_cast<const uint16_t*>(xb + (r * row_bytes + kbytes)), 0);
+      const uint8_t* srow = nullptr;
+      if constexpr (SRC::kPacked) srow = xs + (4 * (tbase + r) + sj) * ngroups;
+      const uint32_t xoff = SRC::kPacked ? r * static_cast<uint32_t>(nC) + static_cast<uint32_t>(kl) : r * row_bytes + kbytes;
+      f.xv[q] = SRC::template raw<NT>(xb + xoff, srow, cj);
       if constexpr (EPI) {
         const char* g3b = reinterpret_cast<const char*>(go3 + tbase * C);
         f.hp[q] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(h_pre + tbase * 4) + 16u * r +
@@ -799,7 +810,7 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
             reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(gi + tbase * nC) + (r * row_bytes + kbytes)), 0);
     }
   };
-  auto compute = [&](const BwdFrag<EPI, GI>& f, int tb) {
+  auto compute = [&](const BwdFrag<EPI, GI, SRC>& f, int tb) {
     const int64_t tbase = block_base(tb);
     const int rows = block_rows(tbase);
     // dot(go, proj_out) of token tbase + col, over the four 8-wide d groups.
@@ -816,6 +827,9 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
       const float d = __shfl(dot, 4 * grp + q, kWave);  // token tbase + 4 * grp + q
       scale[q] = d * (f.inv[q] * f.inv[q]) / static_cast<float>(nC);
     }
+    u32x4 xv[4];  // x as bf16
+#pragma unroll
+    for (int q = 0; q < 4; ++q) xv[q] = SRC::bits(f.xv[q], cj);
     f32x4 acc[8];
     if constexpr (kValu) {
       // VALU build: acc[m][q] = sum_d go[token 4 grp + q][d] * W[d][kl + m] as
@@ -850,7 +864,7 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
         const int r = 4 * grp + q;
         if (r < rows) {
           float xf[8], o[8];
-          unpack8(f.xv[q], xf);
+          unpack8(xv[q], xf);
 #pragma unroll
           for (int m = 0; m < 8; ++m) o[m] = f.inv[q] * acc[m][q] - scale[q] * xf[m];
           if constexpr (EPI) {
@@ -902,7 +916,7 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
         uint32_t e[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t w = f.xv[q][m >> 1];
+          const uint32_t w = xv[q][m >> 1];
           e[q] = (m & 1) ? (w >> 16) : (w & 0xffffu);
         }
         const u32x2 av = {e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
@@ -917,9 +931,9 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const uint16_t* __restrict__ 
   };
   // NBUF = 3: two blocks in flight while one computes (three rotating
   // fragments, three blocks per trip); NBUF = 2: one.
-  BwdFrag<EPI, GI> f0, f1;
+  BwdFrag<EPI, GI, SRC> f0, f1;
   if constexpr (NBUF == 3) {
-    BwdFrag<EPI, GI> f2;
+    BwdFrag<EPI, GI, SRC> f2;
     load(f0, 0);
     load(f1, pos(1));
     int i = 0;
@@ -1049,10 +1063,12 @@ __global__ __launch_bounds__(256) void k1_dw_zero(uint16_t* __restrict__ dW, int
 
 // Element-wise weight gradient for shapes the matrix-core path does not take:
 // one thread per (d, k), tokens summed in order.
-__global__ __launch_bounds__(256) void k1_dw_scalar(const uint16_t* __restrict__ x,
+template <typename SRC>
+__global__ __launch_bounds__(256) void k1_dw_scalar(const typename SRC::Elem* __restrict__ x,
                                                     const uint16_t* __restrict__ go,
                                                     const float* __restrict__ inv_rms,
-                                                    uint16_t* __restrict__ dW, int64_t T, int nC) {
+                                                    uint16_t* __restrict__ dW, int64_t T, int nC, int C,
+                                                    const uint8_t* __restrict__ xs) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= static_cast<int64_t>(kDout) * nC) return;
   const int d = static_cast<int>(i / nC);
@@ -1060,7 +1076,7 @@ __global__ __launch_bounds__(256) void k1_dw_scalar(const uint16_t* __restrict__
   float acc = 0.f;
   for (int64_t t = 0; t < T; ++t) {
     const float g = bf16_to_f32(f32_to_bf16(bf16_to_f32(go[t * kDout + d]) * inv_rms[t]));
-    acc = __builtin_fmaf(g, bf16_to_f32(x[t * nC + k]), acc);
+    acc = __builtin_fmaf(g, SRC::elem(x, xs, t, k, nC, C), acc);
   }
   dW[i] = f32_to_bf16(acc);
 }
@@ -1102,15 +1118,15 @@ __global__ __launch_bounds__(256) void k1_fwd_scalar(const uint16_t* __restrict_
 
 // ACC: grad_x already holds the pre-map's K3 term; store bf16(that + bf16(dx)),
 // and with an incoming gradient gi (may be null) bf16(gi + bf16(that + bf16(dx))).
-template <bool ACC>
-__global__ __launch_bounds__(256) void k1_bwd_scalar(const uint16_t* __restrict__ x,
+template <bool ACC, typename SRC>
+__global__ __launch_bounds__(256) void k1_bwd_scalar(const typename SRC::Elem* __restrict__ x,
                                                      const uint16_t* __restrict__ W,
                                                      const uint16_t* __restrict__ go,
                                                      const uint16_t* __restrict__ proj,
                                                      const float* __restrict__ inv_rms,
                                                      uint16_t* __restrict__ gx,
                                                      const uint16_t* __restrict__ gi,
-                                                     int64_t T, int nC) {
+                                                     int64_t T, int nC, int C, const uint8_t* __restrict__ xs) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + wave;
@@ -1124,14 +1140,13 @@ __global__ __launch_bounds__(256) void k1_bwd_scalar(const uint16_t* __restrict_
   }
   const float inv = inv_rms[t];
   const float scale = dot * (inv * inv) / static_cast<float>(nC);
-  const uint16_t* xr = x + t * nC;
   uint16_t* gr = gx + t * nC;
   for (int k = lane; k < nC; k += kWave) {
     float s = 0.f;
 #pragma unroll
     for (int d = 0; d < kDout; ++d)
       s = __builtin_fmaf(g[d], bf16_to_f32(W[static_cast<int64_t>(d) * nC + k]), s);
-    const float v = inv * s - scale * bf16_to_f32(xr[k]);
+    const float v = inv * s - scale * SRC::elem(x, xs, t, k, nC, C);
     if constexpr (ACC) {
       float u = bf16_to_f32(f32_to_bf16(bf16_to_f32(gr[k]) + bf16_to_f32(f32_to_bf16(v))));
       if (gi) u += bf16_to_f32(gi[t * nC + k]);
@@ -1352,14 +1367,23 @@ int k1_fwd_run(const uint16_t* x_flat, const uint16_t* W, uint16_t* out, float* 
   return launch_status();
 }
 
-template <bool ACC>
-void launch_k1_bwd_scalar(hipStream_t s, const uint16_t* x, const uint16_t* W, const uint16_t* go, const uint16_t* proj,
-                          const float* inv_rms, uint16_t* gx, const uint16_t* gi, int64_t T, int nC) {
+template <bool ACC, typename SRC = Bf16Src>
+void launch_k1_bwd_scalar(hipStream_t s, const typename SRC::Elem* x, const uint16_t* W, const uint16_t* go,
+                          const uint16_t* proj, const float* inv_rms, uint16_t* gx, const uint16_t* gi, int64_t T,
+                          int nC, int C = 1, const uint8_t* xs = nullptr) {
   for_launches(T, 256, 4, [&](int64_t t, int64_t n) {
-    k1_bwd_scalar<ACC><<<dim3(blocks_for(n, 4)), 256, 0, s>>>(x + t * nC, W, go + t * kDout, proj + t * kDout,
-                                                              inv_rms + t, gx + t * nC, gi ? gi + t * nC : nullptr, n,
-                                                              nC);
+    k1_bwd_scalar<ACC, SRC><<<dim3(blocks_for(n, 4)), 256, 0, s>>>(
+        x + t * nC, W, go + t * kDout, proj + t * kDout, inv_rms + t, gx + t * nC, gi ? gi + t * nC : nullptr, n, nC, C,
+        SRC::kPacked ? xs + t * 4 * pack_groups(C) : nullptr);
   });
+}
+
+// grad_W element-wise.
+template <typename SRC = Bf16Src>
+void launch_k1_dw_scalar(hipStream_t s, const typename SRC::Elem* x, const uint16_t* go, const float* inv_rms,
+                         uint16_t* dW, int64_t T, int nC, int C = 1, const uint8_t* xs = nullptr) {
+  k1_dw_scalar<SRC><<<dim3(blocks_for(static_cast<int64_t>(kDout) * nC, 256)), 256, 0, s>>>(x, go, inv_rms, dW, T, nC,
+                                                                                           C, xs);
 }
 
 // Number of runs of k1_bwd_mfma for T tokens (nblocks blocks of 16) and
@@ -1380,11 +1404,12 @@ int64_t k1_bwd_nruns(int64_t T, int64_t nslices, int64_t max_blocks, int64_t min
   return n > nmin ? n : nmin;
 }
 
-template <bool DW, bool EPI = false, bool GI = false>
-void launch_k1_bwd_mfma(hipStream_t s, const uint16_t* x, const uint16_t* W, const uint16_t* go,
+template <bool DW, bool EPI = false, bool GI = false, typename SRC = Bf16Src>
+void launch_k1_bwd_mfma(hipStream_t s, const typename SRC::Elem* x, const uint16_t* W, const uint16_t* go,
                         const uint16_t* proj, const float* inv_rms, uint16_t* gx, float* partial, int64_t T, int nC,
                         const BwdSlices& sl, int64_t nruns, const uint16_t* go3 = nullptr,
-                        const float* h_pre = nullptr, int C = 1, const uint16_t* gi = nullptr) {
+                        const float* h_pre = nullptr, int C = 1, const uint16_t* gi = nullptr,
+                        const uint8_t* xs = nullptr) {
   const dim3 grid(blocks_for(nruns * sl.n, 4));
   constexpr int nbuf = EPI ? kBwdEpiBufs : kBwdBufs;
   // dx alone: one workgroup per CU (LDS reserved that the kernel does not
@@ -1399,9 +1424,9 @@ void launch_k1_bwd_mfma(hipStream_t s, const uint16_t* x, const uint16_t* W, con
   auto launch = [&](auto fullk, auto nt) {
     constexpr bool FULLK = decltype(fullk)::value, NT = decltype(nt)::value;
     static const unsigned lds =
-        lds_reserve(reinterpret_cast<const void*>(&k1_bwd_mfma<DW, FULLK, EPI, GI, NT, nbuf>), kLdsCapOne);
-    k1_bwd_mfma<DW, FULLK, EPI, GI, NT, nbuf><<<grid, 256, cap ? lds : 0u, s>>>(
-        x, W, go, proj, inv_rms, gx, partial, go3, h_pre, gi, T, nC, sl, nruns, C);
+        lds_reserve(reinterpret_cast<const void*>(&k1_bwd_mfma<DW, FULLK, EPI, GI, NT, nbuf, SRC>), kLdsCapOne);
+    k1_bwd_mfma<DW, FULLK, EPI, GI, NT, nbuf, SRC><<<grid, 256, cap ? lds : 0u, s>>>(
+        x, W, go, proj, inv_rms, gx, partial, go3, h_pre, gi, T, nC, sl, nruns, C, xs);
   };
   auto rows = [&](auto nt) {
     sl.len % 128 == 0 ? launch(std::true_type{}, nt) : launch(std::false_type{}, nt);
@@ -1414,7 +1439,7 @@ void launch_k1_bwd_mfma(hipStream_t s, const uint16_t* x, const uint16_t* W, con
   // T = 30011, C = 1001 267.7 / 272.7 and T = 4000, C = 100 27.7 / 29.1).  dx alone
   // is equal.
   if constexpr (DW) {
-    if (nC % 64 != 0 || !aligned16(x)) return rows(std::false_type{});
+    if (nC * sizeof(typename SRC::Elem) % 128 != 0 || !SRC::aligned(x)) return rows(std::false_type{});
   }
   rows(std::true_type{});
 }
@@ -1553,8 +1578,7 @@ extern "C" int fmhc_k1_bwd(const uint16_t* x_flat, const uint16_t* W, const uint
   }
   const int st = fmhc_k1_bwd_dx(x_flat, W, grad_out, proj_out, inv_rms, grad_x, T, nC, D_out, stream);
   if (st != FMHC_OK) return st;
-  k1_dw_scalar<<<dim3(blocks_for(static_cast<int64_t>(kDout) * nC, 256)), 256, 0, s>>>(
-      x_flat, grad_out, inv_rms, grad_W, T, nc);
+  launch_k1_dw_scalar(s, x_flat, grad_out, inv_rms, grad_W, T, nc);
   return launch_status();
 }
 
@@ -1603,7 +1627,8 @@ int64_t k1_bwd_premap_ws_bytes(int64_t T, int64_t C) {
   return T > 0 && k1_bwd_premap_fused(C) ? k1_bwd_dw_bytes(T, bwd_premap_slices(C)) : 0;
 }
 
-int k1_bwd_premap(const uint16_t* x_flat, const uint16_t* W, const uint16_t* grad_proj,
+template <typename SRC>
+int k1_bwd_premap(const typename SRC::Elem* x_flat, const uint8_t* xs, const uint16_t* W, const uint16_t* grad_proj,
                   const uint16_t* proj, const float* inv_rms, const uint16_t* go3, const float* h_pre,
                   const uint16_t* grad_x_in, uint16_t* grad_x, uint16_t* grad_W, void* workspace,
                   int64_t workspace_bytes, int64_t T, int64_t C, const K2ParamSums& k2_sums, hipStream_t s) {
@@ -1621,22 +1646,67 @@ int k1_bwd_premap(const uint16_t* x_flat, const uint16_t* W, const uint16_t* gra
     const int64_t nruns = k1_bwd_runs(T, sl.n);
     float* partial = static_cast<float*>(workspace);
     if (grad_x_in)
-      launch_k1_bwd_mfma<true, true, true>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl, nruns,
-                                           go3, h_pre, static_cast<int>(C), grad_x_in);
+      launch_k1_bwd_mfma<true, true, true, SRC>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl,
+                                                nruns, go3, h_pre, static_cast<int>(C), grad_x_in, xs);
     else
-      launch_k1_bwd_mfma<true, true>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl, nruns,
-                                     go3, h_pre, static_cast<int>(C));
+      launch_k1_bwd_mfma<true, true, false, SRC>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl,
+                                                 nruns, go3, h_pre, static_cast<int>(C), nullptr, xs);
     const int st = launch_status();
     if (st != FMHC_OK) return st;
     return launch_dw_reduce(partial, grad_W, nruns, sl, nc, k2_sums, kNPar, s);
   }
-  launch_k1_bwd_scalar<true>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, grad_x_in, T, nc);
+  const int c = static_cast<int>(C);
+  launch_k1_bwd_scalar<true, SRC>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, grad_x_in, T, nc, c, xs);
   const int st = launch_status();
   if (st != FMHC_OK) return st;
-  k1_dw_scalar<<<dim3(blocks_for(static_cast<int64_t>(kDout) * nC, 256)), 256, 0, s>>>(
-      x_flat, grad_proj, inv_rms, grad_W, T, nc);
+  launch_k1_dw_scalar<SRC>(s, x_flat, grad_proj, inv_rms, grad_W, T, nc, c, xs);
   launch_k2_param_reduce(k2_sums, s);
   return launch_status();
 }
 
+template int k1_bwd_premap<Bf16Src>(const uint16_t*, const uint8_t*, const uint16_t*, const uint16_t*, const uint16_t*,
+                                    const float*, const uint16_t*, const float*, const uint16_t*, uint16_t*, uint16_t*,
+                                    void*, int64_t, int64_t, int64_t, const K2ParamSums&, hipStream_t);
+template int k1_bwd_premap<Pack8Src>(const int8_t*, const uint8_t*, const uint16_t*, const uint16_t*, const uint16_t*,
+                                     const float*, const uint16_t*, const float*, const uint16_t*, uint16_t*, uint16_t*,
+                                     void*, int64_t, int64_t, int64_t, const K2ParamSums&, hipStream_t);
+
 }  // namespace fmhc
+
+extern "C" int64_t fmhc_k1_bwd_pack8_workspace_bytes(int64_t T, int64_t C) {
+  if (T <= 0 || C <= 0 || C > (int64_t{1} << 24)) return 0;
+  return fmhc::k1_bwd_premap_ws_bytes(T, C);
+}
+
+extern "C" int fmhc_k1_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const uint16_t* W,
+                                 const uint16_t* grad_out, const uint16_t* proj_out, const float* inv_rms,
+                                 uint16_t* grad_x, uint16_t* grad_W, void* workspace, int64_t workspace_bytes,
+                                 int64_t T, int64_t C, int64_t n, void* stream) {
+  using namespace fmhc;
+  if (T < 0 || C <= 0 || C > (int64_t{1} << 24) || n != 4 || !grad_W) return FMHC_ERR_INVALID_ARGUMENT;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t nC = 4 * C;
+  const int nc = static_cast<int>(nC), c = static_cast<int>(C);
+  if (T == 0) {  // grad_W of an empty batch is zero
+    k1_dw_zero<<<dim3(blocks_for(static_cast<int64_t>(kDout) * nC, 256)), 256, 0, s>>>(grad_W, nc);
+    return launch_status();
+  }
+  if (!x_codes || !x_scales || !W || !grad_out || !proj_out || !inv_rms || !grad_x) return FMHC_ERR_INVALID_ARGUMENT;
+  if (k1_bwd_premap_fused(C)) {
+    if (!workspace || workspace_bytes < k1_bwd_premap_ws_bytes(T, C) || !aligned16(workspace))
+      return FMHC_ERR_INVALID_ARGUMENT;
+    const BwdSlices sl = bwd_premap_slices(C);
+    const int64_t nruns = k1_bwd_runs(T, sl.n);
+    float* partial = static_cast<float*>(workspace);
+    launch_k1_bwd_mfma<true, false, false, Pack8Src>(s, x_codes, W, grad_out, proj_out, inv_rms, grad_x, partial, T, nc,
+                                                     sl, nruns, nullptr, nullptr, c, nullptr, x_scales);
+    const int st = launch_status();
+    if (st != FMHC_OK) return st;
+    return launch_dw_reduce(partial, grad_W, nruns, sl, nc, K2ParamSums{}, 0, s);
+  }
+  launch_k1_bwd_scalar<false, Pack8Src>(s, x_codes, W, grad_out, proj_out, inv_rms, grad_x, nullptr, T, nc, c, x_scales);
+  const int st = launch_status();
+  if (st != FMHC_OK) return st;
+  launch_k1_dw_scalar<Pack8Src>(s, x_codes, grad_out, inv_rms, grad_W, T, nc, c, x_scales);
+  return launch_status();
+}

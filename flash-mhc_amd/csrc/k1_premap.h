@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "k2_chain.h"
+#include "pack8.h"
 
 namespace fmhc {
 
@@ -66,10 +67,17 @@ int64_t k1_bwd_premap_ws_bytes(int64_t T, int64_t C);
 // grad_x = bf16(grad_x_in + that).  `workspace`: k1_bwd_premap_ws_bytes(T, C),
 // 16-byte aligned.  K2's parameter gradients
 // (k2_bwd_partials) are summed by the same launch as grad_W's partials.
-int k1_bwd_premap(const uint16_t* x_flat, const uint16_t* W, const uint16_t* grad_proj,
+// SRC: x in bf16 (xs unused), or its codes and scales xs (pack8.h).
+template <typename SRC>
+int k1_bwd_premap(const typename SRC::Elem* x_flat, const uint8_t* xs, const uint16_t* W, const uint16_t* grad_proj,
                   const uint16_t* proj, const float* inv_rms, const uint16_t* go3, const float* h_pre,
                   const uint16_t* grad_x_in, uint16_t* grad_x, uint16_t* grad_W, void* workspace,
                   int64_t workspace_bytes, int64_t T, int64_t C, const K2ParamSums& k2_sums, hipStream_t s);
+
+// fmhc_k3_bwd for either source of x (grad_x null: grad_h_pre only).
+template <typename SRC>
+int k3_bwd_run(const typename SRC::Elem* x, const uint8_t* xs, const float* h_pre, const uint16_t* grad_out,
+               uint16_t* grad_x, float* grad_h_pre, int64_t T, int C, hipStream_t s);
 
 // fmhc_k2_bwd without its last launch: K2's backward writes grad_proj and the
 // per-workgroup parameter partials, and *sums describes what remains to sum

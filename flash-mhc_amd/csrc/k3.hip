@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "fmhc_common.h"
+#include "k1_premap.h"
 
 namespace fmhc {
 
@@ -52,13 +53,14 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_fwd_kernel(const uin
 // (fmhc_common.h), which the pre-map backward's split kernel reproduces;
 // otherwise one FMA chain per lane over its groups and its elements of the
 // row's tail, then group_sum.
-template <typename WALK, bool GX, bool CANON>
-__global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_bwd_kernel(const uint16_t* __restrict__ x,
+// SRC: x in bf16, or in 8 bits with scales xs (pack8.h).
+template <typename WALK, bool GX, bool CANON, typename SRC>
+__global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_bwd_kernel(const typename SRC::Elem* __restrict__ x,
                                                         const float* __restrict__ h_pre,
                                                         const uint16_t* __restrict__ go,
                                                         uint16_t* __restrict__ grad_x,
                                                         float* __restrict__ grad_h_pre,
-                                                        int64_t T, int C) {
+                                                        int64_t T, int C, const uint8_t* __restrict__ xs) {
   constexpr int LPT = WALK::LPT;
   constexpr bool LOOP = WALK::LOOP, WHOLE = WALK::WHOLE;
   static_assert(!CANON || LPT >= 16, "slice order: whole 16-lane rows");
@@ -83,10 +85,11 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_bwd_kernel(const uin
   if (live) {
   const float* hp = h_pre + tok * 4;
   const float h0 = hp[0], h1 = hp[1], h2 = hp[2], h3 = hp[3];
-  const uint16_t* x0 = x + tok * 4 * C;
-  const uint16_t* x1 = x0 + C;
-  const uint16_t* x2 = x1 + C;
-  const uint16_t* x3 = x2 + C;
+  using Row = typename SRC::template Row<WHOLE>;
+  const Row x0 = Row::at(x, xs, tok * 4, C);
+  const Row x1 = x0.next(C);
+  const Row x2 = x1.next(C);
+  const Row x3 = x2.next(C);
   const uint16_t* grow = go + tok * C;
   uint16_t* gx0 = grad_x + tok * 4 * C;
   uint16_t* gx1 = gx0 + C;
@@ -97,10 +100,10 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_bwd_kernel(const uin
     constexpr int VEC = decltype(vec)::value;
     float q[VEC], a[VEC], b[VEC], c[VEC], d[VEC], o[VEC];
     Lanes<VEC, WHOLE>::load(grow, g, q);
-    Lanes<VEC, WHOLE>::load(x0, g, a);
-    Lanes<VEC, WHOLE>::load(x1, g, b);
-    Lanes<VEC, WHOLE>::load(x2, g, c);
-    Lanes<VEC, WHOLE>::load(x3, g, d);
+    x0.load(g, a);
+    x1.load(g, b);
+    x2.load(g, c);
+    x3.load(g, d);
     if constexpr (GX) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[e] = h0 * q[e];
@@ -234,23 +237,24 @@ int launch_k3_fwd(const uint16_t* x, const float* h_pre, uint16_t* out, int64_t 
   return launch_status();
 }
 
-template <bool GX>
-int launch_k3_bwd(const uint16_t* x, const float* h_pre, const uint16_t* go, uint16_t* grad_x,
+template <bool GX, typename SRC>
+int launch_k3_bwd(const typename SRC::Elem* x, const uint8_t* xs, const float* h_pre, const uint16_t* go, uint16_t* grad_x,
                   float* grad_h_pre, int64_t T, int C, hipStream_t s) {
   const bool canon = k3_canon(C, lanes_per_token(C));
-  with_row_walk(C, aligned16(x) && aligned16(go) && aligned16(grad_x), [&](auto w) {
+  with_row_walk(C, SRC::aligned(x) && aligned16(go) && aligned16(grad_x), [&](auto w) {
     constexpr int L = decltype(w)::LPT;
     auto launch = [&](auto walk, auto canon_c) {
       using Walk = decltype(walk);
       constexpr bool CANON = decltype(canon_c)::value;
       // Residency cap (fmhc_common.h): with grad_x and one group per lane.
-      static const unsigned own = own_lds(reinterpret_cast<const void*>(&k3_bwd_kernel<Walk, GX, CANON>));
+      static const unsigned own = own_lds(reinterpret_cast<const void*>(&k3_bwd_kernel<Walk, GX, CANON, SRC>));
       for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
         const dim3 grid(blocks_for(n, tokens_per_block(L)));
         unsigned lds = 0;
         if (GX && FMHC_LDS_CAP && !Walk::LOOP) lds = cap_lds(own, grid.x, block_of<L>(), L, C / 8, Walk::CAP);
-        k3_bwd_kernel<Walk, GX, CANON><<<grid, block_of<L>(), lds, s>>>(
-            x + t * 4 * C, h_pre + t * 4, go + t * C, GX ? grad_x + t * 4 * C : nullptr, grad_h_pre + t * 4, n, C);
+        k3_bwd_kernel<Walk, GX, CANON, SRC><<<grid, block_of<L>(), lds, s>>>(
+            x + t * 4 * C, h_pre + t * 4, go + t * C, GX ? grad_x + t * 4 * C : nullptr, grad_h_pre + t * 4, n, C,
+            SRC::kPacked ? xs + t * 4 * pack_groups(C) : nullptr);
       });
     };
     if constexpr (L >= 16) {
@@ -273,6 +277,18 @@ bool bad_sizes(int64_t T, int64_t C, int64_t n) {
 
 }  // namespace
 
+template <typename SRC>
+int k3_bwd_run(const typename SRC::Elem* x, const uint8_t* xs, const float* h_pre, const uint16_t* grad_out,
+               uint16_t* grad_x, float* grad_h_pre, int64_t T, int C, hipStream_t s) {
+  return grad_x ? launch_k3_bwd<true, SRC>(x, xs, h_pre, grad_out, grad_x, grad_h_pre, T, C, s)
+                : launch_k3_bwd<false, SRC>(x, xs, h_pre, grad_out, nullptr, grad_h_pre, T, C, s);  // grad_h_pre only
+}
+
+template int k3_bwd_run<Bf16Src>(const uint16_t*, const uint8_t*, const float*, const uint16_t*, uint16_t*, float*,
+                                 int64_t, int, hipStream_t);
+template int k3_bwd_run<Pack8Src>(const int8_t*, const uint8_t*, const float*, const uint16_t*, uint16_t*, float*,
+                                  int64_t, int, hipStream_t);
+
 }  // namespace fmhc
 
 extern "C" int fmhc_k3_fwd(const uint16_t* x, const float* h_pre, uint16_t* out, int64_t T,
@@ -293,7 +309,5 @@ extern "C" int fmhc_k3_bwd(const uint16_t* x, const float* h_pre, const uint16_t
   if (T == 0) return FMHC_OK;
   if (!x || !h_pre || !grad_out || !grad_h_pre) return FMHC_ERR_INVALID_ARGUMENT;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int c = static_cast<int>(C);
-  return grad_x ? launch_k3_bwd<true>(x, h_pre, grad_out, grad_x, grad_h_pre, T, c, s)
-                : launch_k3_bwd<false>(x, h_pre, grad_out, nullptr, grad_h_pre, T, c, s);  // grad_h_pre only
+  return k3_bwd_run<Bf16Src>(x, nullptr, h_pre, grad_out, grad_x, grad_h_pre, T, static_cast<int>(C), s);
 }

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "fmhc_common.h"
+#include "pack8.h"
 
 namespace fmhc {
 
@@ -87,9 +88,107 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_kernel(const uin
   row_tail<WHOLE>(C, sub, [&](int c) { mix(Vec<1>{}, c); });
 }
 
-template <typename WALK, bool EARLY>
-__global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const uint16_t* __restrict__ x,
-                                                        const uint16_t* __restrict__ lo,
+// The forward that also leaves x and lo in 8 bits (pack8.h) for the backward:
+// out as k4_fwd_kernel gives it, and the codes and scales of the rows it has in
+// registers anyway, which a pass of its own would read again.  A quad of lanes
+// holds a group of 32 columns; the lane at a row's end with fewer than 8 columns
+// left moves them one by one.
+template <typename WALK>
+__global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
+    const uint16_t* __restrict__ x, const uint16_t* __restrict__ lo, const float* __restrict__ H,
+    const float* __restrict__ h_post, uint16_t* __restrict__ out, int8_t* __restrict__ xq, uint8_t* __restrict__ xs,
+    int8_t* __restrict__ lq, uint8_t* __restrict__ ls, int64_t T, int C) {
+  constexpr int LPT = WALK::LPT;
+  constexpr bool LOOP = WALK::LOOP, WHOLE = WALK::WHOLE;
+  static_assert(LPT % 4 == 0, "a group's quad of lanes");
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t tok = token_of_lane<LPT>(lane);
+  if (tok >= T) return;
+  const int sub = sub_of_lane<LPT>();
+  const int G = pack_groups(C);
+
+  float h[4][4], p[4];
+  {
+    const float* Ht = H + tok * 16;
+    const float* pt = h_post + tok * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = pt[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[i][j] = Ht[i * 4 + j];
+    }
+  }
+  const uint16_t* x0 = x + tok * 4 * C;
+  const uint16_t* lrow = lo + tok * C;
+  uint16_t* o0 = out + tok * 4 * C;
+  int8_t* q0 = xq + tok * 4 * C;
+  uint8_t* s0 = xs + tok * 4 * G;
+
+  // Lane group g: columns 8 g .. 8 g + 7, of which n are in the row.
+  auto round = [&](int g) __attribute__((always_inline)) {
+    const int n = C - 8 * g;
+    const bool whole = WHOLE ? n > 0 : n >= 8;
+    float v[5][8];  // lo, then the streams
+    auto fetch = [&](const uint16_t* row, float (&f)[8]) __attribute__((always_inline)) {
+      if (whole) {
+        Lanes<8, WHOLE>::load(row, g, f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = !WHOLE && e < n ? bf16_to_f32(row[8 * g + e]) : 0.f;
+      }
+    };
+    fetch(lrow, v[0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fetch(x0 + j * int64_t{C}, v[1 + j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float acc = p[i] * v[0][e];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_fmaf(h[i][j], v[1 + j][e], acc);
+        o[e] = acc;
+      }
+      uint16_t* orow = o0 + i * int64_t{C};
+      if (whole) {
+        Lanes<8, WHOLE>::store(orow, g, o);
+      } else if constexpr (!WHOLE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < n) orow[8 * g + e] = f32_to_bf16(o[e]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      const uint32_t E = pack_scale(quad_max(max_bits8(v[k])));  // the whole quad is here
+      const u32x2 q = encode8(v[k], E);
+      int8_t* qrow = k == 0 ? lq + tok * C : q0 + (k - 1) * int64_t{C};
+      uint8_t* srow = k == 0 ? ls + tok * G : s0 + (k - 1) * int64_t{G};
+      if (whole) {
+        st_codes<WHOLE>(qrow + 8 * g, q);
+      } else if constexpr (!WHOLE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < n) qrow[8 * g + e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+      }
+      if ((g & 3) == 0 && n > 0) srow[g >> 2] = static_cast<uint8_t>(E);
+    }
+  };
+  // Quads enter whole: a quad's first lane holds a group's first columns.
+  if constexpr (!LOOP) {
+    if ((sub & ~3) < 4 * G) round(sub);
+  } else {
+    for (int g = sub; (g & ~3) < 4 * G; g += LPT) round(g);
+  }
+}
+
+// SRC: where x and lo are read from (bf16 rows, or their 8-bit copies with
+// scales xs and los; pack8.h).  The arithmetic and the order of the sums are
+// the same.
+template <typename WALK, bool EARLY, typename SRC>
+__global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const typename SRC::Elem* __restrict__ x,
+                                                        const typename SRC::Elem* __restrict__ lo,
                                                         const float* __restrict__ H,
                                                         const float* __restrict__ h_post,
                                                         const uint16_t* __restrict__ go,
@@ -97,7 +196,8 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const uin
                                                         uint16_t* __restrict__ grad_lo,
                                                         float* __restrict__ grad_H,
                                                         float* __restrict__ grad_hp,
-                                                        int64_t T, int C) {
+                                                        int64_t T, int C, const uint8_t* __restrict__ xs,
+                                                        const uint8_t* __restrict__ los) {
   constexpr int LPT = WALK::LPT;
   constexpr bool LOOP = WALK::LOOP, WHOLE = WALK::WHOLE;
   constexpr int WPT = LPT > kWave ? LPT / kWave : 1;  // waves per token
@@ -130,19 +230,20 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const uin
       for (int j = 0; j < 4; ++j) h[i][j] = Ht[i * 4 + j];
     }
   }
-  const uint16_t* xr[4];
+  using Row = typename SRC::template Row<WHOLE>;
+  Row xr[4];
   const uint16_t* gr[4];
   uint16_t* gxr[4];
-  xr[0] = x + tok * 4 * C;
+  xr[0] = Row::at(x, xs, tok * 4, C);
   gr[0] = go + tok * 4 * C;
   gxr[0] = grad_x + tok * 4 * C;
 #pragma unroll
   for (int j = 1; j < 4; ++j) {
-    xr[j] = xr[j - 1] + C;
+    xr[j] = xr[j - 1].next(C);
     gr[j] = gr[j - 1] + C;
     gxr[j] = gxr[j - 1] + C;
   }
-  const uint16_t* lrow = lo + tok * C;
+  const Row lrow = Row::at(lo, los, tok, C);
   uint16_t* glrow = grad_lo + tok * C;
 
   auto round = [&](auto vec, int g) __attribute__((always_inline)) {
@@ -150,14 +251,14 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const uin
     float q[4][VEC], l[VEC];
 #pragma unroll
     for (int i = 0; i < 4; ++i) Lanes<VEC, WHOLE>::load(gr[i], g, q[i]);
-    Lanes<VEC, WHOLE>::load(lrow, g, l);
+    lrow.load(g, l);
 
     // EARLY: the iteration's x rows load with grad_out and lo, before its
     // first store (the compiler keeps a load behind an earlier store).
-    float xs[EARLY ? 4 : 1][VEC];
+    float xe[EARLY ? 4 : 1][VEC];
     if constexpr (EARLY) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) Lanes<VEC, WHOLE>::load(xr[j], g, xs[j]);
+      for (int j = 0; j < 4; ++j) xr[j].load(g, xe[j]);
     }
     // grad_lo and the grad_h_post partial sums.
     {
@@ -182,9 +283,9 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const uin
       float xl[VEC], o[VEC];
       const float* xv = xl;
       if constexpr (EARLY)
-        xv = xs[j];
+        xv = xe[j];
       else
-        Lanes<VEC, WHOLE>::load(xr[j], g, xl);
+        xr[j].load(g, xl);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -278,12 +379,32 @@ int launch_k4_fwd(const uint16_t* x, const uint16_t* lo, const float* H, const f
   return launch_status();
 }
 
+int launch_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* hp, uint16_t* out,
+                        int8_t* xq, uint8_t* xs, int8_t* lq, uint8_t* ls, int64_t T, int C, hipStream_t s) {
+  const bool aligned = C % 8 == 0 && aligned16(x) && aligned16(lo) && aligned16(out) && Pack8Src::aligned(xq) &&
+                       Pack8Src::aligned(lq);
+  const int G = pack_groups(C);
+  // Lanes for whole groups of 32 columns.
+  with_row_walk(G * kPackGroup, aligned, [&](auto w) {
+    using Walk = decltype(w);
+    constexpr int L = Walk::LPT;
+    for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
+      const dim3 grid(blocks_for(n, tokens_per_block(L)));
+      k4_fwd_pack8_kernel<Walk><<<grid, block_of<L>(), 0, s>>>(
+          x + t * 4 * C, lo + t * C, H + t * 16, hp + t * 4, out + t * 4 * C, xq + t * 4 * C, xs + t * 4 * G,
+          lq + t * C, ls + t * G, n, C);
+    });
+  });
+  return launch_status();
+}
+
 constexpr int64_t kK4EarlyLanes = int64_t{16384} * 64;
 
-int launch_k4_bwd(const uint16_t* x, const uint16_t* lo, const float* H, const float* hp,
+template <typename SRC>
+int launch_k4_bwd(const typename SRC::Elem* x, const typename SRC::Elem* lo, const float* H, const float* hp,
                   const uint16_t* go, uint16_t* gx, uint16_t* glo, float* gH, float* ghp,
-                  int64_t T, int C, hipStream_t s) {
-  const bool aligned = aligned16(x) && aligned16(lo) && aligned16(go) && aligned16(gx) && aligned16(glo);
+                  int64_t T, int C, hipStream_t s, const uint8_t* xs = nullptr, const uint8_t* los = nullptr) {
+  const bool aligned = SRC::aligned(x) && SRC::aligned(lo) && aligned16(go) && aligned16(gx) && aligned16(glo);
   with_row_walk(C, aligned, [&](auto w) {
     using Walk = decltype(w);
     constexpr int L = Walk::LPT;
@@ -292,14 +413,15 @@ int launch_k4_bwd(const uint16_t* x, const uint16_t* lo, const float* H, const f
       constexpr bool E = decltype(early)::value;
       // Residency cap (fmhc_common.h) with one group per lane, up to 256 lanes
       // (T = 30000, C = 3000 440 us with and without).
-      static const unsigned own = own_lds(reinterpret_cast<const void*>(&k4_bwd_kernel<W, E>));
+      static const unsigned own = own_lds(reinterpret_cast<const void*>(&k4_bwd_kernel<W, E, SRC>));
       for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
         const dim3 grid(blocks_for(n, tokens_per_block(L)));
         unsigned lds = 0;
         if (FMHC_LDS_CAP && C / 8 <= L && L <= 256) lds = cap_lds(own, grid.x, block_of<L>(), L, C / 8, Walk::CAP);
-        k4_bwd_kernel<W, E><<<grid, block_of<L>(), lds, s>>>(
+        k4_bwd_kernel<W, E, SRC><<<grid, block_of<L>(), lds, s>>>(
             x + t * 4 * C, lo + t * C, H + t * 16, hp + t * 4, go + t * 4 * C, gx + t * 4 * C, glo + t * C,
-            gH + t * 16, ghp + t * 4, n, C);
+            gH + t * 16, ghp + t * 4, n, C, SRC::kPacked ? xs + t * 4 * pack_groups(C) : nullptr,
+            SRC::kPacked ? los + t * pack_groups(C) : nullptr);
       });
     };
     // EARLY: all of a lane's loads go out before its first store, so a wave
@@ -349,6 +471,32 @@ extern "C" int fmhc_k4_bwd(const uint16_t* x, const uint16_t* lo, const float* H
   if (!x || !lo || !H || !h_post || !grad_out || !grad_x || !grad_lo || !grad_H || !grad_h_post)
     return FMHC_ERR_INVALID_ARGUMENT;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return launch_k4_bwd(x, lo, H, h_post, grad_out, grad_x, grad_lo, grad_H, grad_h_post, T, static_cast<int>(C),
+  return launch_k4_bwd<Bf16Src>(x, lo, H, h_post, grad_out, grad_x, grad_lo, grad_H, grad_h_post, T, static_cast<int>(C),
                        s);
+}
+
+extern "C" int fmhc_k4_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const int8_t* lo_codes,
+                                 const uint8_t* lo_scales, const float* H, const float* h_post,
+                                 const uint16_t* grad_out, uint16_t* grad_x, uint16_t* grad_lo, float* grad_H,
+                                 float* grad_h_post, int64_t T, int64_t C, int64_t n, void* stream) {
+  using namespace fmhc;
+  if (bad_sizes(T, C, n)) return FMHC_ERR_INVALID_ARGUMENT;
+  if (T == 0) return FMHC_OK;
+  if (!x_codes || !x_scales || !lo_codes || !lo_scales || !H || !h_post || !grad_out || !grad_x || !grad_lo ||
+      !grad_H || !grad_h_post)
+    return FMHC_ERR_INVALID_ARGUMENT;
+  return launch_k4_bwd<Pack8Src>(x_codes, lo_codes, H, h_post, grad_out, grad_x, grad_lo, grad_H, grad_h_post, T,
+                                 static_cast<int>(C), static_cast<hipStream_t>(stream), x_scales, lo_scales);
+}
+
+extern "C" int fmhc_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* h_post,
+                                 uint16_t* out, int8_t* x_codes, uint8_t* x_scales, int8_t* lo_codes,
+                                 uint8_t* lo_scales, int64_t T, int64_t C, int64_t n, void* stream) {
+  using namespace fmhc;
+  if (bad_sizes(T, C, n)) return FMHC_ERR_INVALID_ARGUMENT;
+  if (T == 0) return FMHC_OK;
+  if (!x || !lo || !H || !h_post || !out || !x_codes || !x_scales || !lo_codes || !lo_scales)
+    return FMHC_ERR_INVALID_ARGUMENT;
+  return launch_k4_fwd_pack8(x, lo, H, h_post, out, x_codes, x_scales, lo_codes, lo_scales, T, static_cast<int>(C),
+                             static_cast<hipStream_t>(stream));
 }

@@ -262,11 +262,12 @@ __global__ __launch_bounds__(kFinishThreads) void k1_finish_k2_k3(
 // token order.  grad_proj and the parameter partials are those of K3's
 // backward followed by k2_bwd_small, bit for bit, with one launch and one
 // chain of load latencies fewer.
-template <int LPT, bool CANON>
+// SRC: x in bf16, or in 8 bits with scales xs (pack8.h).
+template <int LPT, bool CANON, typename SRC>
 __global__ __launch_bounds__(kK2BwdTok * LPT) void k3_reduce_k2_bwd(
-    const uint16_t* __restrict__ x, const uint16_t* __restrict__ go3, const uint16_t* __restrict__ proj,
+    const typename SRC::Elem* __restrict__ x, const uint16_t* __restrict__ go3, const uint16_t* __restrict__ proj,
     const K2Params P, const float* __restrict__ g_hpost, const float* __restrict__ g_H,
-    uint16_t* __restrict__ grad_proj, float* __restrict__ partial, int64_t T, int C) {
+    uint16_t* __restrict__ grad_proj, float* __restrict__ partial, int64_t T, int C, const uint8_t* __restrict__ xs) {
   static_assert(LPT == 32 || LPT == 64, "half a wave or one wave per token");
   constexpr int kThreads = kK2BwdTok * LPT;
   __shared__ K2Smem sm;
@@ -288,20 +289,21 @@ __global__ __launch_bounds__(kK2BwdTok * LPT) void k3_reduce_k2_bwd(
   // in k3_bwd_kernel's order (with CANON the slice order of slice_sums_add).
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   const int ng = C / 8;
-  const uint16_t* x0 = x + t * 4 * C;
-  const uint16_t* x1 = x0 + C;
-  const uint16_t* x2 = x1 + C;
-  const uint16_t* x3 = x2 + C;
+  using Row = typename SRC::template Row<false>;
+  const Row x0 = Row::at(x, xs, t * 4, C);
+  const Row x1 = x0.next(C);
+  const Row x2 = x1.next(C);
+  const Row x3 = x2.next(C);
   const uint16_t* grow = go3 + t * C;
   auto round = [&](auto vec, int g, float (&acc)[4]) __attribute__((always_inline)) {
     constexpr int VEC = decltype(vec)::value;
     float gq[VEC], a[VEC], b[VEC], c[VEC], d[VEC];
     // Ordinary loads: K1's backward reads both again right after.
     Lanes<VEC, false>::load(grow, g, gq);
-    Lanes<VEC, false>::load(x0, g, a);
-    Lanes<VEC, false>::load(x1, g, b);
-    Lanes<VEC, false>::load(x2, g, c);
-    Lanes<VEC, false>::load(x3, g, d);
+    x0.load(g, a);
+    x1.load(g, b);
+    x2.load(g, c);
+    x3.load(g, d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       acc[0] = __builtin_fmaf(a[e], gq[e], acc[0]);
@@ -520,22 +522,24 @@ extern "C" int64_t fmhc_premap_bwd_workspace_bytes(int64_t T, int64_t C) {
   return premap_ws(T, C).total;
 }
 
-extern "C" int fmhc_premap_bwd(const uint16_t* x, const uint16_t* W, const void* alpha_pre,
-                               const void* alpha_post, const void* alpha_res, const void* bias,
-                               const void* perm, int param_dtype, const float* h_pre, const uint16_t* proj,
-                               const float* inv_rms, const uint16_t* grad_layer_input,
-                               const float* grad_h_post, const float* grad_H_merged,
-                               const uint16_t* grad_x_in, uint16_t* grad_x,
-                               uint16_t* grad_W, void* grad_alpha_pre, void* grad_alpha_post,
-                               void* grad_alpha_res, void* grad_bias, void* workspace,
-                               int64_t workspace_bytes, int64_t T, int64_t C, int64_t n, void* stream) {
+namespace {
+
+// The backward for either source of x (bf16, or codes with scales xs; pack8.h).
+template <typename SRC>
+int premap_bwd_run(const typename SRC::Elem* x, const uint8_t* xs, const uint16_t* W, const void* alpha_pre,
+                   const void* alpha_post, const void* alpha_res, const void* bias, const void* perm, int param_dtype,
+                   const float* h_pre, const uint16_t* proj, const float* inv_rms, const uint16_t* grad_layer_input,
+                   const float* grad_h_post, const float* grad_H_merged, const uint16_t* grad_x_in, uint16_t* grad_x,
+                   uint16_t* grad_W, void* grad_alpha_pre, void* grad_alpha_post, void* grad_alpha_res,
+                   void* grad_bias, void* workspace, int64_t workspace_bytes, int64_t T, int64_t C, int64_t n,
+                   void* stream) {
   using namespace fmhc;
   if (T < 0 || C <= 0 || C > (int64_t{1} << 24) || n != 4 || !param_dtype_ok(param_dtype))
     return FMHC_ERR_INVALID_ARGUMENT;
   if (!W || !alpha_pre || !alpha_post || !alpha_res || !bias || !perm || !grad_W || !grad_alpha_pre ||
       !grad_alpha_post || !grad_alpha_res || !grad_bias)
     return FMHC_ERR_INVALID_ARGUMENT;
-  if (T > 0 && (!x || !h_pre || !proj || !inv_rms || !grad_layer_input || !grad_x)) return FMHC_ERR_INVALID_ARGUMENT;
+  if (T > 0 && (!x || (SRC::kPacked && !xs) || !h_pre || !proj || !inv_rms || !grad_layer_input || !grad_x)) return FMHC_ERR_INVALID_ARGUMENT;
   if (T > 0 && grad_x_in) {  // grad_x_in is read while grad_x is written: no overlap
     const auto a = reinterpret_cast<uintptr_t>(grad_x_in), b = reinterpret_cast<uintptr_t>(grad_x);
     const auto bytes = static_cast<uintptr_t>(T * n * C * 2);
@@ -549,13 +553,15 @@ extern "C" int fmhc_premap_bwd(const uint16_t* x, const uint16_t* W, const void*
     return FMHC_ERR_INVALID_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (FMHC_PREMAP_SPLIT && premap_split_ok(x, W, proj, inv_rms, grad_x, grad_layer_input, grad_x_in, T, C)) {
+  if constexpr (FMHC_PREMAP_SPLIT && !SRC::kPacked) {
+    if (premap_split_ok(x, W, proj, inv_rms, grad_x, grad_layer_input, grad_x_in, T, C)) {
     K2Params P;
     if (!k2_params(alpha_pre, alpha_post, alpha_res, bias, perm, param_dtype, P)) return FMHC_ERR_INVALID_ARGUMENT;
     return premap_bwd_split(x, W, proj, inv_rms, grad_layer_input, h_pre, grad_h_post, grad_H_merged, grad_x_in,
                             grad_x, grad_W, P, grad_alpha_pre, grad_alpha_post, grad_alpha_res, grad_bias,
                             reinterpret_cast<float*>(ws + w.k2), reinterpret_cast<float*>(ws + w.k1), ws + w.ring, T,
                             C, s);
+    }
   }
   float* gh = T > 0 ? reinterpret_cast<float*>(ws + w.gh) : nullptr;
   uint16_t* gp = T > 0 ? reinterpret_cast<uint16_t*>(ws + w.gp) : nullptr;
@@ -577,8 +583,8 @@ extern "C" int fmhc_premap_bwd(const uint16_t* x, const uint16_t* W, const void*
     const bool canon = k3_canon(C, lanes);
     auto launch = [&](auto lpt_c, auto canon_c) {
       constexpr int L = decltype(lpt_c)::value;
-      k3_reduce_k2_bwd<L, decltype(canon_c)::value><<<grid, kK2BwdTok * L, 0, s>>>(
-          x, grad_layer_input, proj, P, grad_h_post, grad_H_merged, gp, partial, T, static_cast<int>(C));
+      k3_reduce_k2_bwd<L, decltype(canon_c)::value, SRC><<<grid, kK2BwdTok * L, 0, s>>>(
+          x, grad_layer_input, proj, P, grad_h_post, grad_H_merged, gp, partial, T, static_cast<int>(C), xs);
     };
     using I64 = std::integral_constant<int, 64>;
     using I32 = std::integral_constant<int, 32>;
@@ -590,14 +596,46 @@ extern "C" int fmhc_premap_bwd(const uint16_t* x, const uint16_t* W, const void*
     sums = K2ParamSums{partial, static_cast<int64_t>(grid.x), grad_alpha_pre, grad_alpha_post, grad_alpha_res,
                        grad_bias, P.bf16};
   } else {
-    if (T > 0) st = fmhc_k3_bwd(x, h_pre, grad_layer_input, fused ? nullptr : grad_x, gh, T, C, n, stream);
+    if (T > 0)
+      st = k3_bwd_run<SRC>(x, xs, h_pre, grad_layer_input, fused ? nullptr : grad_x, gh, T, static_cast<int>(C), s);
     if (st == FMHC_OK)
       st = k2_bwd_partials(proj, P, gh, grad_h_post, grad_H_merged, gp, grad_alpha_pre, grad_alpha_post,
                            grad_alpha_res, grad_bias, T > 0 ? ws + w.k2 : nullptr, T > 0 ? w.k1 - w.k2 : 0, T, s,
                            &sums);
   }
   if (st == FMHC_OK)
-    st = k1_bwd_premap(x, W, gp, proj, inv_rms, grad_layer_input, h_pre, grad_x_in, grad_x, grad_W,
+    st = k1_bwd_premap<SRC>(x, xs, W, gp, proj, inv_rms, grad_layer_input, h_pre, grad_x_in, grad_x, grad_W,
                        fused ? ws + w.k1 : nullptr, fused ? w.total - w.k1 : 0, T, C, sums, s);
   return st;
+}
+
+}  // namespace
+
+extern "C" int fmhc_premap_bwd(const uint16_t* x, const uint16_t* W, const void* alpha_pre,
+                               const void* alpha_post, const void* alpha_res, const void* bias,
+                               const void* perm, int param_dtype, const float* h_pre, const uint16_t* proj,
+                               const float* inv_rms, const uint16_t* grad_layer_input,
+                               const float* grad_h_post, const float* grad_H_merged,
+                               const uint16_t* grad_x_in, uint16_t* grad_x,
+                               uint16_t* grad_W, void* grad_alpha_pre, void* grad_alpha_post,
+                               void* grad_alpha_res, void* grad_bias, void* workspace,
+                               int64_t workspace_bytes, int64_t T, int64_t C, int64_t n, void* stream) {
+  return premap_bwd_run<fmhc::Bf16Src>(x, nullptr, W, alpha_pre, alpha_post, alpha_res, bias, perm, param_dtype, h_pre,
+                                       proj, inv_rms, grad_layer_input, grad_h_post, grad_H_merged, grad_x_in, grad_x,
+                                       grad_W, grad_alpha_pre, grad_alpha_post, grad_alpha_res, grad_bias, workspace,
+                                       workspace_bytes, T, C, n, stream);
+}
+
+extern "C" int fmhc_premap_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const uint16_t* W,
+                                     const void* alpha_pre, const void* alpha_post, const void* alpha_res,
+                                     const void* bias, const void* perm, int param_dtype, const float* h_pre,
+                                     const uint16_t* proj, const float* inv_rms, const uint16_t* grad_layer_input,
+                                     const float* grad_h_post, const float* grad_H_merged, const uint16_t* grad_x_in,
+                                     uint16_t* grad_x, uint16_t* grad_W, void* grad_alpha_pre, void* grad_alpha_post,
+                                     void* grad_alpha_res, void* grad_bias, void* workspace, int64_t workspace_bytes,
+                                     int64_t T, int64_t C, int64_t n, void* stream) {
+  return premap_bwd_run<fmhc::Pack8Src>(x_codes, x_scales, W, alpha_pre, alpha_post, alpha_res, bias, perm, param_dtype,
+                                        h_pre, proj, inv_rms, grad_layer_input, grad_h_post, grad_H_merged, grad_x_in,
+                                        grad_x, grad_W, grad_alpha_pre, grad_alpha_post, grad_alpha_res, grad_bias,
+                                        workspace, workspace_bytes, T, C, n, stream);
 }

@@ -23,6 +23,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libflash_mhc_hip.so"
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
+_F32 = ctypes.c_float
 
 # name -> argtypes, following include/flash_mhc_hip.h
 SIGNATURES: dict[str, list] = {
@@ -44,6 +45,16 @@ SIGNATURES: dict[str, list] = {
     "fmhc_k3_bwd": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P],
     "fmhc_k4_fwd": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P],
     "fmhc_k4_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P],
+    "fmhc_pack8": [_P, _INT, _P, _P, _I64, _I64, _P],
+    "fmhc_unpack8": [_P, _P, _P, _INT, _I64, _I64, _P],
+    "fmhc_k4_fwd_pack8": [_P] * 9 + [_I64] * 3 + [_P],
+    "fmhc_k4_bwd_pack8": [_P] * 11 + [_I64] * 3 + [_P],
+    "fmhc_k1_bwd_pack8": [_P] * 9 + [_I64] * 4 + [_P],
+    "fmhc_k1_bwd_pack8_workspace_bytes": [_I64, _I64],
+    "fmhc_premap_bwd_pack8": [_P] * 8 + [_INT] + [_P] * 14 + [_I64, _I64, _I64, _I64, _P],
+    "fmhc_layer_norm_fwd": [_P] * 8 + [_INT, _INT, _I64, _I64, _F32, _P],
+    "fmhc_layer_norm_bwd": [_P] * 11 + [_I64, _INT, _INT, _I64, _I64, _P],
+    "fmhc_layer_norm_bwd_workspace_bytes": [_I64, _I64],
     "fmhc_error_string": [ctypes.c_int],
     "fmhc_abi_version": [],
 }
@@ -54,9 +65,11 @@ RESTYPES = {
     "fmhc_premap_fwd_workspace_bytes": ctypes.c_int64,
     "fmhc_k2_bwd_workspace_bytes": ctypes.c_int64,
     "fmhc_premap_bwd_workspace_bytes": ctypes.c_int64,
+    "fmhc_k1_bwd_pack8_workspace_bytes": ctypes.c_int64,
+    "fmhc_layer_norm_bwd_workspace_bytes": ctypes.c_int64,
 }
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

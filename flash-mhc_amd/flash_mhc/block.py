@@ -34,6 +34,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as _checkpoint
 
+from . import activation8 as _a8
 from . import ops as _ops
 
 
@@ -101,6 +102,19 @@ class MHCLiteBlock(nn.Module):
             default, which is the reference's block (no RMSNorm weight) with
             an identical state_dict.  The fused path folds it into the
             projection: rmsnorm(x) * g @ W^T == rmsnorm(x) @ (W * g)^T.
+        activation_bits: 16 keeps x_streams and the layer output for the
+            backward as they are; 8 keeps their 8-bit codes instead
+            (``flash_mhc.activation8``), about half the bytes: the forward is
+            unchanged, the backward reads what the codes stand for.  Applies to
+            the fused path with its pre-map op (the default switches), where it
+            takes the place of activation_checkpointing; other paths keep
+            the tensors.
+        pre_norm: give the block a layer norm ``norm`` of the layer's input, and
+            the residual around it: the layer maps u to F, the block uses
+            u + F(norm(u)).  Off by default (the layer contains both, as in
+            the reference).  With activation_bits=8 the norm keeps 8-bit codes
+            too.
+        norm_eps: the norm's epsilon.
     """
 
     def __init__(
@@ -111,6 +125,9 @@ class MHCLiteBlock(nn.Module):
         triton_fused: bool = True,
         activation_checkpointing: bool = False,
         rmsnorm_weight: bool = False,
+        activation_bits: int = 16,
+        pre_norm: bool = False,
+        norm_eps: float = 1e-5,
     ) -> None:
         super().__init__()
         self.n = n_streams
@@ -119,6 +136,9 @@ class MHCLiteBlock(nn.Module):
         self.layer = layer
         self.triton_fused = triton_fused
         self.activation_checkpointing = activation_checkpointing
+        if activation_bits not in (8, 16):
+            raise ValueError(f"activation_bits must be 16 or 8, got {activation_bits}")
+        self.activation_bits = activation_bits
 
         self.n_fact = math.factorial(n_streams)
 
@@ -135,6 +155,12 @@ class MHCLiteBlock(nn.Module):
             self.rms_weight = nn.Parameter(torch.ones(self.nC))
         else:
             self.rms_weight = None
+        if pre_norm:
+            from .norm import LayerNorm
+
+            self.norm = LayerNorm(hidden_size, eps=norm_eps, activation_bits=activation_bits)
+        else:
+            self.norm = None
 
     # -- shared pieces ------------------------------------------------------
 
@@ -145,6 +171,12 @@ class MHCLiteBlock(nn.Module):
             and torch.is_grad_enabled()
             and x_streams.requires_grad
         )
+
+    def _apply_layer(self, layer_input: torch.Tensor, kwargs) -> torch.Tensor:
+        """The layer, with pre_norm around it: u + F(norm(u))."""
+        if self.norm is None:
+            return self.layer(layer_input, **kwargs)
+        return layer_input + self.layer(self.norm(layer_input), **kwargs)
 
     def _coefficients(
         self, proj: torch.Tensor, dt: torch.dtype
@@ -226,6 +258,10 @@ class MHCLiteBlock(nn.Module):
             # store rather than by autograd.
             args = (x_streams, self._projection_weight(x_streams.dtype), self.alpha_pre, self.alpha_post,
                     self.alpha_res, self.W_all.bias, self.perm_mat)
+            if self._keeps_codes():
+                layer_input, H_merged, h_post, _h_pre, _proj, _inv, x_sink, codes, scales = (
+                    torch.ops.flash_mhc.mhc_pre_map_pack8(*args))
+                return layer_input, H_merged, h_post, x_sink if xgrad else x_streams, codes, scales
             if use_ckpt:
                 # K1 + K2 as one op, K3 as a second one whose backward hands
                 # the layer input's gradient to the first (the fused pre-map
@@ -254,7 +290,14 @@ class MHCLiteBlock(nn.Module):
         layer_input = torch.ops.flash_mhc.fused_pre_map(x_streams, h_pre.float())
         return layer_input, H_merged.float(), h_post.float()
 
-    def _mhc_post_res_triton(self, x_streams, layer_output, H_merged, h_post, x_sink=None):
+    def _keeps_codes(self) -> bool:
+        """The fused path with its pre-map op keeps 8-bit codes for this forward's backward."""
+        return self.activation_bits == 8 and torch.is_grad_enabled()
+
+    def _mhc_post_res_triton(self, x_streams, layer_output, H_merged, h_post, x_sink=None, codes=None, scales=None):
+        if codes is not None:
+            return torch.ops.flash_mhc.mhc_post_res_pack8(x_streams, x_sink, codes, scales, layer_output, H_merged,
+                                                          h_post)[0]
         if x_sink is not None:
             return torch.ops.flash_mhc.mhc_post_res(x_streams, x_sink, layer_output, H_merged, h_post)
         return torch.ops.flash_mhc.fused_post_res(x_streams, layer_output, H_merged, h_post)
@@ -286,10 +329,16 @@ class MHCLiteBlock(nn.Module):
         device implementations instead of through the dispatcher.  Same
         kernels, same values, same x-gradient sink."""
         p = self._parameters
+        if self._keeps_codes():
+            layer_input, H_merged, h_post, x_sink, codes, scales = _a8.pre_map_eager(
+                x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
+                self.W_all.bias, self._buffers["perm_mat"])
+            layer_output = self._apply_layer(layer_input, kwargs)
+            return _a8.post_res_eager(x_streams, x_sink, codes, scales, layer_output, H_merged, h_post)
         layer_input, H_merged, h_post, x_sink = _ops.pre_map_eager(
             x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
             self.W_all.bias, self._buffers["perm_mat"])
-        layer_output = self.layer(layer_input, **kwargs)
+        layer_output = self._apply_layer(layer_input, kwargs)
         return _ops.post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post)
 
     def _forward_nograd(self, x_streams: torch.Tensor, **kwargs) -> torch.Tensor:
@@ -302,7 +351,7 @@ class MHCLiteBlock(nn.Module):
         layer_input, coeffs = _ops.pre_map_nograd(
             x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
             self.W_all.bias, self._buffers["perm_mat"])
-        layer_output = self.layer(layer_input, **kwargs)
+        layer_output = self._apply_layer(layer_input, kwargs)
         return _ops.post_res_nograd(x_streams, layer_output, coeffs)
 
     # -- common driver ------------------------------------------------------
@@ -315,7 +364,7 @@ class MHCLiteBlock(nn.Module):
             # takes (x_streams, layer_output, H_merged, h_post, *extra).
             layer_input, *coeffs = pre_map(x_streams, use_ckpt)
 
-            layer_output = self.layer(layer_input, **kwargs)
+            layer_output = self._apply_layer(layer_input, kwargs)
 
             if use_ckpt and checkpoint_post_res:
                 return _checkpoint(post_res, x_streams, layer_output, *coeffs, use_reentrant=False)

@@ -18,6 +18,13 @@ Reference counterparts (alint77/flash-mHC):
   k3_bwd     <- src/flash_mhc/kernels.py:720-853  _fused_pre_map_bwd_fused_kernel_n4
   k4_fwd     <- src/flash_mhc/kernels.py:384-481  _fused_post_res_fwd_kernel_n4
   k4_bwd     <- src/flash_mhc/kernels.py:487-665  _fused_post_res_bwd_fused_kernel_n4
+
+Without a counterpart there:
+  pack8, unpack8             activations to 8 bits and back
+  k4_fwd_pack8, k4_bwd_pack8, k1_bwd_pack8, premap_bwd_pack8
+                             K4's forward that keeps its inputs in 8 bits, and
+                             the backward passes that read them
+  layer_norm_fwd, layer_norm_bwd
 """
 
 from __future__ import annotations
@@ -521,3 +528,256 @@ def k4_bwd(grad_out: torch.Tensor, x_streams: torch.Tensor, layer_output: torch.
                              T, C, n, _abi.stream_of(x_streams))
     _abi.check(st, "k4_bwd")
     return grad_x, grad_layer_output, grad_H, grad_h_post
+
+
+# ---------------------------------------------------------------------------
+# Activations in 8 bits (the format: include/flash_mhc_hip.h)
+
+PACK_GROUP = 32  # columns that share a scale
+DTYPES = {_F32: 0, _BF16: 1, torch.float16: 2}  # FMHC_DTYPE_*
+
+
+def pack_groups(C: int) -> int:
+    """Scales of a row of C columns."""
+    return (C + PACK_GROUP - 1) // PACK_GROUP
+
+
+def _dtype_code(dt: torch.dtype, name: str) -> int:
+    code = DTYPES.get(dt)
+    if code is None:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {dt}")
+    return code
+
+
+def _rows(shape) -> tuple[int, int]:
+    """(rows, C) of a tensor's shape (..., C)."""
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"expected shape (..., C) with C >= 1, got {tuple(shape)}")
+    rows = 1
+    for d in shape[:-1]:
+        rows *= d
+    return rows, shape[-1]
+
+
+def empty_packed(shape, dev) -> tuple[torch.Tensor, torch.Tensor]:
+    """Unwritten (codes, scales) for a tensor of this shape."""
+    codes = torch.empty(shape, device=dev, dtype=torch.int8)
+    scales = torch.empty((*shape[:-1], pack_groups(shape[-1])), device=dev, dtype=torch.uint8)
+    return codes, scales
+
+
+def _require_packed(codes, scales, name: str, shape, dev) -> None:
+    shape = tuple(shape)
+    _require(codes, f"{name}_codes", torch.int8, shape, dev)
+    _require(scales, f"{name}_scales", torch.uint8, (*shape[:-1], pack_groups(shape[-1])), dev)
+
+
+def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """codes (..., C) int8 and scales (..., ceil(C / 32)) uint8 of x (..., C)."""
+    dev = _device_of(x)
+    code = _dtype_code(x.dtype, "x")
+    rows, C = _rows(x.shape)
+    _require(x, "x", x.dtype, x.shape, dev)
+    codes, scales = empty_packed(x.shape, dev)
+    lib = _abi.load()
+    with _OnDevice(dev):
+        st = lib.fmhc_pack8(x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), rows, C, _abi.stream_of(x))
+    _abi.check(st, "pack8")
+    return codes, scales
+
+
+def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = _BF16) -> torch.Tensor:
+    """The values of pack8's codes and scales, in dtype."""
+    dev = _device_of(codes)
+    code = _dtype_code(dtype, "dtype")
+    rows, C = _rows(codes.shape)
+    _require_packed(codes, scales, "x", codes.shape, dev)
+    x = torch.empty(codes.shape, device=dev, dtype=dtype)
+    lib = _abi.load()
+    with _OnDevice(dev):
+        st = lib.fmhc_unpack8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), code, rows, C, _abi.stream_of(codes))
+    _abi.check(st, "unpack8")
+    return x
+
+
+def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: torch.Tensor, h_post: torch.Tensor):
+    """k4_fwd's out with x_streams and layer_output packed in the same pass:
+    (out, x_codes, x_scales, lo_codes, lo_scales)."""
+    dev = _device_of(x_streams)
+    T, n, C = _streams_shape(x_streams)
+    _require(x_streams, "x_streams", _BF16, (T, n, C), dev)
+    _require(layer_output, "layer_output", _BF16, (T, C), dev)
+    _require(H_merged, "H_merged", _F32, (T, n, n), dev)
+    _require(h_post, "h_post", _F32, (T, n), dev)
+    out = torch.empty_like(x_streams)
+    xq, xs = empty_packed((T, n, C), dev)
+    lq, ls = empty_packed((T, C), dev)
+    lib = _abi.load()
+    with _OnDevice(dev):
+        st = lib.fmhc_k4_fwd_pack8(x_streams.data_ptr(), layer_output.data_ptr(), H_merged.data_ptr(),
+                                   h_post.data_ptr(), out.data_ptr(), xq.data_ptr(), xs.data_ptr(), lq.data_ptr(),
+                                   ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))
+    _abi.check(st, "k4_fwd_pack8")
+    return out, xq, xs, lq, ls
+
+
+def k4_bwd_pack8(grad_out: torch.Tensor, x_codes: torch.Tensor, x_scales: torch.Tensor, lo_codes: torch.Tensor,
+                 lo_scales: torch.Tensor, H_merged: torch.Tensor, h_post: torch.Tensor):
+    """k4_bwd's outputs from packed x_streams and layer_output."""
+    dev = _device_of(x_codes)
+    T, n, C = _streams_shape(x_codes)
+    _require_packed(x_codes, x_scales, "x", (T, n, C), dev)
+    _require_packed(lo_codes, lo_scales, "lo", (T, C), dev)
+    _require(H_merged, "H_merged", _F32, (T, n, n), dev)
+    _require(h_post, "h_post", _F32, (T, n), dev)
+    _require(grad_out, "grad_out", _BF16, (T, n, C), dev)
+    grad_x = torch.empty_like(grad_out)
+    grad_lo = torch.empty((T, C), device=dev, dtype=_BF16)
+    grad_H = torch.empty((T, n, n), device=dev, dtype=_F32)
+    grad_h_post = torch.empty((T, n), device=dev, dtype=_F32)
+    lib = _abi.load()
+    with _OnDevice(dev):
+        st = lib.fmhc_k4_bwd_pack8(x_codes.data_ptr(), x_scales.data_ptr(), lo_codes.data_ptr(), lo_scales.data_ptr(),
+                                   H_merged.data_ptr(), h_post.data_ptr(), grad_out.data_ptr(), grad_x.data_ptr(),
+                                   grad_lo.data_ptr(), grad_H.data_ptr(), grad_h_post.data_ptr(), T, C, n,
+                                   _abi.stream_of(x_codes))
+    _abi.check(st, "k4_bwd_pack8")
+    return grad_x, grad_lo, grad_H, grad_h_post
+
+
+def k1_bwd_pack8(grad_out: torch.Tensor, x_codes: torch.Tensor, x_scales: torch.Tensor, W: torch.Tensor,
+                 proj_out: torch.Tensor, inv_rms: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(grad_x (T, 4, C), grad_W (32, 4 C)) of K1 from packed streams."""
+    dev = _device_of(x_codes)
+    T, n, C = _streams_shape(x_codes)
+    _require_packed(x_codes, x_scales, "x", (T, n, C), dev)
+    _require(W, "W", _BF16, (D_OUT, n * C), dev)
+    _require(grad_out, "grad_out", _BF16, (T, D_OUT), dev)
+    _require(proj_out, "proj_out", _BF16, (T, D_OUT), dev)
+    _require(inv_rms, "inv_rms", _F32, (T,), dev)
+    grad_x = torch.empty((T, n, C), device=dev, dtype=_BF16)
+    grad_W = torch.empty((D_OUT, n * C), device=dev, dtype=_BF16)
+    lib = _abi.load()
+    ws = _workspace(int(lib.fmhc_k1_bwd_pack8_workspace_bytes(T, C)), dev)
+    with _OnDevice(dev):
+        st = lib.fmhc_k1_bwd_pack8(x_codes.data_ptr(), x_scales.data_ptr(), W.data_ptr(), grad_out.data_ptr(),
+                                   proj_out.data_ptr(), inv_rms.data_ptr(), grad_x.data_ptr(), grad_W.data_ptr(),
+                                   _ptr_or_none(ws), 0 if ws is None else ws.numel(), T, C, n,
+                                   _abi.stream_of(x_codes))
+    _abi.check(st, "k1_bwd_pack8")
+    return grad_x, grad_W
+
+
+def premap_bwd_pack8(x_codes: torch.Tensor, x_scales: torch.Tensor, W: torch.Tensor, alpha_pre: torch.Tensor,
+                     alpha_post: torch.Tensor, alpha_res: torch.Tensor, bias: torch.Tensor, perm: torch.Tensor,
+                     h_pre: torch.Tensor, proj: torch.Tensor, inv_rms: torch.Tensor, grad_layer_input: torch.Tensor,
+                     grad_h_post: torch.Tensor | None, grad_H: torch.Tensor | None,
+                     grad_x_in: torch.Tensor | None = None):
+    """premap_bwd's outputs from packed streams."""
+    dev = _device_of(x_codes)
+    T, n, C = _streams_shape(x_codes)
+    _require_packed(x_codes, x_scales, "x", (T, n, C), dev)
+    _require(W, "W", _BF16, (D_OUT, n * C), dev)
+    pdt = _k2_params(alpha_pre, alpha_post, alpha_res, bias, perm, dev)
+    _require(h_pre, "h_pre", _F32, (T, n), dev)
+    _require(proj, "proj", _BF16, (T, D_OUT), dev)
+    _require(inv_rms, "inv_rms", _F32, (T,), dev)
+    _require(grad_layer_input, "grad_layer_input", _BF16, (T, C), dev)
+    if grad_h_post is not None:
+        _require(grad_h_post, "grad_h_post", _F32, (T, n), dev)
+    if grad_H is not None:
+        _require(grad_H, "grad_H_merged", _F32, (T, n, n), dev)
+    if grad_x_in is not None:
+        _require(grad_x_in, "grad_x_in", _BF16, (T, n, C), dev)
+    gx = torch.empty((T, n, C), device=dev, dtype=_BF16)
+    gW = torch.empty((D_OUT, n * C), device=dev, dtype=_BF16)
+    ga = [torch.empty((1,), device=dev, dtype=alpha_pre.dtype) for _ in range(3)]
+    gb = torch.empty((D_OUT,), device=dev, dtype=alpha_pre.dtype)
+    lib = _abi.load()
+    ws = torch.empty((max(int(lib.fmhc_premap_bwd_workspace_bytes(T, C)), 16),), device=dev, dtype=torch.uint8)
+    with _OnDevice(dev):
+        st = lib.fmhc_premap_bwd_pack8(
+            x_codes.data_ptr(), x_scales.data_ptr(), W.data_ptr(), alpha_pre.data_ptr(), alpha_post.data_ptr(),
+            alpha_res.data_ptr(), bias.data_ptr(), perm.data_ptr(), pdt, h_pre.data_ptr(), proj.data_ptr(),
+            inv_rms.data_ptr(), grad_layer_input.data_ptr(), _ptr_or_none(grad_h_post), _ptr_or_none(grad_H),
+            _ptr_or_none(grad_x_in), gx.data_ptr(), gW.data_ptr(), ga[0].data_ptr(), ga[1].data_ptr(),
+            ga[2].data_ptr(), gb.data_ptr(), ws.data_ptr(), ws.numel(), T, C, n, _abi.stream_of(x_codes))
+    _abi.check(st, "premap_bwd_pack8")
+    return gx, gW, ga[0], ga[1], ga[2], gb
+
+
+# ---------------------------------------------------------------------------
+# Layer norm
+
+
+def _norm_params(weight, bias, dtype: torch.dtype, C: int, dev) -> torch.dtype:
+    """Check the norm's weight and bias (either may be None) and return their dtype."""
+    have = [t for t in (weight, bias) if t is not None]
+    if not have:
+        return _F32
+    pdt = have[0].dtype
+    if pdt is not _F32 and pdt is not dtype:
+        raise TypeError(f"weight and bias must be float32 or x's dtype {dtype}, got {pdt}")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _require(t, name, pdt, (C,), dev)
+    return pdt
+
+
+def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                   stats: bool = True, packed: bool = False):
+    """(y, mean, rstd, codes, scales) of x (..., C): y in x's dtype, mean and rstd
+    (...,) fp32 (None without stats), codes and scales pack8's of x (None unless
+    packed)."""
+    dev = _device_of(x)
+    code = _dtype_code(x.dtype, "x")
+    T, C = _rows(x.shape)
+    _require(x, "x", x.dtype, x.shape, dev)
+    pdt = _norm_params(weight, bias, x.dtype, C, dev)
+    y = torch.empty_like(x)
+    mean = torch.empty(x.shape[:-1], device=dev, dtype=_F32) if stats else None
+    rstd = torch.empty(x.shape[:-1], device=dev, dtype=_F32) if stats else None
+    q, s = empty_packed(x.shape, dev) if packed else (None, None)
+    lib = _abi.load()
+    with _OnDevice(dev):
+        st = lib.fmhc_layer_norm_fwd(x.data_ptr(), _ptr_or_none(weight), _ptr_or_none(bias), y.data_ptr(),
+                                     _ptr_or_none(mean), _ptr_or_none(rstd), _ptr_or_none(q), _ptr_or_none(s), code,
+                                     DTYPES[pdt], T, C, eps, _abi.stream_of(x))
+    _abi.check(st, "layer_norm_fwd")
+    return y, mean, rstd, q, s
+
+
+def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Tensor | None,
+                   scales: torch.Tensor | None, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None,
+                   param_dtype: torch.dtype, need_weight: bool = True, need_bias: bool = True):
+    """(grad_x, grad_weight, grad_bias) of layer_norm_fwd, from x or from its codes
+    and scales; a parameter's gradient is in param_dtype, None where not needed."""
+    dev = _device_of(grad_y)
+    code = _dtype_code(grad_y.dtype, "grad_y")
+    T, C = _rows(grad_y.shape)
+    _require(grad_y, "grad_y", grad_y.dtype, grad_y.shape, dev)
+    if (x is None) == (codes is None):
+        raise ValueError("layer_norm_bwd takes x, or its codes and scales")
+    if x is not None:
+        _require(x, "x", grad_y.dtype, grad_y.shape, dev)
+    else:
+        _require_packed(codes, scales, "x", grad_y.shape, dev)
+    _require(mean, "mean", _F32, grad_y.shape[:-1], dev)
+    _require(rstd, "rstd", _F32, grad_y.shape[:-1], dev)
+    if param_dtype is not _F32 and param_dtype is not grad_y.dtype:
+        raise TypeError(f"param_dtype must be float32 or grad_y's dtype {grad_y.dtype}, got {param_dtype}")
+    if weight is not None:
+        _require(weight, "weight", param_dtype, (C,), dev)
+    gx = torch.empty_like(grad_y)
+    gw = torch.empty((C,), device=dev, dtype=param_dtype) if need_weight else None
+    gb = torch.empty((C,), device=dev, dtype=param_dtype) if need_bias else None
+    lib = _abi.load()
+    ws = _workspace(int(lib.fmhc_layer_norm_bwd_workspace_bytes(T, C)), dev) if need_weight or need_bias else None
+    with _OnDevice(dev):
+        st = lib.fmhc_layer_norm_bwd(grad_y.data_ptr(), _ptr_or_none(x), _ptr_or_none(codes), _ptr_or_none(scales),
+                                     mean.data_ptr(), rstd.data_ptr(), _ptr_or_none(weight), gx.data_ptr(),
+                                     _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws),
+                                     0 if ws is None else ws.numel(), code, DTYPES[param_dtype], T, C,
+                                     _abi.stream_of(grad_y))
+    _abi.check(st, "layer_norm_bwd")
+    return gx, gw, gb

@@ -39,12 +39,18 @@ extern "C" {
 #define FMHC_ERR_SCRATCH_LIMIT 2    /* fmhc_premap_fwd_noalloc: shape needs more than its scratch */
 #define FMHC_ERR_HIP_BASE 1000      /* + hipError_t from the launch */
 
-#define FMHC_ABI_VERSION 7
+#define FMHC_ABI_VERSION 8
 
 /* Storage dtype of the block parameters K2 reads (alpha_pre, alpha_post,
  * alpha_res, bias, perm: all five the same) and of their gradients. */
 #define FMHC_PARAM_F32 0
 #define FMHC_PARAM_BF16 1
+
+/* Storage dtype of the tensors that fmhc_pack8 / fmhc_unpack8 and the layer
+ * norm take. */
+#define FMHC_DTYPE_F32 0
+#define FMHC_DTYPE_BF16 1
+#define FMHC_DTYPE_F16 2
 
 /* K1 forward: fused RMSNorm + projection.
  *   inv_rms[t] = rsqrt(sum_k x[t,k]^2 / nC + 1e-6)
@@ -238,6 +244,87 @@ int fmhc_k4_bwd(const uint16_t* x, const uint16_t* lo, const float* H, const flo
                 const uint16_t* grad_out, uint16_t* grad_x, uint16_t* grad_lo,
                 float* grad_H, float* grad_h_post,
                 int64_t T, int64_t C, int64_t n, void* stream);
+
+/* ---- Activations kept in 8 bits ------------------------------------------
+ * No counterpart in the reference, which keeps bf16 activations or recomputes.
+ *
+ * A row of C columns is cut into G = ceil(C / 32) groups of 32 columns (the
+ * last one shorter).  A group has one scale byte and every element one signed
+ * code, with a = max |x| over the group:
+ *   E    = clamp(exponent field of fp32(a), 7, 254), or 255 where a is Inf or NaN
+ *   code = clamp(round_half_even(x / 2^(E - 133)), -127, 127), or 0 where E = 255
+ * which stand for code * 2^(E - 133), exactly a bf16 value (E = 255: NaN).
+ * Codes are (rows, C) int8, scales (rows, G) uint8, contiguous, at any
+ * alignment. */
+
+/* codes and scales of x (rows, C) in `dtype` (FMHC_DTYPE_*), and back (values
+ * rounded to nearest even where `dtype` cannot hold them: fp16's range). */
+int fmhc_pack8(const void* x, int dtype, int8_t* codes, uint8_t* scales, int64_t rows, int64_t C,
+               void* stream);
+int fmhc_unpack8(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int64_t rows,
+                 int64_t C, void* stream);
+
+/* fmhc_k4_fwd that also packs x (codes (T, n, C), scales (T, n, G)) and lo
+ * (codes (T, C), scales (T, G)) in the same pass.  out has fmhc_k4_fwd's bits,
+ * the codes fmhc_pack8's. */
+int fmhc_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* h_post,
+                      uint16_t* out, int8_t* x_codes, uint8_t* x_scales, int8_t* lo_codes,
+                      uint8_t* lo_scales, int64_t T, int64_t C, int64_t n, void* stream);
+/* fmhc_k4_bwd from packed x and lo: the bits that fmhc_k4_bwd gives for the
+ * unpacked tensors. */
+int fmhc_k4_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const int8_t* lo_codes,
+                      const uint8_t* lo_scales, const float* H, const float* h_post,
+                      const uint16_t* grad_out, uint16_t* grad_x, uint16_t* grad_lo, float* grad_H,
+                      float* grad_h_post, int64_t T, int64_t C, int64_t n, void* stream);
+
+/* fmhc_k1_bwd from packed streams: x_codes (T, n, C), x_scales (T, n, G), W
+ * (32, n C), grad_x (T, n, C), grad_W (32, n C); values as fmhc_k1_bwd gives
+ * them for the unpacked x up to the order of fp32 sums (the same bits where
+ * C % 8 == 0).  `workspace`: at least fmhc_k1_bwd_pack8_workspace_bytes(T, C)
+ * bytes, 16-byte aligned (may be NULL where that is 0). */
+int fmhc_k1_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const uint16_t* W,
+                      const uint16_t* grad_out, const uint16_t* proj_out, const float* inv_rms,
+                      uint16_t* grad_x, uint16_t* grad_W, void* workspace, int64_t workspace_bytes,
+                      int64_t T, int64_t C, int64_t n, void* stream);
+int64_t fmhc_k1_bwd_pack8_workspace_bytes(int64_t T, int64_t C);
+
+/* fmhc_premap_bwd from packed streams: the bits that fmhc_premap_bwd gives for
+ * the unpacked x.  `workspace`: fmhc_premap_bwd_workspace_bytes(T, C). */
+int fmhc_premap_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const uint16_t* W,
+                          const void* alpha_pre, const void* alpha_post, const void* alpha_res,
+                          const void* bias, const void* perm, int param_dtype, const float* h_pre,
+                          const uint16_t* proj, const float* inv_rms,
+                          const uint16_t* grad_layer_input, const float* grad_h_post,
+                          const float* grad_H_merged, const uint16_t* grad_x_in, uint16_t* grad_x,
+                          uint16_t* grad_W, void* grad_alpha_pre, void* grad_alpha_post,
+                          void* grad_alpha_res, void* grad_bias, void* workspace,
+                          int64_t workspace_bytes, int64_t T, int64_t C, int64_t n, void* stream);
+
+/* ---- Layer norm ------------------------------------------------------------
+ * No counterpart in the reference.  x, y (T, C) in `dtype`; weight and bias (C,)
+ * in `param_dtype`, which is FMHC_DTYPE_F32 or `dtype`, either of them NULL (1
+ * and 0); statistics and sums in fp32, every output rounded once.
+ *   mean[t] = sum_c x[t,c] / C
+ *   rstd[t] = rsqrt(sum_c (x[t,c] - mean[t])^2 / C + eps)
+ *   y[t,c]  = (x[t,c] - mean[t]) rstd[t] weight[c] + bias[c]
+ * mean and rstd (T,) may be NULL.  With x_codes and x_scales (both or neither)
+ * x is also packed, as fmhc_pack8 does, in the same pass. */
+int fmhc_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* mean,
+                        float* rstd, int8_t* x_codes, uint8_t* x_scales, int dtype, int param_dtype,
+                        int64_t T, int64_t C, float eps, void* stream);
+/* Backward, from x or (x NULL) from its codes and scales, with
+ * h = (x - mean) rstd, g = grad_y weight:
+ *   grad_x[t,c]    = rstd[t] (g[t,c] - sum_c g / C - h[t,c] sum_c g h / C)
+ *   grad_weight[c] = sum_t grad_y[t,c] h[t,c],  grad_bias[c] = sum_t grad_y[t,c]
+ * grad_weight and grad_bias, in param_dtype, may be NULL; with either,
+ * `workspace` has at least fmhc_layer_norm_bwd_workspace_bytes(T, C) bytes,
+ * 16-byte aligned.  Sums are added in a fixed order. */
+int fmhc_layer_norm_bwd(const void* grad_y, const void* x, const int8_t* x_codes,
+                        const uint8_t* x_scales, const float* mean, const float* rstd,
+                        const void* weight, void* grad_x, void* grad_weight, void* grad_bias,
+                        void* workspace, int64_t workspace_bytes, int dtype, int param_dtype,
+                        int64_t T, int64_t C, void* stream);
+int64_t fmhc_layer_norm_bwd_workspace_bytes(int64_t T, int64_t C);
 
 /* Human-readable text for a status code.  Never returns NULL.
  * No counterpart in the reference (Triton raises Python exceptions). */

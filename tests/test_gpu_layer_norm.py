@@ -1,0 +1,275 @@
+"""GPU tests of layer norm, forward and backward, with its input kept as it is and in 8 bits.
+
+Values are compared with 64-bit ones; how far they may be off is derived in
+oracle/act8_oracle.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import flash_mhc
+from oracle import act8_oracle as A
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+DEV = "cuda"
+EPS = 1e-5
+
+
+def rnd(shape, seed, scale=1.0, mean=0.0, dtype=BF16):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale + mean).to(dtype)
+
+
+def inputs(T, C, dtype, pdt, seed=0):
+    x = rnd((T, C), seed, 1.0, 0.25, dtype)
+    x[::5] *= 50
+    w, b = rnd((C,), seed + 1, 0.2, 1.0, pdt), rnd((C,), seed + 2, 0.2, 0.0, pdt)
+    return x.to(DEV), w.to(DEV), b.to(DEV), rnd((T, C), seed + 3, dtype=dtype).to(DEV)
+
+
+def run(x, w, b, g, bits, eps=EPS):
+    leaves = [None if t is None else t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+    y = flash_mhc.layer_norm(leaves[0], leaves[1], leaves[2], eps, activation_bits=bits)
+    have = [t for t in leaves if t is not None]
+    gr = iter(torch.autograd.grad(y, have, g))
+    return y.detach(), *[None if t is None else next(gr) for t in leaves]
+
+
+def verify(x, w, b, g, bits, eps=EPS):
+    y, gx, gw, gb = run(x, w, b, g, bits, eps)
+    A.check("y", y, *A.ln_fwd(x, w, b, eps))
+    kept = A.unpack8(*A.pack8(x)) if bits == 8 else x
+    r = A.ln_bwd(g, x, kept, w, eps)
+    A.check("grad_x", gx.reshape(-1, x.shape[-1]), *r["x"])
+    assert gx.dtype is x.dtype and y.dtype is x.dtype
+    if w is not None:
+        A.check("grad_w", gw, *r["w"])
+        assert gw.dtype is w.dtype
+    if b is not None:
+        A.check("grad_b", gb, *r["b"])
+
+
+TYPES = [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32), (F32, F32)]
+# One lane group to rows past the registers; whole, ragged and single columns.
+SIZES = [(1, 1), (1, 7), (3, 8), (2, 33), (5, 64), (40, 65), (33, 100), (70, 128), (31, 256), (17, 300), (9, 512),
+         (20, 777), (6, 1000), (5, 1024), (9, 1535), (7, 2048), (3, 2560), (5, 4096), (2, 4099), (2, 6000), (2, 8192),
+         (3, 12000), (2, 16384), (3, 16385), (2, 20000)]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T,C", SIZES)
+def test_sizes(T, C, bits):
+    verify(*inputs(T, C, BF16, BF16), bits)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("dtype,pdt", TYPES)
+@pytest.mark.parametrize("T,C", [(1, 40), (37, 100), (600, 264), (130, 1024), (65, 1001), (3, 4096), (2, 17000)])
+def test_types(T, C, dtype, pdt, bits):
+    verify(*inputs(T, C, dtype, pdt), bits)
+
+
+@pytest.mark.parametrize("T,C", [(5000, 32), (4097, 520), (3000, 2000)])
+def test_many_rows(T, C):
+    for bits in (16, 8):
+        verify(*inputs(T, C, BF16, F32), bits)
+
+
+@pytest.mark.parametrize("C", [24, 520, 20000])
+def test_without_parameters(C):
+    x, w, b, g = inputs(7, C, BF16, BF16)
+    for bits in (16, 8):
+        verify(x, None, None, g, bits)
+        verify(x, w, None, g, bits)
+        verify(x, None, b, g, bits)
+
+
+def test_far_mean():
+    """A mean far from the spread: the variance is around the mean.  bf16 values
+    near 256 are multiples of 2, exact in fp32, so the tolerance is the usual one."""
+    x = (rnd((9, 512), 1, 8.0, 256.0)).to(DEV)
+    _x, w, b, g = inputs(9, 512, BF16, BF16)
+    verify(x, w, b, g, 16)
+    xf = rnd((9, 512), 1, 1.0, 100.0, F32).to(DEV)
+    verify(xf, w.float(), b.float(), g.float(), 16)
+
+
+def test_constant_and_zero_rows():
+    x, w, b, g = inputs(4, 96, F32, F32)
+    x[0], x[1] = 0.0, 4.0  # sums and means of 4.0 are exact
+    y, gx, gw, gb = run(x, w, b, g, 16)
+    assert torch.equal(y[:2], b.expand(2, -1))
+    verify(x, w, b, g, 16)
+
+
+def test_inf_and_nan_stay_in_their_row():
+    x, w, b, g = inputs(6, 300, BF16, BF16)
+    clean = run(x, w, b, g, 8)
+    x[2, 17], x[4, 299] = float("inf"), float("nan")
+    for bits in (16, 8):
+        y, gx, _gw, _gb = run(x, w, b, g, bits)
+        ok = [0, 1, 3, 5]
+        assert torch.equal(y[ok], clean[0][ok]) and torch.isnan(y[[2, 4]]).any(1).all()
+        assert torch.isfinite(gx[ok]).all()
+        if bits == 8:
+            assert torch.equal(gx[ok], clean[1][ok])
+
+
+def test_zero_gradient_rows():
+    """Padded rows with no gradient: they get none and give none."""
+    x, w, b, g = inputs(50, 200, BF16, F32)
+    g[30:] = 0
+    _y, gx, gw, gb = run(x, w, b, g, 16)
+    assert float(gx[30:].float().abs().sum()) == 0
+    r = A.ln_bwd(g[:30], x[:30], x[:30], w, EPS)
+    A.check("grad_w", gw, *r["w"])
+    A.check("grad_b", gb, *r["b"])
+
+
+def test_against_differences():
+    """grad_x, grad_w, grad_b against central differences of the 64-bit forward.
+    f = sum(y g) is smooth; step s gives an error of order s^2, with s = 1e-4
+    1e-8 of the values, far below fp32's; 2e-3 of the gradient's norm bounds
+    what the fp32 gradients may be off by a wide margin."""
+    x, w, b, g = inputs(3, 24, F32, F32)
+    x[::5] /= 50
+    _y, gx, gw, gb = run(x, w, b, g, 16)
+    X, W, B, Gr = (t.double().cpu() for t in (x, w, b, g))
+    f = lambda X, W, B: float((A.ln_fwd(X, W, B, EPS)[0] * Gr).sum())
+    for name, t, grad in (("x", X, gx), ("w", W, gw), ("b", B, gb)):
+        num = torch.zeros_like(t)
+        for i in range(t.numel()):
+            e = torch.zeros_like(t).view(-1)
+            e[i] = 1e-4
+            e = e.view_as(t)
+            hi = f(*[u + e if u is t else u for u in (X, W, B)])
+            lo = f(*[u - e if u is t else u for u in (X, W, B)])
+            num.view(-1)[i] = (hi - lo) / 2e-4
+        assert float((num - grad.double().cpu()).norm()) <= 2e-3 * float(num.norm()), name
+
+
+def test_eval_and_ops_agree():
+    for T, C in ((1, 4096), (9, 100)):
+        x, w, b, g = inputs(T, C, BF16, BF16)
+        y = run(x, w, b, g, 16)[0]
+        with torch.no_grad():
+            assert torch.equal(flash_mhc.layer_norm(x, w, b, EPS), y)
+            assert torch.equal(flash_mhc.layer_norm(x, w, b, EPS, activation_bits=8), y)
+        for op in (torch.ops.flash_mhc.layer_norm, torch.ops.flash_mhc.layer_norm_pack8):
+            leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+            out = op(*leaves, EPS)
+            assert torch.equal(out[0], y)
+            if len(out) == 5:
+                assert all(torch.equal(a.cpu(), r) for a, r in zip(out[3:], A.pack8(x)))
+            bits = 16 if len(out) == 3 else 8
+            for a, r in zip(torch.autograd.grad(out[0], leaves, g), run(x, w, b, g, bits)[1:]):
+                assert torch.equal(a, r)
+
+
+def test_some_gradients_only():
+    x, w, b, g = inputs(9, 72, BF16, BF16)
+    want = run(x, w, b, g, 16)
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1)):
+        leaves = [t.clone().requires_grad_(bool(n)) for t, n in zip((x, w, b), need)]
+        y = flash_mhc.layer_norm(*leaves, EPS)
+        y.backward(g)
+        for t, n, r in zip(leaves, need, want[1:]):
+            assert (t.grad is not None) == bool(n)
+            if n:
+                assert torch.equal(t.grad, r)
+
+
+def test_strided_unaligned_and_leading_dims():
+    x, w, b, g = inputs(24, 104, BF16, BF16)
+    want = run(x, w, b, g, 8)
+    wide = torch.empty(24, 208, device=DEV, dtype=BF16)
+    wide[:, ::2] = x
+    xt = wide[:, ::2].requires_grad_(True)
+    gt = torch.empty(104, 24, device=DEV, dtype=BF16).copy_(g.t()).t()
+    y = flash_mhc.layer_norm(xt, w, b, EPS, activation_bits=8)
+    assert torch.equal(y, want[0])
+    assert torch.equal(torch.autograd.grad(y, xt, gt)[0], want[1])
+    off = torch.empty(1 + x.numel(), device=DEV, dtype=BF16)[1:].view_as(x).copy_(x)  # 2 bytes off
+    for a, r in zip(run(off, w, b, g, 8), want):
+        assert a.shape == r.shape
+        assert float((a.double() - r.double()).norm()) <= 2.0 ** -8 * float(r.double().norm())
+    for a, r in zip(run(x.view(2, 3, 4, 104), w, b, g.view(2, 3, 4, 104), 8), want):
+        assert torch.equal(a.reshape(r.shape), r)
+    # A gradient broadcast from one value.
+    xs = x.clone().requires_grad_(True)
+    flash_mhc.layer_norm(xs, w, b, EPS).sum().backward()
+    assert torch.equal(xs.grad, run(x, w, b, torch.ones_like(g), 16)[1])
+
+
+def test_empty():
+    x = torch.empty(0, 40, device=DEV, dtype=BF16).requires_grad_(True)
+    w = torch.ones(40, device=DEV).requires_grad_(True)
+    b = torch.ones(40, device=DEV).requires_grad_(True)
+    y = flash_mhc.layer_norm(x, w, b, EPS, activation_bits=8)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], torch.empty_like(y))
+    assert gx.shape == (0, 40) and float(gw.abs().sum()) == 0 and float(gb.abs().sum()) == 0
+
+
+def test_deterministic_on_two_streams():
+    x, w, b, g = inputs(3000, 520, BF16, BF16)
+    want = run(x, w, b, g, 8)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(run(x, w, b, g, 8))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for r in got:
+        assert all(torch.equal(a, c) for a, c in zip(r, want))
+
+
+def test_captured():
+    x, w, b, g = inputs(700, 1024, BF16, BF16)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = flash_mhc.layer_norm(*leaves, EPS, activation_bits=8)
+        return (y.detach(), *torch.autograd.grad(y, leaves, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):  # two graphs, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(inputs(700, 1024, BF16, BF16, seed=20 + k)[0])
+        for graph in graphs:
+            graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+def test_module():
+    m = flash_mhc.LayerNorm(96, activation_bits=8).to(DEV)
+    ref = torch.nn.LayerNorm(96).to(DEV)
+    assert list(m.state_dict()) == list(ref.state_dict())
+    m.load_state_dict(ref.state_dict())
+    x = rnd((5, 96), 1, dtype=F32).to(DEV)
+    A.check("y", m(x), *A.ln_fwd(x, m.weight, m.bias, m.eps))
+    y = m.double()(x.double())  # a dtype that the kernels do not take
+    assert y.dtype is torch.float64
+    comp = torch.compile(flash_mhc.LayerNorm(96).to(DEV), fullgraph=True, backend="aot_eager")
+    xs = x.clone().requires_grad_(True)
+    comp(xs).square().sum().backward()
+    xe = x.clone().requires_grad_(True)
+    flash_mhc.LayerNorm(96).to(DEV)(xe).square().sum().backward()
+    assert torch.equal(xs.grad, xe.grad)
