@@ -1,0 +1,697 @@
+// The layer norm's kernels, for the translation unit of one storage type.
+//
+// A row is held by LPT lanes, R groups of 8 columns each, from its loads to its
+// stores; a lane keeps the same columns for every row of its workgroup, so the
+// weight and bias and (backward) the sums of grad_w and grad_b stay in registers.
+// The next row's loads are issued before the current row is computed.  The
+// lane at a row's end with fewer than 8 columns left takes the row's last 8
+// instead: every load is one vector inside the row, sums leave out the columns
+// that the lane before holds too, and stores write those once more with the
+// same values.
+#pragma once
+
+#include "layer_norm.h"
+
+namespace fmhc {
+
+namespace {
+
+// 8 elements as loaded.
+template <int DT>
+struct LnRaw {
+  u32x4 a;
+};
+template <>
+struct LnRaw<FMHC_DTYPE_F32> {
+  u32x4 a, b;
+};
+
+template <int DT, bool NT>
+__device__ __forceinline__ LnRaw<DT> ln_load(const typename Elems<DT>::S* p) {
+  LnRaw<DT> r;
+  r.a = NT ? ld16_stream(p) : ld16(p);
+  if constexpr (DT == FMHC_DTYPE_F32) r.b = NT ? ld16_stream(p + 4) : ld16(p + 4);
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void ln_unpack(const LnRaw<DT>& r, float (&f)[8]) {
+  if constexpr (DT == FMHC_DTYPE_BF16) {
+    unpack8(r.a, f);
+  } else if constexpr (DT == FMHC_DTYPE_F16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = Elems<DT>::widen(r.a[i] & 0xffffu);
+      f[2 * i + 1] = Elems<DT>::widen(r.a[i] >> 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = __uint_as_float(r.a[i]);
+      f[4 + i] = __uint_as_float(r.b[i]);
+    }
+  }
+}
+
+// A value that the compiler takes as new.
+template <int DT>
+__device__ __forceinline__ void ln_opaque(LnRaw<DT>& r) {
+  asm volatile("" : "+v"(r.a.x), "+v"(r.a.y), "+v"(r.a.z), "+v"(r.a.w));
+  if constexpr (DT == FMHC_DTYPE_F32) asm volatile("" : "+v"(r.b.x), "+v"(r.b.y), "+v"(r.b.z), "+v"(r.b.w));
+}
+
+// x in the backward: as it is, or codes with their group's scale.
+template <int DT, bool KEPT>
+struct LnX {
+  using Elem = typename Elems<DT>::S;
+  LnRaw<DT> r;
+};
+template <int DT>
+struct LnX<DT, true> {
+  using Elem = int8_t;
+  u32x2 q;
+  uint32_t e0, e1;  // the first and the last column's (a lane's last group only)
+};
+
+// The values of 8 codes from column c on, those of round k < R - 1 in one group.
+template <int R>
+__device__ __forceinline__ void ln_decode(u32x2 q, uint32_t e0, uint32_t e1, int k, int c, float (&f)[8]) {
+  const float u0 = pack_unit(e0);
+  if (k < R - 1) return decode8(q, u0, f);
+  const float u1 = pack_unit(e1);
+  const int n0 = kPackGroup - (c & (kPackGroup - 1));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = code_at(q.x, i) * (i < n0 ? u0 : u1);
+    f[4 + i] = code_at(q.y, i) * (4 + i < n0 ? u0 : u1);
+  }
+}
+
+// Where lane group g of a row of C >= 8 columns is: 8 columns from `c` on, of
+// which the first `skip` belong to the group before (8: the group is past the
+// row's end).
+struct LnPlace {
+  int c, skip;
+};
+__device__ __forceinline__ LnPlace ln_place(int g, int C) {
+  const int c0 = 8 * g, c = c0 < C - 8 ? c0 : C - 8;
+  return LnPlace{c, c0 - c < 8 ? c0 - c : 8};
+}
+
+template <int DT>
+__device__ __forceinline__ void ln_param8(const void* p, bool f32, int c, float none, float (&f)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = none;
+  } else if (f32) {
+    Elems<FMHC_DTYPE_F32>::load8<false>(static_cast<const float*>(p) + c, f);
+  } else {
+    Elems<DT>::template load8<false>(static_cast<const typename Elems<DT>::S*>(p) + c, f);
+  }
+}
+
+// Sums over a row's LPT lanes of a workgroup of BLOCK threads, in every lane.
+// With several waves per row their sums go through `red` in wave order; the two
+// halves of `red` take turns, so one barrier is enough: a wave writes a half
+// again only behind the other half's barrier, which every reader has passed.
+template <int LPT, int BLOCK, int N>
+struct LnSums {
+  static constexpr int WPR = LPT > kWave ? LPT / kWave : 1;
+  float (*red)[BLOCK / kWave][N];  // [2]
+  int half = 0;
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+    if constexpr (WPR == 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = group_sum<LPT>(v[i]);
+    } else {
+      const int wave = static_cast<int>(threadIdx.x) >> 6;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+      if ((threadIdx.x & (kWave - 1)) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) red[half][wave][i] = v[i];
+      }
+      __syncthreads();
+      const int first = wave & ~(WPR - 1);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] = red[half][first][i];
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) v[i] += red[half][first + w][i];
+      }
+      half ^= 1;
+    }
+  }
+};
+
+constexpr int kLnFwdBlock = 256;
+constexpr int kLnBwdBlock = 512;
+
+// Threads of a forward workgroup: a row's lanes fit.
+template <int LPT>
+constexpr int ln_fwd_block() {
+  return LPT > kLnFwdBlock ? LPT : kLnFwdBlock;
+}
+
+template <int DT, int LPT, int R, bool NT, bool KEEP>
+__global__ __launch_bounds__(ln_fwd_block<LPT>()) void ln_fwd_kernel(
+    const typename Elems<DT>::S* __restrict__ x, const LnParams P, typename Elems<DT>::S* __restrict__ y,
+    float* __restrict__ mean_out, float* __restrict__ rstd_out, int8_t* __restrict__ codes,
+    uint8_t* __restrict__ scales, int64_t T, int C, float eps) {
+  constexpr int BLOCK = ln_fwd_block<LPT>(), SLOTS = BLOCK / LPT;
+  __shared__ float red[2][BLOCK / kWave][1];
+  LnSums<LPT, BLOCK, 1> row_sum{red};
+  const int sub = static_cast<int>(threadIdx.x) % LPT, slot = static_cast<int>(threadIdx.x) / LPT;
+  const int G = pack_groups(C);
+  const float n_inv = 1.f / static_cast<float>(C);
+
+  LnPlace at[R];
+  float w[R][8], b[R][8];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    at[k] = ln_place(sub + k * LPT, C);
+    ln_param8<DT>(P.w, P.f32, at[k].c, 1.f, w[k]);
+    ln_param8<DT>(P.b, P.f32, at[k].c, 0.f, b[k]);
+  }
+  // Only a lane's last group can be short or past the row's end.
+  auto inside = [&](int k, int e) { return k < R - 1 || e >= at[k].skip; };
+
+  // Every thread walks as many rows (the barriers of LnSums), those past the
+  // last one on the last one's data, without storing.
+  const int64_t step = static_cast<int64_t>(gridDim.x) * SLOTS;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * SLOTS;
+  LnRaw<DT> raw[R];
+  auto load = [&](int64_t t) {
+    const auto* row = x + (t < T ? t : T - 1) * C;
+#pragma unroll
+    for (int k = 0; k < R; ++k) raw[k] = ln_load<DT, NT>(row + at[k].c);
+  };
+  load(first + slot);
+  for (int64_t t0 = first; t0 < T; t0 += step) {
+    const int64_t t = t0 + slot;
+    float v[R][8];
+#pragma unroll
+    for (int k = 0; k < R; ++k) ln_unpack<DT>(raw[k], v[k]);
+    if (t0 + step < T) load(t + step);
+    __builtin_amdgcn_sched_barrier(0);
+
+    uint32_t E[R];
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t bits = inside(k, e) ? __float_as_uint(v[k][e]) & 0x7fffffffu : 0u;
+          m = bits > m ? bits : m;
+        }
+        E[k] = pack_scale(quad_max(m));
+      }
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[0] += inside(k, e) ? v[k][e] : 0.f;
+    row_sum(s);
+    // Divided, not multiplied with 1 / C: the mean of equal values is that value.
+    const float mean = s[0] / static_cast<float>(C);
+    float s2[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = inside(k, e) ? v[k][e] - mean : 0.f;
+        s2[0] = __builtin_fmaf(d, d, s2[0]);
+      }
+    row_sum(s2);
+    const float rstd = rsqrtf(s2[0] * n_inv + eps);
+    if (t < T) {
+      auto* out = y + t * C;
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (k == R - 1 && at[k].skip == 8) continue;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __builtin_fmaf((v[k][e] - mean) * rstd, w[k][e], b[k][e]);
+        Elems<DT>::template store8<NT>(out + at[k].c, o);
+        if constexpr (KEEP) {
+          const u32x2 q = encode8(v[k], E[k]);
+          int8_t* dst = codes + t * C + at[k].c;
+          if (k < R - 1 || at[k].skip == 0) {
+            st_codes<NT>(dst, q);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e >= at[k].skip) dst[e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+          }
+          const int g = sub + k * LPT;
+          if ((g & 3) == 0) scales[t * G + (g >> 2)] = static_cast<uint8_t>(E[k]);
+        }
+      }
+      if (sub == 0) {
+        if (mean_out) mean_out[t] = mean;
+        if (rstd_out) rstd_out[t] = rstd;
+      }
+    }
+  }
+}
+
+// partial (may be null): this workgroup's sums, [2][ln_cols(C)]: grad_w, grad_b.
+template <int DT, int LPT, int R, bool NT, bool KEPT>
+__global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
+    const typename Elems<DT>::S* __restrict__ gy, const typename LnX<DT, KEPT>::Elem* __restrict__ x,
+    const uint8_t* __restrict__ scales, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+    const LnParams P, typename Elems<DT>::S* __restrict__ gx, float* __restrict__ partial, int64_t T, int C) {
+  constexpr int BLOCK = kLnBwdBlock, SLOTS = BLOCK / LPT;
+  __shared__ float red[2][BLOCK / kWave][2];
+  LnSums<LPT, BLOCK, 2> row_sums{red};
+  const int sub = static_cast<int>(threadIdx.x) % LPT, slot = static_cast<int>(threadIdx.x) / LPT;
+  const int G = pack_groups(C);
+  const float n_inv = 1.f / static_cast<float>(C);
+
+  // Five groups per lane leave no registers for the weight: LDS holds it.
+  constexpr bool W_LDS = R >= 5;
+  __shared__ f32x4 wl[W_LDS ? 2 * R * LPT : 1];
+  LnPlace at[R];
+  float w[W_LDS ? 1 : R][8], dw[R][8], db[R][8];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    at[k] = ln_place(sub + k * LPT, C);
+    ln_param8<DT>(P.w, P.f32, at[k].c, 1.f, w[W_LDS ? 0 : k]);
+    if (W_LDS && slot == 0) {
+      wl[2 * k * LPT + sub] = f32x4{w[0][0], w[0][1], w[0][2], w[0][3]};
+      wl[(2 * k + 1) * LPT + sub] = f32x4{w[0][4], w[0][5], w[0][6], w[0][7]};
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[k][e] = db[k][e] = 0.f;
+  }
+  if constexpr (W_LDS) __syncthreads();
+  auto weight = [&](int k, float (&f)[8]) __attribute__((always_inline)) {
+    if constexpr (W_LDS) {
+      const f32x4 lo = wl[2 * k * LPT + sub], hi = wl[(2 * k + 1) * LPT + sub];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = lo[e];
+        f[4 + e] = hi[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = w[k][e];
+    }
+  };
+
+  const int64_t step = static_cast<int64_t>(gridDim.x) * SLOTS;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * SLOTS;
+  LnRaw<DT> rg[R];
+  LnX<DT, KEPT> rx[R];
+  float mean_n, rstd_n;
+  auto load = [&](int64_t tt) {
+    const int64_t t = tt < T ? tt : T - 1;
+    const auto* grow = gy + t * C;
+    const auto* xrow = x + t * C;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      rg[k] = ln_load<DT, NT>(grow + at[k].c);
+      if constexpr (KEPT) {
+        rx[k].q = ld_codes<NT>(xrow + at[k].c);
+        rx[k].e0 = scales[t * G + (at[k].c >> 5)];
+        // Eight columns off a multiple of 8 may end in another group of 32.
+        rx[k].e1 = k < R - 1 ? rx[k].e0 : scales[t * G + ((at[k].c + 7) >> 5)];
+      } else {
+        rx[k].r = ln_load<DT, NT>(xrow + at[k].c);
+      }
+    }
+    mean_n = mean_in[t];
+    rstd_n = rstd_in[t];
+  };
+  load(first + slot);
+  for (int64_t t0 = first; t0 < T; t0 += step) {
+    const int64_t t = t0 + slot;
+    const float mean = mean_n, rstd = rstd_n;
+    // Few groups per lane stay in fp32 between the sums and the stores; more
+    // stay as loaded and are widened again (16 VGPRs of the 61 per group).
+    constexpr bool HOLD = R <= 3;
+    LnRaw<DT> cg[R];
+    LnX<DT, KEPT> cx[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      cg[k] = rg[k];
+      cx[k] = rx[k];
+    }
+    if (t0 + step < T) load(t + step);
+    __builtin_amdgcn_sched_barrier(0);
+    float q[HOLD ? R : 1][8], h[HOLD ? R : 1][8];
+    auto widen = [&](int k, float (&qk)[8], float (&hk)[8]) __attribute__((always_inline)) {
+      ln_unpack<DT>(cg[k], qk);
+      if constexpr (KEPT)
+        ln_decode<R>(cx[k].q, cx[k].e0, cx[k].e1, k, at[k].c, hk);
+      else
+        ln_unpack<DT>(cx[k].r, hk);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hk[e] = (hk[e] - mean) * rstd;
+    };
+
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float (&qk)[8] = q[HOLD ? k : 0];
+      float (&hk)[8] = h[HOLD ? k : 0];
+      widen(k, qk, hk);
+      float wk[8];
+      weight(k, wk);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float g = k < R - 1 || e >= at[k].skip ? qk[e] * wk[e] : 0.f;
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, hk[e], s[1]);
+      }
+    }
+    row_sums(s);
+    if constexpr (!HOLD) {
+      // The compiler is not to keep the widened values after all.
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        ln_opaque(cg[k]);
+        if constexpr (KEPT)
+          asm volatile("" : "+v"(cx[k].q.x), "+v"(cx[k].q.y));
+        else
+          ln_opaque(cx[k].r);
+      }
+    }
+    if (t < T) {
+      // rstd (g - c1 - h c2)
+      const float k1 = s[0] * n_inv * rstd, k2 = s[1] * n_inv * rstd;
+      auto* out = gx + t * C;
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        float (&qk)[8] = q[HOLD ? k : 0];
+        float (&hk)[8] = h[HOLD ? k : 0];
+        if constexpr (!HOLD) widen(k, qk, hk);
+        float wk[8], o[8];
+        weight(k, wk);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          o[e] = __builtin_fmaf(-hk[e], k2, __builtin_fmaf(qk[e] * wk[e], rstd, -k1));
+          dw[k][e] = __builtin_fmaf(qk[e], hk[e], dw[k][e]);
+          db[k][e] += qk[e];
+        }
+        if (k < R - 1 || at[k].skip < 8) Elems<DT>::template store8<NT>(out + at[k].c, o);
+      }
+    }
+  }
+  if (!partial) return;
+  // The workgroup's rows: the threads that hold the same columns, in slot order.
+  constexpr int kPitch = BLOCK + 4;
+  __shared__ float acc[16 * kPitch];
+  const int64_t cols = (C + 7) / 8 * 8;
+  float* dst = partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      acc[e * kPitch + threadIdx.x] = dw[k][e];
+      acc[(8 + e) * kPitch + threadIdx.x] = db[k][e];
+    }
+    __syncthreads();
+    for (int i = static_cast<int>(threadIdx.x); i < 16 * LPT; i += BLOCK) {
+      const int which = i / (8 * LPT), j = i % (8 * LPT), own = j / 8, e = j % 8;
+      const float* src = acc + (8 * which + e) * kPitch + own;
+      float v = src[0];
+#pragma unroll
+      for (int sl = 1; sl < SLOTS; ++sl) v += src[sl * LPT];
+      const LnPlace p = ln_place(own + k * LPT, C);
+      if (e >= p.skip) dst[which * cols + p.c + e] = v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows of fewer than 8 columns, and rows that no registers hold: one workgroup
+// per row, which is read again for every use, one element per lane.
+constexpr int kLnAnyBlock = 256;
+
+__device__ __forceinline__ float ln_any_sum(float v, float* red) {
+  v = wave_sum(v);
+  __syncthreads();  // red is free again
+  if ((threadIdx.x & (kWave - 1)) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = red[0];
+#pragma unroll
+  for (int i = 1; i < kLnAnyBlock / kWave; ++i) s += red[i];
+  return s;
+}
+
+template <int DT>
+__device__ __forceinline__ float ln_param(const void* p, bool f32, int c, float none) {
+  if (!p) return none;
+  return f32 ? static_cast<const float*>(p)[c] : Elems<DT>::load(static_cast<const typename Elems<DT>::S*>(p) + c);
+}
+
+// x[t, c] in the backward.
+template <int DT, bool KEPT>
+__device__ __forceinline__ float ln_any_x(const typename LnX<DT, KEPT>::Elem* x, const uint8_t* scales, int64_t t, int c,
+                                          int C) {
+  if constexpr (KEPT)
+    return static_cast<float>(x[t * C + c]) * pack_unit(scales[t * pack_groups(C) + (c >> 5)]);
+  else
+    return Elems<DT>::load(x + t * C + c);
+}
+
+template <int DT>
+__global__ __launch_bounds__(kLnAnyBlock) void ln_fwd_any(const typename Elems<DT>::S* __restrict__ x, const LnParams P,
+                                                          typename Elems<DT>::S* __restrict__ y,
+                                                          float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                          int8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                          int64_t T, int C, float eps) {
+  __shared__ float red[kLnAnyBlock / kWave];
+  const int lane = static_cast<int>(threadIdx.x);
+  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
+    const auto* row = x + t * C;
+    float s = 0.f, s2 = 0.f;
+    for (int c = lane; c < C; c += kLnAnyBlock) s += Elems<DT>::load(row + c);
+    const float mean = ln_any_sum(s, red) / static_cast<float>(C);
+    for (int c = lane; c < C; c += kLnAnyBlock) {
+      const float d = Elems<DT>::load(row + c) - mean;
+      s2 = __builtin_fmaf(d, d, s2);
+    }
+    const float rstd = rsqrtf(ln_any_sum(s2, red) / static_cast<float>(C) + eps);
+    for (int c = lane; c < C; c += kLnAnyBlock)
+      Elems<DT>::store(y + t * C + c, __builtin_fmaf((Elems<DT>::load(row + c) - mean) * rstd,
+                                                     ln_param<DT>(P.w, P.f32, c, 1.f), ln_param<DT>(P.b, P.f32, c, 0.f)));
+    if (codes) {
+      // A lane takes 8 columns, a quad of lanes a group of 32.
+      for (int g = lane; (g & ~3) < 4 * pack_groups(C); g += kLnAnyBlock) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 8 * g + e < C ? Elems<DT>::load(row + 8 * g + e) : 0.f;
+        const uint32_t E = pack_scale(quad_max(max_bits8(f)));
+        const u32x2 q = encode8(f, E);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * g + e < C) codes[t * C + 8 * g + e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+        if ((g & 3) == 0 && 8 * g < C) scales[t * pack_groups(C) + (g >> 2)] = static_cast<uint8_t>(E);
+      }
+    }
+    if (lane == 0) {
+      if (mean_out) mean_out[t] = mean;
+      if (rstd_out) rstd_out[t] = rstd;
+    }
+  }
+}
+
+template <int DT, bool KEPT>
+__global__ __launch_bounds__(kLnAnyBlock) void ln_bwd_any(const typename Elems<DT>::S* __restrict__ gy,
+                                                          const typename LnX<DT, KEPT>::Elem* __restrict__ x,
+                                                          const uint8_t* __restrict__ scales,
+                                                          const float* __restrict__ mean_in,
+                                                          const float* __restrict__ rstd_in, const LnParams P,
+                                                          typename Elems<DT>::S* __restrict__ gx, int64_t T, int C) {
+  __shared__ float red[kLnAnyBlock / kWave];
+  const int lane = static_cast<int>(threadIdx.x);
+  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
+    const float mean = mean_in[t], rstd = rstd_in[t];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = lane; c < C; c += kLnAnyBlock) {
+      const float g = Elems<DT>::load(gy + t * C + c) * ln_param<DT>(P.w, P.f32, c, 1.f);
+      s1 += g;
+      s2 = __builtin_fmaf(g, (ln_any_x<DT, KEPT>(x, scales, t, c, C) - mean) * rstd, s2);
+    }
+    const float c1 = ln_any_sum(s1, red) / static_cast<float>(C), c2 = ln_any_sum(s2, red) / static_cast<float>(C);
+    for (int c = lane; c < C; c += kLnAnyBlock) {
+      const float g = Elems<DT>::load(gy + t * C + c) * ln_param<DT>(P.w, P.f32, c, 1.f);
+      const float h = (ln_any_x<DT, KEPT>(x, scales, t, c, C) - mean) * rstd;
+      Elems<DT>::store(gx + t * C + c, rstd * (g - c1 - h * c2));
+    }
+  }
+}
+
+// Their grad_w and grad_b: a workgroup takes 256 columns and rows blockIdx.y,
+// blockIdx.y + gridDim.y, ..., into `partial` as ln_bwd_kernel's workgroup
+// blockIdx.y.
+template <int DT, bool KEPT>
+__global__ __launch_bounds__(kLnAnyBlock) void ln_columns_any(const typename Elems<DT>::S* __restrict__ gy,
+                                                              const typename LnX<DT, KEPT>::Elem* __restrict__ x,
+                                                              const uint8_t* __restrict__ scales,
+                                                              const float* __restrict__ mean_in,
+                                                              const float* __restrict__ rstd_in,
+                                                              float* __restrict__ partial, int64_t T, int C) {
+  const int64_t cols = (C + 7) / 8 * 8;
+  const int c = static_cast<int>(blockIdx.x) * kLnAnyBlock + static_cast<int>(threadIdx.x);
+  if (c >= C) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t t = blockIdx.y; t < T; t += gridDim.y) {
+    const float q = Elems<DT>::load(gy + t * C + c);
+    dw = __builtin_fmaf(q, (ln_any_x<DT, KEPT>(x, scales, t, c, C) - mean_in[t]) * rstd_in[t], dw);
+    db += q;
+  }
+  float* dst = partial + static_cast<int64_t>(blockIdx.y) * 2 * cols;
+  dst[c] = dw;
+  dst[cols + c] = db;
+}
+
+// grad_w and grad_b from the workgroups' sums: 16 vectors of four columns per
+// workgroup, 16 shares of the parts, added in order.
+template <int DT>
+__global__ __launch_bounds__(256) void ln_reduce_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
+                                                        int C, bool f32, void* __restrict__ gw, void* __restrict__ gb) {
+  constexpr int kVecs = 16, kShares = 256 / kVecs;
+  __shared__ f32x4 acc[kShares][kVecs];
+  const int v = static_cast<int>(threadIdx.x) % kVecs, share = static_cast<int>(threadIdx.x) / kVecs;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * kVecs + v) * 4;  // of 2 cols, a multiple of 16
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (i < 2 * cols) {
+    const float* src = partial + i;
+#pragma unroll 4
+    for (int64_t p = share; p < parts; p += kShares) s += *reinterpret_cast<const f32x4*>(src + p * 2 * cols);
+  }
+  acc[share][v] = s;
+  __syncthreads();
+  if (share != 0 || i >= 2 * cols) return;
+#pragma unroll
+  for (int k = 1; k < kShares; ++k) s += acc[k][v];
+  void* dst = i < cols ? gw : gb;
+  if (!dst) return;
+  const int64_t c = i < cols ? i : i - cols;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (c + e < C) {
+      if (f32)
+        static_cast<float*>(dst)[c + e] = s[e];
+      else
+        Elems<DT>::store(static_cast<typename Elems<DT>::S*>(dst) + c + e, s[e]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// How rows are laid over lanes.
+
+template <int kLpt, int kR>
+struct LnWalk {
+  static constexpr int LPT = kLpt, R = kR;
+};
+
+// f(LnWalk) for T rows of C columns, 8 or more, held by registers with at most
+// RMAX groups per lane; false where there is no such layout.
+template <int RMAX, typename F>
+bool with_ln_walk(int64_t T, int C, F&& f) {
+  if (C < 8) return false;
+  const int groups = (C + 7) / 8;
+  auto rounds = [&](auto lpt, int r) {
+    constexpr int L = decltype(lpt)::value;
+    switch (r) {
+      case 1: f(LnWalk<L, 1>{}); return;
+      case 2: f(LnWalk<L, 2>{}); return;
+      case 3: f(LnWalk<L, 3>{}); return;
+      case 4: if constexpr (RMAX >= 4) f(LnWalk<L, 4>{}); return;
+      default: if constexpr (RMAX >= 5 && L <= 128) f(LnWalk<L, 5>{}); return;
+    }
+  };
+  using std::integral_constant;
+  if (groups <= 8) f(LnWalk<8, 1>{});
+  else if (groups <= 16) f(LnWalk<16, 1>{});
+  else if (groups <= 32) f(LnWalk<32, 1>{});
+  else if (groups <= 64) f(LnWalk<64, 1>{});
+  else if (groups <= 64 * RMAX && (groups <= 128 || T >= 1024)) rounds(integral_constant<int, 64>{}, (groups + 63) / 64);
+  else if (groups <= 128 * RMAX && (groups <= 256 || T >= 512)) rounds(integral_constant<int, 128>{}, (groups + 127) / 128);
+  else if (groups <= 512 * (RMAX < 4 ? RMAX : 4)) rounds(integral_constant<int, 512>{}, (groups + 511) / 512);
+  else return false;
+  return true;
+}
+
+}  // namespace
+
+template <int DT>
+int ln_fwd_run(const LnFwdArgs& a, hipStream_t s) {
+  using S = typename Elems<DT>::S;
+  const auto* x = static_cast<const S*>(a.x);
+  auto* y = static_cast<S*>(a.y);
+  const bool nt = a.C % 8 == 0 && aligned16(x) && aligned16(y) && (!a.codes || Pack8Src::aligned(a.codes));
+  const bool held = with_ln_walk<(DT == FMHC_DTYPE_F32 ? 3 : 5)>(a.T, a.C, [&](auto walk) {
+    constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, BLOCK = ln_fwd_block<LPT>();
+    auto launch = [&](auto ntc, auto keep) {
+      constexpr bool NT = decltype(ntc)::value, KEEP = decltype(keep)::value;
+      auto* kernel = &ln_fwd_kernel<DT, LPT, R, NT, KEEP>;
+      const int64_t want = (a.T + BLOCK / LPT - 1) / (BLOCK / LPT);
+      const int64_t most = 256 * 8;
+      kernel<<<dim3(static_cast<unsigned>(want < most ? want : most)), BLOCK, 0, s>>>(x, a.P, y, a.mean, a.rstd, a.codes,
+                                                                                    a.scales, a.T, a.C, a.eps);
+    };
+    auto pick = [&](auto ntc) { a.codes ? launch(ntc, std::true_type{}) : launch(ntc, std::false_type{}); };
+    nt ? pick(std::true_type{}) : pick(std::false_type{});
+  });
+  if (!held) {
+    const int64_t most = 4096;
+    ln_fwd_any<DT><<<dim3(static_cast<unsigned>(a.T < most ? a.T : most)), kLnAnyBlock, 0, s>>>(
+        x, a.P, y, a.mean, a.rstd, a.codes, a.scales, a.T, a.C, a.eps);
+  }
+  return launch_status();
+}
+
+template <int DT>
+int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
+  using S = typename Elems<DT>::S;
+  const auto* gy = static_cast<const S*>(a.gy);
+  auto* gx = static_cast<S*>(a.gx);
+  const int64_t cols = ln_cols(a.C);
+  int64_t parts = 0;
+  auto run = [&](auto kept) {
+    constexpr bool KEPT = decltype(kept)::value;
+    using X = typename LnX<DT, KEPT>::Elem;
+    const X* x = nullptr;
+    if constexpr (KEPT)
+      x = a.codes;
+    else
+      x = static_cast<const X*>(a.x);
+    const bool nt = a.C % 8 == 0 && aligned16(gy) && aligned16(gx) &&
+                    (reinterpret_cast<uintptr_t>(x) & (KEPT ? 7u : 15u)) == 0;
+    const bool held = with_ln_walk<(DT == FMHC_DTYPE_F32 ? 3 : 5)>(a.T, a.C, [&](auto walk) {
+      constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, SLOTS = kLnBwdBlock / LPT;
+      const int64_t want = (a.T + SLOTS - 1) / SLOTS;
+      parts = want < kLnParts ? want : kLnParts;
+      auto launch = [&](auto ntc) {
+        ln_bwd_kernel<DT, LPT, R, decltype(ntc)::value, KEPT><<<dim3(static_cast<unsigned>(parts)), kLnBwdBlock, 0, s>>>(
+            gy, x, a.scales, a.mean, a.rstd, a.P, gx, a.partial, a.T, a.C);
+      };
+      nt ? launch(std::true_type{}) : launch(std::false_type{});
+    });
+    if (!held) {
+      const int64_t most = 4096;
+      ln_bwd_any<DT, KEPT><<<dim3(static_cast<unsigned>(a.T < most ? a.T : most)), kLnAnyBlock, 0, s>>>(
+          gy, x, a.scales, a.mean, a.rstd, a.P, gx, a.T, a.C);
+      if (a.partial) {
+        parts = a.T < kLnParts ? a.T : kLnParts;
+        ln_columns_any<DT, KEPT><<<dim3(blocks_for(a.C, kLnAnyBlock), static_cast<unsigned>(parts)), kLnAnyBlock, 0, s>>>(
+            gy, x, a.scales, a.mean, a.rstd, a.partial, a.T, a.C);
+      }
+    }
+  };
+  a.x ? run(std::false_type{}) : run(std::true_type{});
+  const int st = launch_status();
+  if (st != FMHC_OK || !a.partial) return st;
+  ln_reduce_kernel<DT><<<dim3(blocks_for(2 * cols, 64)), 256, 0, s>>>(a.partial, parts, cols, a.C, a.P.f32, a.gw, a.gb);
+  return launch_status();
+}
+
+}  // namespace fmhc

@@ -33,7 +33,7 @@ LIB_PATH = LIB_DIR / LIB_NAME
 PROBE_LIB_PATH = LIB_DIR / "libflash_mhc_probe.so"
 
 SOURCES = ("k1.hip", "k2.hip", "k3.hip", "k4.hip", "premap.hip", "premap_resident.hip", "premap_split.hip",
-           "pack8.hip", "layer_norm.hip", "abi.hip")
+           "pack8.hip", "layer_norm.hip", "layer_norm_f32.hip", "layer_norm_bf16.hip", "layer_norm_f16.hip", "abi.hip")
 PROBE_SOURCES = ("stream_probe.hip",)
 
 ARCH = "gfx950"
