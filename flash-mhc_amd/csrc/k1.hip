@@ -634,6 +634,7 @@ struct BwdFrag {
   u32x4 gv, pv;   // go / proj_out row of token tbase + col, d = 8 * grp .. + 8
   float inv[4];   // inv_rms of tokens tbase + 4 * grp + q
   typename SRC::Raw xv[4];  // x of those tokens, k = kl .. kl + 8
+  float ic[SRC::kPacked ? 1 : 0];  // 8 bits: inv_rms of token tbase + col
   u32x4 g3[EPI ? 4 : 1];  // EPI: the K3 output gradient of those tokens at the lane's c
   float hp[EPI ? 4 : 1];  // EPI: their h_pre of the lane's stream j
   u32x4 gi[GI ? 4 : 1];   // GI: x's incoming gradient at the lane's 8 k
@@ -780,6 +781,7 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
     f.gv = ld16(reinterpret_cast<const char*>(go + tbase * kDout) + goff);
     f.pv = ld16(reinterpret_cast<const char*>(proj + tbase * kDout) + goff);
     const char* ib = reinterpret_cast<const char*>(inv_rms + tbase);
+    if constexpr (SRC::kPacked) f.ic[0] = inv_rms[tbase + rg];
     const char* xb = reinterpret_cast<const char*>(x + tbase * nC);
     // The lane's four tokens are consecutive: a full block reads their
     // inv_rms with one 16-byte load (the block-uniform branch below).
@@ -822,14 +824,24 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
     for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(gf[e], pf[e], dot);
     dot = rows_sum(dot);  // the wave is converged here
     float scale[4];
+    if constexpr (SRC::kPacked) {
+      // One division per lane, for token tbase + col, instead of four.
+      const float sc = dot * (f.ic[0] * f.ic[0]) / static_cast<float>(nC);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float d = __shfl(dot, 4 * grp + q, kWave);  // token tbase + 4 * grp + q
-      scale[q] = d * (f.inv[q] * f.inv[q]) / static_cast<float>(nC);
+      for (int q = 0; q < 4; ++q) scale[q] = __shfl(sc, 4 * grp + q, kWave);  // token tbase + 4 * grp + q
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float d = __shfl(dot, 4 * grp + q, kWave);  // token tbase + 4 * grp + q
+        scale[q] = d * (f.inv[q] * f.inv[q]) / static_cast<float>(nC);
+      }
     }
-    u32x4 xv[4];  // x as bf16
+    // 8 bits: widened once, for grad_x and for grad_W's operand.
+    float xw[SRC::kPacked ? 4 : 1][8];
+    if constexpr (SRC::kPacked) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) xv[q] = SRC::bits(f.xv[q], cj);
+      for (int q = 0; q < 4; ++q) SRC::widen(f.xv[q], cj, xw[q]);
+    }
     f32x4 acc[8];
     if constexpr (kValu) {
       // VALU build: acc[m][q] = sum_d go[token 4 grp + q][d] * W[d][kl + m] as
@@ -864,7 +876,12 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
         const int r = 4 * grp + q;
         if (r < rows) {
           float xf[8], o[8];
-          unpack8(xv[q], xf);
+          if constexpr (SRC::kPacked) {
+#pragma unroll
+            for (int m = 0; m < 8; ++m) xf[m] = xw[q][m];
+          } else {
+            unpack8(f.xv[q], xf);
+          }
 #pragma unroll
           for (int m = 0; m < 8; ++m) o[m] = f.inv[q] * acc[m][q] - scale[q] * xf[m];
           if constexpr (EPI) {
@@ -913,13 +930,18 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
 #pragma unroll
       for (int m = 0; m < 8; ++m) {
         // A: element m of the 4 tokens' x vectors.
-        uint32_t e[4];
+        u32x2 av;
+        if constexpr (SRC::kPacked) {  // exact: a value has seven significant bits
+          av = u32x2{pack_bf16x2(xw[0][m], xw[1][m]), pack_bf16x2(xw[2][m], xw[3][m])};
+        } else {
+          uint32_t e[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t w = xv[q][m >> 1];
-          e[q] = (m & 1) ? (w >> 16) : (w & 0xffffu);
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t w = f.xv[q][m >> 1];
+            e[q] = (m & 1) ? (w >> 16) : (w & 0xffffu);
+          }
+          av = u32x2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
         }
-        const u32x2 av = {e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const u32x2 bv = {bh[h][0], bh[h][1]};
@@ -1213,7 +1235,10 @@ constexpr int kBwdNTB = 8;
 constexpr int kBwdDwNTB = 64;
 // Fragments in flight in k1_bwd_mfma's block loop (two blocks load while one
 // computes): the K1 op kernels, and the pre-map variants (EPI), whose extra
-// operands leave no registers for a third buffer at two waves per SIMD.
+// operands leave no registers for a third buffer at two waves per SIMD, and the
+// kernels that read x in 8 bits, whose buffers are smaller but whose VALU work
+// (4 more operations per two elements) one wave per SIMD does not hide: two
+// buffers and two waves T = 16384, C = 4096 172 us, three and one 193, four 202.
 constexpr int kBwdBufs = 3;
 constexpr int kBwdEpiBufs = 2;
 constexpr int kBwdDwMinNTB = 4;
@@ -1411,7 +1436,7 @@ void launch_k1_bwd_mfma(hipStream_t s, const typename SRC::Elem* x, const uint16
                         const float* h_pre = nullptr, int C = 1, const uint16_t* gi = nullptr,
                         const uint8_t* xs = nullptr) {
   const dim3 grid(blocks_for(nruns * sl.n, 4));
-  constexpr int nbuf = EPI ? kBwdEpiBufs : kBwdBufs;
+  constexpr int nbuf = EPI || SRC::kPacked ? kBwdEpiBufs : kBwdBufs;
   // dx alone: one workgroup per CU (LDS reserved that the kernel does not
   // use; its registers allow two) up to C = 2560 per stream.  Measured in
   // the six-kernel step (GB/s, two workgroups per CU against one): T = 65536,
@@ -1645,12 +1670,19 @@ int k1_bwd_premap(const typename SRC::Elem* x_flat, const uint8_t* xs, const uin
     const BwdSlices sl = bwd_premap_slices(C);
     const int64_t nruns = k1_bwd_runs(T, sl.n);
     float* partial = static_cast<float*>(workspace);
-    if (grad_x_in)
-      launch_k1_bwd_mfma<true, true, true, SRC>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl,
-                                                nruns, go3, h_pre, static_cast<int>(C), grad_x_in, xs);
-    else
-      launch_k1_bwd_mfma<true, true, false, SRC>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl,
+    auto run = [&](auto src) {
+      using S = decltype(src);
+      if (grad_x_in)
+        launch_k1_bwd_mfma<true, true, true, S>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl, nruns,
+                                                go3, h_pre, static_cast<int>(C), grad_x_in, xs);
+      else
+        launch_k1_bwd_mfma<true, true, false, S>(s, x_flat, W, grad_proj, proj, inv_rms, grad_x, partial, T, nc, sl,
                                                  nruns, go3, h_pre, static_cast<int>(C), nullptr, xs);
+    };
+    if (SRC::kPacked && C % 8 == 0)
+      run(std::conditional_t<SRC::kPacked, Pack8WholeSrc, SRC>{});
+    else
+      run(SRC{});
     const int st = launch_status();
     if (st != FMHC_OK) return st;
     return launch_dw_reduce(partial, grad_W, nruns, sl, nc, k2_sums, kNPar, s);
@@ -1698,8 +1730,11 @@ extern "C" int fmhc_k1_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales,
     const BwdSlices sl = bwd_premap_slices(C);
     const int64_t nruns = k1_bwd_runs(T, sl.n);
     float* partial = static_cast<float*>(workspace);
-    launch_k1_bwd_mfma<true, false, false, Pack8Src>(s, x_codes, W, grad_out, proj_out, inv_rms, grad_x, partial, T, nc,
-                                                     sl, nruns, nullptr, nullptr, c, nullptr, x_scales);
+    auto run = [&](auto src) {
+      launch_k1_bwd_mfma<true, false, false, decltype(src)>(s, x_codes, W, grad_out, proj_out, inv_rms, grad_x, partial, T,
+                                                            nc, sl, nruns, nullptr, nullptr, c, nullptr, x_scales);
+    };
+    C % 8 == 0 ? run(Pack8WholeSrc{}) : run(Pack8Src{});
     const int st = launch_status();
     if (st != FMHC_OK) return st;
     return launch_dw_reduce(partial, grad_W, nruns, sl, nc, K2ParamSums{}, 0, s);

@@ -91,9 +91,11 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_kernel(const uin
 // The forward that also leaves x and lo in 8 bits (pack8.h) for the backward:
 // out as k4_fwd_kernel gives it, and the codes and scales of the rows it has in
 // registers anyway, which a pass of its own would read again.  A quad of lanes
-// holds a group of 32 columns; the lane at a row's end with fewer than 8 columns
-// left moves them one by one.
-template <typename WALK>
+// holds a group of 32 columns.  The lane at a row's end with fewer than 8
+// columns left takes the row's last 8: it leaves those of the lane before out of
+// its group's maximum, and stores them once more with the same values.  SHORT:
+// rows of fewer than 8 columns, one element at a time.
+template <typename WALK, bool SHORT>
 __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
     const uint16_t* __restrict__ x, const uint16_t* __restrict__ lo, const float* __restrict__ H,
     const float* __restrict__ h_post, uint16_t* __restrict__ out, int8_t* __restrict__ xq, uint8_t* __restrict__ xs,
@@ -127,14 +129,15 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
   // Lane group g: columns 8 g .. 8 g + 7, of which n are in the row.
   auto round = [&](int g) __attribute__((always_inline)) {
     const int n = C - 8 * g;
-    const bool whole = WHOLE ? n > 0 : n >= 8;
-    float v[5][8];  // lo, then the streams
+    const int c = SHORT || n >= 8 ? 8 * g : C - 8;  // the eight columns it holds
+    const int skip = 8 * g - c;                     // (8 or more: past the row's end)
+    float v[5][8];                                  // lo, then the streams
     auto fetch = [&](const uint16_t* row, float (&f)[8]) __attribute__((always_inline)) {
-      if (whole) {
-        Lanes<8, WHOLE>::load(row, g, f);
-      } else {
+      if constexpr (SHORT) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = !WHOLE && e < n ? bf16_to_f32(row[8 * g + e]) : 0.f;
+        for (int e = 0; e < 8; ++e) f[e] = e < n ? bf16_to_f32(row[c + e]) : 0.f;
+      } else {
+        Lanes<8, WHOLE>::load(row + c, 0, f);
       }
     };
     fetch(lrow, v[0]);
@@ -151,26 +154,36 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
         o[e] = acc;
       }
       uint16_t* orow = o0 + i * int64_t{C};
-      if (whole) {
-        Lanes<8, WHOLE>::store(orow, g, o);
-      } else if constexpr (!WHOLE) {
+      if constexpr (SHORT) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e < n) orow[8 * g + e] = f32_to_bf16(o[e]);
+          if (e < n) orow[c + e] = f32_to_bf16(o[e]);
+      } else if (n > 0) {
+        Lanes<8, WHOLE>::store(orow + c, 0, o);
       }
     }
 #pragma unroll
     for (int k = 0; k < 5; ++k) {
-      const uint32_t E = pack_scale(quad_max(max_bits8(v[k])));  // the whole quad is here
+      uint32_t m = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // SHORT: zeros past the end; WHOLE: a lane's columns are its own, or none are in the row.
+        const uint32_t b = __float_as_uint(v[k][e]) & 0x7fffffffu;
+        const bool own = SHORT || (WHOLE ? n > 0 : e >= skip);
+        m = own && b > m ? b : m;
+      }
+      const uint32_t E = pack_scale(quad_max(m));  // the whole quad is here
       const u32x2 q = encode8(v[k], E);
       int8_t* qrow = k == 0 ? lq + tok * C : q0 + (k - 1) * int64_t{C};
       uint8_t* srow = k == 0 ? ls + tok * G : s0 + (k - 1) * int64_t{G};
-      if (whole) {
-        st_codes<WHOLE>(qrow + 8 * g, q);
-      } else if constexpr (!WHOLE) {
+      if constexpr (SHORT) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e < n) qrow[8 * g + e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+          if (e < n) qrow[c + e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+      } else if (WHOLE ? n > 0 : n >= 8) {
+        st_codes<WHOLE>(qrow + c, q);
+      } else if (!WHOLE && n > 0) {
+        st_last_codes(qrow + 8 * g, q, n);
       }
       if ((g & 3) == 0 && n > 0) srow[g >> 2] = static_cast<uint8_t>(E);
     }
@@ -385,16 +398,20 @@ int launch_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, c
                        Pack8Src::aligned(lq);
   const int G = pack_groups(C);
   // Lanes for whole groups of 32 columns.
-  with_row_walk(G * kPackGroup, aligned, [&](auto w) {
+  auto run = [&](auto w, auto few) {
     using Walk = decltype(w);
     constexpr int L = Walk::LPT;
     for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
       const dim3 grid(blocks_for(n, tokens_per_block(L)));
-      k4_fwd_pack8_kernel<Walk><<<grid, block_of<L>(), 0, s>>>(
+      k4_fwd_pack8_kernel<Walk, decltype(few)::value><<<grid, block_of<L>(), 0, s>>>(
           x + t * 4 * C, lo + t * C, H + t * 16, hp + t * 4, out + t * 4 * C, xq + t * 4 * C, xs + t * 4 * G,
           lq + t * C, ls + t * G, n, C);
     });
-  });
+  };
+  if (C < 8)
+    run(RowWalk<8, false, false>{}, std::true_type{});
+  else
+    with_row_walk(G * kPackGroup, aligned, [&](auto w) { run(w, std::false_type{}); });
   return launch_status();
 }
 

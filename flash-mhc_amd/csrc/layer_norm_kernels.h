@@ -72,18 +72,14 @@ struct LnX<DT, true> {
   uint32_t e0, e1;  // the first and the last column's (a lane's last group only)
 };
 
-// The values of 8 codes from column c on, those of round k < R - 1 in one group.
-template <int R>
+// The values of 8 codes from column c on, in one group for round k < R - 1 and
+// in rows of whole groups of 8 (NT).
+template <int R, bool NT>
 __device__ __forceinline__ void ln_decode(u32x2 q, uint32_t e0, uint32_t e1, int k, int c, float (&f)[8]) {
-  const float u0 = pack_unit(e0);
-  if (k < R - 1) return decode8(q, u0, f);
-  const float u1 = pack_unit(e1);
-  const int n0 = kPackGroup - (c & (kPackGroup - 1));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = code_at(q.x, i) * (i < n0 ? u0 : u1);
-    f[4 + i] = code_at(q.y, i) * (4 + i < n0 ? u0 : u1);
-  }
+  if (NT || k < R - 1)
+    decode8(q, pack_unit(e0), f);
+  else
+    decode8(q, pack_unit(e0), pack_unit(e1), kPackGroup - (c & (kPackGroup - 1)), f);
 }
 
 // Where lane group g of a row of C >= 8 columns is: 8 columns from `c` on, of
@@ -240,9 +236,7 @@ __global__ __launch_bounds__(ln_fwd_block<LPT>()) void ln_fwd_kernel(
           if (k < R - 1 || at[k].skip == 0) {
             st_codes<NT>(dst, q);
           } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e >= at[k].skip) dst[e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+            st_last_codes(dst + at[k].skip, q, 8 - at[k].skip);
           }
           const int g = sub + k * LPT;
           if ((g & 3) == 0) scales[t * G + (g >> 2)] = static_cast<uint8_t>(E[k]);
@@ -316,7 +310,7 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
         rx[k].q = ld_codes<NT>(xrow + at[k].c);
         rx[k].e0 = scales[t * G + (at[k].c >> 5)];
         // Eight columns off a multiple of 8 may end in another group of 32.
-        rx[k].e1 = k < R - 1 ? rx[k].e0 : scales[t * G + ((at[k].c + 7) >> 5)];
+        rx[k].e1 = NT || k < R - 1 ? rx[k].e0 : scales[t * G + ((at[k].c + 7) >> 5)];
       } else {
         rx[k].r = ln_load<DT, NT>(xrow + at[k].c);
       }
@@ -344,7 +338,7 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
     auto widen = [&](int k, float (&qk)[8], float (&hk)[8]) __attribute__((always_inline)) {
       ln_unpack<DT>(cg[k], qk);
       if constexpr (KEPT)
-        ln_decode<R>(cx[k].q, cx[k].e0, cx[k].e1, k, at[k].c, hk);
+        ln_decode<R, NT>(cx[k].q, cx[k].e0, cx[k].e1, k, at[k].c, hk);
       else
         ln_unpack<DT>(cx[k].r, hk);
 #pragma unroll

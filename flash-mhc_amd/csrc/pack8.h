@@ -48,17 +48,33 @@ __device__ __forceinline__ float pack_unit(uint32_t E) {
   return __uint_as_float(E == kPackNan ? 0x7fc00000u : (E - 6u) << 23);
 }
 
-__device__ __forceinline__ float code_at(uint32_t w, int i) {
-  return static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+// Code I of a word as fp32.  A bit field extraction, which the compiler folds
+// into the conversion's operand (from a shift and a narrowing cast it makes two
+// to three instructions).
+template <int I>
+__device__ __forceinline__ float code_at(uint32_t w) {
+  return static_cast<float>(static_cast<int>(__builtin_amdgcn_sbfe(static_cast<int>(w), 8 * I, 8)));
+}
+
+// The 8 codes as fp32.
+__device__ __forceinline__ void codes8(u32x2 q, float (&f)[8]) {
+  f[0] = code_at<0>(q.x), f[1] = code_at<1>(q.x), f[2] = code_at<2>(q.x), f[3] = code_at<3>(q.x);
+  f[4] = code_at<0>(q.y), f[5] = code_at<1>(q.y), f[6] = code_at<2>(q.y), f[7] = code_at<3>(q.y);
 }
 
 // The values of 8 codes of one group.
-__device__ __forceinline__ void decode8(u32x2 q, float unit, float f[8]) {
+__device__ __forceinline__ void decode8(u32x2 q, float unit, float (&f)[8]) {
+  codes8(q, f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = code_at(q.x, i) * unit;
-    f[4 + i] = code_at(q.y, i) * unit;
-  }
+  for (int i = 0; i < 8; ++i) f[i] *= unit;
+}
+
+// The same where the group of 32 ends behind n0 columns (8 or more: all of them
+// have u0).
+__device__ __forceinline__ void decode8(u32x2 q, float u0, float u1, int n0, float (&f)[8]) {
+  codes8(q, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] *= i < n0 ? u0 : u1;
 }
 
 // The largest magnitude's bits (NaN above Inf above every number).
@@ -110,6 +126,24 @@ __device__ __forceinline__ u32x2 encode8(const float f[8], uint32_t E) {
   return q;
 }
 
+// The last n codes (1 to 7) of 8, to p on: one store per bit of n.
+__device__ __forceinline__ void st_last_codes(int8_t* p, u32x2 q, int n) {
+  uint64_t v = (static_cast<uint64_t>(q.y) << 32 | q.x) >> (8 * (8 - n));
+  typedef uint32_t u32_byte __attribute__((aligned(1)));
+  typedef uint16_t u16_byte __attribute__((aligned(1)));
+  if (n & 4) {
+    *reinterpret_cast<u32_byte*>(p) = static_cast<uint32_t>(v);
+    p += 4;
+    v >>= 32;
+  }
+  if (n & 2) {
+    *reinterpret_cast<u16_byte*>(p) = static_cast<uint16_t>(v);
+    p += 2;
+    v >>= 16;
+  }
+  if (n & 1) *p = static_cast<int8_t>(v);
+}
+
 // Where a kernel reads rows from: bf16, or codes and scales.  A Row is one row
 // of C columns; load<8>(g) its element group g (8 columns), load<1>(c) one
 // element.  NT: with the nontemporal hint (whole, aligned groups).  Kernels
@@ -128,14 +162,12 @@ struct Bf16Src {
     }
   };
   static bool aligned(const Elem* x) { return aligned16(x); }
-  // Eight columns as loaded, and as bf16 bits; c is the first one's place in its
-  // row.
+  // Eight columns as loaded; c is the first one's place in its row.
   using Raw = u32x4;
   template <bool NT>
   __device__ static __forceinline__ Raw raw(const char* at, const uint8_t*, int) {
     return Lanes<8, NT>::raw(reinterpret_cast<const uint16_t*>(at), 0);
   }
-  __device__ static __forceinline__ u32x4 bits(const Raw& v, int) { return v; }
   // Column k of token t, whose nC columns are streams of C.
   __device__ static __forceinline__ float elem(const Elem* x, const uint8_t*, int64_t t, int k, int nC, int) {
     return bf16_to_f32(x[t * nC + k]);
@@ -174,23 +206,27 @@ struct Pack8Src {
   __device__ static __forceinline__ Raw raw(const char* at, const uint8_t* row_scales, int c) {
     return Raw{ld_codes<NT>(reinterpret_cast<const int8_t*>(at)), row_scales[c >> 5], row_scales[(c + 7) >> 5]};
   }
-  // Exact: a value has seven significant bits.
-  __device__ static __forceinline__ u32x4 bits(const Raw& v, int c) {
-    const float u0 = pack_unit(v.e0), u1 = pack_unit(v.e1);
-    const int n0 = kPackGroup - (c & (kPackGroup - 1));  // columns of the first group from c on
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = code_at(v.q.x, i) * (i < n0 ? u0 : u1);
-      f[4 + i] = code_at(v.q.y, i) * (4 + i < n0 ? u0 : u1);
-    }
-    return pack8(f);
+  __device__ static __forceinline__ void widen(const Raw& v, int c, float (&f)[8]) {
+    decode8(v.q, pack_unit(v.e0), pack_unit(v.e1), kPackGroup - (c & (kPackGroup - 1)), f);
   }
   __device__ static __forceinline__ float elem(const Elem* x, const uint8_t* scales, int64_t t, int k, int nC, int C) {
     const int j = k / C;
     return static_cast<float>(x[t * nC + k]) *
            pack_unit(scales[(t * (nC / C) + j) * pack_groups(C) + ((k - j * C) >> 5)]);
   }
+};
+
+// Rows of C % 8 == 0: eight columns from a multiple of 8 on have one scale.
+struct Pack8WholeSrc : Pack8Src {
+  struct Raw {
+    u32x2 q;
+    uint32_t e;
+  };
+  template <bool NT>
+  __device__ static __forceinline__ Raw raw(const char* at, const uint8_t* row_scales, int c) {
+    return Raw{ld_codes<NT>(reinterpret_cast<const int8_t*>(at)), row_scales[c >> 5]};
+  }
+  __device__ static __forceinline__ void widen(const Raw& v, int, float (&f)[8]) { decode8(v.q, pack_unit(v.e), f); }
 };
 
 }  // namespace fmhc
