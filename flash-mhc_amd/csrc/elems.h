@@ -76,8 +76,9 @@ struct Elems<FMHC_DTYPE_F32> {
       a[i] = __float_as_uint(f[i]);
       b[i] = __float_as_uint(f[4 + i]);
     }
-    NT ? st16_stream(p, a) : st16(p, a);
-    NT ? st16_stream(p + 4, b) : st16(p + 4, b);
+    // Never with the hint: each of the two stores fills half of its lines.
+    st16(p, a);
+    st16(p + 4, b);
   }
   __device__ static __forceinline__ float load(const S* p) { return *p; }
   __device__ static __forceinline__ void store(S* p, float v) { *p = v; }
