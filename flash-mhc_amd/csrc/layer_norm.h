@@ -52,9 +52,10 @@ int ln_fwd_run(const LnFwdArgs& a, hipStream_t s);
 template <int DT>
 int ln_bwd_run(const LnBwdArgs& a, hipStream_t s);
 
-// Workgroups of the backward, each of which leaves sums of all columns: at most
-// this many (one of eight waves per CU).
-constexpr int64_t kLnParts = 256;
+// Workgroups of the backward, each of which leaves sums of all columns, at most:
+// one of eight waves per CU, two where a lane has one group of columns (and the
+// registers for them).
+constexpr int64_t kLnParts = 512;
 // Columns of a workgroup's sums.
 inline int64_t ln_cols(int64_t C) { return (C + 7) / 8 * 8; }
 

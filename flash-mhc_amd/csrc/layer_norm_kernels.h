@@ -263,36 +263,15 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
   const int G = pack_groups(C);
   const float n_inv = 1.f / static_cast<float>(C);
 
-  // Five groups per lane leave no registers for the weight: LDS holds it.
-  constexpr bool W_LDS = R >= 5;
-  __shared__ f32x4 wl[W_LDS ? 2 * R * LPT : 1];
   LnPlace at[R];
-  float w[W_LDS ? 1 : R][8], dw[R][8], db[R][8];
+  float w[R][8], dw[R][8], db[R][8];
 #pragma unroll
   for (int k = 0; k < R; ++k) {
     at[k] = ln_place(sub + k * LPT, C);
-    ln_param8<DT>(P.w, P.f32, at[k].c, 1.f, w[W_LDS ? 0 : k]);
-    if (W_LDS && slot == 0) {
-      wl[2 * k * LPT + sub] = f32x4{w[0][0], w[0][1], w[0][2], w[0][3]};
-      wl[(2 * k + 1) * LPT + sub] = f32x4{w[0][4], w[0][5], w[0][6], w[0][7]};
-    }
+    ln_param8<DT>(P.w, P.f32, at[k].c, 1.f, w[k]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[k][e] = db[k][e] = 0.f;
   }
-  if constexpr (W_LDS) __syncthreads();
-  auto weight = [&](int k, float (&f)[8]) __attribute__((always_inline)) {
-    if constexpr (W_LDS) {
-      const f32x4 lo = wl[2 * k * LPT + sub], hi = wl[(2 * k + 1) * LPT + sub];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[e] = lo[e];
-        f[4 + e] = hi[e];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = w[k][e];
-    }
-  };
 
   const int64_t step = static_cast<int64_t>(gridDim.x) * SLOTS;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * SLOTS;
@@ -351,11 +330,9 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
       float (&qk)[8] = q[HOLD ? k : 0];
       float (&hk)[8] = h[HOLD ? k : 0];
       widen(k, qk, hk);
-      float wk[8];
-      weight(k, wk);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float g = k < R - 1 || e >= at[k].skip ? qk[e] * wk[e] : 0.f;
+        const float g = k < R - 1 || e >= at[k].skip ? qk[e] * w[k][e] : 0.f;
         s[0] += g;
         s[1] = __builtin_fmaf(g, hk[e], s[1]);
       }
@@ -381,11 +358,10 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
         float (&qk)[8] = q[HOLD ? k : 0];
         float (&hk)[8] = h[HOLD ? k : 0];
         if constexpr (!HOLD) widen(k, qk, hk);
-        float wk[8], o[8];
-        weight(k, wk);
+        float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          o[e] = __builtin_fmaf(-hk[e], k2, __builtin_fmaf(qk[e] * wk[e], rstd, -k1));
+          o[e] = __builtin_fmaf(-hk[e], k2, __builtin_fmaf(qk[e] * w[k][e], rstd, -k1));
           dw[k][e] = __builtin_fmaf(qk[e], hk[e], dw[k][e]);
           db[k][e] += qk[e];
         }
@@ -545,25 +521,34 @@ __global__ __launch_bounds__(kLnAnyBlock) void ln_columns_any(const typename Ele
 }
 
 // grad_w and grad_b from the workgroups' sums: 16 vectors of four columns per
-// workgroup, 16 shares of the parts, added in order.
+// workgroup, 64 shares of the parts, added in order.  A chain of load latencies:
+// with 16 shares a thread walks up to 32 parts.
+constexpr int kLnReduceBlock = 1024;
 template <int DT>
-__global__ __launch_bounds__(256) void ln_reduce_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
+__global__ __launch_bounds__(kLnReduceBlock) void ln_reduce_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
                                                         int C, bool f32, void* __restrict__ gw, void* __restrict__ gb) {
-  constexpr int kVecs = 16, kShares = 256 / kVecs;
+  constexpr int kVecs = 16, kShares = kLnReduceBlock / kVecs;
   __shared__ f32x4 acc[kShares][kVecs];
   const int v = static_cast<int>(threadIdx.x) % kVecs, share = static_cast<int>(threadIdx.x) / kVecs;
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * kVecs + v) * 4;  // of 2 cols, a multiple of 16
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (i < 2 * cols) {
     const float* src = partial + i;
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t p = share; p < parts; p += kShares) s += *reinterpret_cast<const f32x4*>(src + p * 2 * cols);
   }
   acc[share][v] = s;
   __syncthreads();
+  if (share < 8) {
+#pragma unroll
+    for (int k = 8; k < kShares; k += 8) s += acc[share + k][v];
+  }
+  __syncthreads();
+  if (share < 8) acc[share][v] = s;
+  __syncthreads();
   if (share != 0 || i >= 2 * cols) return;
 #pragma unroll
-  for (int k = 1; k < kShares; ++k) s += acc[k][v];
+  for (int k = 1; k < 8; ++k) s += acc[k][v];
   void* dst = i < cols ? gw : gb;
   if (!dst) return;
   const int64_t c = i < cols ? i : i - cols;
@@ -598,7 +583,7 @@ bool with_ln_walk(int64_t T, int C, F&& f) {
       case 1: f(LnWalk<L, 1>{}); return;
       case 2: f(LnWalk<L, 2>{}); return;
       case 3: f(LnWalk<L, 3>{}); return;
-      case 4: if constexpr (RMAX >= 4) f(LnWalk<L, 4>{}); return;
+      case 4: if constexpr (RMAX >= 4 || L == 512) f(LnWalk<L, 4>{}); return;
       default: if constexpr (RMAX >= 5 && L <= 128) f(LnWalk<L, 5>{}); return;
     }
   };
@@ -608,8 +593,9 @@ bool with_ln_walk(int64_t T, int C, F&& f) {
   else if (groups <= 32) f(LnWalk<32, 1>{});
   else if (groups <= 64) f(LnWalk<64, 1>{});
   else if (groups <= 64 * RMAX && (groups <= 128 || T >= 1024)) rounds(integral_constant<int, 64>{}, (groups + 63) / 64);
-  else if (groups <= 128 * RMAX && (groups <= 256 || T >= 512)) rounds(integral_constant<int, 128>{}, (groups + 127) / 128);
-  else if (groups <= 512 * (RMAX < 4 ? RMAX : 4)) rounds(integral_constant<int, 512>{}, (groups + 511) / 512);
+  else if (groups <= 128 * RMAX && (groups <= 256 || T >= 8192)) rounds(integral_constant<int, 128>{}, (groups + 127) / 128);
+  else if (groups <= 256 * RMAX && (groups <= 512 || T >= 512)) rounds(integral_constant<int, 256>{}, (groups + 255) / 256);
+  else if (groups <= 512 * 4) rounds(integral_constant<int, 512>{}, (groups + 511) / 512);
   else return false;
   return true;
 }
@@ -660,10 +646,11 @@ int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
       x = static_cast<const X*>(a.x);
     const bool nt = a.C % 8 == 0 && aligned16(gy) && aligned16(gx) &&
                     (reinterpret_cast<uintptr_t>(x) & (KEPT ? 7u : 15u)) == 0;
-    const bool held = with_ln_walk<(DT == FMHC_DTYPE_F32 ? 3 : 5)>(a.T, a.C, [&](auto walk) {
+    const bool held = with_ln_walk<3>(a.T, a.C, [&](auto walk) {
       constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, SLOTS = kLnBwdBlock / LPT;
       const int64_t want = (a.T + SLOTS - 1) / SLOTS;
-      parts = want < kLnParts ? want : kLnParts;
+      const int64_t most = R == 1 ? kLnParts : kLnParts / 2;
+      parts = want < most ? want : most;
       auto launch = [&](auto ntc) {
         ln_bwd_kernel<DT, LPT, R, decltype(ntc)::value, KEPT><<<dim3(static_cast<unsigned>(parts)), kLnBwdBlock, 0, s>>>(
             gy, x, a.scales, a.mean, a.rstd, a.P, gx, a.partial, a.T, a.C);
@@ -684,7 +671,7 @@ int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
   a.x ? run(std::false_type{}) : run(std::true_type{});
   const int st = launch_status();
   if (st != FMHC_OK || !a.partial) return st;
-  ln_reduce_kernel<DT><<<dim3(blocks_for(2 * cols, 64)), 256, 0, s>>>(a.partial, parts, cols, a.C, a.P.f32, a.gw, a.gb);
+  ln_reduce_kernel<DT><<<dim3(blocks_for(2 * cols, 64)), kLnReduceBlock, 0, s>>>(a.partial, parts, cols, a.C, a.P.f32, a.gw, a.gb);
   return launch_status();
 }
 
