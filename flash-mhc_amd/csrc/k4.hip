@@ -95,7 +95,8 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_kernel(const uin
 // columns left takes the row's last 8: it leaves those of the lane before out of
 // its group's maximum, and stores them once more with the same values.  SHORT:
 // rows of fewer than 8 columns, one element at a time.
-template <typename WALK, bool SHORT>
+// PACKX: x too, not lo alone (a block's pre-map has packed it already).
+template <typename WALK, bool SHORT, bool PACKX>
 __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
     const uint16_t* __restrict__ x, const uint16_t* __restrict__ lo, const float* __restrict__ H,
     const float* __restrict__ h_post, uint16_t* __restrict__ out, int8_t* __restrict__ xq, uint8_t* __restrict__ xs,
@@ -123,8 +124,8 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
   const uint16_t* x0 = x + tok * 4 * C;
   const uint16_t* lrow = lo + tok * C;
   uint16_t* o0 = out + tok * 4 * C;
-  int8_t* q0 = xq + tok * 4 * C;
-  uint8_t* s0 = xs + tok * 4 * G;
+  int8_t* q0 = PACKX ? xq + tok * 4 * C : nullptr;
+  uint8_t* s0 = PACKX ? xs + tok * 4 * G : nullptr;
 
   // Lane group g: columns 8 g .. 8 g + 7, of which n are in the row.
   auto round = [&](int g) __attribute__((always_inline)) {
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
       }
     }
 #pragma unroll
-    for (int k = 0; k < 5; ++k) {
+    for (int k = 0; k < (PACKX ? 5 : 1); ++k) {
       uint32_t m = 0u;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -394,6 +395,7 @@ int launch_k4_fwd(const uint16_t* x, const uint16_t* lo, const float* H, const f
 
 int launch_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* hp, uint16_t* out,
                         int8_t* xq, uint8_t* xs, int8_t* lq, uint8_t* ls, int64_t T, int C, hipStream_t s) {
+  // (A null xq counts as aligned.)
   const bool aligned = C % 8 == 0 && aligned16(x) && aligned16(lo) && aligned16(out) && Pack8Src::aligned(xq) &&
                        Pack8Src::aligned(lq);
   const int G = pack_groups(C);
@@ -401,12 +403,16 @@ int launch_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, c
   auto run = [&](auto w, auto few) {
     using Walk = decltype(w);
     constexpr int L = Walk::LPT;
-    for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
-      const dim3 grid(blocks_for(n, tokens_per_block(L)));
-      k4_fwd_pack8_kernel<Walk, decltype(few)::value><<<grid, block_of<L>(), 0, s>>>(
-          x + t * 4 * C, lo + t * C, H + t * 16, hp + t * 4, out + t * 4 * C, xq + t * 4 * C, xs + t * 4 * G,
-          lq + t * C, ls + t * G, n, C);
-    });
+    auto launch = [&](auto packx) {
+      constexpr bool PX = decltype(packx)::value;
+      for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
+        const dim3 grid(blocks_for(n, tokens_per_block(L)));
+        k4_fwd_pack8_kernel<Walk, decltype(few)::value, PX><<<grid, block_of<L>(), 0, s>>>(
+            x + t * 4 * C, lo + t * C, H + t * 16, hp + t * 4, out + t * 4 * C, PX ? xq + t * 4 * C : nullptr,
+            PX ? xs + t * 4 * G : nullptr, lq + t * C, ls + t * G, n, C);
+      });
+    };
+    xq ? launch(std::true_type{}) : launch(std::false_type{});
   };
   if (C < 8)
     run(RowWalk<8, false, false>{}, std::true_type{});
@@ -512,7 +518,7 @@ extern "C" int fmhc_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const fl
   using namespace fmhc;
   if (bad_sizes(T, C, n)) return FMHC_ERR_INVALID_ARGUMENT;
   if (T == 0) return FMHC_OK;
-  if (!x || !lo || !H || !h_post || !out || !x_codes || !x_scales || !lo_codes || !lo_scales)
+  if (!x || !lo || !H || !h_post || !out || !x_codes != !x_scales || !lo_codes || !lo_scales)
     return FMHC_ERR_INVALID_ARGUMENT;
   return launch_k4_fwd_pack8(x, lo, H, h_post, out, x_codes, x_scales, lo_codes, lo_scales, T, static_cast<int>(C),
                              static_cast<hipStream_t>(stream));

@@ -15,11 +15,16 @@ bits that the bf16 backward gives on the unpacked tensors.
                                     the block's two ops (MHCLiteBlock with
                                     ``activation_bits=8``): mhc_pre_map packs x,
                                     and mhc_post_res reads the same codes
+  pre_map_eager, post_res_eager     the block in eager mode: post-res's forward,
+                                    the block's last kernel, packs x and the
+                                    layer output while it has them in registers
 
 No counterpart in the reference, whose backward reads bf16 tensors.
 """
 
 from __future__ import annotations
+
+import weakref
 
 import torch
 import torch.library
@@ -29,7 +34,6 @@ from .ops import (
     _check_k2_shapes,
     _check_n4,
     _coeff,
-    _mhc_post_res_cuda,
     _mhc_pre_map_cuda,
     _mhc_pre_map_fake,
     _params,
@@ -154,9 +158,13 @@ def _fused_rmsnorm_project_bwd_pack8_cuda(grad_out, x_codes, x_scales, W, proj_o
 
 @torch.library.impl(_lib, "mhc_pre_map_pack8", "CUDA")
 def _mhc_pre_map_pack8_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat):
+    _check_n4(x_streams, "flash_mhc::mhc_pre_map_pack8 supports n=4 only")
     x = x_streams.contiguous()
-    outs = _mhc_pre_map_cuda(x, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat)
-    return (*outs, *_k.pack8(x))
+    # A launch of its own: inside K1's kernels, which have two waves per SIMD or
+    # one and all registers in use, the packing took as long as on its own (T =
+    # 65536, C = 1024 135 -> 269 us, alone 132).
+    packed = _k.pack8(x)
+    return (*_mhc_pre_map_cuda(x, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat), *packed)
 
 
 @torch.library.impl(_lib, "mhc_pre_map_backward_pack8", "CUDA")
@@ -197,8 +205,10 @@ def _mhc_pre_map_backward_pack8_cuda(grad_layer_input, grad_H_merged, grad_h_pos
 
 @torch.library.impl(_lib, "mhc_post_res_pack8", "CUDA")
 def _mhc_post_res_pack8_cuda(x_streams, x_sink, x_codes, x_scales, layer_output, H_merged, h_post):
-    lo = layer_output.contiguous()
-    return (_mhc_post_res_cuda(x_streams, x_sink, lo, H_merged, h_post), *_k.pack8(lo))
+    _check_n4(x_streams, "flash_mhc::mhc_post_res_pack8 supports n=4 only")
+    out, _xq, _xs, lo_codes, lo_scales = _k.k4_fwd_pack8(x_streams.contiguous(), layer_output.contiguous(),
+                                                         _coeff(H_merged), _coeff(h_post), pack_x=False)
+    return out, lo_codes, lo_scales
 
 
 # ---------------------------------------------------------------------------
@@ -256,52 +266,88 @@ torch.library.register_autograd("flash_mhc::mhc_post_res_pack8", _mhc_post_res_p
                                 setup_context=_setup_mhc_post_res)
 
 
+class _Kept:
+    """The codes of a block's streams, on their way from post-res, whose forward
+    makes and saves them, to the pre-map's backward, which runs after
+    post-res's."""
+
+    __slots__ = ("version", "post", "codes")
+
+    def __init__(self, version: int):
+        self.version = version  # of the streams when the pre-map read them
+        self.post = None        # weak: post-res's node leads to the pre-map's
+        self.codes = None
+
+    def take(self):
+        """(x_codes, x_scales).  Post-res's backward has left them here; where it
+        was not part of this backward (a loss on the layer's input alone), they
+        are still with post-res's node."""
+        codes, self.codes = self.codes, None
+        if codes is not None:
+            return codes
+        post = self.post() if self.post is not None else None
+        if post is None:
+            raise RuntimeError(
+                "activation_bits=8: the block's output is gone, and its 8-bit activations with it; keep the output "
+                "until its layer input's gradient is taken, or use activation_bits=16")
+        return post.saved_tensors[:2]
+
+
 class _PreMapEager(torch.autograd.Function):
-    """mhc_pre_map_pack8 with its registered autograd, without the op's dispatch
-    (ops._PreMapEager with 8-bit codes).  Returns (layer_input, H_merged,
-    h_post, x_sink, x_codes, x_scales)."""
+    """mhc_pre_map without the op's dispatch (ops._PreMapEager), whose backward
+    reads the streams' codes from `kept`.  Returns (layer_input, H_merged,
+    h_post, x_sink)."""
 
     @staticmethod
-    def forward(ctx, x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat):
-        li, H, hq, h_pre, proj, inv_rms, x_sink, codes, scales = _mhc_pre_map_pack8_cuda(
-            x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat)
-        ctx.save_for_backward(codes, scales, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre, proj, inv_rms)
-        ctx.mark_non_differentiable(codes, scales)
+    def forward(ctx, x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, kept):
+        li, H, hq, h_pre, proj, inv_rms, x_sink = _mhc_pre_map_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res,
+                                                                     bias, perm_mat)
+        ctx.kept = kept
+        ctx.save_for_backward(W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre, proj, inv_rms)
         ctx.set_materialize_grads(False)
-        return li, H, hq, x_sink, codes, scales
+        return li, H, hq, x_sink
 
     @staticmethod
-    def backward(ctx, g_li, g_H, g_hq, g_sink, _gc, _gs):
-        grads = _mhc_pre_map_backward_pack8_cuda(g_li, g_H, g_hq, None, None, g_sink, *ctx.saved_tensors)
-        return (*grads, None)
+    def backward(ctx, g_li, g_H, g_hq, g_sink):
+        saved = ctx.saved_tensors
+        grads = _mhc_pre_map_backward_pack8_cuda(g_li, g_H, g_hq, None, None, g_sink, *ctx.kept.take(), *saved)
+        return (*grads, None, None)
 
 
 class _PostResEager(torch.autograd.Function):
-    """mhc_post_res_pack8 with its registered autograd, without the op's
-    dispatch: x's gradient goes to x_sink."""
+    """mhc_post_res without the op's dispatch, which packs x and the layer output
+    in its own pass (fused_post_res_pack8's kernel): x's gradient goes to x_sink."""
 
     @staticmethod
-    def forward(ctx, x_streams, x_sink, x_codes, x_scales, layer_output, H_merged, h_post):
-        out, lo_codes, lo_scales = _mhc_post_res_pack8_cuda(x_streams, x_sink, x_codes, x_scales, layer_output,
-                                                            H_merged, h_post)
-        ctx.save_for_backward(x_codes, x_scales, lo_codes, lo_scales, H_merged, h_post)
+    def forward(ctx, x_streams, x_sink, layer_output, H_merged, h_post, kept):
+        if x_streams._version != kept.version:
+            raise RuntimeError("the streams were modified by an inplace operation between the block's pre-map and "
+                               "post-res, which both need them")
+        out, *codes = _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post)
+        ctx.kept = kept
+        kept.post = weakref.ref(ctx)
+        ctx.save_for_backward(*codes, H_merged, h_post)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        g_x, g_lo, g_H, g_hp = _fused_post_res_backward_pack8_cuda(grad_out, *ctx.saved_tensors)
-        return None, g_x, None, None, g_lo, g_H, g_hp
+        saved = ctx.saved_tensors
+        ctx.kept.codes = saved[:2]
+        g_x, g_lo, g_H, g_hp = _fused_post_res_backward_pack8_cuda(grad_out, *saved)
+        return None, g_x, g_lo, g_H, g_hp, None
 
 
 def pre_map_eager(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat):
-    """(layer_input, H_merged, h_post, x_sink, x_codes, x_scales) of
-    mhc_pre_map_pack8, recorded for autograd without the op's dispatch."""
-    return _PreMapEager.apply(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat)
+    """(layer_input, H_merged, h_post, x_sink, kept) of mhc_pre_map, recorded for
+    autograd without the op's dispatch; `kept` goes to post_res_eager for the
+    same streams, whose forward packs them for this one's backward."""
+    kept = _Kept(x_streams._version)
+    return (*_PreMapEager.apply(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, kept), kept)
 
 
-def post_res_eager(x_streams, x_sink, x_codes, x_scales, layer_output, H_merged, h_post):
-    """mhc_post_res_pack8's out, recorded for autograd without the op's dispatch."""
-    return _PostResEager.apply(x_streams, x_sink, x_codes, x_scales, layer_output, H_merged, h_post)
+def post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept):
+    """mhc_post_res, recorded for autograd without the op's dispatch, keeping codes."""
+    return _PostResEager.apply(x_streams, x_sink, layer_output, H_merged, h_post, kept)
 
 
 # ---------------------------------------------------------------------------

@@ -330,11 +330,11 @@ class MHCLiteBlock(nn.Module):
         kernels, same values, same x-gradient sink."""
         p = self._parameters
         if self._keeps_codes():
-            layer_input, H_merged, h_post, x_sink, codes, scales = _a8.pre_map_eager(
+            layer_input, H_merged, h_post, x_sink, kept = _a8.pre_map_eager(
                 x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
                 self.W_all.bias, self._buffers["perm_mat"])
             layer_output = self._apply_layer(layer_input, kwargs)
-            return _a8.post_res_eager(x_streams, x_sink, codes, scales, layer_output, H_merged, h_post)
+            return _a8.post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept)
         layer_input, H_merged, h_post, x_sink = _ops.pre_map_eager(
             x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
             self.W_all.bias, self._buffers["perm_mat"])

@@ -600,9 +600,10 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = _BF1
     return x
 
 
-def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: torch.Tensor, h_post: torch.Tensor):
-    """k4_fwd's out with x_streams and layer_output packed in the same pass:
-    (out, x_codes, x_scales, lo_codes, lo_scales)."""
+def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: torch.Tensor, h_post: torch.Tensor,
+                 pack_x: bool = True):
+    """k4_fwd's out with x_streams (unless pack_x is false) and layer_output packed
+    in the same pass: (out, x_codes, x_scales, lo_codes, lo_scales)."""
     dev = _device_of(x_streams)
     T, n, C = _streams_shape(x_streams)
     _require(x_streams, "x_streams", _BF16, (T, n, C), dev)
@@ -610,13 +611,13 @@ def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: 
     _require(H_merged, "H_merged", _F32, (T, n, n), dev)
     _require(h_post, "h_post", _F32, (T, n), dev)
     out = torch.empty_like(x_streams)
-    xq, xs = empty_packed((T, n, C), dev)
+    xq, xs = empty_packed((T, n, C), dev) if pack_x else (None, None)
     lq, ls = empty_packed((T, C), dev)
     lib = _abi.load()
     with _OnDevice(dev):
         st = lib.fmhc_k4_fwd_pack8(x_streams.data_ptr(), layer_output.data_ptr(), H_merged.data_ptr(),
-                                   h_post.data_ptr(), out.data_ptr(), xq.data_ptr(), xs.data_ptr(), lq.data_ptr(),
-                                   ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))
+                                   h_post.data_ptr(), out.data_ptr(), _ptr_or_none(xq), _ptr_or_none(xs),
+                                   lq.data_ptr(), ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))
     _abi.check(st, "k4_fwd_pack8")
     return out, xq, xs, lq, ls
 

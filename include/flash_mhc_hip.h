@@ -266,7 +266,7 @@ int fmhc_unpack8(const int8_t* codes, const uint8_t* scales, void* x, int dtype,
 
 /* fmhc_k4_fwd that also packs x (codes (T, n, C), scales (T, n, G)) and lo
  * (codes (T, C), scales (T, G)) in the same pass.  out has fmhc_k4_fwd's bits,
- * the codes fmhc_pack8's. */
+ * the codes fmhc_pack8's.  x_codes and x_scales may both be NULL: lo only. */
 int fmhc_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* h_post,
                       uint16_t* out, int8_t* x_codes, uint8_t* x_scales, int8_t* lo_codes,
                       uint8_t* lo_scales, int64_t T, int64_t C, int64_t n, void* stream);

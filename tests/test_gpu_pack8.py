@@ -436,12 +436,71 @@ def test_block_under_checkpoint_and_offload():
         out = blk(xs)
     for a, b in zip(torch.autograd.grad(out, [xs, *blk.parameters()], g), want):
         same(a, b)
-    # A second use of the layer input, beside the block's output.
-    aux = {}
-    blk.layer.register_forward_hook(lambda m, i, o: aux.__setitem__("li", i[0]))
+
+
+def test_block_gradients_in_parts():
+    """The pre-map's backward gets the streams' codes from post-res's node,
+    whichever parts of the graph a backward runs."""
+    C, T = 64, 40
+    blk = make_block(C, activation_bits=8)
+    x, g = streams(T, C, 4).to(DEV), rnd((T, 4, C), 5).to(DEV)
+    seen = {}
+    blk.layer.register_forward_hook(lambda m, i, o: seen.__setitem__("li", i[0]))
+    aux = lambda: seen["li"].float().square().sum()
+    xs = x.clone().requires_grad_(True)
+    params = list(blk.parameters())
     out = blk(xs)
-    (gx,) = torch.autograd.grad(aux["li"].float().square().sum(), [xs])
-    assert bool(torch.isfinite(gx).all()) and float(gx.float().abs().sum()) > 0
+    whole = torch.autograd.grad(out, [xs, *params], g, retain_graph=True)
+    both = torch.autograd.grad([out, aux()], [xs], [g, None], retain_graph=True)[0]
+    alone = torch.autograd.grad(aux(), [xs], retain_graph=True)[0]  # a loss on the layer's input
+    again = torch.autograd.grad(out, [xs, *params], g)
+    for a, b in zip(whole, again):
+        same(a, b)
+    # The layer's gradient first, then the rest with another loss.
+    out = blk(xs)
+    at = [n for n, _p in blk.named_parameters()].index("layer.0.weight")
+    same(torch.autograd.grad(out, [params[at]], g)[0], whole[1 + at])
+    same(torch.autograd.grad(aux(), [xs], retain_graph=True)[0], alone)
+    # Against the 16-bit block: codes of x alone come in, a few percent.
+    ref = make_block(C)
+    ref.layer.register_forward_hook(lambda m, i, o: seen.__setitem__("li", i[0]))
+    out16 = ref(xs)
+    for got, want in ((alone, torch.autograd.grad(aux(), [xs], retain_graph=True)[0]),
+                      (both, torch.autograd.grad([out16, aux()], [xs], [g, None])[0])):
+        got, want = got.double(), want.double()
+        assert float((got - want).norm()) <= 0.04 * float(want.norm())
+    # The output and its codes gone: refused, not wrong.
+    out = blk(xs)
+    del out
+    with pytest.raises(RuntimeError, match="keep the output"):
+        torch.autograd.grad(aux(), [xs])
+
+
+def test_block_refuses_changed_streams():
+    C, T = 64, 8
+    blk = make_block(C, activation_bits=8)
+    x = streams(T, C, 4).to(DEV)
+    blk.layer.register_forward_pre_hook(lambda m, i: [x.mul_(2)] and None)
+    with pytest.raises(RuntimeError, match="inplace"):
+        blk(x)
+
+
+def test_block_frozen_parts():
+    """Frozen streams and coefficients, a trained layer; and the reverse."""
+    C, T = 64, 24
+    blk = make_block(C, activation_bits=8)
+    x, g = streams(T, C, 4).to(DEV), rnd((T, 4, C), 5).to(DEV)
+    _out, want = grads(blk, x, g)
+    at = [n for n, _p in blk.named_parameters()].index("layer.0.weight")
+    for p in blk.parameters():
+        p.requires_grad_(False)
+    w = blk.layer[0].weight.requires_grad_(True)
+    blk(x).backward(g)
+    same(w.grad, want[1 + at])
+    w.requires_grad_(False)
+    xs = x.clone().requires_grad_(True)
+    blk(xs).backward(g)
+    same(xs.grad, want[0])
 
 
 def test_block_eval_keeps_nothing():
