@@ -43,8 +43,14 @@ _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
 _lib.define("pack8(Tensor x) -> (Tensor codes, Tensor scales)")
 _lib.define("unpack8(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor")
+# fused_post_res_pack8 in eager mode is an autograd Function around the device
+# implementation (_FusedPostResEager); where it is traced it becomes
+# fused_post_res_pack8_traced, which has its fake and registered autograd.
 _lib.define(
     "fused_post_res_pack8(Tensor x_streams, Tensor layer_output, Tensor H_merged, Tensor h_post) -> (Tensor out, Tensor x_codes, Tensor x_scales, Tensor lo_codes, Tensor lo_scales)"
+)
+_lib.define(
+    "fused_post_res_pack8_traced(Tensor x_streams, Tensor layer_output, Tensor H_merged, Tensor h_post) -> (Tensor out, Tensor x_codes, Tensor x_scales, Tensor lo_codes, Tensor lo_scales)"
 )
 _lib.define(
     "fused_post_res_backward_pack8(Tensor grad_out, Tensor x_codes, Tensor x_scales, Tensor lo_codes, Tensor lo_scales, Tensor H_merged, Tensor h_post) -> (Tensor grad_x, Tensor grad_layer_output, Tensor grad_H_merged, Tensor grad_h_post)"
@@ -85,6 +91,7 @@ def _unpack8_fake(codes, scales, dtype):
     return codes.new_empty(codes.shape, dtype=dtype)
 
 
+@torch.library.register_fake("flash_mhc::fused_post_res_pack8_traced")
 @torch.library.register_fake("flash_mhc::fused_post_res_pack8")
 def _fused_post_res_pack8_fake(x_streams, layer_output, H_merged, h_post):
     return (torch.empty_like(x_streams, memory_format=torch.contiguous_format), *_packed_like(x_streams),
@@ -136,6 +143,7 @@ def _unpack8_cuda(codes, scales, dtype):
     return _k.unpack8(codes.contiguous(), scales.contiguous(), dtype)
 
 
+@torch.library.impl(_lib, "fused_post_res_pack8_traced", "CUDA")
 @torch.library.impl(_lib, "fused_post_res_pack8", "CUDA")
 def _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post):
     _check_n4(x_streams, "flash_mhc::fused_post_res_pack8 supports n=4 only")
@@ -228,8 +236,33 @@ def _fused_post_res_pack8_backward(ctx, grad_out, *_codes):
     return torch.ops.flash_mhc.fused_post_res_backward_pack8(grad_out, *ctx.saved_tensors)
 
 
-torch.library.register_autograd("flash_mhc::fused_post_res_pack8", _fused_post_res_pack8_backward,
+torch.library.register_autograd("flash_mhc::fused_post_res_pack8_traced", _fused_post_res_pack8_backward,
                                 setup_context=_setup_post_res)
+
+
+class _FusedPostResEager(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x_streams, layer_output, H_merged, h_post):
+        outs = _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post)
+        ctx.save_for_backward(*outs[1:], H_merged, h_post)
+        ctx.mark_non_differentiable(*outs[1:])
+        ctx.set_materialize_grads(False)
+        return outs
+
+    @staticmethod
+    def backward(ctx, grad_out, *_codes):
+        if grad_out is None:
+            return None, None, None, None
+        return _fused_post_res_backward_pack8_cuda(grad_out, *ctx.saved_tensors)
+
+
+@torch.library.impl(_lib, "fused_post_res_pack8", "AutogradCUDA")
+def _fused_post_res_pack8_autograd(x_streams, layer_output, H_merged, h_post):
+    from .block import _plain_eager
+
+    if _plain_eager(x_streams):
+        return _FusedPostResEager.apply(x_streams, layer_output, H_merged, h_post)
+    return torch.ops.flash_mhc.fused_post_res_pack8_traced(x_streams, layer_output, H_merged, h_post)
 
 
 def _setup_pre_map(ctx, inputs, output):

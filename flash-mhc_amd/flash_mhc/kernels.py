@@ -769,6 +769,16 @@ def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Te
         raise TypeError(f"param_dtype must be float32 or grad_y's dtype {grad_y.dtype}, got {param_dtype}")
     if weight is not None:
         _require(weight, "weight", param_dtype, (C,), dev)
+    return launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias)
+
+
+def launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias):
+    """layer_norm_bwd for operands that are known to be right: what
+    layer_norm_fwd took and gave, and autograd's gradient of its y, contiguous."""
+    dev = grad_y.device
+    code = DTYPES[grad_y.dtype]
+    C = grad_y.shape[-1]
+    T = grad_y.numel() // C
     gx = torch.empty_like(grad_y)
     gw = torch.empty((C,), device=dev, dtype=param_dtype) if need_weight else None
     gb = torch.empty((C,), device=dev, dtype=param_dtype) if need_bias else None

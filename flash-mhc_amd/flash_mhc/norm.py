@@ -123,8 +123,8 @@ class _LayerNormEager(torch.autograd.Function):
     def backward(ctx, grad_y):
         x, codes, scales, mean, rstd, weight = ctx.saved_tensors
         _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
-        gx, gw, gb = _k.layer_norm_bwd(grad_y.contiguous(), x, codes, scales, mean, rstd, weight, ctx.param_dtype,
-                                       need_weight, need_bias)
+        gx, gw, gb = _k.launch_layer_norm_bwd(grad_y.contiguous(), x, codes, scales, mean, rstd, weight,
+                                              ctx.param_dtype, need_weight, need_bias)
         return gx, gw, gb, None, None
 
 

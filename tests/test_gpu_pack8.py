@@ -522,3 +522,29 @@ def test_block_other_switches(flags, monkeypatch):
     same(out, ref)
     for a, b in zip(got, want):
         assert float((a.double() - b.double()).norm()) <= 0.06 * float(b.double().norm()) + 1e-3
+
+
+def test_post_res_compiled_and_nograd():
+    """The op in a compiled graph, without autograd and in inference mode."""
+    T, C = 33, 96
+    x, lo, H, hp, go = mix_inputs(T, C)
+    leaves = [t.clone().requires_grad_(True) for t in (x, lo, H, hp)]
+    f = lambda x, lo, H, hp: OPS.fused_post_res_pack8(x, lo, H, hp)[0] * 2
+    want = f(*leaves)
+    gw = torch.autograd.grad(want, leaves, go)
+    comp = torch.compile(f, fullgraph=True, backend="aot_eager")
+    out = comp(*leaves)
+    same(out, want)
+    for a, b in zip(torch.autograd.grad(out, leaves, go), gw):
+        same(a, b)
+    with torch.no_grad():
+        for a, b in zip(OPS.fused_post_res_pack8(x, lo, H, hp), OPS.fused_post_res_pack8(*leaves)):
+            same(a, b)
+            assert not a.requires_grad
+    with torch.inference_mode():
+        same(OPS.fused_post_res_pack8(x, lo, H, hp)[0], OPS.fused_post_res(x, lo, H, hp))
+    # Only some gradients asked for; gradients into the codes do not exist.
+    some = [x, lo.clone().requires_grad_(True), H, hp]
+    out, *codes = OPS.fused_post_res_pack8(*some)
+    assert not any(c.requires_grad for c in codes)
+    same(torch.autograd.grad(out, some[1], go)[0], OPS.fused_post_res_backward(go, x, lo, H, hp)[1])
