@@ -727,7 +727,11 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
   const int sj = kStream ? kl / C : 0;
   const int cj = kStream ? kl - sj * C : 0;
   const uint32_t c3bytes = 2u * static_cast<uint32_t>(cj);
-  const int ngroups = SRC::kPacked ? pack_groups(C) : 0;  // scales of a stream's row
+  // 8 bits: scales of a stream's row, the lane's first within a token's four
+  // rows of them, and the step to the one of its last column.
+  const int ngroups = SRC::kPacked ? pack_groups(C) : 0;
+  const uint32_t s0 = static_cast<uint32_t>(sj * ngroups + (cj >> 5));
+  const uint32_t s10 = static_cast<uint32_t>(((cj + 7) >> 5) - (cj >> 5));
   f32x4 dacc[DW ? 8 : 1][2];
 #pragma unroll
   for (int m = 0; m < (DW ? 8 : 1); ++m) dacc[m][0] = dacc[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -773,6 +777,14 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
   auto block_base = [&](int tb) { return (run + static_cast<int64_t>(tb) * nruns) * 16; };
   // Valid rows of the block starting at tbase (16 except in the last block).
   auto block_rows = [&](int64_t tbase) { return static_cast<int>(T - tbase < 16 ? T - tbase : 16); };
+  // Offset of the lane's row q, of `step` elements, in a block whose last row is
+  // `last` (rows past it re-read it): a sum and a minimum, where a product of
+  // the row costs as much as four of either.
+  auto row_off = [&](uint32_t step, int q, int last) {
+    const uint32_t off = static_cast<uint32_t>(4 * grp) * step + static_cast<uint32_t>(q) * step;
+    const uint32_t end = static_cast<uint32_t>(last) * step;
+    return off < end ? off : end;
+  };
   auto load = [&](BwdFrag<EPI, GI, SRC>& f, int tb) {
     const int64_t tbase = block_base(tb);
     const int last = block_rows(tbase) - 1;  // rows past the end re-read the last one
@@ -795,10 +807,12 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
       const int r0 = 4 * grp + q;
       const uint32_t r = static_cast<uint32_t>(r0 < last ? r0 : last);
       if (last != 15) f.inv[q] = *reinterpret_cast<const float*>(ib + 4u * r);
-      const uint8_t* srow = nullptr;
-      if constexpr (SRC::kPacked) srow = xs + (4 * (tbase + r) + sj) * ngroups;
-      const uint32_t xoff = SRC::kPacked ? r * static_cast<uint32_t>(nC) + static_cast<uint32_t>(kl) : r * row_bytes + kbytes;
-      f.xv[q] = SRC::template raw<NT>(xb + xoff, srow, cj);
+      if constexpr (SRC::kPacked)
+        f.xv[q] = SRC::template raw<NT>(xb, row_off(static_cast<uint32_t>(nC), q, last) + static_cast<uint32_t>(kl),
+                                        xs + 4 * tbase * ngroups, row_off(4u * static_cast<uint32_t>(ngroups), q, last) + s0,
+                                        s10);
+      else
+        f.xv[q] = SRC::template raw<NT>(xb + (r * row_bytes + kbytes));
       if constexpr (EPI) {
         const char* g3b = reinterpret_cast<const char*>(go3 + tbase * C);
         f.hp[q] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(h_pre + tbase * 4) + 16u * r +
@@ -1239,6 +1253,9 @@ constexpr int kBwdDwNTB = 64;
 // kernels that read x in 8 bits, whose buffers are smaller but whose VALU work
 // (4 more operations per two elements) one wave per SIMD does not hide: two
 // buffers and two waves T = 16384, C = 4096 172 us, three and one 193, four 202.
+// At two waves it is bound by the memory's mix of reads and twice as many
+// written bytes (805 MB, 4.7 TB/s; the VALU is issued 45% of the time): a third
+// buffer beside two waves 174, loads and stores without a branch 177.
 constexpr int kBwdBufs = 3;
 constexpr int kBwdEpiBufs = 2;
 constexpr int kBwdDwMinNTB = 4;

@@ -162,10 +162,10 @@ struct Bf16Src {
     }
   };
   static bool aligned(const Elem* x) { return aligned16(x); }
-  // Eight columns as loaded; c is the first one's place in its row.
+  // Eight columns as loaded.
   using Raw = u32x4;
   template <bool NT>
-  __device__ static __forceinline__ Raw raw(const char* at, const uint8_t*, int) {
+  __device__ static __forceinline__ Raw raw(const char* at) {
     return Lanes<8, NT>::raw(reinterpret_cast<const uint16_t*>(at), 0);
   }
   // Column k of token t, whose nC columns are streams of C.
@@ -202,9 +202,12 @@ struct Pack8Src {
     u32x2 q;
     uint32_t e0, e1;
   };
+  // From wave-uniform bases: the first column's code at x + off, its scale at
+  // scales + soff, the last one's `step` (0 or 1) behind it.
   template <bool NT>
-  __device__ static __forceinline__ Raw raw(const char* at, const uint8_t* row_scales, int c) {
-    return Raw{ld_codes<NT>(reinterpret_cast<const int8_t*>(at)), row_scales[c >> 5], row_scales[(c + 7) >> 5]};
+  __device__ static __forceinline__ Raw raw(const char* x, uint32_t off, const uint8_t* scales, uint32_t soff,
+                                            uint32_t step) {
+    return Raw{ld_codes<NT>(reinterpret_cast<const int8_t*>(x + off)), scales[soff], scales[soff + step]};
   }
   __device__ static __forceinline__ void widen(const Raw& v, int c, float (&f)[8]) {
     decode8(v.q, pack_unit(v.e0), pack_unit(v.e1), kPackGroup - (c & (kPackGroup - 1)), f);
@@ -223,8 +226,8 @@ struct Pack8WholeSrc : Pack8Src {
     uint32_t e;
   };
   template <bool NT>
-  __device__ static __forceinline__ Raw raw(const char* at, const uint8_t* row_scales, int c) {
-    return Raw{ld_codes<NT>(reinterpret_cast<const int8_t*>(at)), row_scales[c >> 5]};
+  __device__ static __forceinline__ Raw raw(const char* x, uint32_t off, const uint8_t* scales, uint32_t soff, uint32_t) {
+    return Raw{ld_codes<NT>(reinterpret_cast<const int8_t*>(x + off)), scales[soff]};
   }
   __device__ static __forceinline__ void widen(const Raw& v, int, float (&f)[8]) { decode8(v.q, pack_unit(v.e), f); }
 };
