@@ -571,32 +571,42 @@ struct LnWalk {
   static constexpr int LPT = kLpt, R = kR;
 };
 
+// Groups per lane at most with LPT lanes per row, where RMAX fit: five only with
+// up to two waves per row, four always with eight (no more lanes to take).
+template <int RMAX, int LPT>
+constexpr int ln_most_rounds() {
+  return LPT == 512 ? 4 : LPT <= 128 || RMAX < 4 ? RMAX : 4;
+}
+
 // f(LnWalk) for T rows of C columns, 8 or more, held by registers with at most
 // RMAX groups per lane; false where there is no such layout.
 template <int RMAX, typename F>
 bool with_ln_walk(int64_t T, int C, F&& f) {
   if (C < 8) return false;
   const int groups = (C + 7) / 8;
-  auto rounds = [&](auto lpt, int r) {
-    constexpr int L = decltype(lpt)::value;
-    switch (r) {
-      case 1: f(LnWalk<L, 1>{}); return;
-      case 2: f(LnWalk<L, 2>{}); return;
-      case 3: f(LnWalk<L, 3>{}); return;
-      case 4: if constexpr (RMAX >= 4 || L == 512) f(LnWalk<L, 4>{}); return;
-      default: if constexpr (RMAX >= 5 && L <= 128) f(LnWalk<L, 5>{}); return;
+  auto rounds = [&](auto lpt, bool may) {
+    constexpr int L = decltype(lpt)::value, most = ln_most_rounds<RMAX, L>();
+    static_assert(most >= 3 && most <= 5);
+    const int r = (groups + L - 1) / L;
+    if (!may || r > most) return false;
+    if (r == 1) f(LnWalk<L, 1>{});
+    else if (r == 2) f(LnWalk<L, 2>{});
+    else if (r == 3) f(LnWalk<L, 3>{});
+    else if constexpr (most >= 4) {
+      if (r == 4) f(LnWalk<L, 4>{});
+      else if constexpr (most >= 5) f(LnWalk<L, 5>{});
     }
+    return true;
   };
   using std::integral_constant;
   if (groups <= 8) f(LnWalk<8, 1>{});
   else if (groups <= 16) f(LnWalk<16, 1>{});
   else if (groups <= 32) f(LnWalk<32, 1>{});
   else if (groups <= 64) f(LnWalk<64, 1>{});
-  else if (groups <= 64 * RMAX && (groups <= 128 || T >= 1024)) rounds(integral_constant<int, 64>{}, (groups + 63) / 64);
-  else if (groups <= 128 * RMAX && (groups <= 256 || T >= 8192)) rounds(integral_constant<int, 128>{}, (groups + 127) / 128);
-  else if (groups <= 256 * RMAX && (groups <= 512 || T >= 512)) rounds(integral_constant<int, 256>{}, (groups + 255) / 256);
-  else if (groups <= 512 * 4) rounds(integral_constant<int, 512>{}, (groups + 511) / 512);
-  else return false;
+  else return rounds(integral_constant<int, 64>{}, groups <= 128 || T >= 1024) ||
+              rounds(integral_constant<int, 128>{}, groups <= 256 || T >= 8192) ||
+              rounds(integral_constant<int, 256>{}, groups <= 512 || T >= 512) ||
+              rounds(integral_constant<int, 512>{}, true);
   return true;
 }
 

@@ -273,3 +273,21 @@ def test_module():
     xe = x.clone().requires_grad_(True)
     flash_mhc.LayerNorm(96).to(DEV)(xe).square().sum().backward()
     assert torch.equal(xs.grad, xe.grad)
+
+
+# Every way to lay rows over lanes: the lanes per row depend on the columns and
+# the rows.  Memory that held NaN shows a row that is not written.
+@pytest.mark.parametrize("T,C", [(4, 8193), (4, 10240), (520, 4100), (520, 8192), (520, 8200), (520, 10240), (520, 10250),
+                                 (520, 16384), (1030, 1030), (1030, 1544), (1030, 2560), (1030, 2568), (8200, 1540),
+                                 (8200, 2564), (8200, 4104)])
+def test_layouts(T, C):
+    x, w, b, g = inputs(T, C, BF16, F32)
+    held = [torch.full((T, C), float("nan"), dtype=BF16, device=DEV) for _ in range(8)]
+    del held
+    verify(x, w, b, g, 16 if T > 8000 else 8)
+
+
+@pytest.mark.parametrize("T", [3, 530, 1030])
+def test_layouts_fp32(T):
+    for C in (1536, 1544, 6000, 8200) if T < 1000 else (1544,):
+        verify(*inputs(T, C, F32, F32), 16)
