@@ -28,6 +28,7 @@ import weakref
 
 import torch
 import torch.library
+from torch.autograd.function import once_differentiable
 
 from . import kernels as _k
 from .ops import (
@@ -250,6 +251,7 @@ class _FusedPostResEager(torch.autograd.Function):
         return outs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out, *_codes):
         if grad_out is None:
             return None, None, None, None
@@ -341,6 +343,7 @@ class _PreMapEager(torch.autograd.Function):
         return li, H, hq, x_sink
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g_li, g_H, g_hq, g_sink):
         saved = ctx.saved_tensors
         grads = _mhc_pre_map_backward_pack8_cuda(g_li, g_H, g_hq, None, None, g_sink, *ctx.kept.take(), *saved)
@@ -363,6 +366,7 @@ class _PostResEager(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         saved = ctx.saved_tensors
         ctx.kept.codes = saved[:2]

@@ -14,6 +14,7 @@ import torch
 import torch.library
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import kernels as _k
 from .activation8 import _packed_like
@@ -120,6 +121,7 @@ class _LayerNormEager(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_y):
         x, codes, scales, mean, rstd, weight = ctx.saved_tensors
         _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
@@ -146,7 +148,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     or of x's dtype.  Statistics and sums are fp32, y and every gradient are
     rounded once.  activation_bits: 16 keeps x for the backward, 8 its 8-bit
     codes (the backward's normalised input is then that of the codes, with the
-    statistics of x)."""
+    statistics of x).  Differentiable once: a gradient of its gradients raises."""
     _check(x, weight, bias, activation_bits)
     packed = activation_bits == 8
     if _plain_eager(x):

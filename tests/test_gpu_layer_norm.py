@@ -291,3 +291,47 @@ def test_layouts(T, C):
 def test_layouts_fp32(T):
     for C in (1536, 1544, 6000, 8200) if T < 1000 else (1544,):
         verify(*inputs(T, C, F32, F32), 16)
+
+
+def test_opcheck():
+    x, w, b, g = inputs(7, 72, BF16, F32)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y, mean, rstd, q, s = torch.ops.flash_mhc.layer_norm_pack8(x, w, b, EPS)
+    check = torch.library.opcheck
+    check(torch.ops.flash_mhc.layer_norm, (*leaves, EPS))
+    check(torch.ops.flash_mhc.layer_norm, (leaves[0], None, None, EPS))
+    check(torch.ops.flash_mhc.layer_norm_pack8, (*leaves, EPS))
+    check(torch.ops.flash_mhc.layer_norm_backward, (g, x, None, None, mean, rstd, w, F32, True, True))
+    check(torch.ops.flash_mhc.layer_norm_backward, (g, None, q, s, mean, rstd, w, F32, True, False))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_differentiable_once(bits):
+    x, w, b, _g = inputs(5, 48, F32, F32)
+    x.requires_grad_(True)
+    (gx,) = torch.autograd.grad(flash_mhc.layer_norm(x, w, b, activation_bits=bits).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gx.square().sum().backward()
+
+
+@pytest.mark.parametrize("C", [2048, 2051])
+def test_past_32_bits(C):
+    """Over 2^32 elements: 2100 copies of the same rows have the same results.  (One
+    copy alone is summed in another order: fewer rows take more lanes each.)"""
+    n, reps = 1000, 2100
+    T = n * reps
+    assert T * C > 1 << 32
+    x, w, b, g = inputs(n, C, BF16, BF16)
+    t, d = x.repeat(reps, 1), g.repeat(reps, 1)
+    y, mean, rstd, q, s = torch.ops.flash_mhc.layer_norm_pack8(t, w, b, EPS)
+    bwd = torch.ops.flash_mhc.layer_norm_backward
+    gx = bwd(d, t, None, None, mean, rstd, w, BF16, True, True)[0]
+    gx8 = bwd(d, None, q, s, mean, rstd, w, BF16, False, False)[0]
+    for o in (y, mean, rstd, q, s, gx, gx8):
+        for k in (reps // 2, reps - 1):
+            assert torch.equal(o[k * n:(k + 1) * n], o[:n])
+    A.check("y", y[:n], *A.ln_fwd(x, w, b, EPS))
+    A.check("grad_x", gx[:n], *A.ln_bwd(g, x, x, w, EPS)["x"])
+    A.check("grad_x of 8 bits", gx8[:n], *A.ln_bwd(g, x, A.unpack8(*A.pack8(x)), w, EPS)["x"])
+    del t, d, y, mean, rstd, q, s, gx, gx8, o
+    torch.cuda.empty_cache()

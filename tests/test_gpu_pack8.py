@@ -548,3 +548,89 @@ def test_post_res_compiled_and_nograd():
     out, *codes = OPS.fused_post_res_pack8(*some)
     assert not any(c.requires_grad for c in codes)
     same(torch.autograd.grad(out, some[1], go)[0], OPS.fused_post_res_backward(go, x, lo, H, hp)[1])
+
+
+def test_opcheck():
+    """Schemas, fakes, autograd registration and tracing of the ops."""
+    T, C = 5, 40
+    x, lo, H, hp, go = mix_inputs(T, C)
+    q, s = flash_mhc.pack8(x)
+    lq, ls = flash_mhc.pack8(lo)
+    xx, args, li, hpre, proj, inv = premap_state(T, C)
+    xq, xs = flash_mhc.pack8(xx)
+    grad = lambda *ts: [t.clone().requires_grad_(True) for t in ts]
+    check = torch.library.opcheck
+    check(OPS.pack8, (x,))
+    check(OPS.unpack8, (q, s, BF16))
+    check(OPS.fused_post_res_pack8, (x, lo, H, hp))
+    check(OPS.fused_post_res_pack8_traced, tuple(grad(x, lo, H, hp)))
+    check(OPS.fused_post_res_backward_pack8, (go, q, s, lq, ls, H, hp))
+    check(OPS.fused_rmsnorm_project_bwd_pack8, (proj, xq, xs, args[0], proj, inv))
+    check(OPS.mhc_pre_map_pack8, (*grad(xx, *args[:-1]), args[-1]), test_utils=("test_schema", "test_faketensor"))
+    check(OPS.mhc_pre_map_backward_pack8, (li, None, None, None, None, None, xq, xs, *args, hpre, proj, inv))
+    check(OPS.mhc_post_res_pack8, (x, torch.empty_like(x), q, s, lo, H, hp))
+
+
+def premap_state(T, C):
+    """x, mhc_pre_map's other arguments, and some of its outputs."""
+    blk = make_block(C)
+    x = streams(T, C, 5).to(DEV)
+    args = (*(p.detach() for p in (blk.W_all.weight, blk.alpha_pre, blk.alpha_post, blk.alpha_res, blk.W_all.bias)),
+            blk.perm_mat)
+    li, _H, _hq, hpre, proj, inv, _sink = OPS.mhc_pre_map(x, *args)
+    return x, args, li, hpre, proj, inv
+
+
+@pytest.mark.parametrize("kw", [{}, {"pre_norm": True}])
+def test_block_differentiable_once(kw):
+    blk = make_block(64, activation_bits=8, **kw)
+    x = streams(6, 64, 3).to(DEV).requires_grad_(True)
+    (gx,) = torch.autograd.grad(blk(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gx.float().square().sum().backward()
+
+
+@pytest.mark.parametrize("C", [2048, 2051])
+def test_past_32_bits(C):
+    """Over 2^32 elements: 530 copies of the same tokens have the same results."""
+    n, reps = 1000, 530
+    T = n * reps
+    assert T * 4 * C > 1 << 32
+    x, lo, H, hp, go = mix_inputs(n, C)
+    xx, args, li, hpre, proj, inv = premap_state(n, C)
+    many = lambda t: t.repeat(reps, *[1] * (t.dim() - 1))
+    parts = [slice(0, n), slice((reps // 2) * n, (reps // 2 + 1) * n), slice(T - n, T)]
+
+    def compare(outs, want):
+        for o, w in zip(outs, want):
+            for p in parts:
+                same(o[p], w)
+
+    big = many(x)
+    codes = flash_mhc.pack8(big)
+    want = flash_mhc.pack8(x)
+    compare(codes, want)
+    back = flash_mhc.unpack8(*codes)
+    compare([back], [flash_mhc.unpack8(*want)])
+    del back, codes
+    rest = [many(t) for t in (lo, H, hp)]
+    outs = OPS.fused_post_res_pack8(big, *rest)
+    want = OPS.fused_post_res_pack8(x, lo, H, hp)
+    compare(outs, want)
+    del big
+    rest, outs = rest[1:], outs[1:]
+    big = many(go)
+    got = OPS.fused_post_res_backward_pack8(big, *outs, *rest)
+    compare(got, OPS.fused_post_res_backward_pack8(go, *want[1:], H, hp))
+    del got, big
+    xq, xs = flash_mhc.pack8(xx)
+    got = OPS.fused_rmsnorm_project_bwd_pack8(many(proj), many(xq), many(xs), args[0], many(proj), many(inv))
+    want = OPS.fused_rmsnorm_project_bwd_pack8(proj, xq, xs, args[0], proj, inv)
+    compare(got[:1], want[:1])
+    del got
+    got = OPS.mhc_pre_map_backward_pack8(many(li), None, None, None, None, None, many(xq), many(xs), *args, many(hpre),
+                                         many(proj), many(inv))
+    want = OPS.mhc_pre_map_backward_pack8(li, None, None, None, None, None, xq, xs, *args, hpre, proj, inv)
+    compare(got[:1], want[:1])
+    del got
+    torch.cuda.empty_cache()
