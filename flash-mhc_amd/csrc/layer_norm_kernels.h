@@ -722,7 +722,11 @@ int ln_fwd_run(const LnFwdArgs& a, hipStream_t s) {
       constexpr bool NT = decltype(ntc)::value, KEEP = decltype(keep)::value;
       auto* kernel = &ln_fwd_kernel<DT, LPT, R, NT, KEEP>;
       const int64_t want = (a.T + BLOCK / LPT - 1) / (BLOCK / LPT);
-      const int64_t most = 256 * 8;
+      // Eight workgroups per CU; with rows of up to one wave of 16-bit elements more,
+      // from four rows per slot on (T = 262144, C = 1024 202 -> 174 us, T = 65536,
+      // C = 2048 94 -> 90; at two rows per slot T = 30011, C = 2560 54 -> 69; C = 1024
+      // in fp32 98 -> 100, C = 8192 packed 61 -> 64).
+      const int64_t deep = LPT <= kWave && DT != FMHC_DTYPE_F32 ? want / 4 : 0, most = deep > 256 * 8 ? deep : 256 * 8;
       kernel<<<dim3(static_cast<unsigned>(want < most ? want : most)), BLOCK, 0, s>>>(x, a.P, y, a.mean, a.rstd, a.codes,
                                                                                     a.scales, a.T, a.C, a.eps);
     };
