@@ -7,8 +7,8 @@
 namespace fmhc {
 
 // load8 / store8: 8 consecutive elements at any address that is a multiple of
-// the element's size, with the nontemporal hint or not; load / store: one.
-// Stores round to nearest even.
+// the element's size, with the nontemporal hint or not; load / store: one;
+// rounded: what a store leaves.  Stores round to nearest even.
 template <int DT>
 struct Elems;
 
@@ -25,6 +25,7 @@ struct Elems<FMHC_DTYPE_BF16> {
   }
   __device__ static __forceinline__ float load(const S* p) { return bf16_to_f32(*p); }
   __device__ static __forceinline__ void store(S* p, float v) { *p = f32_to_bf16(v); }
+  __device__ static __forceinline__ float rounded(float v) { return bf16_to_f32(f32_to_bf16(v)); }
 };
 
 template <>
@@ -54,6 +55,7 @@ struct Elems<FMHC_DTYPE_F16> {
   }
   __device__ static __forceinline__ float load(const S* p) { return widen(*p); }
   __device__ static __forceinline__ void store(S* p, float v) { *p = narrow(v); }
+  __device__ static __forceinline__ float rounded(float v) { return widen(narrow(v)); }
 };
 
 template <>
@@ -82,6 +84,7 @@ struct Elems<FMHC_DTYPE_F32> {
   }
   __device__ static __forceinline__ float load(const S* p) { return *p; }
   __device__ static __forceinline__ void store(S* p, float v) { *p = v; }
+  __device__ static __forceinline__ float rounded(float v) { return v; }
 };
 
 // f(integral_constant of the type), or FMHC_ERR_INVALID_ARGUMENT.

@@ -38,6 +38,7 @@ struct LnBwdArgs {
   const float* mean;
   const float* rstd;
   LnParams P;            // b unused
+  const void* gi;        // a gradient of x from elsewhere, added to gx; may be null
   void* gx;
   float* partial;        // null: no parameter gradients
   void* gw;              // may be null

@@ -4,7 +4,7 @@
 //   forward   mean = sum_c x / C,  rstd = rsqrt(sum_c (x - mean)^2 / C + eps)
 //             y = h w + b,  h = (x - mean) rstd
 //   backward  g = gy w,  h = (x' - mean) rstd   (x' is x, or what its codes stand for)
-//             grad_x = rstd (g - sum_c g / C - h sum_c g h / C)
+//             grad_x = rstd (g - sum_c g / C - h sum_c g h / C)   (+ x's gradient from elsewhere)
 //             grad_w = sum_t gy h,  grad_b = sum_t gy
 //
 // Everything is fp32 but the stored tensors, each rounded once.  The variance is
@@ -68,11 +68,13 @@ extern "C" int64_t fmhc_layer_norm_bwd_workspace_bytes(int64_t T, int64_t C) {
 }
 
 extern "C" int fmhc_layer_norm_bwd(const void* grad_y, const void* x, const int8_t* x_codes, const uint8_t* x_scales,
-                                   const float* mean, const float* rstd, const void* weight, void* grad_x,
-                                   void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
-                                   int dtype, int param_dtype, int64_t T, int64_t C, void* stream) {
+                                   const float* mean, const float* rstd, const void* weight,
+                                   const void* grad_x_in, void* grad_x, void* grad_weight, void* grad_bias,
+                                   void* workspace, int64_t workspace_bytes, int dtype, int param_dtype, int64_t T,
+                                   int64_t C, void* stream) {
   using namespace fmhc;
-  if (bad_sizes(T, C) || bad_types(dtype, param_dtype) || !x_codes != !x_scales || (x && x_codes))
+  if (bad_sizes(T, C) || bad_types(dtype, param_dtype) || !x_codes != !x_scales || (x && x_codes) ||
+      (grad_x_in && grad_x_in == grad_x))
     return FMHC_ERR_INVALID_ARGUMENT;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool f32 = param_dtype == FMHC_DTYPE_F32;
@@ -86,7 +88,7 @@ extern "C" int fmhc_layer_norm_bwd(const void* grad_y, const void* x, const int8
   const bool params = grad_weight || grad_bias;
   if (params && (!workspace || workspace_bytes < ln_workspace(T, C) || !aligned16(workspace)))
     return FMHC_ERR_INVALID_ARGUMENT;
-  const LnBwdArgs a{grad_y, x,      x_codes, x_scales, mean, rstd, LnParams{weight, nullptr, f32}, grad_x,
+  const LnBwdArgs a{grad_y, x,      x_codes, x_scales, mean, rstd, LnParams{weight, nullptr, f32}, grad_x_in, grad_x,
                     params ? static_cast<float*>(workspace) : nullptr, grad_weight, grad_bias, T, static_cast<int>(C)};
   return with_dtype(dtype, [&](auto dt) { return ln_bwd_run<decltype(dt)::value>(a, s); });
 }

@@ -250,12 +250,22 @@ __global__ __launch_bounds__(ln_fwd_block<LPT>()) void ln_fwd_kernel(
   }
 }
 
+// The residual around a norm gives x a second gradient.  With GI it is added here,
+// to the rounded one, as adding the two tensors would: that pass reads both and
+// writes their sum, here one is read (MHCLiteBlock with pre_norm).
+template <int DT, int N>
+__device__ __forceinline__ void ln_add_grad(const float (&gi)[N], float (&o)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) o[e] = gi[e] + Elems<DT>::rounded(o[e]);
+}
+
 // partial (may be null): this workgroup's sums, [2][ln_cols(C)]: grad_w, grad_b.
-template <int DT, int LPT, int R, bool NT, bool KEPT>
+template <int DT, int LPT, int R, bool NT, bool KEPT, bool GI>
 __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
     const typename Elems<DT>::S* __restrict__ gy, const typename LnX<DT, KEPT>::Elem* __restrict__ x,
     const uint8_t* __restrict__ scales, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
-    const LnParams P, typename Elems<DT>::S* __restrict__ gx, float* __restrict__ partial, int64_t T, int C) {
+    const LnParams P, const typename Elems<DT>::S* __restrict__ gi, typename Elems<DT>::S* __restrict__ gx,
+    float* __restrict__ partial, int64_t T, int C) {
   constexpr int BLOCK = kLnBwdBlock, SLOTS = BLOCK / LPT;
   __shared__ float red[2][BLOCK / kWave][2];
   LnSums<LPT, BLOCK, 2> row_sums{red};
@@ -277,6 +287,7 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
   const int64_t first = static_cast<int64_t>(blockIdx.x) * SLOTS;
   LnRaw<DT> rg[R];
   LnX<DT, KEPT> rx[R];
+  LnRaw<DT> ri[GI ? R : 1];
   float mean_n, rstd_n;
   auto load = [&](int64_t tt) {
     const int64_t t = tt < T ? tt : T - 1;
@@ -293,6 +304,7 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
       } else {
         rx[k].r = ln_load<DT, NT>(xrow + at[k].c);
       }
+      if constexpr (GI) ri[k] = ln_load<DT, NT>(gi + t * C + at[k].c);
     }
     mean_n = mean_in[t];
     rstd_n = rstd_in[t];
@@ -306,10 +318,12 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
     constexpr bool HOLD = R <= 3;
     LnRaw<DT> cg[R];
     LnX<DT, KEPT> cx[R];
+    LnRaw<DT> ci[GI ? R : 1];
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       cg[k] = rg[k];
       cx[k] = rx[k];
+      if constexpr (GI) ci[k] = ri[k];
     }
     if (t0 + step < T) load(t + step);
     __builtin_amdgcn_sched_barrier(0);
@@ -364,6 +378,11 @@ __global__ __launch_bounds__(kLnBwdBlock) void ln_bwd_kernel(
           o[e] = __builtin_fmaf(-hk[e], k2, __builtin_fmaf(qk[e] * w[k][e], rstd, -k1));
           dw[k][e] = __builtin_fmaf(qk[e], hk[e], dw[k][e]);
           db[k][e] += qk[e];
+        }
+        if constexpr (GI) {
+          float f[8];
+          ln_unpack<DT>(ci[k], f);
+          ln_add_grad<DT>(f, o);
         }
         if (k < R - 1 || at[k].skip < 8) Elems<DT>::template store8<NT>(out + at[k].c, o);
       }
@@ -541,6 +560,7 @@ __global__ __launch_bounds__(ln_any_block<N>()) void ln_bwd_any(const typename E
                                                           const uint8_t* __restrict__ scales,
                                                           const float* __restrict__ mean_in,
                                                           const float* __restrict__ rstd_in, const LnParams P,
+                                                          const typename Elems<DT>::S* __restrict__ gi,
                                                           typename Elems<DT>::S* __restrict__ gx, int64_t T, int C) {
   __shared__ float red[ln_any_block<N>() / kWave];
   const int lane = static_cast<int>(threadIdx.x);
@@ -575,6 +595,10 @@ __global__ __launch_bounds__(ln_any_block<N>()) void ln_bwd_any(const typename E
       load(p);
 #pragma unroll
       for (int e = 0; e < N; ++e) g[e] = rstd * (g[e] - c1 - h[e] * c2);
+      if (gi) {
+        ln_any_load<DT>(gi + t * C + p.c, h);
+        ln_add_grad<DT>(h, g);
+      }
       ln_any_store<DT>(gx + t * C + p.c, g);
     }
   }
@@ -749,6 +773,7 @@ template <int DT>
 int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
   using S = typename Elems<DT>::S;
   const auto* gy = static_cast<const S*>(a.gy);
+  const auto* gi = static_cast<const S*>(a.gi);
   auto* gx = static_cast<S*>(a.gx);
   const int64_t cols = ln_cols(a.C);
   int64_t parts = 0;
@@ -760,25 +785,27 @@ int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
       x = a.codes;
     else
       x = static_cast<const X*>(a.x);
-    const bool nt = a.C % 8 == 0 && aligned16(gy) && aligned16(gx) &&
+    const bool nt = a.C % 8 == 0 && aligned16(gy) && aligned16(gx) && aligned16(gi) &&
                     (reinterpret_cast<uintptr_t>(x) & (KEPT ? 7u : 15u)) == 0;
     const bool held = with_ln_walk<3>(a.T, a.C, [&](auto walk) {
       constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, SLOTS = kLnBwdBlock / LPT;
       const int64_t want = (a.T + SLOTS - 1) / SLOTS;
       const int64_t most = R == 1 ? kLnParts : kLnParts / 2;
       parts = want < most ? want : most;
-      auto launch = [&](auto ntc) {
-        ln_bwd_kernel<DT, LPT, R, decltype(ntc)::value, KEPT><<<dim3(static_cast<unsigned>(parts)), kLnBwdBlock, 0, s>>>(
-            gy, x, a.scales, a.mean, a.rstd, a.P, gx, a.partial, a.T, a.C);
+      auto launch = [&](auto ntc, auto add) {
+        ln_bwd_kernel<DT, LPT, R, decltype(ntc)::value, KEPT, decltype(add)::value>
+            <<<dim3(static_cast<unsigned>(parts)), kLnBwdBlock, 0, s>>>(gy, x, a.scales, a.mean, a.rstd, a.P, gi, gx,
+                                                                        a.partial, a.T, a.C);
       };
-      nt ? launch(std::true_type{}) : launch(std::false_type{});
+      auto pick = [&](auto ntc) { gi ? launch(ntc, std::true_type{}) : launch(ntc, std::false_type{}); };
+      nt ? pick(std::true_type{}) : pick(std::false_type{});
     });
     if (!held) {
       auto any = [&](auto n) {
         constexpr int N = decltype(n)::value;
         const int64_t most = 16384;
         ln_bwd_any<DT, KEPT, N><<<dim3(static_cast<unsigned>(a.T < most ? a.T : most)), ln_any_block<N>(), 0, s>>>(
-            gy, x, a.scales, a.mean, a.rstd, a.P, gx, a.T, a.C);
+            gy, x, a.scales, a.mean, a.rstd, a.P, gi, gx, a.T, a.C);
         if (!a.partial) return;
         // Four workgroups per CU: each writes sums of all its columns.
         const unsigned blocks = blocks_for(a.C, kLnColumnsBlock * N);

@@ -53,7 +53,7 @@ SIGNATURES: dict[str, list] = {
     "fmhc_k1_bwd_pack8_workspace_bytes": [_I64, _I64],
     "fmhc_premap_bwd_pack8": [_P] * 8 + [_INT] + [_P] * 14 + [_I64, _I64, _I64, _I64, _P],
     "fmhc_layer_norm_fwd": [_P] * 8 + [_INT, _INT, _I64, _I64, _F32, _P],
-    "fmhc_layer_norm_bwd": [_P] * 11 + [_I64, _INT, _INT, _I64, _I64, _P],
+    "fmhc_layer_norm_bwd": [_P] * 12 + [_I64, _INT, _INT, _I64, _I64, _P],
     "fmhc_layer_norm_bwd_workspace_bytes": [_I64, _I64],
     "fmhc_error_string": [ctypes.c_int],
     "fmhc_abi_version": [],

@@ -176,7 +176,11 @@ class MHCLiteBlock(nn.Module):
         """The layer, with pre_norm around it: u + F(norm(u))."""
         if self.norm is None:
             return self.layer(layer_input, **kwargs)
-        return layer_input + self.layer(self.norm(layer_input), **kwargs)
+        with_residual = getattr(self.norm, "with_residual", None)
+        if with_residual is None:  # another module put in the norm's place
+            return layer_input + self.layer(self.norm(layer_input), **kwargs)
+        normed, residual = with_residual(layer_input)
+        return residual + self.layer(normed, **kwargs)
 
     def _coefficients(
         self, proj: torch.Tensor, dt: torch.dtype

@@ -750,9 +750,11 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
 
 def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Tensor | None,
                    scales: torch.Tensor | None, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None,
-                   param_dtype: torch.dtype, need_weight: bool = True, need_bias: bool = True):
+                   param_dtype: torch.dtype, need_weight: bool = True, need_bias: bool = True,
+                   grad_x_in: torch.Tensor | None = None):
     """(grad_x, grad_weight, grad_bias) of layer_norm_fwd, from x or from its codes
-    and scales; a parameter's gradient is in param_dtype, None where not needed."""
+    and scales; a parameter's gradient is in param_dtype, None where not needed.
+    grad_x_in: a gradient of x from elsewhere, added to grad_x."""
     dev = _device_of(grad_y)
     code = _dtype_code(grad_y.dtype, "grad_y")
     T, C = _rows(grad_y.shape)
@@ -769,12 +771,16 @@ def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Te
         raise TypeError(f"param_dtype must be float32 or grad_y's dtype {grad_y.dtype}, got {param_dtype}")
     if weight is not None:
         _require(weight, "weight", param_dtype, (C,), dev)
-    return launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias)
+    if grad_x_in is not None:
+        _require(grad_x_in, "grad_x_in", grad_y.dtype, grad_y.shape, dev)
+    return launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias,
+                                 grad_x_in)
 
 
-def launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias):
+def launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias,
+                          grad_x_in=None):
     """layer_norm_bwd for operands that are known to be right: what
-    layer_norm_fwd took and gave, and autograd's gradient of its y, contiguous."""
+    layer_norm_fwd took and gave, and autograd's gradients, contiguous."""
     dev = grad_y.device
     code = DTYPES[grad_y.dtype]
     C = grad_y.shape[-1]
@@ -786,7 +792,7 @@ def launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dt
     ws = _workspace(int(lib.fmhc_layer_norm_bwd_workspace_bytes(T, C)), dev) if need_weight or need_bias else None
     with _OnDevice(dev):
         st = lib.fmhc_layer_norm_bwd(grad_y.data_ptr(), _ptr_or_none(x), _ptr_or_none(codes), _ptr_or_none(scales),
-                                     mean.data_ptr(), rstd.data_ptr(), _ptr_or_none(weight), gx.data_ptr(),
+                                     mean.data_ptr(), rstd.data_ptr(), _ptr_or_none(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
                                      _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws),
                                      0 if ws is None else ws.numel(), code, DTYPES[param_dtype], T, C,
                                      _abi.stream_of(grad_y))

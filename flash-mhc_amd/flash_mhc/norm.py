@@ -22,6 +22,10 @@ from .block import _plain_eager
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
+# Whether hooks for all modules are registered (a private name: without it, modules
+# count as hooked).
+_any_global_hook = getattr(torch.nn.modules.module, "_has_any_global_hook", None)
+
 _lib.define("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor y, Tensor mean, Tensor rstd)")
 _lib.define(
     "layer_norm_pack8(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor y, Tensor mean, Tensor rstd, Tensor x_codes, Tensor x_scales)"
@@ -130,6 +134,27 @@ class _LayerNormEager(torch.autograd.Function):
         return gx, gw, gb, None, None
 
 
+class _LayerNormResidualEager(torch.autograd.Function):
+    """(layer_norm(x), x): the gradient of the second, which the residual around a
+    block's layer gives, is added in the norm's backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, packed):
+        ctx.set_materialize_grads(False)
+        return _LayerNormEager.forward(ctx, x, weight, bias, eps, packed), x.view_as(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, grad_skip):
+        if grad_y is None:  # the norm's output was not used
+            return grad_skip, None, None, None, None
+        x, codes, scales, mean, rstd, weight = ctx.saved_tensors
+        _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
+        gx, gw, gb = _k.launch_layer_norm_bwd(grad_y.contiguous(), x, codes, scales, mean, rstd, weight,
+                                              ctx.param_dtype, need_weight, need_bias, _dense(grad_skip))
+        return gx, gw, gb, None, None
+
+
 def _check(x, weight, bias, activation_bits) -> None:
     if activation_bits not in (8, 16):
         raise ValueError(f"activation_bits must be 16 (keep the input as it is) or 8, got {activation_bits}")
@@ -186,12 +211,29 @@ class LayerNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(hidden_size, **kw)) if elementwise_affine else None
         self.bias = nn.Parameter(torch.zeros(hidden_size, **kw)) if elementwise_affine and bias else None
 
+    def _on_kernels(self, x: torch.Tensor) -> bool:
+        pdt = _param_dtype(self.weight, self.bias)
+        return x.is_cuda and x.dtype in _k.DTYPES and (pdt is torch.float32 or pdt is x.dtype)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        w, b = self.weight, self.bias
-        pdt = _param_dtype(w, b)
-        if x.is_cuda and x.dtype in _k.DTYPES and (pdt is torch.float32 or pdt is x.dtype):
-            return layer_norm(x, w, b, self.eps, self.activation_bits)
-        return F.layer_norm(x, (self.hidden_size,), w, b, self.eps)
+        if self._on_kernels(x):
+            return layer_norm(x, self.weight, self.bias, self.eps, self.activation_bits)
+        return F.layer_norm(x, (self.hidden_size,), self.weight, self.bias, self.eps)
+
+    def _hooked(self) -> bool:
+        """A call of this module does more than forward."""
+        return (_any_global_hook is None or _any_global_hook() or type(self).forward is not LayerNorm.forward
+                or bool(self._forward_hooks or self._forward_pre_hooks or self._backward_hooks
+                        or self._backward_pre_hooks))
+
+    def with_residual(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(norm(x), x) for ``x + layer(norm(x))``: the norm's backward adds the
+        gradient that x gets from the residual (as a separate addition would)."""
+        if (torch.is_grad_enabled() and x.requires_grad and not self._hooked() and _plain_eager(x)
+                and self._on_kernels(x)):
+            _check(x, self.weight, self.bias, self.activation_bits)
+            return _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
+        return self(x), x
 
     def extra_repr(self) -> str:
         return f"{self.hidden_size}, eps={self.eps}, activation_bits={self.activation_bits}"

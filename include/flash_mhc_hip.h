@@ -316,14 +316,16 @@ int fmhc_layer_norm_fwd(const void* x, const void* weight, const void* bias, voi
  * h = (x - mean) rstd, g = grad_y weight:
  *   grad_x[t,c]    = rstd[t] (g[t,c] - sum_c g / C - h[t,c] sum_c g h / C)
  *   grad_weight[c] = sum_t grad_y[t,c] h[t,c],  grad_bias[c] = sum_t grad_y[t,c]
+ * grad_x_in (may be NULL, not grad_x): a gradient of x from elsewhere, added to
+ * the rounded grad_x (grad_x = round(grad_x_in + round(that above))).
  * grad_weight and grad_bias, in param_dtype, may be NULL; with either,
  * `workspace` has at least fmhc_layer_norm_bwd_workspace_bytes(T, C) bytes,
  * 16-byte aligned.  Sums are added in a fixed order. */
 int fmhc_layer_norm_bwd(const void* grad_y, const void* x, const int8_t* x_codes,
                         const uint8_t* x_scales, const float* mean, const float* rstd,
-                        const void* weight, void* grad_x, void* grad_weight, void* grad_bias,
-                        void* workspace, int64_t workspace_bytes, int dtype, int param_dtype,
-                        int64_t T, int64_t C, void* stream);
+                        const void* weight, const void* grad_x_in, void* grad_x, void* grad_weight,
+                        void* grad_bias, void* workspace, int64_t workspace_bytes, int dtype,
+                        int param_dtype, int64_t T, int64_t C, void* stream);
 int64_t fmhc_layer_norm_bwd_workspace_bytes(int64_t T, int64_t C);
 
 /* Human-readable text for a status code.  Never returns NULL.

@@ -293,6 +293,71 @@ def test_layouts_fp32(T):
         verify(*inputs(T, C, F32, F32), 16)
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T,C,dtype", [(1, 5, BF16), (3, 40, F16), (70, 300, BF16), (33, 1024, F32), (1100, 2048, BF16),
+                                       (9, 1001, BF16), (40, 4096, F16), (3, 8200, BF16), (2, 16384, BF16),
+                                       (2, 17001, BF16), (2, 17000, F32)])
+def test_with_residual(T, C, dtype, bits):
+    """The bits of two gradients that are added."""
+    x, w, b, g = inputs(T, C, dtype, F32)
+    g2 = rnd((T, C), 9, 0.5, dtype=dtype).to(DEV)
+    norm = flash_mhc.LayerNorm(C, activation_bits=bits).to(DEV)
+    with torch.no_grad():
+        norm.weight.copy_(w)
+        norm.bias.copy_(b)
+    for other in (lambda r: r, lambda r: r.t().contiguous().t()):  # a strided gradient too
+        results = []
+        for fused in (True, False):
+            xs = x.clone().requires_grad_(True)
+            y, r = norm.with_residual(xs) if fused else (norm(xs), xs)
+            assert torch.equal(r, x)
+            results.append((y, *torch.autograd.grad([y, r], [xs, norm.weight, norm.bias], [g, other(g2)])))
+        for a, c in zip(*results):
+            assert torch.equal(a, c)
+    # One of the two only.
+    xs = x.clone().requires_grad_(True)
+    y, r = norm.with_residual(xs)
+    assert torch.equal(torch.autograd.grad(r, xs, g2, retain_graph=True)[0], g2)
+    only = torch.autograd.grad(y, xs, g)[0]
+    xs = x.clone().requires_grad_(True)
+    assert torch.equal(only, torch.autograd.grad(norm(xs), xs, g)[0])
+
+
+def test_with_residual_in_a_block():
+    """Hooks are called, in-place layers work, other norms and frozen inputs too."""
+    torch.manual_seed(0)
+    C = 96
+    layer = torch.nn.Sequential(torch.nn.ReLU(inplace=True), torch.nn.Linear(C, C))
+    blk = flash_mhc.MHCLiteBlock(4, C, layer, pre_norm=True).to(DEV).to(BF16)
+    x = rnd((17, 4, C), 1).to(DEV)
+
+    def step():
+        xs = x.clone().requires_grad_(True)
+        out = blk(xs)
+        return out, *torch.autograd.grad(out.float().square().sum(), [xs, *blk.parameters()])
+
+    want = step()
+    seen = []
+    handle = blk.norm.register_forward_hook(lambda m, a, out: seen.append(out.shape))
+    got = step()
+    handle.remove()
+    assert seen == [(17, C)]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, out: seen.append(type(m).__name__))
+    got = step()
+    handle.remove()
+    assert "LayerNorm" in seen
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    blk.norm.requires_grad_(False)
+    out = blk(x.clone().requires_grad_(True))
+    assert torch.equal(out, want[0])
+    out.float().sum().backward()
+    blk.norm = torch.nn.RMSNorm(C, device=DEV, dtype=BF16)
+    assert torch.isfinite(step()[1]).all()
+
+
 def test_opcheck():
     x, w, b, g = inputs(7, 72, BF16, F32)
     leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]

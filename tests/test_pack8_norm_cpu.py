@@ -64,11 +64,11 @@ F = _FAKE
         lambda L: L.fmhc_layer_norm_fwd(*[F] * 7, None, 1, 0, 2, 8, 1e-5, None),  # codes without scales
         lambda L: L.fmhc_layer_norm_fwd(None, *[F] * 7, 1, 0, 2, 8, 1e-5, None),
         lambda L: L.fmhc_layer_norm_fwd(*[F] * 8, 1, 0, 2, 0, 1e-5, None),
-        lambda L: L.fmhc_layer_norm_bwd(*[F] * 11, 1 << 40, 1, 0, 2, 8, None),  # x and codes
-        lambda L: L.fmhc_layer_norm_bwd(F, None, None, None, *[F] * 7, 1 << 40, 1, 0, 2, 8, None),  # neither
-        lambda L: L.fmhc_layer_norm_bwd(F, F, None, None, *[F] * 7, 8, 1, 0, 2, 8, None),  # workspace too small
-        lambda L: L.fmhc_layer_norm_bwd(F, F, None, None, *[F] * 6, F + 8, 1 << 40, 1, 0, 2, 8, None),
-        lambda L: L.fmhc_layer_norm_bwd(F, F, None, None, F, None, *[F] * 5, 1 << 40, 1, 0, 2, 8, None),  # no rstd
+        lambda L: L.fmhc_layer_norm_bwd(*[F] * 12, 1 << 40, 1, 0, 2, 8, None),  # x and codes
+        lambda L: L.fmhc_layer_norm_bwd(F, None, None, None, *[F] * 8, 1 << 40, 1, 0, 2, 8, None),  # neither
+        lambda L: L.fmhc_layer_norm_bwd(F, F, None, None, *[F] * 3, None, *[F] * 4, 8, 1, 0, 2, 8, None),  # workspace too small
+        lambda L: L.fmhc_layer_norm_bwd(F, F, None, None, *[F] * 3, None, *[F] * 3, F + 8, 1 << 40, 1, 0, 2, 8, None),
+        lambda L: L.fmhc_layer_norm_bwd(F, F, None, None, F, None, F, None, *[F] * 4, 1 << 40, 1, 0, 2, 8, None),  # no rstd
     ],
 )
 def test_entry_points_refuse(call):
