@@ -732,6 +732,16 @@ bool with_ln_walk(int64_t T, int C, F&& f) {
   return true;
 }
 
+// Whether whole aligned rows carry the nontemporal hint.  In fp32, whose loads take
+// half a lane's columns each, only rows of more than one group per lane in up to
+// 256 MiB (hint / none, us, forward and backward: T = 32768, C = 2048 95 / 98 and 141
+// / 151, T = 65536, C = 1024 97 / 100 and 150 / 149; T = 131072, C = 1024 213 / 197
+// and 313 / 294, C = 320 74 / 68 and 106 / 103).
+template <int DT>
+bool ln_hint(int64_t T, int C) {
+  return DT != FMHC_DTYPE_F32 || (C > 512 && T * C <= int64_t{1} << 26);
+}
+
 }  // namespace
 
 template <int DT>
@@ -739,18 +749,18 @@ int ln_fwd_run(const LnFwdArgs& a, hipStream_t s) {
   using S = typename Elems<DT>::S;
   const auto* x = static_cast<const S*>(a.x);
   auto* y = static_cast<S*>(a.y);
-  const bool nt = a.C % 8 == 0 && aligned16(x) && aligned16(y) && (!a.codes || Pack8Src::aligned(a.codes));
+  const bool nt = ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(x) && aligned16(y) && (!a.codes || Pack8Src::aligned(a.codes));
   const bool held = with_ln_walk<(DT == FMHC_DTYPE_F32 ? 3 : 5)>(a.T, a.C, [&](auto walk) {
     constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, BLOCK = ln_fwd_block<LPT>();
     auto launch = [&](auto ntc, auto keep) {
       constexpr bool NT = decltype(ntc)::value, KEEP = decltype(keep)::value;
       auto* kernel = &ln_fwd_kernel<DT, LPT, R, NT, KEEP>;
       const int64_t want = (a.T + BLOCK / LPT - 1) / (BLOCK / LPT);
-      // Eight workgroups per CU; with rows of up to one wave of 16-bit elements more,
-      // from four rows per slot on (T = 262144, C = 1024 202 -> 174 us, T = 65536,
-      // C = 2048 94 -> 90; at two rows per slot T = 30011, C = 2560 54 -> 69; C = 1024
-      // in fp32 98 -> 100, C = 8192 packed 61 -> 64).
-      const int64_t deep = LPT <= kWave && DT != FMHC_DTYPE_F32 ? want / 4 : 0, most = deep > 256 * 8 ? deep : 256 * 8;
+      // Eight workgroups per CU; with rows of up to one wave more, from four rows per
+      // slot on (T = 262144, C = 1024 202 -> 174 us, T = 65536, C = 2048 94 -> 90; at
+      // two rows per slot T = 30011, C = 2560 54 -> 69; with wider rows C = 8192 packed
+      // 61 -> 64).
+      const int64_t deep = LPT <= kWave ? want / 4 : 0, most = deep > 256 * 8 ? deep : 256 * 8;
       kernel<<<dim3(static_cast<unsigned>(want < most ? want : most)), BLOCK, 0, s>>>(x, a.P, y, a.mean, a.rstd, a.codes,
                                                                                     a.scales, a.T, a.C, a.eps);
     };
@@ -785,7 +795,7 @@ int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
       x = a.codes;
     else
       x = static_cast<const X*>(a.x);
-    const bool nt = a.C % 8 == 0 && aligned16(gy) && aligned16(gx) && aligned16(gi) &&
+    const bool nt = ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(gy) && aligned16(gx) && aligned16(gi) &&
                     (reinterpret_cast<uintptr_t>(x) & (KEPT ? 7u : 15u)) == 0;
     const bool held = with_ln_walk<3>(a.T, a.C, [&](auto walk) {
       constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, SLOTS = kLnBwdBlock / LPT;
