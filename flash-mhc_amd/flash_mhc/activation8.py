@@ -241,6 +241,16 @@ torch.library.register_autograd("flash_mhc::fused_post_res_pack8_traced", _fused
                                 setup_context=_setup_post_res)
 
 
+def _eager_post_res_backward(ctx, grad_out, *_codes):
+    if grad_out is None:
+        return None, None, None, None
+    return _fused_post_res_backward_pack8_cuda(grad_out, *ctx.saved_tensors)
+
+
+# For a graph of the gradients: raises where that graph is used.
+_eager_post_res_backward_once = once_differentiable(_eager_post_res_backward)
+
+
 class _FusedPostResEager(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_streams, layer_output, H_merged, h_post):
@@ -251,11 +261,8 @@ class _FusedPostResEager(torch.autograd.Function):
         return outs
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out, *_codes):
-        if grad_out is None:
-            return None, None, None, None
-        return _fused_post_res_backward_pack8_cuda(grad_out, *ctx.saved_tensors)
+    def backward(ctx, *grads):
+        return (_eager_post_res_backward_once if torch.is_grad_enabled() else _eager_post_res_backward)(ctx, *grads)
 
 
 @torch.library.impl(_lib, "fused_post_res_pack8", "AutogradCUDA")

@@ -713,15 +713,16 @@ def premap_bwd_pack8(x_codes: torch.Tensor, x_scales: torch.Tensor, W: torch.Ten
 
 def _norm_params(weight, bias, dtype: torch.dtype, C: int, dev) -> torch.dtype:
     """Check the norm's weight and bias (either may be None) and return their dtype."""
-    have = [t for t in (weight, bias) if t is not None]
-    if not have:
+    first = weight if weight is not None else bias
+    if first is None:
         return _F32
-    pdt = have[0].dtype
+    pdt = first.dtype
     if pdt is not _F32 and pdt is not dtype:
         raise TypeError(f"weight and bias must be float32 or x's dtype {dtype}, got {pdt}")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            _require(t, name, pdt, (C,), dev)
+    if weight is not None:
+        _require(weight, "weight", pdt, (C,), dev)
+    if bias is not None:
+        _require(bias, "bias", pdt, (C,), dev)
     return pdt
 
 
@@ -731,21 +732,36 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Ten
     (...,) fp32 (None without stats), codes and scales pack8's of x (None unless
     packed)."""
     dev = _device_of(x)
+    mean = torch.empty(x.shape[:-1], device=dev, dtype=_F32) if stats else None
+    rstd = torch.empty(x.shape[:-1], device=dev, dtype=_F32) if stats else None
+    y, q, s, _pdt = _layer_norm_fwd(x, weight, bias, eps, dev, _ptr_or_none(mean), _ptr_or_none(rstd), packed)
+    return y, mean, rstd, q, s
+
+
+def layer_norm_fwd_joint(x, weight, bias, eps: float, packed: bool):
+    """(y, stats, codes, scales, the parameters' dtype) of layer_norm_fwd, with mean
+    and rstd the halves of stats (an allocation less, where the host is the bound)."""
+    dev = _device_of(x)
+    T = _rows(x.shape)[0]
+    stats = torch.empty((2 * T,), device=dev, dtype=_F32)
+    mean = stats.data_ptr()
+    y, q, s, pdt = _layer_norm_fwd(x, weight, bias, eps, dev, mean, mean + 4 * T, packed)
+    return y, stats, q, s, pdt
+
+
+def _layer_norm_fwd(x, weight, bias, eps, dev, mean, rstd, packed):
     code = _dtype_code(x.dtype, "x")
     T, C = _rows(x.shape)
     _require(x, "x", x.dtype, x.shape, dev)
     pdt = _norm_params(weight, bias, x.dtype, C, dev)
     y = torch.empty_like(x)
-    mean = torch.empty(x.shape[:-1], device=dev, dtype=_F32) if stats else None
-    rstd = torch.empty(x.shape[:-1], device=dev, dtype=_F32) if stats else None
     q, s = empty_packed(x.shape, dev) if packed else (None, None)
     lib = _abi.load()
     with _OnDevice(dev):
-        st = lib.fmhc_layer_norm_fwd(x.data_ptr(), _ptr_or_none(weight), _ptr_or_none(bias), y.data_ptr(),
-                                     _ptr_or_none(mean), _ptr_or_none(rstd), _ptr_or_none(q), _ptr_or_none(s), code,
-                                     DTYPES[pdt], T, C, eps, _abi.stream_of(x))
+        st = lib.fmhc_layer_norm_fwd(x.data_ptr(), _ptr_or_none(weight), _ptr_or_none(bias), y.data_ptr(), mean, rstd,
+                                     _ptr_or_none(q), _ptr_or_none(s), code, DTYPES[pdt], T, C, eps, _abi.stream_of(x))
     _abi.check(st, "layer_norm_fwd")
-    return y, mean, rstd, q, s
+    return y, q, s, pdt
 
 
 def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Tensor | None,
@@ -773,14 +789,19 @@ def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Te
         _require(weight, "weight", param_dtype, (C,), dev)
     if grad_x_in is not None:
         _require(grad_x_in, "grad_x_in", grad_y.dtype, grad_y.shape, dev)
-    return launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias,
-                                 grad_x_in)
+    return _layer_norm_bwd(grad_y, x, codes, scales, mean.data_ptr(), rstd.data_ptr(), weight, param_dtype, need_weight,
+                           need_bias, grad_x_in)
 
 
-def launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias,
-                          grad_x_in=None):
-    """layer_norm_bwd for operands that are known to be right: what
-    layer_norm_fwd took and gave, and autograd's gradients, contiguous."""
+def layer_norm_bwd_joint(grad_y, x, codes, scales, stats, weight, param_dtype, need_weight, need_bias, grad_x_in=None):
+    """layer_norm_bwd for operands that need no checks: what layer_norm_fwd_joint
+    took and gave, and autograd's gradients, contiguous."""
+    mean = stats.data_ptr()
+    return _layer_norm_bwd(grad_y, x, codes, scales, mean, mean + 2 * stats.numel(), weight, param_dtype, need_weight,
+                           need_bias, grad_x_in)
+
+
+def _layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, need_weight, need_bias, grad_x_in):
     dev = grad_y.device
     code = DTYPES[grad_y.dtype]
     C = grad_y.shape[-1]
@@ -792,7 +813,7 @@ def launch_layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dt
     ws = _workspace(int(lib.fmhc_layer_norm_bwd_workspace_bytes(T, C)), dev) if need_weight or need_bias else None
     with _OnDevice(dev):
         st = lib.fmhc_layer_norm_bwd(grad_y.data_ptr(), _ptr_or_none(x), _ptr_or_none(codes), _ptr_or_none(scales),
-                                     mean.data_ptr(), rstd.data_ptr(), _ptr_or_none(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
+                                     mean, rstd, _ptr_or_none(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
                                      _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws),
                                      0 if ws is None else ws.numel(), code, DTYPES[param_dtype], T, C,
                                      _abi.stream_of(grad_y))

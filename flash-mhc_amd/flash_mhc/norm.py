@@ -111,27 +111,38 @@ torch.library.register_autograd("flash_mhc::layer_norm", _backward, setup_contex
 torch.library.register_autograd("flash_mhc::layer_norm_pack8", _backward, setup_context=_setup)
 
 
+# The two eager Functions' backward.  With a graph of the gradients (create_graph)
+# it goes through once_differentiable, which raises where that graph is used; the
+# check is cheaper than its wrapper, and a step of few rows is bound by the host.
+
+
+def _eager_backward(ctx, grad_y, grad_x=None):
+    if grad_y is None:  # the norm's output was not used
+        return grad_x, None, None, None, None
+    x, codes, scales, stats, weight = ctx.saved_tensors
+    _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
+    gx, gw, gb = _k.layer_norm_bwd_joint(grad_y.contiguous(), x, codes, scales, stats, weight, ctx.param_dtype,
+                                         need_weight, need_bias, _dense(grad_x))
+    return gx, gw, gb, None, None
+
+
+_eager_backward_once = once_differentiable(_eager_backward)
+
+
 class _LayerNormEager(torch.autograd.Function):
     """layer_norm / layer_norm_pack8 with their registered autograd, without the
-    ops' dispatch (at few rows a training step is bound by the host)."""
+    ops' dispatch."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, packed):
         x, weight = x.contiguous(), _dense(weight)
-        y, mean, rstd, codes, scales = _k.layer_norm_fwd(x, weight, _dense(bias), eps, packed=packed)
-        ctx.packed = packed
-        ctx.param_dtype = _param_dtype(weight, bias)
-        ctx.save_for_backward(None if packed else x, codes, scales, mean, rstd, weight)
+        y, stats, codes, scales, ctx.param_dtype = _k.layer_norm_fwd_joint(x, weight, _dense(bias), eps, packed)
+        ctx.save_for_backward(None if packed else x, codes, scales, stats, weight)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
-        x, codes, scales, mean, rstd, weight = ctx.saved_tensors
-        _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
-        gx, gw, gb = _k.launch_layer_norm_bwd(grad_y.contiguous(), x, codes, scales, mean, rstd, weight,
-                                              ctx.param_dtype, need_weight, need_bias)
-        return gx, gw, gb, None, None
+        return (_eager_backward_once if torch.is_grad_enabled() else _eager_backward)(ctx, grad_y)
 
 
 class _LayerNormResidualEager(torch.autograd.Function):
@@ -144,15 +155,8 @@ class _LayerNormResidualEager(torch.autograd.Function):
         return _LayerNormEager.forward(ctx, x, weight, bias, eps, packed), x.view_as(x)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y, grad_skip):
-        if grad_y is None:  # the norm's output was not used
-            return grad_skip, None, None, None, None
-        x, codes, scales, mean, rstd, weight = ctx.saved_tensors
-        _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
-        gx, gw, gb = _k.launch_layer_norm_bwd(grad_y.contiguous(), x, codes, scales, mean, rstd, weight,
-                                              ctx.param_dtype, need_weight, need_bias, _dense(grad_skip))
-        return gx, gw, gb, None, None
+    def backward(ctx, grad_y, grad_x):
+        return (_eager_backward_once if torch.is_grad_enabled() else _eager_backward)(ctx, grad_y, grad_x)
 
 
 def _check(x, weight, bias, activation_bits) -> None:
@@ -174,13 +178,13 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     rounded once.  activation_bits: 16 keeps x for the backward, 8 its 8-bit
     codes (the backward's normalised input is then that of the codes, with the
     statistics of x).  Differentiable once: a gradient of its gradients raises."""
-    _check(x, weight, bias, activation_bits)
     packed = activation_bits == 8
-    if _plain_eager(x):
+    if (packed or activation_bits == 16) and _plain_eager(x):  # the kernels' launchers check the tensors
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                         or (bias is not None and bias.requires_grad)):
             return _LayerNormEager.apply(x, weight, bias, eps, packed)
         return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps, stats=False)[0]
+    _check(x, weight, bias, activation_bits)
     op = torch.ops.flash_mhc.layer_norm_pack8 if packed else torch.ops.flash_mhc.layer_norm
     return op(x, weight, bias, eps)[0]
 
@@ -231,7 +235,6 @@ class LayerNorm(nn.Module):
         gradient that x gets from the residual (as a separate addition would)."""
         if (torch.is_grad_enabled() and x.requires_grad and not self._hooked() and _plain_eager(x)
                 and self._on_kernels(x)):
-            _check(x, self.weight, self.bias, self.activation_bits)
             return _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
         return self(x), x
 
