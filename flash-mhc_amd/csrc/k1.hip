@@ -687,13 +687,18 @@ __global__ __launch_bounds__(256) void k1_bwd_mfma(const typename SRC::Elem* __r
   // one slice and four runs, to sum their grad_W partials in LDS, measured
   // 8% slower.)
   // Workgroups are dispatched round-robin over the 8 XCDs.  Within each
-  // group of 64, workgroup b takes the logical id 8 (b % 8) + (b % 64) / 8:
-  // the workgroups of one run, which read the same go / proj rows, share one
-  // XCD's L2 (8% less HBM traffic), and a group still covers 8 neighbouring
-  // runs at a time.
+  // group of 8 p, workgroup b takes the logical id p (b % 8) + (b % 8 p) / 8:
+  // neighbouring workgroups, which read the same go / proj rows, share one
+  // XCD's L2 (p = 8: 8% less HBM traffic), and a group still covers neighbouring
+  // runs at a time.  With EPI a run's workgroups also read the same go3 rows,
+  // every stream's: where they are a multiple of 8, p is all of them (pre-map
+  // backward T = 16384, C = 4096 436 -> 414 us, from 8 bits 362 -> 342; T = 65536, C =
+  // 2048 853 -> 838, 686 -> 679; all of them at C = 2560, 20: 505 -> 508, and without
+  // EPI at C = 4096 205 -> 208, C = 512 102 -> 108).
   const unsigned bid = blockIdx.x;
-  const unsigned full = gridDim.x & ~63u;
-  const unsigned lid = bid < full ? (bid & ~63u) + 8u * (bid % 8u) + (bid % 64u) / 8u : bid;
+  const unsigned p8 = EPI && sl.n % 32 == 0 ? 2u * static_cast<unsigned>(sl.n) : 64u;
+  const unsigned group = bid / p8 * p8, in = bid - group;
+  const unsigned lid = group + p8 <= gridDim.x ? group + p8 / 8u * (in % 8u) + in / 8u : bid;
   const int64_t wid = static_cast<int64_t>(lid) * 4 + wave;
   const int slice = static_cast<int>(wid % sl.n);
   const int64_t run = wid / sl.n;

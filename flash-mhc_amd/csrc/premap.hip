@@ -539,7 +539,8 @@ int premap_bwd_run(const typename SRC::Elem* x, const uint8_t* xs, const uint16_
   if (!W || !alpha_pre || !alpha_post || !alpha_res || !bias || !perm || !grad_W || !grad_alpha_pre ||
       !grad_alpha_post || !grad_alpha_res || !grad_bias)
     return FMHC_ERR_INVALID_ARGUMENT;
-  if (T > 0 && (!x || (SRC::kPacked && !xs) || !h_pre || !proj || !inv_rms || !grad_layer_input || !grad_x)) return FMHC_ERR_INVALID_ARGUMENT;
+  if (T > 0 && (!x || (SRC::kPacked && !xs) || !h_pre || !proj || !inv_rms || !grad_layer_input || !grad_x))
+    return FMHC_ERR_INVALID_ARGUMENT;
   if (T > 0 && grad_x_in) {  // grad_x_in is read while grad_x is written: no overlap
     const auto a = reinterpret_cast<uintptr_t>(grad_x_in), b = reinterpret_cast<uintptr_t>(grad_x);
     const auto bytes = static_cast<uintptr_t>(T * n * C * 2);
