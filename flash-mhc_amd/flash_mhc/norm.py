@@ -193,7 +193,8 @@ class LayerNorm(nn.Module):
     """``nn.LayerNorm`` over the last axis on the HIP kernels, with the same
     parameters (``weight`` ones, ``bias`` zeros) and state_dict.  Tensors that
     the kernels do not take (not on a GPU, or other dtypes) go through PyTorch's
-    layer norm, as MHCLiteBlock's do through its plain formulation.
+    layer norm, as MHCLiteBlock's do through its plain formulation.  Autocast
+    does not change the kernels' types: the output has x's.
 
     Args:
         hidden_size: C.
@@ -233,7 +234,7 @@ class LayerNorm(nn.Module):
     def with_residual(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(norm(x), x) for ``x + layer(norm(x))``: the norm's backward adds the
         gradient that x gets from the residual (as a separate addition would)."""
-        if (torch.is_grad_enabled() and x.requires_grad and not self._hooked() and _plain_eager(x)
+        if (_plain_eager(x) and torch.is_grad_enabled() and x.requires_grad and not self._hooked()
                 and self._on_kernels(x)):
             return _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
         return self(x), x

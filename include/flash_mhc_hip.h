@@ -308,7 +308,8 @@ int fmhc_premap_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const 
  *   rstd[t] = rsqrt(sum_c (x[t,c] - mean[t])^2 / C + eps)
  *   y[t,c]  = (x[t,c] - mean[t]) rstd[t] weight[c] + bias[c]
  * mean and rstd (T,) may be NULL.  With x_codes and x_scales (both or neither)
- * x is also packed, as fmhc_pack8 does, in the same pass. */
+ * x is also packed, as fmhc_pack8 does, in the same pass.  No output may
+ * overlap an input. */
 int fmhc_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* mean,
                         float* rstd, int8_t* x_codes, uint8_t* x_scales, int dtype, int param_dtype,
                         int64_t T, int64_t C, float eps, void* stream);

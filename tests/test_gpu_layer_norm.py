@@ -400,3 +400,24 @@ def test_past_32_bits(C):
     A.check("grad_x of 8 bits", gx8[:n], *A.ln_bwd(g, x, A.unpack8(*A.pack8(x)), w, EPS)["x"])
     del t, d, y, mean, rstd, q, s, gx, gx8, o
     torch.cuda.empty_cache()
+
+
+def test_one_row_without_leading_dims_and_two_streams_at_once():
+    x, w, b, g = inputs(1, 1000, BF16, F32)
+    verify(x[0], w, b, g[0], 16)
+    verify(x[0], w, b, g[0], 8)
+    # Two forwards and backwards that overlap on two streams, workspaces of their own.
+    many = [inputs(3000, 520, BF16, F32, seed) for seed in (1, 2)]
+    want = [run(*m, 8) for m in many]
+    streams = [torch.cuda.Stream() for _ in many]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for s, m in zip(streams, many):
+        with torch.cuda.stream(s):
+            got.append(run(*m, 8))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for a, c in zip(got, want):
+        for u, v in zip(a, c):
+            assert torch.equal(u, v)

@@ -13,7 +13,7 @@ import flash_mhc
 from flash_mhc import ops as _ops  # noqa: F401
 from oracle import act8_oracle as A
 from oracle import mhc_oracle as O
-from parity import check_bf16, check_fp32
+from parity import block_close, check_bf16, check_fp32
 
 pytestmark = pytest.mark.gpu
 
@@ -634,3 +634,33 @@ def test_past_32_bits(C):
     compare(got[:1], want[:1])
     del got
     torch.cuda.empty_cache()
+
+
+def test_block_reduce_overhead_training():
+    """Inductor with graphs: replays equal the first calls, and eager mode within the block's tolerance."""
+    T, C = 256, 512
+    torch._dynamo.reset()
+    blk = make_block(C, activation_bits=8, pre_norm=True)
+    data = [(streams(T, C, 300 + i).to(DEV), rnd((T, 4, C), 400 + i).to(DEV)) for i in range(3)]
+
+    def step(fn, x, up):
+        blk.zero_grad(set_to_none=True)
+        xi = x.clone().requires_grad_(True)
+        out = fn(xi)
+        out.backward(up)
+        return [out.detach().clone(), xi.grad.clone()] + [p.grad.clone() for p in blk.parameters()]
+
+    eager = [step(blk, x, up) for x, up in data]
+    f = torch.compile(blk, mode="reduce-overhead", fullgraph=True)
+    rounds = []
+    for _ in range(2):
+        res = []
+        for x, up in data:
+            torch.compiler.cudagraph_mark_step_begin()
+            res.append(step(f, x, up))
+        rounds.append(res)
+    for first, again, want in zip(*rounds, eager):
+        for a, b in zip(again, first):
+            same(a, b)
+        block_close("out", again[0], want[0].float())
+        block_close("grad_x", again[1], want[1].float(), rtol=5e-2, atol=1e-1)
