@@ -30,6 +30,7 @@ import torch
 import torch.library
 from torch.autograd.function import once_differentiable
 
+from . import block as _block  # which imports this module: its names are read at call time
 from . import kernels as _k
 from .ops import (
     _check_k2_shapes,
@@ -244,7 +245,8 @@ torch.library.register_autograd("flash_mhc::fused_post_res_pack8_traced", _fused
 def _eager_post_res_backward(ctx, grad_out, *_codes):
     if grad_out is None:
         return None, None, None, None
-    return _fused_post_res_backward_pack8_cuda(grad_out, *ctx.saved_tensors)
+    *codes, H_merged, h_post = ctx.saved_tensors
+    return _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
 
 
 # For a graph of the gradients: raises where that graph is used.
@@ -267,9 +269,7 @@ class _FusedPostResEager(torch.autograd.Function):
 
 @torch.library.impl(_lib, "fused_post_res_pack8", "AutogradCUDA")
 def _fused_post_res_pack8_autograd(x_streams, layer_output, H_merged, h_post):
-    from .block import _plain_eager
-
-    if _plain_eager(x_streams):
+    if _block._plain_eager(x_streams):
         return _FusedPostResEager.apply(x_streams, layer_output, H_merged, h_post)
     return torch.ops.flash_mhc.fused_post_res_pack8_traced(x_streams, layer_output, H_merged, h_post)
 
@@ -375,9 +375,9 @@ class _PostResEager(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        saved = ctx.saved_tensors
-        ctx.kept.codes = saved[:2]
-        g_x, g_lo, g_H, g_hp = _fused_post_res_backward_pack8_cuda(grad_out, *saved)
+        *codes, H_merged, h_post = ctx.saved_tensors
+        ctx.kept.codes = codes[:2]
+        g_x, g_lo, g_H, g_hp = _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
         return None, g_x, g_lo, g_H, g_hp, None
 
 
@@ -405,9 +405,7 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     A group of 32 columns whose largest magnitude is in [2^e, 2^(e + 1)) has the
     scale byte e + 127 (at least 7) and stands for code * 2^(e - 6); a group
     with an Inf or NaN has 255 and stands for NaN throughout."""
-    from .block import _plain_eager
-
-    if _plain_eager(x):
+    if _block._plain_eager(x):
         return _pack8_cuda(x)
     return torch.ops.flash_mhc.pack8(x)
 
@@ -415,8 +413,6 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The tensor that pack8's codes and scales stand for, exact in bf16 and fp32
     (and in fp16 for what was packed from fp16)."""
-    from .block import _plain_eager
-
-    if _plain_eager(codes):
+    if _block._plain_eager(codes):
         return _unpack8_cuda(codes, scales, dtype)
     return torch.ops.flash_mhc.unpack8(codes, scales, dtype)

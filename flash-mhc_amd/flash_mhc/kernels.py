@@ -559,11 +559,22 @@ def _rows(shape) -> tuple[int, int]:
     return rows, shape[-1]
 
 
-def empty_packed(shape, dev) -> tuple[torch.Tensor, torch.Tensor]:
-    """Unwritten (codes, scales) for a tensor of this shape."""
-    codes = torch.empty(shape, device=dev, dtype=torch.int8)
-    scales = torch.empty((*shape[:-1], pack_groups(shape[-1])), device=dev, dtype=torch.uint8)
-    return codes, scales
+def empty_packed(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Unwritten (codes, scales) for a contiguous x."""
+    shape = x.shape
+    return (torch.empty_like(x, dtype=torch.int8),
+            x.new_empty((*shape[:-1], pack_groups(shape[-1])), dtype=torch.uint8))
+
+
+def _launch(what: str, dev: torch.device, fn, *args) -> None:
+    """fn(*args) with dev current (it nearly always is), its status checked."""
+    if torch.cuda.current_device() == dev.index:
+        st = fn(*args)
+    else:
+        with _OnDevice(dev):
+            st = fn(*args)
+    if st != 0:
+        _abi.check(st, what)
 
 
 def _require_packed(codes, scales, name: str, shape, dev) -> None:
@@ -578,11 +589,9 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     code = _dtype_code(x.dtype, "x")
     rows, C = _rows(x.shape)
     _require(x, "x", x.dtype, x.shape, dev)
-    codes, scales = empty_packed(x.shape, dev)
-    lib = _abi.load()
-    with _OnDevice(dev):
-        st = lib.fmhc_pack8(x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), rows, C, _abi.stream_of(x))
-    _abi.check(st, "pack8")
+    codes, scales = empty_packed(x)
+    _launch("pack8", dev, _abi.load().fmhc_pack8, x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), rows, C,
+            _abi.stream_of(x))
     return codes, scales
 
 
@@ -592,11 +601,9 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = _BF1
     code = _dtype_code(dtype, "dtype")
     rows, C = _rows(codes.shape)
     _require_packed(codes, scales, "x", codes.shape, dev)
-    x = torch.empty(codes.shape, device=dev, dtype=dtype)
-    lib = _abi.load()
-    with _OnDevice(dev):
-        st = lib.fmhc_unpack8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), code, rows, C, _abi.stream_of(codes))
-    _abi.check(st, "unpack8")
+    x = torch.empty_like(codes, dtype=dtype)
+    _launch("unpack8", dev, _abi.load().fmhc_unpack8, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), code, rows, C,
+            _abi.stream_of(codes))
     return x
 
 
@@ -611,14 +618,11 @@ def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: 
     _require(H_merged, "H_merged", _F32, (T, n, n), dev)
     _require(h_post, "h_post", _F32, (T, n), dev)
     out = torch.empty_like(x_streams)
-    xq, xs = empty_packed((T, n, C), dev) if pack_x else (None, None)
-    lq, ls = empty_packed((T, C), dev)
-    lib = _abi.load()
-    with _OnDevice(dev):
-        st = lib.fmhc_k4_fwd_pack8(x_streams.data_ptr(), layer_output.data_ptr(), H_merged.data_ptr(),
-                                   h_post.data_ptr(), out.data_ptr(), _ptr_or_none(xq), _ptr_or_none(xs),
-                                   lq.data_ptr(), ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))
-    _abi.check(st, "k4_fwd_pack8")
+    xq, xs = empty_packed(x_streams) if pack_x else (None, None)
+    lq, ls = empty_packed(layer_output)
+    _launch("k4_fwd_pack8", dev, _abi.load().fmhc_k4_fwd_pack8, x_streams.data_ptr(), layer_output.data_ptr(),
+            H_merged.data_ptr(), h_post.data_ptr(), out.data_ptr(), _ptr_or_none(xq), _ptr_or_none(xs), lq.data_ptr(),
+            ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))
     return out, xq, xs, lq, ls
 
 
@@ -632,17 +636,21 @@ def k4_bwd_pack8(grad_out: torch.Tensor, x_codes: torch.Tensor, x_scales: torch.
     _require(H_merged, "H_merged", _F32, (T, n, n), dev)
     _require(h_post, "h_post", _F32, (T, n), dev)
     _require(grad_out, "grad_out", _BF16, (T, n, C), dev)
+    return k4_bwd_pack8_saved(grad_out, x_codes, x_scales, lo_codes, lo_scales, H_merged, h_post)
+
+
+def k4_bwd_pack8_saved(grad_out, x_codes, x_scales, lo_codes, lo_scales, H_merged, h_post):
+    """k4_bwd_pack8 for operands that need no checks: what k4_fwd_pack8 took and
+    gave, and autograd's gradient of its out, contiguous."""
+    T, n, C = x_codes.shape
     grad_x = torch.empty_like(grad_out)
-    grad_lo = torch.empty((T, C), device=dev, dtype=_BF16)
-    grad_H = torch.empty((T, n, n), device=dev, dtype=_F32)
-    grad_h_post = torch.empty((T, n), device=dev, dtype=_F32)
-    lib = _abi.load()
-    with _OnDevice(dev):
-        st = lib.fmhc_k4_bwd_pack8(x_codes.data_ptr(), x_scales.data_ptr(), lo_codes.data_ptr(), lo_scales.data_ptr(),
-                                   H_merged.data_ptr(), h_post.data_ptr(), grad_out.data_ptr(), grad_x.data_ptr(),
-                                   grad_lo.data_ptr(), grad_H.data_ptr(), grad_h_post.data_ptr(), T, C, n,
-                                   _abi.stream_of(x_codes))
-    _abi.check(st, "k4_bwd_pack8")
+    grad_lo = torch.empty_like(lo_codes, dtype=_BF16)
+    grad_H = torch.empty_like(H_merged)
+    grad_h_post = torch.empty_like(h_post)
+    _launch("k4_bwd_pack8", x_codes.device, _abi.load().fmhc_k4_bwd_pack8, x_codes.data_ptr(), x_scales.data_ptr(),
+            lo_codes.data_ptr(), lo_scales.data_ptr(), H_merged.data_ptr(), h_post.data_ptr(), grad_out.data_ptr(),
+            grad_x.data_ptr(), grad_lo.data_ptr(), grad_H.data_ptr(), grad_h_post.data_ptr(), T, C, n,
+            _abi.stream_of(x_codes))
     return grad_x, grad_lo, grad_H, grad_h_post
 
 
@@ -755,12 +763,10 @@ def _layer_norm_fwd(x, weight, bias, eps, dev, mean, rstd, packed):
     _require(x, "x", x.dtype, x.shape, dev)
     pdt = _norm_params(weight, bias, x.dtype, C, dev)
     y = torch.empty_like(x)
-    q, s = empty_packed(x.shape, dev) if packed else (None, None)
-    lib = _abi.load()
-    with _OnDevice(dev):
-        st = lib.fmhc_layer_norm_fwd(x.data_ptr(), _ptr_or_none(weight), _ptr_or_none(bias), y.data_ptr(), mean, rstd,
-                                     _ptr_or_none(q), _ptr_or_none(s), code, DTYPES[pdt], T, C, eps, _abi.stream_of(x))
-    _abi.check(st, "layer_norm_fwd")
+    q, s = empty_packed(x) if packed else (None, None)
+    _launch("layer_norm_fwd", dev, _abi.load().fmhc_layer_norm_fwd, x.data_ptr(), _ptr_or_none(weight),
+            _ptr_or_none(bias), y.data_ptr(), mean, rstd, _ptr_or_none(q), _ptr_or_none(s), code, DTYPES[pdt], T, C, eps,
+            _abi.stream_of(x))
     return y, q, s, pdt
 
 
@@ -807,15 +813,13 @@ def _layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, n
     C = grad_y.shape[-1]
     T = grad_y.numel() // C
     gx = torch.empty_like(grad_y)
-    gw = torch.empty((C,), device=dev, dtype=param_dtype) if need_weight else None
-    gb = torch.empty((C,), device=dev, dtype=param_dtype) if need_bias else None
+    gw = grad_y.new_empty((C,), dtype=param_dtype) if need_weight else None
+    gb = grad_y.new_empty((C,), dtype=param_dtype) if need_bias else None
     lib = _abi.load()
-    ws = _workspace(int(lib.fmhc_layer_norm_bwd_workspace_bytes(T, C)), dev) if need_weight or need_bias else None
-    with _OnDevice(dev):
-        st = lib.fmhc_layer_norm_bwd(grad_y.data_ptr(), _ptr_or_none(x), _ptr_or_none(codes), _ptr_or_none(scales),
-                                     mean, rstd, _ptr_or_none(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
-                                     _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws),
-                                     0 if ws is None else ws.numel(), code, DTYPES[param_dtype], T, C,
-                                     _abi.stream_of(grad_y))
-    _abi.check(st, "layer_norm_bwd")
+    ws_bytes = lib.fmhc_layer_norm_bwd_workspace_bytes(T, C) if need_weight or need_bias else 0
+    ws = _workspace(ws_bytes, dev)
+    _launch("layer_norm_bwd", dev, lib.fmhc_layer_norm_bwd, grad_y.data_ptr(), _ptr_or_none(x), _ptr_or_none(codes),
+            _ptr_or_none(scales), mean, rstd, _ptr_or_none(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
+            _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws), ws_bytes, code, DTYPES[param_dtype], T, C,
+            _abi.stream_of(grad_y))
     return gx, gw, gb
