@@ -549,21 +549,21 @@ def _dtype_code(dt: torch.dtype, name: str) -> int:
     return code
 
 
-def _rows(shape) -> tuple[int, int]:
-    """(rows, C) of a tensor's shape (..., C)."""
+def _rows(x: torch.Tensor, name: str) -> tuple[int, int]:
+    """(rows, C) of x (..., C), which must be contiguous."""
+    shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError(f"expected shape (..., C) with C >= 1, got {tuple(shape)}")
-    rows = 1
-    for d in shape[:-1]:
-        rows *= d
-    return rows, shape[-1]
+    if not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return x.numel() // shape[-1], shape[-1]
 
 
 def empty_packed(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Unwritten (codes, scales) for a contiguous x."""
     shape = x.shape
     return (torch.empty_like(x, dtype=torch.int8),
-            x.new_empty((*shape[:-1], pack_groups(shape[-1])), dtype=torch.uint8))
+            x.new_empty((*shape[:-1], (shape[-1] + PACK_GROUP - 1) // PACK_GROUP), dtype=torch.uint8))
 
 
 def _launch(what: str, dev: torch.device, fn, *args) -> None:
@@ -587,8 +587,7 @@ def pack8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """codes (..., C) int8 and scales (..., ceil(C / 32)) uint8 of x (..., C)."""
     dev = _device_of(x)
     code = _dtype_code(x.dtype, "x")
-    rows, C = _rows(x.shape)
-    _require(x, "x", x.dtype, x.shape, dev)
+    rows, C = _rows(x, "x")
     codes, scales = empty_packed(x)
     _launch("pack8", dev, _abi.load().fmhc_pack8, x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(), rows, C,
             _abi.stream_of(x))
@@ -599,7 +598,7 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = _BF1
     """The values of pack8's codes and scales, in dtype."""
     dev = _device_of(codes)
     code = _dtype_code(dtype, "dtype")
-    rows, C = _rows(codes.shape)
+    rows, C = _rows(codes, "x_codes")
     _require_packed(codes, scales, "x", codes.shape, dev)
     x = torch.empty_like(codes, dtype=dtype)
     _launch("unpack8", dev, _abi.load().fmhc_unpack8, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), code, rows, C,
@@ -750,8 +749,8 @@ def layer_norm_fwd_joint(x, weight, bias, eps: float, packed: bool):
     """(y, stats, codes, scales, the parameters' dtype) of layer_norm_fwd, with mean
     and rstd the halves of stats (an allocation less, where the host is the bound)."""
     dev = _device_of(x)
-    T = _rows(x.shape)[0]
-    stats = torch.empty((2 * T,), device=dev, dtype=_F32)
+    T = _rows(x, "x")[0]
+    stats = x.new_empty((2 * T,), dtype=_F32)
     mean = stats.data_ptr()
     y, q, s, pdt = _layer_norm_fwd(x, weight, bias, eps, dev, mean, mean + 4 * T, packed)
     return y, stats, q, s, pdt
@@ -759,8 +758,7 @@ def layer_norm_fwd_joint(x, weight, bias, eps: float, packed: bool):
 
 def _layer_norm_fwd(x, weight, bias, eps, dev, mean, rstd, packed):
     code = _dtype_code(x.dtype, "x")
-    T, C = _rows(x.shape)
-    _require(x, "x", x.dtype, x.shape, dev)
+    T, C = _rows(x, "x")
     pdt = _norm_params(weight, bias, x.dtype, C, dev)
     y = torch.empty_like(x)
     q, s = empty_packed(x) if packed else (None, None)
@@ -779,8 +777,7 @@ def layer_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor | None, codes: torch.Te
     grad_x_in: a gradient of x from elsewhere, added to grad_x."""
     dev = _device_of(grad_y)
     code = _dtype_code(grad_y.dtype, "grad_y")
-    T, C = _rows(grad_y.shape)
-    _require(grad_y, "grad_y", grad_y.dtype, grad_y.shape, dev)
+    T, C = _rows(grad_y, "grad_y")
     if (x is None) == (codes is None):
         raise ValueError("layer_norm_bwd takes x, or its codes and scales")
     if x is not None:
