@@ -54,8 +54,9 @@ template <int DT>
 int ln_bwd_run(const LnBwdArgs& a, hipStream_t s);
 
 // Workgroups of the backward, each of which leaves sums of all columns, at most:
-// one of eight waves per CU, two where a lane has one group of columns (and the
-// registers for them).
+// one of eight waves per CU, two where a lane has one group of columns and the
+// registers for them (T = 65536, C = 512 one 41.4 us, two 39.8; C = 2048, two groups
+// per lane, one 135, two 140, with twice as many sums to add).
 constexpr int64_t kLnParts = 512;
 // Columns of a workgroup's sums.
 inline int64_t ln_cols(int64_t C) { return (C + 7) / 8 * 8; }

@@ -3,8 +3,11 @@
 // A row is held by LPT lanes, R groups of 8 columns each, from its loads to its
 // stores; a lane keeps the same columns for every row of its workgroup, so the
 // weight and bias and (backward) the sums of grad_w and grad_b stay in registers.
-// The next row's loads are issued before the current row is computed.  The
-// lane at a row's end with fewer than 8 columns left takes the row's last 8
+// The next row's loads are issued before the current row is computed.
+// Bound by HBM (some 10 VALU operations per element): T = 65536, C = 2048 in bf16 the
+// forward takes 92 us (5.8 TB/s; packed 117, 5.8), the backward 131 + 4.6 for the
+// parameters' sums (6.1; from codes 106, 6.4).
+// The lane at a row's end with fewer than 8 columns left takes the row's last 8
 // instead: every load is one vector inside the row, sums leave out the columns
 // that the lane before holds too, and stores write those once more with the
 // same values.
@@ -702,6 +705,18 @@ constexpr int ln_most_rounds() {
 
 // f(LnWalk) for T rows of C columns, 8 or more, held by registers with at most
 // RMAX groups per lane; false where there is no such layout.
+//
+// Many rows take few lanes each: one wave sums a row without LDS and a barrier.
+// Few rows take more, so that every CU has some.  Forward, bf16, fewer lanes / more
+// (us): C = 2048 T = 64 3.9 / 3.3, T = 65536 94 / 99; C = 1536 T = 1024 3.9 / 3.9, T =
+// 4096 6.3 / 8.0; C = 4096 (128 lanes, 256) T = 4096 16.4 / 14.1, T = 8192 24.8 /
+// 24.9, T = 16384 47.8 / 48.6; C = 8192 (256, 512) T = 256 4.7 / 4.3, T = 1024 9.3 /
+// 9.6, T = 4096 25.4 / 28.1.  The backward differs by 2% at most.
+//
+// RMAX: five groups per lane forward in 16-bit types (C = 2560, T = 65536, three
+// instead 117 -> 119, packed 155 -> 163), three in fp32 (four: T = 32768, C = 2048 95
+// -> 102) and in the backward (five: beyond the registers).  320 lanes for rows of 257
+// to 320 groups, none idle: C = 2560, T = 65536 114 -> 126 forward, 167 -> 176 backward.
 template <int RMAX, typename F>
 bool with_ln_walk(int64_t T, int C, F&& f) {
   if (C < 8) return false;
