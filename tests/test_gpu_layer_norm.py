@@ -421,3 +421,55 @@ def test_one_row_without_leading_dims_and_two_streams_at_once():
     for a, c in zip(got, want):
         for u, v in zip(a, c):
             assert torch.equal(u, v)
+
+
+class Fenced:
+    """Outputs inside larger buffers whose other bytes have to stay as they were."""
+
+    def __init__(self):
+        self.held = []
+
+    def __call__(self, shape, dtype):
+        n = torch.empty(shape, dtype=dtype, device="meta").numel() * dtype.itemsize
+        buf = torch.full((n + 1024,), 0xA5, dtype=torch.uint8, device=DEV)
+        self.held.append((buf, n))
+        return buf[512:512 + n].view(dtype).view(shape)
+
+    def check(self):
+        for buf, n in self.held:
+            assert bool((buf[:512] == 0xA5).all()) and bool((buf[512 + n:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("T,C", [(1, 1), (3, 7), (5, 8), (2, 33), (7, 100), (130, 300), (33, 1001), (1030, 1544), (5, 2560),
+                                 (3, 4099), (2, 8200), (2, 16384), (3, 17003)])
+@pytest.mark.parametrize("dtype,code", [(BF16, 1), (F32, 0)])
+def test_writes_stay_inside(T, C, dtype, code):
+    """Every output of layer norm, pack8 and unpack8 is written whole and nothing beside it."""
+    from flash_mhc import _abi
+
+    lib, st = _abi.load(), torch.cuda.current_stream().cuda_stream
+    x, w, b, g = inputs(T, C, dtype, F32)
+    out, G = Fenced(), (C + 31) // 32
+    y, mean, rstd = out((T, C), dtype), out((T,), F32), out((T,), F32)
+    q, s = out((T, C), torch.int8), out((T, G), torch.uint8)
+    P = lambda *ts: [None if t is None else t.data_ptr() for t in ts]
+    _abi.check(lib.fmhc_layer_norm_fwd(*P(x, w, b, y, mean, rstd, q, s), code, 0, T, C, EPS, st), "forward")
+    nbytes = lib.fmhc_layer_norm_bwd_workspace_bytes(T, C)
+    for kept in ((x, None, None), (None, q, s)):
+        for extra in (None, g):
+            gx, gw, gb = out((T, C), dtype), out((C,), F32), out((C,), F32)
+            ws = out((nbytes,), torch.uint8)
+            _abi.check(lib.fmhc_layer_norm_bwd(*P(g, *kept, mean, rstd, w, extra, gx, gw, gb, ws), nbytes, code, 0, T, C,
+                                               st), "backward")
+            a = torch.ops.flash_mhc.layer_norm_backward(g, *kept, mean, rstd, w, F32, True, True)
+            assert torch.equal(gw, a[1]) and torch.equal(gb, a[2])
+            assert torch.equal(gx, a[0] if extra is None else a[0] + g)
+    q2, s2, back = out((T, C), torch.int8), out((T, G), torch.uint8), out((T, C), dtype)
+    _abi.check(lib.fmhc_pack8(*P(x), code, *P(q2, s2), T, C, st), "pack8")
+    _abi.check(lib.fmhc_unpack8(*P(q2, s2, back), code, T, C, st), "unpack8")
+    out.check()
+    want = torch.ops.flash_mhc.layer_norm_pack8(x, w, b, EPS)
+    for a, v in zip((y, mean, rstd, q, s), want):
+        assert torch.equal(a, v)
+    assert torch.equal(q2, q) and torch.equal(s2, s)
+    assert torch.equal(back, flash_mhc.unpack8(q, s, dtype))

@@ -664,3 +664,51 @@ def test_block_reduce_overhead_training():
             same(a, b)
         block_close("out", again[0], want[0].float())
         block_close("grad_x", again[1], want[1].float(), rtol=5e-2, atol=1e-1)
+
+
+@pytest.mark.parametrize("T,C", [(1, 1), (3, 7), (17, 8), (16, 33), (130, 100), (47, 300), (33, 1001), (64, 1024), (5, 2056)])
+def test_writes_stay_inside(T, C):
+    """The outputs of every kernel that reads or writes codes, and nothing beside them."""
+    from flash_mhc import _abi
+
+    held = []
+
+    def out(shape, dtype):
+        n = torch.empty(shape, dtype=dtype, device="meta").numel() * dtype.itemsize
+        buf = torch.full((n + 1024,), 0xA5, dtype=torch.uint8, device=DEV)
+        held.append((buf, n))
+        return buf[512:512 + n].view(dtype).view(shape)
+
+    f32, i8, u8 = torch.float32, torch.int8, torch.uint8
+    lib, st, G = _abi.load(), torch.cuda.current_stream().cuda_stream, (C + 31) // 32
+    P = lambda *ts: [None if t is None else t.data_ptr() for t in ts]
+    x, lo, H, hp, go = mix_inputs(T, C)
+    o, xq, xs, lq, ls = (out((T, 4, C), BF16), out((T, 4, C), i8), out((T, 4, G), u8), out((T, C), i8), out((T, G), u8))
+    _abi.check(lib.fmhc_k4_fwd_pack8(*P(x, lo, H, hp, o, xq, xs, lq, ls), T, C, 4, st), "k4 forward")
+    want = OPS.fused_post_res_pack8(x, lo, H, hp)
+    for a, b in zip((o, xq, xs, lq, ls), want):
+        same(a, b)
+    gx, glo, gH, ghp = out((T, 4, C), BF16), out((T, C), BF16), out((T, 4, 4), f32), out((T, 4), f32)
+    _abi.check(lib.fmhc_k4_bwd_pack8(*P(xq, xs, lq, ls, H, hp, go, gx, glo, gH, ghp), T, C, 4, st), "k4 backward")
+    for a, b in zip((gx, glo, gH, ghp), OPS.fused_post_res_backward_pack8(go, *want[1:], H, hp)):
+        same(a, b)
+    xx, args, li, hpre, proj, inv = premap_state(T, C)
+    q, s = flash_mhc.pack8(xx)
+    gx, gW = out((T, 4, C), BF16), out((32, 4 * C), BF16)
+    nbytes = lib.fmhc_k1_bwd_pack8_workspace_bytes(T, C)
+    ws = out((nbytes,), u8)
+    _abi.check(lib.fmhc_k1_bwd_pack8(*P(q, s, args[0], proj, proj, inv, gx, gW, ws if nbytes else None), nbytes, T, C, 4, st),
+               "k1 backward")
+    for a, b in zip((gx, gW), OPS.fused_rmsnorm_project_bwd_pack8(proj, q, s, args[0], proj, inv)):
+        same(a, b)
+    nbytes = max(lib.fmhc_premap_bwd_workspace_bytes(T, C), 16)
+    for sink in (None, go):
+        gx, gW, ws = out((T, 4, C), BF16), out((32, 4 * C), BF16), out((nbytes,), u8)
+        ga, gb = [out((1,), BF16) for _ in range(3)], out((32,), BF16)
+        _abi.check(lib.fmhc_premap_bwd_pack8(*P(q, s, *args), 1, *P(hpre, proj, inv, li, hp, H, sink, gx, gW, *ga, gb, ws),
+                                             nbytes, T, C, 4, st), "pre-map backward")
+        ref = OPS.mhc_pre_map_backward_pack8(li, H, hp, None, None, sink, q, s, *args, hpre, proj, inv)
+        for a, b in zip((gx, gW, *ga, gb), ref):
+            same(a, b.view_as(a))
+    for buf, n in held:
+        assert bool((buf[:512] == 0xA5).all()) and bool((buf[512 + n:] == 0xA5).all())
