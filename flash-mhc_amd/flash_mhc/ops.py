@@ -244,6 +244,8 @@ def _check_n4(x_streams: torch.Tensor, message: str) -> None:
 
 def _coeff(t: torch.Tensor) -> torch.Tensor:
     # The reference kernels upcast whatever coefficient dtype they receive.
+    if t.dtype is torch.float32 and t.is_contiguous():
+        return t
     return t.to(torch.float32).contiguous()
 
 

@@ -712,3 +712,28 @@ def test_writes_stay_inside(T, C):
             same(a, b.view_as(a))
     for buf, n in held:
         assert bool((buf[:512] == 0xA5).all()) and bool((buf[512 + n:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("kw", [dict(rmsnorm_weight=True), dict(activation_checkpointing=True),
+                                dict(rmsnorm_weight=True, pre_norm=True, activation_checkpointing=True)])
+def test_block_options_eager_and_compiled(kw):
+    """The block's other options beside activation_bits=8: the same bits through the
+    Functions and through the ops, from a strided x too."""
+    T, C = 70, 96
+    torch._dynamo.reset()
+    blk = make_block(C, 3, activation_bits=8, **kw)
+    x, g = streams(T, C, 2).to(DEV), rnd((T, 4, C), 3).to(DEV)
+    out, want = grads(blk, x, g)
+    compiled = torch.compile(blk, fullgraph=True, backend="aot_eager")
+    for fn in (blk, compiled):
+        xs = x.clone().requires_grad_(True)
+        o = fn(xs)
+        same(o, out)
+        for a, b in zip(torch.autograd.grad(o, [xs, *blk.parameters()], g), want):
+            same(a, b)
+    wide = torch.empty(T, C, 4, device=DEV, dtype=BF16).copy_(x.transpose(1, 2)).transpose(1, 2).requires_grad_(True)
+    assert not wide.is_contiguous()
+    o = blk(wide)
+    same(o, out)
+    for a, b in zip(torch.autograd.grad(o, [wide, *blk.parameters()], g.transpose(1, 2).contiguous().transpose(1, 2)), want):
+        same(a, b)
