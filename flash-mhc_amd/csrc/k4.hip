@@ -91,17 +91,19 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_kernel(const uin
 // The forward that also leaves x and lo in 8 bits (pack8.h) for the backward:
 // out as k4_fwd_kernel gives it, and the codes and scales of the rows it has in
 // registers anyway, which a pass of its own would read again (T = 65536, C = 1024
-// 256 us, 6.1 TB/s; the forward alone 188, a pass over x alone 132).  A quad of lanes
+// 257 us, 6.1 TB/s; the forward alone 184, a pass over x alone 132).  A quad of lanes
 // holds a group of 32 columns.  The lane at a row's end with fewer than 8
 // columns left takes the row's last 8: it leaves those of the lane before out of
 // its group's maximum, and stores them once more with the same values.  SHORT:
 // rows of fewer than 8 columns, one element at a time.
 // PACKX: x too, not lo alone (a block's pre-map has packed it already).
-template <typename WALK, bool SHORT, bool PACKX>
+// RES: lo is round(res + lo), the residual around a block's norm and layer, summed
+// here (T = 65536, C = 1024 257 -> 280 us; PyTorch's addition by itself 68).
+template <typename WALK, bool SHORT, bool PACKX, bool RES>
 __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
     const uint16_t* __restrict__ x, const uint16_t* __restrict__ lo, const float* __restrict__ H,
     const float* __restrict__ h_post, uint16_t* __restrict__ out, int8_t* __restrict__ xq, uint8_t* __restrict__ xs,
-    int8_t* __restrict__ lq, uint8_t* __restrict__ ls, int64_t T, int C) {
+    int8_t* __restrict__ lq, uint8_t* __restrict__ ls, int64_t T, int C, const uint16_t* __restrict__ res) {
   constexpr int LPT = WALK::LPT;
   constexpr bool LOOP = WALK::LOOP, WHOLE = WALK::WHOLE;
   static_assert(LPT % 4 == 0, "a group's quad of lanes");
@@ -142,9 +144,15 @@ __global__ __launch_bounds__(block_of<WALK::LPT>()) void k4_fwd_pack8_kernel(
         Lanes<8, WHOLE>::load(row + c, 0, f);
       }
     };
+    float rv[RES ? 8 : 1];
     fetch(lrow, v[0]);
+    if constexpr (RES) fetch(res + tok * C, rv);
 #pragma unroll
     for (int j = 0; j < 4; ++j) fetch(x0 + j * int64_t{C}, v[1 + j]);
+    if constexpr (RES) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[0][e] = bf16_to_f32(f32_to_bf16(rv[e] + v[0][e]));
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float o[8];
@@ -395,25 +403,29 @@ int launch_k4_fwd(const uint16_t* x, const uint16_t* lo, const float* H, const f
 }
 
 int launch_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* hp, uint16_t* out,
-                        int8_t* xq, uint8_t* xs, int8_t* lq, uint8_t* ls, int64_t T, int C, hipStream_t s) {
-  // (A null xq counts as aligned.)
-  const bool aligned = C % 8 == 0 && aligned16(x) && aligned16(lo) && aligned16(out) && Pack8Src::aligned(xq) &&
-                       Pack8Src::aligned(lq);
+                        int8_t* xq, uint8_t* xs, int8_t* lq, uint8_t* ls, int64_t T, int C, hipStream_t s,
+                        const uint16_t* res = nullptr) {
+  // (A null xq or res counts as aligned.)
+  const bool aligned = C % 8 == 0 && aligned16(x) && aligned16(lo) && aligned16(out) && aligned16(res) &&
+                       Pack8Src::aligned(xq) && Pack8Src::aligned(lq);
   const int G = pack_groups(C);
   // Lanes for whole groups of 32 columns.
   auto run = [&](auto w, auto few) {
     using Walk = decltype(w);
     constexpr int L = Walk::LPT;
-    auto launch = [&](auto packx) {
-      constexpr bool PX = decltype(packx)::value;
+    auto launch = [&](auto packx, auto add) {
+      constexpr bool PX = decltype(packx)::value, RES = decltype(add)::value;
       for_launches(T, block_of<L>(), tokens_per_block(L), [&](int64_t t, int64_t n) {
         const dim3 grid(blocks_for(n, tokens_per_block(L)));
-        k4_fwd_pack8_kernel<Walk, decltype(few)::value, PX><<<grid, block_of<L>(), 0, s>>>(
+        k4_fwd_pack8_kernel<Walk, decltype(few)::value, PX, RES><<<grid, block_of<L>(), 0, s>>>(
             x + t * 4 * C, lo + t * C, H + t * 16, hp + t * 4, out + t * 4 * C, PX ? xq + t * 4 * C : nullptr,
-            PX ? xs + t * 4 * G : nullptr, lq + t * C, ls + t * G, n, C);
+            PX ? xs + t * 4 * G : nullptr, lq + t * C, ls + t * G, n, C, RES ? res + t * C : nullptr);
       });
     };
-    xq ? launch(std::true_type{}) : launch(std::false_type{});
+    if (!xq)
+      launch(std::false_type{}, std::false_type{});
+    else
+      res ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
   };
   if (C < 8)
     run(RowWalk<8, false, false>{}, std::true_type{});
@@ -523,4 +535,17 @@ extern "C" int fmhc_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const fl
     return FMHC_ERR_INVALID_ARGUMENT;
   return launch_k4_fwd_pack8(x, lo, H, h_post, out, x_codes, x_scales, lo_codes, lo_scales, T, static_cast<int>(C),
                              static_cast<hipStream_t>(stream));
+}
+
+extern "C" int fmhc_k4_fwd_pack8_residual(const uint16_t* x, const uint16_t* lo, const uint16_t* residual,
+                                          const float* H, const float* h_post, uint16_t* out, int8_t* x_codes,
+                                          uint8_t* x_scales, int8_t* lo_codes, uint8_t* lo_scales, int64_t T, int64_t C,
+                                          int64_t n, void* stream) {
+  using namespace fmhc;
+  if (bad_sizes(T, C, n)) return FMHC_ERR_INVALID_ARGUMENT;
+  if (T == 0) return FMHC_OK;
+  if (!x || !lo || !residual || !H || !h_post || !out || !x_codes || !x_scales || !lo_codes || !lo_scales)
+    return FMHC_ERR_INVALID_ARGUMENT;
+  return launch_k4_fwd_pack8(x, lo, H, h_post, out, x_codes, x_scales, lo_codes, lo_scales, T, static_cast<int>(C),
+                             static_cast<hipStream_t>(stream), residual);
 }

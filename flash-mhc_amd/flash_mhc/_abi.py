@@ -48,6 +48,7 @@ SIGNATURES: dict[str, list] = {
     "fmhc_pack8": [_P, _INT, _P, _P, _I64, _I64, _P],
     "fmhc_unpack8": [_P, _P, _P, _INT, _I64, _I64, _P],
     "fmhc_k4_fwd_pack8": [_P] * 9 + [_I64] * 3 + [_P],
+    "fmhc_k4_fwd_pack8_residual": [_P] * 10 + [_I64] * 3 + [_P],
     "fmhc_k4_bwd_pack8": [_P] * 11 + [_I64] * 3 + [_P],
     "fmhc_k1_bwd_pack8": [_P] * 9 + [_I64] * 4 + [_P],
     "fmhc_k1_bwd_pack8_workspace_bytes": [_I64, _I64],

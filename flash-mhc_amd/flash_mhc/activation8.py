@@ -359,15 +359,18 @@ class _PreMapEager(torch.autograd.Function):
 
 class _PostResEager(torch.autograd.Function):
     """mhc_post_res without the op's dispatch, which packs x and the layer output
-    in its own pass (fused_post_res_pack8's kernel): x's gradient goes to x_sink."""
+    in its own pass (fused_post_res_pack8's kernel): x's gradient goes to x_sink.
+    With a residual the layer output is residual + layer_output."""
 
     @staticmethod
-    def forward(ctx, x_streams, x_sink, layer_output, H_merged, h_post, kept):
+    def forward(ctx, x_streams, x_sink, layer_output, H_merged, h_post, kept, residual):
         if x_streams._version != kept.version:
             raise RuntimeError("the streams were modified by an inplace operation between the block's pre-map and "
                                "post-res, which both need them")
-        out, *codes = _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post)
+        out, *codes = _k.k4_fwd_pack8(x_streams.contiguous(), layer_output.contiguous(), _coeff(H_merged),
+                                      _coeff(h_post), residual=None if residual is None else residual.contiguous())
         ctx.kept = kept
+        ctx.residual = residual is not None
         kept.post = weakref.ref(ctx)
         ctx.save_for_backward(*codes, H_merged, h_post)
         return out
@@ -378,7 +381,7 @@ class _PostResEager(torch.autograd.Function):
         *codes, H_merged, h_post = ctx.saved_tensors
         ctx.kept.codes = codes[:2]
         g_x, g_lo, g_H, g_hp = _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
-        return None, g_x, g_lo, g_H, g_hp, None
+        return None, g_x, g_lo, g_H, g_hp, None, g_lo if ctx.residual else None
 
 
 def pre_map_eager(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat):
@@ -389,9 +392,13 @@ def pre_map_eager(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat
     return (*_PreMapEager.apply(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, kept), kept)
 
 
-def post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept):
-    """mhc_post_res, recorded for autograd without the op's dispatch, keeping codes."""
-    return _PostResEager.apply(x_streams, x_sink, layer_output, H_merged, h_post, kept)
+def post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept, residual=None):
+    """mhc_post_res of layer_output, or of residual + layer_output, recorded for
+    autograd without the op's dispatch, keeping codes."""
+    if residual is not None and (layer_output.shape != residual.shape or layer_output.dtype is not residual.dtype
+                                 or layer_output.device != residual.device):
+        layer_output, residual = residual + layer_output, None  # as PyTorch adds them
+    return _PostResEager.apply(x_streams, x_sink, layer_output, H_merged, h_post, kept, residual)
 
 
 # ---------------------------------------------------------------------------

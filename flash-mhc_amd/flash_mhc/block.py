@@ -172,15 +172,21 @@ class MHCLiteBlock(nn.Module):
             and x_streams.requires_grad
         )
 
-    def _apply_layer(self, layer_input: torch.Tensor, kwargs) -> torch.Tensor:
-        """The layer, with pre_norm around it: u + F(norm(u))."""
+    def _layer_and_residual(self, layer_input: torch.Tensor, kwargs):
+        """(the layer's output, what is added to it): pre_norm gives F(norm(u)) and u,
+        otherwise there is no residual (None)."""
         if self.norm is None:
-            return self.layer(layer_input, **kwargs)
+            return self.layer(layer_input, **kwargs), None
         with_residual = getattr(self.norm, "with_residual", None)
         if with_residual is None:  # another module put in the norm's place
-            return layer_input + self.layer(self.norm(layer_input), **kwargs)
+            return self.layer(self.norm(layer_input), **kwargs), layer_input
         normed, residual = with_residual(layer_input)
-        return residual + self.layer(normed, **kwargs)
+        return self.layer(normed, **kwargs), residual
+
+    def _apply_layer(self, layer_input: torch.Tensor, kwargs) -> torch.Tensor:
+        """The layer, with pre_norm around it: u + F(norm(u))."""
+        layer_output, residual = self._layer_and_residual(layer_input, kwargs)
+        return layer_output if residual is None else residual + layer_output
 
     def _coefficients(
         self, proj: torch.Tensor, dt: torch.dtype
@@ -337,8 +343,8 @@ class MHCLiteBlock(nn.Module):
             layer_input, H_merged, h_post, x_sink, kept = _a8.pre_map_eager(
                 x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
                 self.W_all.bias, self._buffers["perm_mat"])
-            layer_output = self._apply_layer(layer_input, kwargs)
-            return _a8.post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept)
+            layer_output, residual = self._layer_and_residual(layer_input, kwargs)
+            return _a8.post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept, residual)
         layer_input, H_merged, h_post, x_sink = _ops.pre_map_eager(
             x_streams, self._projection_weight(x_streams.dtype), p["alpha_pre"], p["alpha_post"], p["alpha_res"],
             self.W_all.bias, self._buffers["perm_mat"])

@@ -607,9 +607,10 @@ def unpack8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = _BF1
 
 
 def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: torch.Tensor, h_post: torch.Tensor,
-                 pack_x: bool = True):
+                 pack_x: bool = True, residual: torch.Tensor | None = None):
     """k4_fwd's out with x_streams (unless pack_x is false) and layer_output packed
-    in the same pass: (out, x_codes, x_scales, lo_codes, lo_scales)."""
+    in the same pass: (out, x_codes, x_scales, lo_codes, lo_scales).  With a
+    residual (T, C), and pack_x, residual + layer_output takes layer_output's place."""
     dev = _device_of(x_streams)
     T, n, C = _streams_shape(x_streams)
     _require(x_streams, "x_streams", _BF16, (T, n, C), dev)
@@ -619,6 +620,14 @@ def k4_fwd_pack8(x_streams: torch.Tensor, layer_output: torch.Tensor, H_merged: 
     out = torch.empty_like(x_streams)
     xq, xs = empty_packed(x_streams) if pack_x else (None, None)
     lq, ls = empty_packed(layer_output)
+    if residual is not None:
+        _require(residual, "residual", _BF16, (T, C), dev)
+        if not pack_x:
+            raise ValueError("k4_fwd_pack8 takes a residual where it packs x_streams")
+        _launch("k4_fwd_pack8_residual", dev, _abi.load().fmhc_k4_fwd_pack8_residual, x_streams.data_ptr(),
+                layer_output.data_ptr(), residual.data_ptr(), H_merged.data_ptr(), h_post.data_ptr(), out.data_ptr(),
+                xq.data_ptr(), xs.data_ptr(), lq.data_ptr(), ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))
+        return out, xq, xs, lq, ls
     _launch("k4_fwd_pack8", dev, _abi.load().fmhc_k4_fwd_pack8, x_streams.data_ptr(), layer_output.data_ptr(),
             H_merged.data_ptr(), h_post.data_ptr(), out.data_ptr(), _ptr_or_none(xq), _ptr_or_none(xs), lq.data_ptr(),
             ls.data_ptr(), T, C, n, _abi.stream_of(x_streams))

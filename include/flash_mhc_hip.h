@@ -270,6 +270,12 @@ int fmhc_unpack8(const int8_t* codes, const uint8_t* scales, void* x, int dtype,
 int fmhc_k4_fwd_pack8(const uint16_t* x, const uint16_t* lo, const float* H, const float* h_post,
                       uint16_t* out, int8_t* x_codes, uint8_t* x_scales, int8_t* lo_codes,
                       uint8_t* lo_scales, int64_t T, int64_t C, int64_t n, void* stream);
+/* The same for the layer output round(residual + lo), residual (T, C): a layer
+ * with a residual around it.  Its codes are those of the sum. */
+int fmhc_k4_fwd_pack8_residual(const uint16_t* x, const uint16_t* lo, const uint16_t* residual,
+                               const float* H, const float* h_post, uint16_t* out, int8_t* x_codes,
+                               uint8_t* x_scales, int8_t* lo_codes, uint8_t* lo_scales, int64_t T,
+                               int64_t C, int64_t n, void* stream);
 /* fmhc_k4_bwd from packed x and lo: the bits that fmhc_k4_bwd gives for the
  * unpacked tensors. */
 int fmhc_k4_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const int8_t* lo_codes,

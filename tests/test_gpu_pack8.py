@@ -737,3 +737,53 @@ def test_block_options_eager_and_compiled(kw):
     same(o, out)
     for a, b in zip(torch.autograd.grad(o, [wide, *blk.parameters()], g.transpose(1, 2).contiguous().transpose(1, 2)), want):
         same(a, b)
+
+
+@pytest.mark.parametrize("T,C", SIZES)
+def test_post_res_with_residual(T, C):
+    """The bits of post-res of the added tensors, rows of every kind."""
+    from flash_mhc import kernels as K
+
+    x, lo, H, hp, _go = mix_inputs(T, C)
+    r = rnd((T, C), 77).to(DEV)
+    for a, b in zip(K.k4_fwd_pack8(x, lo, H, hp, residual=r), K.k4_fwd_pack8(x, r + lo, H, hp)):
+        same(a, b)
+    off = torch.empty(T * C + 1, device=DEV, dtype=BF16)[1:].view(T, C).copy_(r)  # 2 bytes off
+    for a, b in zip(K.k4_fwd_pack8(x, lo, H, hp, residual=off), K.k4_fwd_pack8(x, r + lo, H, hp)):
+        same(a, b)
+    with pytest.raises(ValueError, match="packs x_streams"):
+        K.k4_fwd_pack8(x, lo, H, hp, pack_x=False, residual=r)
+
+
+class Layer(torch.nn.Module):
+    """A layer with an output of another dtype, another shape, or its input itself."""
+
+    def __init__(self, C, kind):
+        super().__init__()
+        self.lin, self.kind = torch.nn.Linear(C, C, bias=False), kind
+
+    def forward(self, u):
+        if self.kind == "input":
+            return u
+        out = self.lin(u)
+        return {"wide": out.to(torch.bfloat16)[None].squeeze(0), "row": out.mean(0, keepdim=True),
+                "strided": out.t().contiguous().t(), "frozen": out.detach()}[self.kind]
+
+
+@pytest.mark.parametrize("kind", ["input", "wide", "row", "strided", "frozen"])
+def test_block_residual_kinds(kind):
+    """pre_norm in 8 bits: the residual is added in post-res where it can be, with
+    the bits of PyTorch's addition (the op path)."""
+    T, C = 37, 96
+    torch.manual_seed(0)
+    blk = flash_mhc.MHCLiteBlock(4, C, Layer(C, kind), activation_bits=8, pre_norm=True).to(DEV).to(BF16)
+    x, g = streams(T, C, 2).to(DEV), rnd((T, 4, C), 3).to(DEV)
+    xs = x.clone().requires_grad_(True)
+    leaves = [xs, *(p for n, p in blk.named_parameters() if n.startswith(("W_all", "alpha")))]
+    got = blk(xs)
+    gg = torch.autograd.grad(got, leaves, g)
+    torch._dynamo.reset()
+    want = torch.compile(blk, fullgraph=True, backend="aot_eager")(xs)
+    same(got, want)
+    for a, b in zip(gg, torch.autograd.grad(want, leaves, g)):
+        same(a, b)

@@ -47,6 +47,9 @@ F = _FAKE
         lambda L: L.fmhc_k4_fwd_pack8(*[F] * 9, 2, 8, 3, None),  # n != 4
         lambda L: L.fmhc_k4_fwd_pack8(*[F] * 8, None, 2, 8, 4, None),
         lambda L: L.fmhc_k4_fwd_pack8(*[F] * 9, 2, 0, 4, None),
+        lambda L: L.fmhc_k4_fwd_pack8_residual(*[F] * 10, 2, 8, 3, None),
+        lambda L: L.fmhc_k4_fwd_pack8_residual(*[F] * 2, None, *[F] * 7, 2, 8, 4, None),
+        lambda L: L.fmhc_k4_fwd_pack8_residual(*[F] * 6, None, *[F] * 3, 2, 8, 4, None),
         lambda L: L.fmhc_k4_bwd_pack8(*[F] * 11, -2, 8, 4, None),
         lambda L: L.fmhc_k4_bwd_pack8(F, None, *[F] * 9, 2, 8, 4, None),
         lambda L: L.fmhc_k1_bwd_pack8(*[F] * 9, 1 << 40, 2, 8, 5, None),
