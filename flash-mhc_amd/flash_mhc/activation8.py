@@ -28,7 +28,6 @@ import weakref
 
 import torch
 import torch.library
-from torch.autograd.function import once_differentiable
 
 from . import block as _block  # which imports this module: its names are read at call time
 from . import kernels as _k
@@ -39,6 +38,7 @@ from .ops import (
     _mhc_pre_map_cuda,
     _mhc_pre_map_fake,
     _params,
+    differentiable_once,
 )
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
@@ -242,17 +242,6 @@ torch.library.register_autograd("flash_mhc::fused_post_res_pack8_traced", _fused
                                 setup_context=_setup_post_res)
 
 
-def _eager_post_res_backward(ctx, grad_out, *_codes):
-    if grad_out is None:
-        return None, None, None, None
-    *codes, H_merged, h_post = ctx.saved_tensors
-    return _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
-
-
-# For a graph of the gradients: raises where that graph is used.
-_eager_post_res_backward_once = once_differentiable(_eager_post_res_backward)
-
-
 class _FusedPostResEager(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_streams, layer_output, H_merged, h_post):
@@ -263,8 +252,12 @@ class _FusedPostResEager(torch.autograd.Function):
         return outs
 
     @staticmethod
-    def backward(ctx, *grads):
-        return (_eager_post_res_backward_once if torch.is_grad_enabled() else _eager_post_res_backward)(ctx, *grads)
+    @differentiable_once
+    def backward(ctx, grad_out, *_codes):
+        if grad_out is None:
+            return None, None, None, None
+        *codes, H_merged, h_post = ctx.saved_tensors
+        return _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
 
 
 @torch.library.impl(_lib, "fused_post_res_pack8", "AutogradCUDA")
@@ -350,7 +343,7 @@ class _PreMapEager(torch.autograd.Function):
         return li, H, hq, x_sink
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, g_li, g_H, g_hq, g_sink):
         saved = ctx.saved_tensors
         grads = _mhc_pre_map_backward_pack8_cuda(g_li, g_H, g_hq, None, None, g_sink, *ctx.kept.take(), *saved)
@@ -376,7 +369,7 @@ class _PostResEager(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad_out):
         *codes, H_merged, h_post = ctx.saved_tensors
         ctx.kept.codes = codes[:2]

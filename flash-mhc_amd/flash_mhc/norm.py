@@ -14,11 +14,11 @@ import torch
 import torch.library
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import kernels as _k
 from .activation8 import _packed_like
 from .block import _plain_eager
+from .ops import differentiable_once
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
@@ -111,14 +111,11 @@ torch.library.register_autograd("flash_mhc::layer_norm", _backward, setup_contex
 torch.library.register_autograd("flash_mhc::layer_norm_pack8", _backward, setup_context=_setup)
 
 
-# The two eager Functions' backward.  With a graph of the gradients (create_graph)
-# it goes through once_differentiable, which raises where that graph is used; the
-# check is cheaper than its wrapper, and a step of few rows is bound by the host.
+# The two eager Functions' backward.
 
 
-def _eager_backward(ctx, grad_y, grad_x=None):
-    if grad_y is None:  # the norm's output was not used
-        return grad_x, None, None, None, None
+@differentiable_once
+def _eager_gradients(ctx, grad_y, grad_x):
     x, codes, scales, stats, weight = ctx.saved_tensors
     _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
     gx, gw, gb = _k.layer_norm_bwd_joint(grad_y.contiguous(), x, codes, scales, stats, weight, ctx.param_dtype,
@@ -126,7 +123,10 @@ def _eager_backward(ctx, grad_y, grad_x=None):
     return gx, gw, gb, None, None
 
 
-_eager_backward_once = once_differentiable(_eager_backward)
+def _eager_backward(ctx, grad_y, grad_x=None):
+    if grad_y is None:  # the norm's output was not used: x's gradient is the residual's
+        return grad_x, None, None, None, None
+    return _eager_gradients(ctx, grad_y, grad_x)
 
 
 class _LayerNormEager(torch.autograd.Function):
@@ -142,7 +142,7 @@ class _LayerNormEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y):
-        return (_eager_backward_once if torch.is_grad_enabled() else _eager_backward)(ctx, grad_y)
+        return _eager_backward(ctx, grad_y)
 
 
 class _LayerNormResidualEager(torch.autograd.Function):
@@ -156,7 +156,7 @@ class _LayerNormResidualEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y, grad_x):
-        return (_eager_backward_once if torch.is_grad_enabled() else _eager_backward)(ctx, grad_y, grad_x)
+        return _eager_backward(ctx, grad_y, grad_x)
 
 
 def _check(x, weight, bias, activation_bits) -> None:

@@ -34,6 +34,7 @@ Additions (not in the reference):
 
 from __future__ import annotations
 
+import functools
 import os
 from contextlib import contextmanager
 
@@ -435,6 +436,41 @@ def _fused_post_res_backward_cuda(grad_out, x_streams, layer_output, H_merged, h
     _check_n4(x_streams, "flash_mhc::fused_post_res_backward supports n=4 only")
     return _k.k4_bwd(grad_out.contiguous(), x_streams.contiguous(), layer_output.contiguous(),
                      _coeff(H_merged), _coeff(h_post))
+
+
+# ---------------------------------------------------------------------------
+# Backward passes without a derivative.
+
+
+class _Once(torch.autograd.Function):
+    """The gradients unchanged, in a graph that raises where it is used."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("flash_mhc: a gradient of this gradient was asked for, but the operator's backward is "
+                           "once_differentiable")
+
+
+def differentiable_once(backward):
+    """backward(ctx, *grads) of an autograd Function or a registered op whose
+    gradients have no derivative.  They depend on what the forward kept whether or
+    not a gradient that came in requires grad (a linear loss, grad_outputs), so
+    where a graph of them is recorded each is made to raise in it: otherwise they
+    would count as constants there and the terms be lost."""
+
+    @functools.wraps(backward)
+    def once(ctx, *grads):
+        if not torch.is_grad_enabled():  # an ordinary backward
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        return _Once.apply(torch.zeros((), requires_grad=True), *out)
+
+    return once
 
 
 # ---------------------------------------------------------------------------
