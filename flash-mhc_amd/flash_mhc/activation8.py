@@ -39,6 +39,8 @@ from .ops import (
     _mhc_pre_map_fake,
     _params,
     differentiable_once,
+    graph_link,
+    register_no_autograd,
 )
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
@@ -227,15 +229,16 @@ def _mhc_post_res_pack8_cuda(x_streams, x_sink, x_codes, x_scales, layer_output,
 
 
 def _setup_post_res(ctx, inputs, output):
-    _x, _lo, H_merged, h_post = inputs
-    ctx.save_for_backward(*output[1:], H_merged, h_post)
+    x, lo, H_merged, h_post = inputs
+    ctx.save_for_backward(*output[1:], H_merged, h_post, graph_link(x, lo))
     ctx.set_materialize_grads(False)
 
 
+@differentiable_once
 def _fused_post_res_pack8_backward(ctx, grad_out, *_codes):
     if grad_out is None:
         return None, None, None, None
-    return torch.ops.flash_mhc.fused_post_res_backward_pack8(grad_out, *ctx.saved_tensors)
+    return torch.ops.flash_mhc.fused_post_res_backward_pack8(grad_out, *ctx.saved_tensors[:-1])
 
 
 torch.library.register_autograd("flash_mhc::fused_post_res_pack8_traced", _fused_post_res_pack8_backward,
@@ -246,24 +249,25 @@ class _FusedPostResEager(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_streams, layer_output, H_merged, h_post):
         outs = _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post)
-        ctx.save_for_backward(*outs[1:], H_merged, h_post)
+        link = x_streams.new_empty(0)  # a last output, kept for differentiable_once
+        ctx.save_for_backward(*outs[1:], H_merged, h_post, link)
         ctx.mark_non_differentiable(*outs[1:])
         ctx.set_materialize_grads(False)
-        return outs
+        return (*outs, link)
 
     @staticmethod
     @differentiable_once
     def backward(ctx, grad_out, *_codes):
         if grad_out is None:
             return None, None, None, None
-        *codes, H_merged, h_post = ctx.saved_tensors
+        *codes, H_merged, h_post, _link = ctx.saved_tensors
         return _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
 
 
 @torch.library.impl(_lib, "fused_post_res_pack8", "AutogradCUDA")
 def _fused_post_res_pack8_autograd(x_streams, layer_output, H_merged, h_post):
     if _block._plain_eager(x_streams):
-        return _FusedPostResEager.apply(x_streams, layer_output, H_merged, h_post)
+        return _FusedPostResEager.apply(x_streams, layer_output, H_merged, h_post)[:-1]
     return torch.ops.flash_mhc.fused_post_res_pack8_traced(x_streams, layer_output, H_merged, h_post)
 
 
@@ -274,6 +278,7 @@ def _setup_pre_map(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
+@differentiable_once
 def _mhc_pre_map_pack8_backward(ctx, g_li, g_H, g_hq, g_hpre, g_proj, _g_inv, g_sink, _gc, _gs):
     grads = torch.ops.flash_mhc.mhc_pre_map_backward_pack8(g_li, g_H, g_hq, g_hpre, g_proj, g_sink, *ctx.saved_tensors)
     return (*grads, None)
@@ -284,21 +289,26 @@ torch.library.register_autograd("flash_mhc::mhc_pre_map_pack8", _mhc_pre_map_pac
 
 
 def _setup_mhc_post_res(ctx, inputs, output):
-    _x, _sink, codes, scales, _lo, H_merged, h_post = inputs
+    _x, x_sink, codes, scales, lo, H_merged, h_post = inputs
     _out, lo_codes, lo_scales = output
-    ctx.save_for_backward(codes, scales, lo_codes, lo_scales, H_merged, h_post)
+    ctx.save_for_backward(codes, scales, lo_codes, lo_scales, H_merged, h_post, graph_link(x_sink, lo))
     ctx.set_materialize_grads(False)
 
 
+@differentiable_once
 def _mhc_post_res_pack8_backward(ctx, grad_out, _gc, _gs):
     if grad_out is None:
         return (None,) * 7
-    g_x, g_lo, g_H, g_hp = torch.ops.flash_mhc.fused_post_res_backward_pack8(grad_out, *ctx.saved_tensors)
+    g_x, g_lo, g_H, g_hp = torch.ops.flash_mhc.fused_post_res_backward_pack8(grad_out, *ctx.saved_tensors[:-1])
     return None, g_x, None, None, g_lo, g_H, g_hp  # x's gradient goes to the sink
 
 
 torch.library.register_autograd("flash_mhc::mhc_post_res_pack8", _mhc_post_res_pack8_backward,
                                 setup_context=_setup_mhc_post_res)
+
+
+for _op in ("fused_post_res_backward_pack8", "fused_rmsnorm_project_bwd_pack8", "mhc_pre_map_backward_pack8"):
+    register_no_autograd(_op)
 
 
 class _Kept:
@@ -338,14 +348,15 @@ class _PreMapEager(torch.autograd.Function):
         li, H, hq, h_pre, proj, inv_rms, x_sink = _mhc_pre_map_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res,
                                                                      bias, perm_mat)
         ctx.kept = kept
-        ctx.save_for_backward(W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre, proj, inv_rms)
+        # (x_sink, an output, for differentiable_once)
+        ctx.save_for_backward(W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre, proj, inv_rms, x_sink)
         ctx.set_materialize_grads(False)
         return li, H, hq, x_sink
 
     @staticmethod
     @differentiable_once
     def backward(ctx, g_li, g_H, g_hq, g_sink):
-        saved = ctx.saved_tensors
+        *saved, _sink = ctx.saved_tensors
         grads = _mhc_pre_map_backward_pack8_cuda(g_li, g_H, g_hq, None, None, g_sink, *ctx.kept.take(), *saved)
         return (*grads, None, None)
 
@@ -365,13 +376,17 @@ class _PostResEager(torch.autograd.Function):
         ctx.kept = kept
         ctx.residual = residual is not None
         kept.post = weakref.ref(ctx)
-        ctx.save_for_backward(*codes, H_merged, h_post)
-        return out
+        link = out.new_empty(0)  # a second output, kept for differentiable_once
+        ctx.save_for_backward(*codes, H_merged, h_post, link)
+        ctx.set_materialize_grads(False)
+        return out, link
 
     @staticmethod
     @differentiable_once
-    def backward(ctx, grad_out):
-        *codes, H_merged, h_post = ctx.saved_tensors
+    def backward(ctx, grad_out, _link):
+        if grad_out is None:
+            return (None,) * 7
+        *codes, H_merged, h_post, _link = ctx.saved_tensors
         ctx.kept.codes = codes[:2]
         g_x, g_lo, g_H, g_hp = _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
         return None, g_x, g_lo, g_H, g_hp, None, g_lo if ctx.residual else None
@@ -391,7 +406,7 @@ def post_res_eager(x_streams, x_sink, layer_output, H_merged, h_post, kept, resi
     if residual is not None and (layer_output.shape != residual.shape or layer_output.dtype is not residual.dtype
                                  or layer_output.device != residual.device):
         layer_output, residual = residual + layer_output, None  # as PyTorch adds them
-    return _PostResEager.apply(x_streams, x_sink, layer_output, H_merged, h_post, kept, residual)
+    return _PostResEager.apply(x_streams, x_sink, layer_output, H_merged, h_post, kept, residual)[0]
 
 
 # ---------------------------------------------------------------------------

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from . import kernels as _k
 from .activation8 import _packed_like
 from .block import _plain_eager
-from .ops import differentiable_once
+from .ops import differentiable_once, register_no_autograd
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
@@ -93,6 +93,7 @@ def _setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
+@differentiable_once
 def _backward(ctx, grad_y, *_rest):
     # mean and rstd are not differentiable.
     if grad_y is None:
@@ -109,6 +110,7 @@ def _backward(ctx, grad_y, *_rest):
 
 torch.library.register_autograd("flash_mhc::layer_norm", _backward, setup_context=_setup)
 torch.library.register_autograd("flash_mhc::layer_norm_pack8", _backward, setup_context=_setup)
+register_no_autograd("layer_norm_backward")
 
 
 # The two eager Functions' backward.
@@ -116,7 +118,7 @@ torch.library.register_autograd("flash_mhc::layer_norm_pack8", _backward, setup_
 
 @differentiable_once
 def _eager_gradients(ctx, grad_y, grad_x):
-    x, codes, scales, stats, weight = ctx.saved_tensors
+    x, codes, scales, stats, weight = ctx.saved_tensors  # (stats: an output where x is not kept, for the graph's sake)
     _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
     gx, gw, gb = _k.layer_norm_bwd_joint(grad_y.contiguous(), x, codes, scales, stats, weight, ctx.param_dtype,
                                          need_weight, need_bias, _dense(grad_x))
@@ -129,33 +131,39 @@ def _eager_backward(ctx, grad_y, grad_x=None):
     return _eager_gradients(ctx, grad_y, grad_x)
 
 
+def _eager_forward(ctx, x, weight, bias, eps, packed):
+    ctx.set_materialize_grads(False)
+    x, weight = x.contiguous(), _dense(weight)
+    y, stats, codes, scales, ctx.param_dtype = _k.layer_norm_fwd_joint(x, weight, _dense(bias), eps, packed)
+    ctx.save_for_backward(None if packed else x, codes, scales, stats, weight)
+    return y, stats
+
+
 class _LayerNormEager(torch.autograd.Function):
     """layer_norm / layer_norm_pack8 with their registered autograd, without the
-    ops' dispatch."""
+    ops' dispatch: (y, stats) where packed, otherwise y."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, packed):
-        x, weight = x.contiguous(), _dense(weight)
-        y, stats, codes, scales, ctx.param_dtype = _k.layer_norm_fwd_joint(x, weight, _dense(bias), eps, packed)
-        ctx.save_for_backward(None if packed else x, codes, scales, stats, weight)
-        return y
+        y, stats = _eager_forward(ctx, x, weight, bias, eps, packed)
+        return (y, stats) if packed else y
 
     @staticmethod
-    def backward(ctx, grad_y):
+    def backward(ctx, grad_y, _stats=None):
         return _eager_backward(ctx, grad_y)
 
 
 class _LayerNormResidualEager(torch.autograd.Function):
-    """(layer_norm(x), x): the gradient of the second, which the residual around a
-    block's layer gives, is added in the norm's backward."""
+    """(layer_norm(x), x, and stats where packed): the gradient of the second, which
+    the residual around a block's layer gives, is added in the norm's backward."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, packed):
-        ctx.set_materialize_grads(False)
-        return _LayerNormEager.forward(ctx, x, weight, bias, eps, packed), x.view_as(x)
+        y, stats = _eager_forward(ctx, x, weight, bias, eps, packed)
+        return (y, x.view_as(x), stats) if packed else (y, x.view_as(x))
 
     @staticmethod
-    def backward(ctx, grad_y, grad_x):
+    def backward(ctx, grad_y, grad_x, _stats=None):
         return _eager_backward(ctx, grad_y, grad_x)
 
 
@@ -182,7 +190,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if (packed or activation_bits == 16) and _plain_eager(x):  # the kernels' launchers check the tensors
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                         or (bias is not None and bias.requires_grad)):
-            return _LayerNormEager.apply(x, weight, bias, eps, packed)
+            out = _LayerNormEager.apply(x, weight, bias, eps, packed)
+            return out[0] if packed else out
         return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps, stats=False)[0]
     _check(x, weight, bias, activation_bits)
     op = torch.ops.flash_mhc.layer_norm_pack8 if packed else torch.ops.flash_mhc.layer_norm
@@ -236,7 +245,7 @@ class LayerNorm(nn.Module):
         gradient that x gets from the residual (as a separate addition would)."""
         if (_plain_eager(x) and torch.is_grad_enabled() and x.requires_grad and not self._hooked()
                 and self._on_kernels(x)):
-            return _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
+            return _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)[:2]
         return self(x), x
 
     def extra_repr(self) -> str:

@@ -443,11 +443,12 @@ def _fused_post_res_backward_cuda(grad_out, x_streams, layer_output, H_merged, h
 
 
 class _Once(torch.autograd.Function):
-    """The gradients unchanged, in a graph that raises where it is used."""
+    """tensors[links:] unchanged, in a graph that leads to tensors[:links] and raises
+    where it is used."""
 
     @staticmethod
-    def forward(ctx, anchor, *grads):
-        return grads
+    def forward(ctx, links, *tensors):
+        return tensors[links:]
 
     @staticmethod
     def backward(ctx, *grads):
@@ -455,12 +456,33 @@ class _Once(torch.autograd.Function):
                            "once_differentiable")
 
 
+class _Link(torch.autograd.Function):
+    """An empty tensor that leads to its inputs in a graph."""
+
+    @staticmethod
+    def forward(ctx, *tensors):
+        return tensors[0].new_empty(0)
+
+    backward = _Once.backward
+
+
+def graph_link(*tensors):
+    """For a forward that keeps none of some inputs: an empty tensor to keep in
+    their place (None in a compiled graph, which has no gradients of gradients)."""
+    if torch.compiler.is_compiling():
+        return None
+    with torch.enable_grad():
+        return _Link.apply(*tensors)
+
+
 def differentiable_once(backward):
     """backward(ctx, *grads) of an autograd Function or a registered op whose
     gradients have no derivative.  They depend on what the forward kept whether or
     not a gradient that came in requires grad (a linear loss, grad_outputs), so
     where a graph of them is recorded each is made to raise in it: otherwise they
-    would count as constants there and the terms be lost."""
+    would count as constants there and the terms be lost.  The graph has to lead to
+    every input that they depend on, since torch.autograd.grad runs no other
+    nodes: ctx keeps the input itself, an output, or a graph_link."""
 
     @functools.wraps(backward)
     def once(ctx, *grads):
@@ -468,9 +490,22 @@ def differentiable_once(backward):
             return backward(ctx, *grads)
         with torch.no_grad():
             out = backward(ctx, *grads)
-        return _Once.apply(torch.zeros((), requires_grad=True), *out)
+        links = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+        links.append(torch.zeros((), requires_grad=True))
+        return _Once.apply(len(links), *links, *out)
 
     return once
+
+
+def register_no_autograd(op: str) -> None:
+    """A backward op called by itself, with inputs that require grad: its outputs
+    raise where they are differentiated (without a formula, torch only warns and
+    takes them as constants)."""
+
+    def backward(ctx, *_grads):
+        raise RuntimeError(f"flash_mhc::{op} is a backward pass, which is once_differentiable: it has no derivative")
+
+    torch.library.register_autograd(f"flash_mhc::{op}", backward)
 
 
 # ---------------------------------------------------------------------------

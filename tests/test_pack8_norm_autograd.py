@@ -35,10 +35,13 @@ def dev(request, monkeypatch):
 
 
 def _twice(loss, leaf, match="once_differentiable"):
-    """loss + |grad loss|^2 differentiated; the first gradient is right to take."""
+    """The gradient of loss + |grad loss|^2, through all nodes and through those that lead to the leaf."""
     (g,) = torch.autograd.grad(loss, leaf, create_graph=True)
+    total = loss + g.float().square().sum()
     with pytest.raises(RuntimeError, match=match):
-        (loss + g.float().square().sum()).backward()
+        total.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match=match):
+        torch.autograd.grad(total, leaf)
 
 
 def _weights(y):
@@ -58,6 +61,9 @@ def test_layer_norm_once(dev, bits, score):
     x, w = _grad(rnd((5, 48), 1).to(dev)), rnd((48,), 2).to(dev)
     for weight in (w, _grad(w.clone()), None):
         _twice(SCORES[score](flash_mhc.layer_norm(x, weight, activation_bits=bits)), x)
+        # With respect to what is no leaf, and is not kept either.
+        u = x * 1.5
+        _twice(SCORES[score](flash_mhc.layer_norm(u * 1, weight, activation_bits=bits)), u)
     # A parameter's gradient too.
     weight = _grad(w.clone())
     _twice(SCORES[score](flash_mhc.layer_norm(x, weight, activation_bits=bits)), weight)
@@ -79,6 +85,15 @@ def test_norm_with_residual_once(dev, use, score):
         _twice(loss, x)
 
 
+def _mixed(out, leaves):
+    """grad_H with respect to x, and grad_h_post with respect to the layer output."""
+    x, lo, H, hp = leaves
+    gH, ghp = torch.autograd.grad(out.float().sum(), [H, hp], create_graph=True)
+    for g, t in ((gH, x), (ghp, lo)):
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            torch.autograd.grad(g.sum(), t, retain_graph=True)
+
+
 @pytest.mark.parametrize("score", SCORES)
 def test_post_res_once(dev, score):
     T, C = 6, 40
@@ -87,6 +102,11 @@ def test_post_res_once(dev, score):
     op = OPS.fused_post_res_pack8 if dev == "cuda" else lambda *a: flash_mhc.activation8._FusedPostResEager.apply(*a)
     for leaf in leaves:
         _twice(SCORES[score](op(*leaves)[0].float()), leaf)
+    inner = [t * 1.5 for t in leaves]
+    for t in inner:
+        _twice(SCORES[score](op(*(t * 1 for t in inner))[0].float()), t)
+    # grad_H depends on x and grad_h_post on the layer output.
+    _mixed(op(*leaves)[0], leaves)
 
 
 @pytest.mark.parametrize("score", SCORES)
@@ -96,6 +116,12 @@ def test_block_once(dev, kw, score):
     x = _grad(rnd((6, 4, 64), 3, dtype=BF16).to(dev))
     for leaf in (x, blk.W_all.weight, blk.layer.weight):
         _twice(SCORES[score](blk._forward_triton(x).float()), leaf)
+    u = x * 1.5
+    _twice(SCORES[score](blk._forward_triton(u * 1).float()), u)
+    # The gradient of a coefficient's bias depends on the layer's output.
+    (gb,) = torch.autograd.grad(SCORES[score](blk._forward_triton(x).float()), blk.W_all.bias, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(gb.float().sum(), blk.layer.weight)
 
 
 def test_gradients_with_a_graph_have_the_same_values(dev):
@@ -112,3 +138,77 @@ def test_gradients_with_a_graph_have_the_same_values(dev):
     y = flash_mhc.layer_norm(x, _grad(w.clone())) * p
     (gp,) = torch.autograd.grad(y.square().sum(), p, create_graph=True)  # 2 p sum y^2, not through the norm's backward
     torch.autograd.grad(gp.sum(), p)
+
+
+# The same through the registered ops: called by name, under a dispatch mode, with
+# tensor subclasses.
+
+
+@pytest.fixture(params=["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def opdev(request):
+    """The registered ops: on the CPU with stand-ins, on the GPU with the kernels."""
+    if request.param == "cpu":
+        with cpu.registered():
+            yield request.param
+    else:
+        yield request.param
+
+
+def premap_args(dev, C=32, T=6):
+    x, W = rnd((T, 4, C), 1, dtype=BF16), rnd((32, 4 * C), 2, 0.1, BF16)
+    alphas = [torch.tensor([a]) for a in (0.25, 0.375, 0.5)]
+    perm = flash_mhc.build_permutation_matrices(4)[0]
+    return [t.to(dev) for t in (x, W, *alphas, rnd((32,), 3, 0.1), perm)]
+
+
+@pytest.mark.parametrize("score", SCORES)
+@pytest.mark.parametrize("op", [OPS.layer_norm, OPS.layer_norm_pack8])
+def test_layer_norm_ops_once(opdev, op, score):
+    x, w = _grad(rnd((5, 48), 1).to(opdev)), rnd((48,), 2).to(opdev)
+    for weight in (w, _grad(w.clone()), None):
+        _twice(SCORES[score](op(x, weight, None, 1e-5)[0]), x)
+        u = x * 1.5
+        _twice(SCORES[score](op(u * 1, weight, None, 1e-5)[0]), u)
+
+
+@pytest.mark.parametrize("score", SCORES)
+def test_post_res_ops_once(opdev, score):
+    T, C = 6, 40
+    x, lo, H, hp = rnd((T, 4, C), 1, dtype=BF16), rnd((T, C), 2, dtype=BF16), rnd((T, 4, 4), 3), rnd((T, 4), 4)
+    leaves = [_grad(t.to(opdev)) for t in (x, lo, H, hp)]
+    op = OPS.fused_post_res_pack8_traced
+    for leaf in leaves:
+        _twice(SCORES[score](op(*leaves)[0].float()), leaf)
+    inner = [t * 1.5 for t in leaves]
+    for t in inner:
+        _twice(SCORES[score](op(*(t * 1 for t in inner))[0].float()), t)
+    _mixed(op(*leaves)[0], leaves)
+
+
+@pytest.mark.parametrize("score", SCORES)
+def test_block_ops_once(opdev, score):
+    x, *params, perm = premap_args(opdev)
+    leaves = [_grad(t) for t in (x, *params)]
+    li, H, hq, _hpre, _proj, _inv, sink, codes, scales = OPS.mhc_pre_map_pack8(*leaves, perm)
+    out = OPS.mhc_post_res_pack8(x, sink, codes, scales, li, H, hq)[0].float()
+    for leaf in leaves[:2]:
+        _twice(SCORES[score](out), leaf)
+
+
+def test_backward_ops_have_no_derivative(opdev):
+    """The backward ops themselves: called with inputs that require grad."""
+    T, C = 6, 32
+    x, W, ap, apo, ar, b, perm = premap_args(opdev)
+    g, w = _grad(rnd((T, C), 5, dtype=BF16).to(opdev)), rnd((C,), 6).to(opdev)
+    _y, mean, rstd, q, s = OPS.layer_norm_pack8(x[:, 0].contiguous(), w, None, 1e-5)
+    outs = [OPS.layer_norm_backward(g, None, q, s, mean, rstd, w, F32, True, True)]
+    li, H, hq, hpre, proj, inv, _sink, xq, xs = OPS.mhc_pre_map_pack8(x, W, ap, apo, ar, b, perm)
+    lq, ls = OPS.pack8(li)
+    outs.append(OPS.fused_post_res_backward_pack8(_grad(rnd((T, 4, C), 7, dtype=BF16).to(opdev)), xq, xs, lq, ls, H, hq))
+    outs.append(OPS.fused_rmsnorm_project_bwd_pack8(_grad(proj.clone()), xq, xs, W, proj, inv))
+    outs.append(OPS.mhc_pre_map_backward_pack8(g, None, None, None, None, None, xq, xs, W, ap, apo, ar, b, perm, hpre,
+                                               proj, inv))
+    for out in outs:
+        for t in out:
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                t.float().sum().backward(retain_graph=True)
