@@ -249,7 +249,7 @@ class _FusedPostResEager(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_streams, layer_output, H_merged, h_post):
         outs = _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post)
-        link = x_streams.new_empty(0)  # a last output, kept for differentiable_once
+        link = H_merged.new_empty(0)  # a last output, kept for differentiable_once
         ctx.save_for_backward(*outs[1:], H_merged, h_post, link)
         ctx.mark_non_differentiable(*outs[1:])
         ctx.set_materialize_grads(False)
@@ -348,15 +348,15 @@ class _PreMapEager(torch.autograd.Function):
         li, H, hq, h_pre, proj, inv_rms, x_sink = _mhc_pre_map_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res,
                                                                      bias, perm_mat)
         ctx.kept = kept
-        # (x_sink, an output, for differentiable_once)
-        ctx.save_for_backward(W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre, proj, inv_rms, x_sink)
+        # (h_post, an output that post-res keeps as well, for differentiable_once)
+        ctx.save_for_backward(W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre, proj, inv_rms, hq)
         ctx.set_materialize_grads(False)
         return li, H, hq, x_sink
 
     @staticmethod
     @differentiable_once
     def backward(ctx, g_li, g_H, g_hq, g_sink):
-        *saved, _sink = ctx.saved_tensors
+        *saved, _hq = ctx.saved_tensors
         grads = _mhc_pre_map_backward_pack8_cuda(g_li, g_H, g_hq, None, None, g_sink, *ctx.kept.take(), *saved)
         return (*grads, None, None)
 
@@ -376,7 +376,7 @@ class _PostResEager(torch.autograd.Function):
         ctx.kept = kept
         ctx.residual = residual is not None
         kept.post = weakref.ref(ctx)
-        link = out.new_empty(0)  # a second output, kept for differentiable_once
+        link = H_merged.new_empty(0)  # a second output, kept for differentiable_once
         ctx.save_for_backward(*codes, H_merged, h_post, link)
         ctx.set_materialize_grads(False)
         return out, link

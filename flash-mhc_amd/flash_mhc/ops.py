@@ -461,7 +461,7 @@ class _Link(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, *tensors):
-        return tensors[0].new_empty(0)
+        return tensors[0].new_empty(0, dtype=torch.float32)
 
     backward = _Once.backward
 

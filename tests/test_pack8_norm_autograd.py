@@ -41,7 +41,7 @@ def _twice(loss, leaf, match="once_differentiable"):
     with pytest.raises(RuntimeError, match=match):
         total.backward(retain_graph=True)
     with pytest.raises(RuntimeError, match=match):
-        torch.autograd.grad(total, leaf)
+        torch.autograd.grad(total, leaf, retain_graph=True)
 
 
 def _weights(y):
