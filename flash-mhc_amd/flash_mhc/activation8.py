@@ -41,6 +41,7 @@ from .ops import (
     differentiable_once,
     graph_link,
     register_no_autograd,
+    without_tangents,
 )
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
@@ -149,12 +150,14 @@ def _unpack8_cuda(codes, scales, dtype):
 
 @torch.library.impl(_lib, "fused_post_res_pack8_traced", "CUDA")
 @torch.library.impl(_lib, "fused_post_res_pack8", "CUDA")
+@without_tangents
 def _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post):
     _check_n4(x_streams, "flash_mhc::fused_post_res_pack8 supports n=4 only")
     return _k.k4_fwd_pack8(x_streams.contiguous(), layer_output.contiguous(), _coeff(H_merged), _coeff(h_post))
 
 
 @torch.library.impl(_lib, "fused_post_res_backward_pack8", "CUDA")
+@without_tangents
 def _fused_post_res_backward_pack8_cuda(grad_out, x_codes, x_scales, lo_codes, lo_scales, H_merged, h_post):
     _check_n4(x_codes, "flash_mhc::fused_post_res_backward_pack8 supports n=4 only")
     return _k.k4_bwd_pack8(grad_out.contiguous(), x_codes.contiguous(), x_scales.contiguous(), lo_codes.contiguous(),
@@ -162,6 +165,7 @@ def _fused_post_res_backward_pack8_cuda(grad_out, x_codes, x_scales, lo_codes, l
 
 
 @torch.library.impl(_lib, "fused_rmsnorm_project_bwd_pack8", "CUDA")
+@without_tangents
 def _fused_rmsnorm_project_bwd_pack8_cuda(grad_out, x_codes, x_scales, W, proj_out, inv_rms):
     _check_n4(x_codes, "flash_mhc::fused_rmsnorm_project_bwd_pack8 supports n=4 only")
     return _k.k1_bwd_pack8(grad_out.contiguous(), x_codes.contiguous(), x_scales.contiguous(),
@@ -169,6 +173,7 @@ def _fused_rmsnorm_project_bwd_pack8_cuda(grad_out, x_codes, x_scales, W, proj_o
 
 
 @torch.library.impl(_lib, "mhc_pre_map_pack8", "CUDA")
+@without_tangents
 def _mhc_pre_map_pack8_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat):
     _check_n4(x_streams, "flash_mhc::mhc_pre_map_pack8 supports n=4 only")
     x = x_streams.contiguous()
@@ -180,6 +185,7 @@ def _mhc_pre_map_pack8_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res, bias
 
 
 @torch.library.impl(_lib, "mhc_pre_map_backward_pack8", "CUDA")
+@without_tangents
 def _mhc_pre_map_backward_pack8_cuda(grad_layer_input, grad_H_merged, grad_h_post, grad_h_pre, grad_proj, grad_x_sink,
                                      x_codes, x_scales, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre,
                                      proj, inv_rms):
@@ -216,6 +222,7 @@ def _mhc_pre_map_backward_pack8_cuda(grad_layer_input, grad_H_merged, grad_h_pos
 
 
 @torch.library.impl(_lib, "mhc_post_res_pack8", "CUDA")
+@without_tangents
 def _mhc_post_res_pack8_cuda(x_streams, x_sink, x_codes, x_scales, layer_output, H_merged, h_post):
     _check_n4(x_streams, "flash_mhc::mhc_post_res_pack8 supports n=4 only")
     out, _xq, _xs, lo_codes, lo_scales = _k.k4_fwd_pack8(x_streams.contiguous(), layer_output.contiguous(),

@@ -269,6 +269,7 @@ class MHCLiteBlock(nn.Module):
             args = (x_streams, self._projection_weight(x_streams.dtype), self.alpha_pre, self.alpha_post,
                     self.alpha_res, self.W_all.bias, self.perm_mat)
             if self._keeps_codes():
+                _ops.refuse_tangents(*args)
                 layer_input, H_merged, h_post, _h_pre, _proj, _inv, x_sink, codes, scales = (
                     torch.ops.flash_mhc.mhc_pre_map_pack8(*args))
                 return layer_input, H_merged, h_post, x_sink if xgrad else x_streams, codes, scales

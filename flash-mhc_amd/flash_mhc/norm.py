@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from . import kernels as _k
 from .activation8 import _packed_like
 from .block import _plain_eager
-from .ops import differentiable_once, register_no_autograd
+from .ops import differentiable_once, refuse_tangents, register_no_autograd, without_tangents
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
@@ -60,16 +60,19 @@ def _dense(t):
 
 
 @torch.library.impl(_lib, "layer_norm", "CUDA")
+@without_tangents
 def _layer_norm_cuda(x, weight, bias, eps):
     return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps)[:3]
 
 
 @torch.library.impl(_lib, "layer_norm_pack8", "CUDA")
+@without_tangents
 def _layer_norm_pack8_cuda(x, weight, bias, eps):
     return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps, packed=True)
 
 
 @torch.library.impl(_lib, "layer_norm_backward", "CUDA")
+@without_tangents
 def _layer_norm_backward_cuda(grad_y, x, x_codes, x_scales, mean, rstd, weight, param_dtype, need_weight, need_bias):
     gx, gw, gb = _k.layer_norm_bwd(grad_y.contiguous(), _dense(x), _dense(x_codes), _dense(x_scales),
                                    mean.contiguous(), rstd.contiguous(), _dense(weight), param_dtype, need_weight,
@@ -185,15 +188,18 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     or of x's dtype.  Statistics and sums are fp32, y and every gradient are
     rounded once.  activation_bits: 16 keeps x for the backward, 8 its 8-bit
     codes (the backward's normalised input is then that of the codes, with the
-    statistics of x).  Differentiable once: a gradient of its gradients raises."""
+    statistics of x).  Differentiable once, in reverse mode: a gradient of its
+    gradients raises, and so does a dual tensor."""
     packed = activation_bits == 8
     if (packed or activation_bits == 16) and _plain_eager(x):  # the kernels' launchers check the tensors
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                         or (bias is not None and bias.requires_grad)):
             out = _LayerNormEager.apply(x, weight, bias, eps, packed)
             return out[0] if packed else out
+        refuse_tangents(x, weight, bias)
         return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps, stats=False)[0]
     _check(x, weight, bias, activation_bits)
+    refuse_tangents(x, weight, bias)
     op = torch.ops.flash_mhc.layer_norm_pack8 if packed else torch.ops.flash_mhc.layer_norm
     return op(x, weight, bias, eps)[0]
 

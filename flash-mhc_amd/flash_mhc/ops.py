@@ -40,6 +40,7 @@ from contextlib import contextmanager
 
 import torch
 import torch.library
+from torch.autograd import forward_ad as _forward_ad
 
 from . import kernels as _k
 
@@ -439,6 +440,33 @@ def _fused_post_res_backward_cuda(grad_out, x_streams, layer_output, H_merged, h
 
 
 # ---------------------------------------------------------------------------
+# Forward-mode differentiation, which the kernels do not have.
+
+
+def refuse_tangents(*tensors) -> None:
+    """Raise if one of tensors is a dual tensor.  An autograd Function does so by
+    itself; a kernel launched outside of one would drop the tangent."""
+    # (The level is a private name: without it, every tensor is asked.)
+    if getattr(_forward_ad, "_current_level", 0) < 0 or torch.compiler.is_compiling():
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("flash_mhc: this operator has no forward-mode derivative, and an input is a dual "
+                                      "tensor")
+
+
+def without_tangents(fn):
+    """fn(*args), refusing dual tensors among them."""
+
+    @functools.wraps(fn)
+    def refusing(*args):
+        refuse_tangents(*args)
+        return fn(*args)
+
+    return refusing
+
+
+# ---------------------------------------------------------------------------
 # Backward passes without a derivative.
 
 
@@ -486,6 +514,7 @@ def differentiable_once(backward):
 
     @functools.wraps(backward)
     def once(ctx, *grads):
+        refuse_tangents(*grads)
         if not torch.is_grad_enabled():  # an ordinary backward
             return backward(ctx, *grads)
         with torch.no_grad():

@@ -12,7 +12,7 @@ from contextlib import contextmanager
 import torch
 
 import flash_mhc
-from flash_mhc import activation8, block, kernels, norm
+from flash_mhc import activation8, block, kernels, norm, ops
 from oracle import act8_oracle as A
 from oracle_cpu_ops import _k1_bwd, _k4, _k4_bwd, _pre_map, _pre_map_bwd
 
@@ -120,7 +120,7 @@ def registered():
     lib = torch.library.Library("flash_mhc", "IMPL")
     try:
         for name, fn in REGISTERED.items():
-            lib.impl(name, fn, "CPU")
+            lib.impl(name, fn if name == "pack8" else ops.without_tangents(fn), "CPU")
         yield
     finally:
         lib._destroy()

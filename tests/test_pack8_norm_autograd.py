@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import flash_mhc
 import pack8_cpu_kernels as cpu
@@ -212,3 +213,71 @@ def test_backward_ops_have_no_derivative(opdev):
         for t in out:
             with pytest.raises(RuntimeError, match="once_differentiable"):
                 t.float().sum().backward(retain_graph=True)
+
+
+# ---------------------------------------------------------------------------
+# Forward mode: there is no derivative in it, and a tangent is not dropped.
+
+
+def _dual(t):
+    return fwAD.make_dual(t, torch.ones_like(t))
+
+
+def _refuses(call):
+    with pytest.raises(NotImplementedError, match="forward.mode"):
+        call()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_layer_norm_refuses_dual_tensors(dev, bits):
+    x, w, b = (rnd(s, i).to(dev) for i, s in enumerate(((5, 48), (48,), (48,))))
+    norm = lambda *a: flash_mhc.layer_norm(*a, activation_bits=bits)
+    with fwAD.dual_level():
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad():
+                for k in range(3):
+                    args = [x, w, b]
+                    args[k] = _dual(args[k])
+                    _refuses(lambda: norm(*args))
+                    _refuses(lambda: norm(x.clone().requires_grad_(True), args[1], _dual(b)))
+                assert torch.equal(norm(x, w, b), norm(x, w, b))  # ordinary tensors within a level
+        y = norm(_grad(x.clone()), w, b)
+        _refuses(lambda: y.backward(_dual(torch.ones_like(y))))
+    with pytest.raises(NotImplementedError, match="forward.mode"):
+        torch.func.jvp(lambda t: norm(t, w, b), (x,), (x,))
+
+
+def test_block_refuses_dual_tensors(dev):
+    blk = cpu.make_block(32, pre_norm=True).to(dev).requires_grad_(False)
+    x = rnd((6, 4, 32), 1, dtype=BF16).to(dev)
+    with fwAD.dual_level():
+        _refuses(lambda: blk._forward_triton(_dual(x)))
+
+
+def test_ops_refuse_dual_tensors(opdev):
+    T, C = 6, 32
+    x, W, ap, apo, ar, b, perm = premap_args(opdev)
+    params = (W, ap, apo, ar, b, perm)
+    w = rnd((C,), 6).to(opdev)
+    lo = x[:, 0].contiguous()
+    _y, mean, rstd, q, s = OPS.layer_norm_pack8(lo, w, None, 1e-5)
+    li, H, hq, hpre, proj, inv, sink, xq, xs = OPS.mhc_pre_map_pack8(x, *params)
+    post_res = OPS.fused_post_res_pack8 if opdev == "cuda" else OPS.fused_post_res_pack8_traced
+    with fwAD.dual_level():
+        for call in (
+            lambda: OPS.layer_norm(lo, _dual(w), None, 1e-5),
+            lambda: OPS.layer_norm_pack8(_dual(lo), w, None, 1e-5),
+            lambda: OPS.layer_norm_backward(_dual(lo), None, q, s, mean, rstd, w, F32, True, True),
+            lambda: OPS.mhc_pre_map_pack8(_dual(x), *params),
+            lambda: OPS.mhc_pre_map_backward_pack8(_dual(li), None, None, None, None, None, xq, xs, *params, hpre, proj, inv),
+            lambda: OPS.mhc_post_res_pack8(x, sink, xq, xs, li, _dual(H), hq),
+            lambda: post_res(x, _dual(li), H, hq),
+            lambda: OPS.fused_post_res_backward_pack8(_dual(x), xq, xs, q, s, H, hq),
+            lambda: OPS.fused_rmsnorm_project_bwd_pack8(_dual(proj), xq, xs, W, proj, inv),
+        ):
+            _refuses(call)
+    blk = cpu.make_block(C).to(opdev).requires_grad_(False)
+    with fwAD.dual_level():
+        _refuses(lambda: blk._mhc_pre_map_triton(_dual(x)))
+    with pytest.raises(NotImplementedError, match="forward.mode"):
+        torch.func.jvp(lambda t: blk._mhc_pre_map_triton(t)[0], (x,), (x,))
