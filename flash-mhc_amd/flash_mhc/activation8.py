@@ -278,9 +278,22 @@ def _fused_post_res_pack8_autograd(x_streams, layer_output, H_merged, h_post):
     return torch.ops.flash_mhc.fused_post_res_pack8_traced(x_streams, layer_output, H_merged, h_post)
 
 
+def _version(x):
+    """Counts x's changes in place (inference tensors are not changed where gradients are recorded)."""
+    return None if x.is_inference() else x._version
+
+
+def _check_version(x, version) -> None:
+    # autograd's own check is of tensors that are kept, and x is not.
+    if _version(x) != version:
+        raise RuntimeError("the streams were modified by an inplace operation between the block's pre-map and "
+                           "post-res, which both need them")
+
+
 def _setup_pre_map(ctx, inputs, output):
-    _x, *params = inputs
+    x, *params = inputs
     _li, _H, _hq, h_pre, proj, inv_rms, _sink, codes, scales = output
+    codes._streams_version = _version(x)  # for mhc_post_res_pack8, also while a graph is traced
     ctx.save_for_backward(codes, scales, *params, h_pre, proj, inv_rms)
     ctx.set_materialize_grads(False)
 
@@ -296,7 +309,10 @@ torch.library.register_autograd("flash_mhc::mhc_pre_map_pack8", _mhc_pre_map_pac
 
 
 def _setup_mhc_post_res(ctx, inputs, output):
-    _x, x_sink, codes, scales, lo, H_merged, h_post = inputs
+    x, x_sink, codes, scales, lo, H_merged, h_post = inputs
+    # (Codes from elsewhere, or from another compiled graph, have no version.)
+    if hasattr(codes, "_streams_version"):
+        _check_version(x, codes._streams_version)
     _out, lo_codes, lo_scales = output
     ctx.save_for_backward(codes, scales, lo_codes, lo_scales, H_merged, h_post, graph_link(x_sink, lo))
     ctx.set_materialize_grads(False)
@@ -325,7 +341,7 @@ class _Kept:
 
     __slots__ = ("version", "post", "codes")
 
-    def __init__(self, version: int):
+    def __init__(self, version):
         self.version = version  # of the streams when the pre-map read them
         self.post = None        # weak: post-res's node leads to the pre-map's
         self.codes = None
@@ -375,9 +391,7 @@ class _PostResEager(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x_streams, x_sink, layer_output, H_merged, h_post, kept, residual):
-        if x_streams._version != kept.version:
-            raise RuntimeError("the streams were modified by an inplace operation between the block's pre-map and "
-                               "post-res, which both need them")
+        _check_version(x_streams, kept.version)
         out, *codes = _k.k4_fwd_pack8(x_streams.contiguous(), layer_output.contiguous(), _coeff(H_merged),
                                       _coeff(h_post), residual=None if residual is None else residual.contiguous())
         ctx.kept = kept
@@ -403,7 +417,7 @@ def pre_map_eager(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat
     """(layer_input, H_merged, h_post, x_sink, kept) of mhc_pre_map, recorded for
     autograd without the op's dispatch; `kept` goes to post_res_eager for the
     same streams, whose forward packs them for this one's backward."""
-    kept = _Kept(x_streams._version)
+    kept = _Kept(_version(x_streams))
     return (*_PreMapEager.apply(x_streams, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, kept), kept)
 
 

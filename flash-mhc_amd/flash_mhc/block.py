@@ -108,7 +108,9 @@ class MHCLiteBlock(nn.Module):
             unchanged, the backward reads what the codes stand for.  Applies to
             the fused path with its pre-map op (the default switches), where it
             takes the place of activation_checkpointing; other paths keep
-            the tensors.
+            the tensors.  The layer must not change x_streams in place: that
+            raises, except where torch.compile breaks the graph in the layer,
+            which leaves it unnoticed (16 bits raise in the backward there).
         pre_norm: give the block a layer norm ``norm`` of the layer's input, and
             the residual around it: the layer maps u to F, the block uses
             u + F(norm(u)).  Off by default (the layer contains both, as in

@@ -281,3 +281,83 @@ def test_ops_refuse_dual_tensors(opdev):
         _refuses(lambda: blk._mhc_pre_map_triton(_dual(x)))
     with pytest.raises(NotImplementedError, match="forward.mode"):
         torch.func.jvp(lambda t: blk._mhc_pre_map_triton(t)[0], (x,), (x,))
+
+
+# ---------------------------------------------------------------------------
+# The streams changed in place between the pre-map, which packs them, and post-res,
+# which mixes them: refused on the op path as in eager mode.
+
+
+class Changing(torch.nn.Module):
+    """A layer that is also given the streams."""
+
+    def __init__(self, C, how=None, breaks=False):
+        super().__init__()
+        self.lin, self.how, self.breaks = torch.nn.Linear(C, C), how, breaks
+
+    def forward(self, u, x=None):
+        if self.how == "whole":
+            x.mul_(2)
+        elif self.how == "part":
+            x[1:].add_(3)
+        elif self.how == "item":
+            x[0, 0, 0] = 3
+        elif self.how == "view":
+            x.view(-1).relu_()
+        elif self.how == "detached":
+            x.detach().zero_()
+        if self.breaks:
+            torch._dynamo.graph_break()
+        return self.lin(u)
+
+
+def _forward(blk, route):
+    if route == "ops":
+        return blk._forward_triton
+    torch._dynamo.reset()
+    return torch.compile(blk._forward_triton, backend=route, fullgraph=not blk.layer.breaks)
+
+
+ROUTES = ["ops", "eager", "aot_eager", "inductor"]
+
+
+@pytest.fixture(params=["1", "0"])
+def op_route(request, opdev, monkeypatch):
+    """The block on the ops, with the x-gradient's sink or without it."""
+    monkeypatch.setattr(flash_mhc.block, "_plain_eager", lambda x: False)
+    monkeypatch.setenv("FLASH_MHC_FUSED_XGRAD", request.param)
+    return opdev
+
+
+@pytest.mark.parametrize("route,how", [(r, "whole") for r in ROUTES] + [
+    (r, how) for r in ROUTES[:3] for how in ("part", "item", "view", "detached")])
+def test_block_ops_refuse_changed_streams(op_route, route, how):
+    C = 32
+    blk = cpu.make_block(C, layer=Changing(C, how)).to(op_route)
+    x = _grad(rnd((6, 4, C), 1, dtype=BF16).to(op_route)) * 1
+    with pytest.raises(Exception, match="inplace"):
+        blk_out = _forward(blk, route)(x, x=x)
+        torch.autograd.grad(blk_out.sum(), blk.W_all.weight)
+
+
+@pytest.mark.parametrize("breaks", [False, True])
+@pytest.mark.parametrize("route", ROUTES)
+def test_block_ops_take_streams_changed_before(op_route, route, breaks):
+    """No version but the one between pre-map and post-res counts: buffers filled
+    anew for every step, stacks of blocks, layers that break the graph.  (Inductor
+    rounds the layer's bf16 intermediates at other places, 2^-8 each, and a
+    weight's gradient is a sum of such terms, within 2^-6 of its largest.)"""
+    C, T = 32, 6
+    blks = [cpu.make_block(C, s, layer=Changing(C, breaks=breaks)).to(op_route) for s in (1, 2)]
+    fns = [_forward(b, route) for b in blks]
+    buf = torch.zeros(T, 4, C, dtype=BF16, device=op_route)
+    for step in range(3):
+        buf.copy_(rnd((T, 4, C), step, dtype=BF16))
+        y = fns[0](buf)
+        y = fns[1](y + 0)
+        got = torch.autograd.grad(y.float().square().sum(), [p for b in blks for p in b.parameters()])
+        want = blks[1]._forward_triton(blks[0]._forward_triton(buf.clone()))
+        want = torch.autograd.grad(want.float().square().sum(), [p for b in blks for p in b.parameters()])
+        for a, b in zip(got, want):
+            assert torch.allclose(a.float(), b.float(), rtol=2 ** -6, atol=2 ** -6 * float(b.abs().max()))
+        buf.add_(1)
