@@ -179,10 +179,10 @@ class MHCLiteBlock(nn.Module):
         otherwise there is no residual (None)."""
         if self.norm is None:
             return self.layer(layer_input, **kwargs), None
-        with_residual = getattr(self.norm, "with_residual", None)
-        if with_residual is None:  # another module put in the norm's place
+        # (Of its class: a wrapper that passes attributes on is another module.)
+        if getattr(type(self.norm), "with_residual", None) is None:
             return self.layer(self.norm(layer_input), **kwargs), layer_input
-        normed, residual = with_residual(layer_input)
+        normed, residual = self.norm.with_residual(layer_input)
         return self.layer(normed, **kwargs), residual
 
     def _apply_layer(self, layer_input: torch.Tensor, kwargs) -> torch.Tensor:

@@ -241,8 +241,12 @@ class LayerNorm(nn.Module):
         return F.layer_norm(x, (self.hidden_size,), self.weight, self.bias, self.eps)
 
     def _hooked(self) -> bool:
-        """A call of this module does more than forward."""
-        return (_any_global_hook is None or _any_global_hook() or type(self).forward is not LayerNorm.forward
+        """A call of this module does more than LayerNorm.forward."""
+        cls = type(self)
+        return (_any_global_hook is None or _any_global_hook() or cls.forward is not LayerNorm.forward
+                or cls.__call__ is not nn.Module.__call__ or cls._call_impl is not nn.Module._call_impl
+                or "forward" in self.__dict__ or "_call_impl" in self.__dict__
+                or getattr(self, "_compiled_call_impl", None) is not None
                 or bool(self._forward_hooks or self._forward_pre_hooks or self._backward_hooks
                         or self._backward_pre_hooks))
 

@@ -361,3 +361,86 @@ def test_block_ops_take_streams_changed_before(op_route, route, breaks):
         for a, b in zip(got, want):
             assert torch.allclose(a.float(), b.float(), rtol=2 ** -6, atol=2 ** -6 * float(b.abs().max()))
         buf.add_(1)
+
+
+# ---------------------------------------------------------------------------
+# What a block with pre_norm calls is its norm, whatever was put around it.
+
+
+class _CallsTwice(flash_mhc.LayerNorm):
+    def __call__(self, x):
+        return super().__call__(x) * 2
+
+
+class _Wrapper(torch.nn.Module):
+    """Attributes are those of the wrapped module, as offloading and sharding wrappers have it."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def __getattr__(self, name):
+        try:
+            return super().__getattr__(name)
+        except AttributeError:
+            return getattr(super().__getattr__("inner"), name)
+
+    def forward(self, x):
+        return self.inner(x) * 2
+
+
+def _instance_forward(norm):
+    plain = norm.forward
+    norm.forward = lambda x: plain(x) * 2
+    return norm
+
+
+def _instance_call(norm):
+    plain = norm._call_impl
+    norm._call_impl = lambda x: plain(x) * 2
+    return norm
+
+
+def _subclass(norm):
+    norm.__class__ = _CallsTwice
+    return norm
+
+
+def _hook(norm):
+    norm.register_forward_hook(lambda m, a, out: out * 2)
+    return norm
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("change", [_instance_forward, _instance_call, _subclass, _hook, _Wrapper])
+def test_block_calls_its_norm(dev, change, bits):
+    """A norm that gives twice its output: the same as a layer that takes twice its input, in training too."""
+    C = 32
+    layer = torch.nn.Linear(C, C, bias=False)
+    blk = cpu.make_block(C, layer=layer, pre_norm=True).to(dev)
+    blk.activation_bits = blk.norm.activation_bits = bits
+    if dev == "cpu" and bits == 16:
+        pytest.skip("the 16-bit block has no stand-ins")
+    x, g = rnd((6, 4, C), 1, dtype=BF16).to(dev), rnd((6, 4, C), 2, dtype=BF16).to(dev)
+
+    def step():
+        xs = _grad(x.clone())
+        out = blk._forward_triton(xs)
+        return out.detach(), torch.autograd.grad(out, xs, g)[0]
+
+    once = step()
+    blk.norm = change(blk.norm)
+    changed = step()
+    with torch.no_grad():
+        layer.weight.mul_(0.5)  # exact
+    again = step()
+    for a, b in zip(again, once):
+        assert torch.equal(a, b)
+    assert not torch.equal(changed[0], once[0]) and not torch.equal(changed[1], once[1])
+
+
+def test_hooked():
+    norm = flash_mhc.LayerNorm(8)
+    assert not norm._hooked()
+    norm.compile(backend="eager")
+    assert norm._hooked()
