@@ -777,7 +777,9 @@ int ln_fwd_run(const LnFwdArgs& a, hipStream_t s) {
       // slot on (T = 262144, C = 1024 202 -> 174 us, T = 65536, C = 2048 94 -> 90; at
       // two rows per slot T = 30011, C = 2560 54 -> 69; with wider rows C = 8192 packed
       // 61 -> 64).
-      const int64_t deep = LPT <= kWave ? want / 4 : 0, most = deep > 256 * 8 ? deep : 256 * 8;
+      // A launch has fewer than 2^32 threads; the workgroups walk the rest of the rows.
+      const int64_t deep = LPT <= kWave ? want / 4 : 0, fit = ((int64_t{1} << 32) - 1) / BLOCK;
+      const int64_t many = deep > 256 * 8 ? deep : 256 * 8, most = many < fit ? many : fit;
       kernel<<<dim3(static_cast<unsigned>(want < most ? want : most)), BLOCK, 0, s>>>(x, a.P, y, a.mean, a.rstd, a.codes,
                                                                                     a.scales, a.T, a.C, a.eps);
     };
