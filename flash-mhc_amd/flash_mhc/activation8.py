@@ -29,6 +29,7 @@ import weakref
 import torch
 import torch.library
 
+from . import _abi
 from . import block as _block  # which imports this module: its names are read at call time
 from . import kernels as _k
 from .ops import (
@@ -334,16 +335,31 @@ for _op in ("fused_post_res_backward_pack8", "fused_rmsnorm_project_bwd_pack8", 
     register_no_autograd(_op)
 
 
+def _stream_of(t) -> int:
+    return _abi.stream_of(t) if t.is_cuda else 0
+
+
+def _borrow(tensors, stream: int) -> None:
+    """Use tensors that were made on `stream` on the current one: after what made
+    them, and their memory is not given away before that use is over."""
+    dev = tensors[0].device
+    now = torch.cuda.current_stream(dev)
+    now.wait_stream(torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev))
+    for t in tensors:
+        t.record_stream(now)
+
+
 class _Kept:
     """The codes of a block's streams, on their way from post-res, whose forward
     makes and saves them, to the pre-map's backward, which runs after
     post-res's."""
 
-    __slots__ = ("version", "post", "codes")
+    __slots__ = ("version", "post", "stream", "codes")
 
     def __init__(self, version):
         self.version = version  # of the streams when the pre-map read them
         self.post = None        # weak: post-res's node leads to the pre-map's
+        self.stream = 0         # that post-res ran on, the pre-map's unless the layer left another one current
         self.codes = None
 
     def take(self):
@@ -351,14 +367,16 @@ class _Kept:
         was not part of this backward (a loss on the layer's input alone), they
         are still with post-res's node."""
         codes, self.codes = self.codes, None
-        if codes is not None:
-            return codes
-        post = self.post() if self.post is not None else None
-        if post is None:
-            raise RuntimeError(
-                "activation_bits=8: the block's output is gone, and its 8-bit activations with it; keep the output "
-                "until its layer input's gradient is taken, or use activation_bits=16")
-        return post.saved_tensors[:2]
+        if codes is None:
+            post = self.post() if self.post is not None else None
+            if post is None:
+                raise RuntimeError(
+                    "activation_bits=8: the block's output is gone, and its 8-bit activations with it; keep the output "
+                    "until its layer input's gradient is taken, or use activation_bits=16")
+            codes = post.saved_tensors[:2]
+        if _stream_of(codes[0]) != self.stream:
+            _borrow(codes, self.stream)
+        return codes
 
 
 class _PreMapEager(torch.autograd.Function):
@@ -397,6 +415,7 @@ class _PostResEager(torch.autograd.Function):
         ctx.kept = kept
         ctx.residual = residual is not None
         kept.post = weakref.ref(ctx)
+        kept.stream = _stream_of(out)
         link = H_merged.new_empty(0)  # a second output, kept for differentiable_once
         ctx.save_for_backward(*codes, H_merged, h_post, link)
         ctx.set_materialize_grads(False)

@@ -444,3 +444,86 @@ def test_hooked():
     assert not norm._hooked()
     norm.compile(backend="eager")
     assert norm._hooked()
+
+
+# ---------------------------------------------------------------------------
+# The streams' codes go from post-res to the pre-map's backward.
+
+
+def _li_loss(blk, seen):
+    blk.layer.register_forward_hook(lambda m, i, o: seen.__setitem__("li", i[0]))
+
+
+@pytest.mark.parametrize("way", ["whole", "input alone"])
+def test_codes_on_another_stream(monkeypatch, way):
+    """The codes are made on post-res's stream and read on the pre-map's: with stand-ins that count where they are."""
+    cpu.eager(monkeypatch)
+    a8 = flash_mhc.activation8
+    now, borrowed = [1], []
+    monkeypatch.setattr(a8, "_stream_of", lambda t: now[0])
+    monkeypatch.setattr(a8, "_borrow", lambda tensors, stream: borrowed.append((len(tensors), stream)))
+    blk, seen = cpu.make_block(32), {}
+    _li_loss(blk, seen)
+    x = _grad(rnd((6, 4, 32), 1, dtype=BF16))
+    for during, expect in ((1, []), (2, [(2, 2)])):
+        handle = blk.layer.register_forward_hook(lambda m, i, o: now.__setitem__(0, during))
+        now[0] = 1
+        out = blk._forward_triton(x)
+        handle.remove()
+        now[0] = 1
+        (out if way == "whole" else seen["li"]).float().sum().backward()
+        assert borrowed == expect
+
+
+class _Leaves(torch.nn.Module):
+    """A layer that leaves another stream current."""
+
+    def __init__(self, C, stream):
+        super().__init__()
+        self.lin, self.stream = torch.nn.Linear(C, C), stream
+
+    def forward(self, u):
+        if self.stream is not None:
+            self.stream.wait_stream(torch.cuda.current_stream())
+            torch.cuda.set_stream(self.stream)
+        return self.lin(u)
+
+
+@pytest.mark.gpu
+def test_layer_that_leaves_another_stream_current():
+    """The same gradients, and the allocator is told of the codes' second stream."""
+    C, T = 256, 2048
+    x, g = (rnd((T, 4, C), i, dtype=BF16).cuda() for i in (1, 2))
+    home = torch.cuda.current_stream()
+
+    def step(stream, alone):
+        seen = {}
+        torch.manual_seed(0)  # the layer's weights
+        blk = cpu.make_block(C, layer=_Leaves(C, stream)).cuda()
+        _li_loss(blk, seen)
+        xs = _grad(x.clone())
+        home.synchronize()
+        try:
+            out = blk(xs)
+            torch.cuda.current_stream().synchronize()
+        finally:
+            torch.cuda.set_stream(home)
+        loss, up = (seen["li"], g[:, 0].contiguous()) if alone else (out, g)
+        leaves = [xs, blk.W_all.weight]
+        got = torch.autograd.grad(loss, leaves, up)
+        del out, loss, seen
+        torch.cuda.synchronize()
+        return got
+
+    marked = []
+    with pytest.MonkeyPatch.context() as m:
+        record = torch.Tensor.record_stream
+        m.setattr(torch.Tensor, "record_stream", lambda t, s: (marked.append(s), record(t, s))[1])
+        for alone in (False, True):
+            want = step(None, alone)
+            assert not marked
+            got = step(torch.cuda.Stream(), alone)
+            assert marked == [home, home]
+            marked.clear()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
