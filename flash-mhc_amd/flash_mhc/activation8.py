@@ -427,7 +427,10 @@ class _PostResEager(torch.autograd.Function):
         if grad_out is None:
             return (None,) * 7
         *codes, H_merged, h_post, _link = ctx.saved_tensors
-        ctx.kept.codes = codes[:2]
+        # Not where no pre-map's backward will take them (frozen streams and coefficients).
+        _x, x_sink, _lo, H, hp, _kept, _res = ctx.needs_input_grad
+        if x_sink or H or hp:
+            ctx.kept.codes = codes[:2]
         g_x, g_lo, g_H, g_hp = _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
         return None, g_x, g_lo, g_H, g_hp, None, g_lo if ctx.residual else None
 

@@ -527,3 +527,31 @@ def test_layer_that_leaves_another_stream_current():
             marked.clear()
             for a, b in zip(got, want):
                 assert torch.equal(a, b)
+
+
+def test_frozen_block_frees_its_codes(dev):
+    """A trained layer in a block whose streams and coefficients are frozen: once its
+    backward is over no codes are left, whoever still holds the output."""
+    C, T = 256, 512
+    blk = cpu.make_block(C).to(dev).requires_grad_(False)
+    blk.layer.requires_grad_(True)
+    x, g = (rnd((T, 4, C), i, dtype=BF16).to(dev) for i in (1, 2))
+    kept = []
+    with pytest.MonkeyPatch.context() as m:
+        init = flash_mhc.activation8._Kept.__init__
+        m.setattr(flash_mhc.activation8._Kept, "__init__", lambda self, v: (kept.append(self), init(self, v))[1])
+        out = blk._forward_triton(x)
+    before = torch.cuda.memory_allocated() if dev == "cuda" else 0
+    out.backward(g)
+    assert blk.layer.weight.grad is not None and len(kept) == 1 and kept[0].codes is None
+    if dev == "cuda":
+        freed = before - torch.cuda.memory_allocated() + 2 * sum(p.numel() for p in blk.layer.parameters())
+        assert freed >= T * 5 * C  # the codes of x and of the layer's output
+    # Where a later backward may take them they stay.
+    blk.requires_grad_(True)
+    xs = _grad(x.clone())
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(flash_mhc.activation8._Kept, "__init__", lambda self, v: (kept.append(self), init(self, v))[1])
+        out = blk._forward_triton(xs)
+    torch.autograd.grad(out, blk.layer.weight, g)
+    assert kept[1].codes is not None
