@@ -121,7 +121,7 @@ register_no_autograd("layer_norm_backward")
 
 @differentiable_once
 def _eager_gradients(ctx, grad_y, grad_x):
-    x, codes, scales, stats, weight = ctx.saved_tensors  # (stats: an output where x is not kept, for the graph's sake)
+    x, codes, scales, stats, weight = ctx.saved_tensors
     _nx, need_weight, need_bias, _ne, _np = ctx.needs_input_grad
     gx, gw, gb = _k.layer_norm_bwd_joint(grad_y.contiguous(), x, codes, scales, stats, weight, ctx.param_dtype,
                                          need_weight, need_bias, _dense(grad_x))
@@ -135,21 +135,21 @@ def _eager_backward(ctx, grad_y, grad_x=None):
 
 
 def _eager_forward(ctx, x, weight, bias, eps, packed):
+    """(y,), or (y, stats) where ctx keeps something else than x or weight itself."""
     ctx.set_materialize_grads(False)
-    x, weight = x.contiguous(), _dense(weight)
-    y, stats, codes, scales, ctx.param_dtype = _k.layer_norm_fwd_joint(x, weight, _dense(bias), eps, packed)
-    ctx.save_for_backward(None if packed else x, codes, scales, stats, weight)
-    return y, stats
+    xc, wc = x.contiguous(), _dense(weight)
+    y, stats, codes, scales, ctx.param_dtype = _k.layer_norm_fwd_joint(xc, wc, _dense(bias), eps, packed)
+    ctx.save_for_backward(None if packed else xc, codes, scales, stats, wc)
+    return (y, stats) if packed or xc is not x or wc is not weight else (y,)
 
 
 class _LayerNormEager(torch.autograd.Function):
     """layer_norm / layer_norm_pack8 with their registered autograd, without the
-    ops' dispatch: (y, stats) where packed, otherwise y."""
+    ops' dispatch: y, and what _eager_forward adds."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, packed):
-        y, stats = _eager_forward(ctx, x, weight, bias, eps, packed)
-        return (y, stats) if packed else y
+        return _eager_forward(ctx, x, weight, bias, eps, packed)
 
     @staticmethod
     def backward(ctx, grad_y, _stats=None):
@@ -157,16 +157,15 @@ class _LayerNormEager(torch.autograd.Function):
 
 
 class _LayerNormResidualEager(torch.autograd.Function):
-    """(layer_norm(x), x, and stats where packed): the gradient of the second, which
-    the residual around a block's layer gives, is added in the norm's backward."""
+    """(x, layer_norm(x)): the gradient of the first, which the residual around a
+    block's layer gives, is added in the norm's backward."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, packed):
-        y, stats = _eager_forward(ctx, x, weight, bias, eps, packed)
-        return (y, x.view_as(x), stats) if packed else (y, x.view_as(x))
+        return (x.view_as(x), *_eager_forward(ctx, x, weight, bias, eps, packed))
 
     @staticmethod
-    def backward(ctx, grad_y, grad_x, _stats=None):
+    def backward(ctx, grad_x, grad_y, _stats=None):
         return _eager_backward(ctx, grad_y, grad_x)
 
 
@@ -194,8 +193,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if (packed or activation_bits == 16) and _plain_eager(x):  # the kernels' launchers check the tensors
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                         or (bias is not None and bias.requires_grad)):
-            out = _LayerNormEager.apply(x, weight, bias, eps, packed)
-            return out[0] if packed else out
+            return _LayerNormEager.apply(x, weight, bias, eps, packed)[0]
         refuse_tangents(x, weight, bias)
         return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps, stats=False)[0]
     _check(x, weight, bias, activation_bits)
@@ -255,7 +253,8 @@ class LayerNorm(nn.Module):
         gradient that x gets from the residual (as a separate addition would)."""
         if (_plain_eager(x) and torch.is_grad_enabled() and x.requires_grad and not self._hooked()
                 and self._on_kernels(x)):
-            return _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)[:2]
+            r, y, *_ = _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
+            return y, r
         return self(x), x
 
     def extra_repr(self) -> str:

@@ -65,6 +65,11 @@ def test_layer_norm_once(dev, bits, score):
         # With respect to what is no leaf, and is not kept either.
         u = x * 1.5
         _twice(SCORES[score](flash_mhc.layer_norm(u * 1, weight, activation_bits=bits)), u)
+        # Kept as a copy.
+        u = x.t().contiguous() * 1.5
+        _twice(SCORES[score](flash_mhc.layer_norm(u.t(), weight, activation_bits=bits)), u)
+    wide = _grad(rnd((48, 2), 2).to(dev))
+    _twice(SCORES[score](flash_mhc.layer_norm(x, wide[:, 0], activation_bits=bits)), wide)
     # A parameter's gradient too.
     weight = _grad(w.clone())
     _twice(SCORES[score](flash_mhc.layer_norm(x, weight, activation_bits=bits)), weight)
@@ -75,7 +80,10 @@ def test_layer_norm_once(dev, bits, score):
 def test_norm_with_residual_once(dev, use, score):
     norm = flash_mhc.LayerNorm(48).to(dev)
     x = _grad(rnd((5, 48), 1).to(dev))
-    y, r = norm.with_residual(x * 1.5)
+    if score == "linear":
+        y, r = norm.with_residual((x * 1.5).t().contiguous().t())
+    else:
+        y, r = norm.with_residual(x * 1.5)
     used = {"norm": [y], "residual": [r], "both": [y, r]}[use]
     loss = sum(SCORES[score](t) for t in used)
     if use == "residual":  # the identity, which has all its derivatives
