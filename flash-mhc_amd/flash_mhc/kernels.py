@@ -739,6 +739,9 @@ def _norm_params(weight, bias, dtype: torch.dtype, C: int, dev) -> torch.dtype:
         _require(weight, "weight", pdt, (C,), dev)
     if bias is not None:
         _require(bias, "bias", pdt, (C,), dev)
+    # Null stands for no weight and no bias: a tensor without memory of its own (a wrapper) is not to pass for it.
+    if (weight is not None and not weight.data_ptr()) or (bias is not None and not bias.data_ptr()):
+        raise TypeError("weight and bias must have memory that the kernels can read (not a wrapper subclass's)")
     return pdt
 
 

@@ -55,6 +55,11 @@ def _layer_norm_backward_fake(grad_y, x, x_codes, x_scales, mean, rstd, weight, 
             grad_y.new_empty((C if need_bias else 0,), dtype=param_dtype))
 
 
+def _ordinary(*params) -> bool:
+    """None, or tensors and parameters of no subclass, whose memory the kernels can read."""
+    return all(t is None or type(t) is nn.Parameter or type(t) is torch.Tensor for t in params)
+
+
 def _dense(t):
     return None if t is None else t.contiguous()
 
@@ -190,7 +195,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     statistics of x).  Differentiable once, in reverse mode: a gradient of its
     gradients raises, and so does a dual tensor."""
     packed = activation_bits == 8
-    if (packed or activation_bits == 16) and _plain_eager(x):  # the kernels' launchers check the tensors
+    if (packed or activation_bits == 16) and _plain_eager(x) and _ordinary(weight, bias):  # the kernels' launchers check the tensors
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                         or (bias is not None and bias.requires_grad)):
             return _LayerNormEager.apply(x, weight, bias, eps, packed)[0]
@@ -252,7 +257,7 @@ class LayerNorm(nn.Module):
         """(norm(x), x) for ``x + layer(norm(x))``: the norm's backward adds the
         gradient that x gets from the residual (as a separate addition would)."""
         if (_plain_eager(x) and torch.is_grad_enabled() and x.requires_grad and not self._hooked()
-                and self._on_kernels(x)):
+                and self._on_kernels(x) and _ordinary(self.weight, self.bias)):
             r, y, *_ = _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
             return y, r
         return self(x), x

@@ -563,3 +563,52 @@ def test_frozen_block_frees_its_codes(dev):
         out = blk._forward_triton(xs)
     torch.autograd.grad(out, blk.layer.weight, g)
     assert kept[1].codes is not None
+
+
+# ---------------------------------------------------------------------------
+# Parameters that are wrappers (sharded, quantised) have no memory of their own.
+
+
+class _Held(torch.Tensor):
+    """A wrapper subclass: ops run on what it holds."""
+
+    seen: list = []
+
+    @staticmethod
+    def __new__(cls, held):
+        return torch.Tensor._make_wrapper_subclass(cls, held.shape, dtype=held.dtype, device=held.device)
+
+    def __init__(self, held):
+        self.held = held
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        cls.seen.append(func)
+        return func(*(a.held if isinstance(a, _Held) else a for a in args), **(kwargs or {}))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_wrapped_parameters(opdev, monkeypatch, bits):
+    if opdev == "cpu":
+        cpu.eager(monkeypatch)
+    x, w, b = (rnd(s, i).to(opdev) for i, s in enumerate(((5, 48), (48,), (48,))))
+    want = flash_mhc.layer_norm(x, w, b)
+    norm = flash_mhc.LayerNorm(48, activation_bits=bits).to(opdev)
+    for args in ((x, _Held(w), b), (x, w, _Held(b))):
+        _Held.seen.clear()
+        assert torch.equal(flash_mhc.layer_norm(*args, activation_bits=bits), want)
+        del norm.weight, norm.bias
+        norm.weight, norm.bias = args[1:]
+        y, _r = norm.with_residual(_grad(x.clone()))
+        assert torch.equal(y, want)
+        assert OPS.layer_norm.default in _Held.seen or OPS.layer_norm_pack8.default in _Held.seen
+
+
+def test_launcher_refuses_parameters_without_memory(monkeypatch):
+    from flash_mhc import kernels as K
+
+    monkeypatch.setattr(K, "_device_of", lambda t: t.device)
+    x, w = rnd((5, 48), 1), rnd((48,), 2)
+    for weight, bias in ((_Held(w), None), (w, _Held(w))):
+        with pytest.raises(TypeError, match="wrapper"):
+            K.layer_norm_fwd(x, weight, bias, 1e-5)
