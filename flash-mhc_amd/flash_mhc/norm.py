@@ -240,6 +240,8 @@ class LayerNorm(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self._on_kernels(x):
+            if self.weight is None and x.shape[-1:] != (self.hidden_size,):  # (weight's shape is checked)
+                raise ValueError(f"expected x of shape (..., {self.hidden_size}), got {tuple(x.shape)}")
             return layer_norm(x, self.weight, self.bias, self.eps, self.activation_bits)
         return F.layer_norm(x, (self.hidden_size,), self.weight, self.bias, self.eps)
 
@@ -257,7 +259,7 @@ class LayerNorm(nn.Module):
         """(norm(x), x) for ``x + layer(norm(x))``: the norm's backward adds the
         gradient that x gets from the residual (as a separate addition would)."""
         if (_plain_eager(x) and torch.is_grad_enabled() and x.requires_grad and not self._hooked()
-                and self._on_kernels(x) and _ordinary(self.weight, self.bias)):
+                and self._on_kernels(x) and _ordinary(self.weight, self.bias) and x.shape[-1:] == (self.hidden_size,)):
             r, y, *_ = _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
             return y, r
         return self(x), x

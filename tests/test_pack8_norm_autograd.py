@@ -612,3 +612,19 @@ def test_launcher_refuses_parameters_without_memory(monkeypatch):
     for weight, bias in ((_Held(w), None), (w, _Held(w))):
         with pytest.raises(TypeError, match="wrapper"):
             K.layer_norm_fwd(x, weight, bias, 1e-5)
+
+
+# ---------------------------------------------------------------------------
+# The module's width.
+
+
+@pytest.mark.parametrize("affine", [True, False])
+def test_module_refuses_another_width(dev, affine):
+    norm = flash_mhc.LayerNorm(48, elementwise_affine=affine).to(dev)
+    assert norm(rnd((2, 3, 48), 1).to(dev)).shape == (2, 3, 48)
+    for shape in ((5, 40), (48, 5), *([()] if dev == "cuda" or not affine else [])):
+        x = rnd(shape, 1).to(dev)
+        for call in (norm, norm.with_residual):
+            for leaf in (x, _grad(x.clone())):
+                with pytest.raises((ValueError, RuntimeError)):
+                    call(leaf)
