@@ -149,12 +149,13 @@ def _unpack8_cuda(codes, scales, dtype):
     return _k.unpack8(codes.contiguous(), scales.contiguous(), dtype)
 
 
-@torch.library.impl(_lib, "fused_post_res_pack8_traced", "CUDA")
-@torch.library.impl(_lib, "fused_post_res_pack8", "CUDA")
-@without_tangents
 def _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post):
     _check_n4(x_streams, "flash_mhc::fused_post_res_pack8 supports n=4 only")
     return _k.k4_fwd_pack8(x_streams.contiguous(), layer_output.contiguous(), _coeff(H_merged), _coeff(h_post))
+
+
+for _op in ("fused_post_res_pack8_traced", "fused_post_res_pack8"):
+    torch.library.impl(_lib, _op, "CUDA")(without_tangents(_fused_post_res_pack8_cuda))
 
 
 @torch.library.impl(_lib, "fused_post_res_backward_pack8", "CUDA")

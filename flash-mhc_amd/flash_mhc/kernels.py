@@ -739,10 +739,16 @@ def _norm_params(weight, bias, dtype: torch.dtype, C: int, dev) -> torch.dtype:
         _require(weight, "weight", pdt, (C,), dev)
     if bias is not None:
         _require(bias, "bias", pdt, (C,), dev)
-    # Null stands for no weight and no bias: a tensor without memory of its own (a wrapper) is not to pass for it.
-    if (weight is not None and not weight.data_ptr()) or (bias is not None and not bias.data_ptr()):
-        raise TypeError("weight and bias must have memory that the kernels can read (not a wrapper subclass's)")
     return pdt
+
+
+def _param_ptr(t: torch.Tensor | None):
+    if t is None:
+        return None
+    p = t.data_ptr()
+    if not p:  # null stands for no parameter
+        raise TypeError("weight and bias must have memory that the kernels can read (not a wrapper subclass's)")
+    return p
 
 
 def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
@@ -774,8 +780,8 @@ def _layer_norm_fwd(x, weight, bias, eps, dev, mean, rstd, packed):
     pdt = _norm_params(weight, bias, x.dtype, C, dev)
     y = torch.empty_like(x)
     q, s = empty_packed(x) if packed else (None, None)
-    _launch("layer_norm_fwd", dev, _abi.load().fmhc_layer_norm_fwd, x.data_ptr(), _ptr_or_none(weight),
-            _ptr_or_none(bias), y.data_ptr(), mean, rstd, _ptr_or_none(q), _ptr_or_none(s), code, DTYPES[pdt], T, C, eps,
+    _launch("layer_norm_fwd", dev, _abi.load().fmhc_layer_norm_fwd, x.data_ptr(), _param_ptr(weight),
+            _param_ptr(bias), y.data_ptr(), mean, rstd, _ptr_or_none(q), _ptr_or_none(s), code, DTYPES[pdt], T, C, eps,
             _abi.stream_of(x))
     return y, q, s, pdt
 
@@ -828,7 +834,7 @@ def _layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, n
     ws_bytes = lib.fmhc_layer_norm_bwd_workspace_bytes(T, C) if need_weight or need_bias else 0
     ws = _workspace(ws_bytes, dev)
     _launch("layer_norm_bwd", dev, lib.fmhc_layer_norm_bwd, grad_y.data_ptr(), _ptr_or_none(x), _ptr_or_none(codes),
-            _ptr_or_none(scales), mean, rstd, _ptr_or_none(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
+            _ptr_or_none(scales), mean, rstd, _param_ptr(weight), _ptr_or_none(grad_x_in), gx.data_ptr(),
             _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws), ws_bytes, code, DTYPES[param_dtype], T, C,
             _abi.stream_of(grad_y))
     return gx, gw, gb

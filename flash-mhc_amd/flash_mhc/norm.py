@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from . import kernels as _k
 from .activation8 import _packed_like
 from .block import _plain_eager
-from .ops import differentiable_once, refuse_tangents, register_no_autograd, without_tangents
+from .ops import _forward_ad, differentiable_once, refuse_tangents, register_no_autograd, without_tangents
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
@@ -55,9 +55,7 @@ def _layer_norm_backward_fake(grad_y, x, x_codes, x_scales, mean, rstd, weight, 
             grad_y.new_empty((C if need_bias else 0,), dtype=param_dtype))
 
 
-def _ordinary(*params) -> bool:
-    """None, or tensors and parameters of no subclass, whose memory the kernels can read."""
-    return all(t is None or type(t) is nn.Parameter or type(t) is torch.Tensor for t in params)
+_ORDINARY = (type(None), nn.Parameter, torch.Tensor)  # no subclass: the kernels can read its memory
 
 
 def _dense(t):
@@ -195,11 +193,13 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     statistics of x).  Differentiable once, in reverse mode: a gradient of its
     gradients raises, and so does a dual tensor."""
     packed = activation_bits == 8
-    if (packed or activation_bits == 16) and _plain_eager(x) and _ordinary(weight, bias):  # the kernels' launchers check the tensors
+    if (packed or activation_bits == 16) and _plain_eager(x) and type(weight) in _ORDINARY and type(bias) in _ORDINARY:
+        # (The kernels' launchers check the tensors.)
         if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                         or (bias is not None and bias.requires_grad)):
             return _LayerNormEager.apply(x, weight, bias, eps, packed)[0]
-        refuse_tangents(x, weight, bias)
+        if _forward_ad._current_level >= 0:
+            refuse_tangents(x, weight, bias)
         return _k.layer_norm_fwd(x.contiguous(), _dense(weight), _dense(bias), eps, stats=False)[0]
     _check(x, weight, bias, activation_bits)
     refuse_tangents(x, weight, bias)
@@ -259,7 +259,8 @@ class LayerNorm(nn.Module):
         """(norm(x), x) for ``x + layer(norm(x))``: the norm's backward adds the
         gradient that x gets from the residual (as a separate addition would)."""
         if (_plain_eager(x) and torch.is_grad_enabled() and x.requires_grad and not self._hooked()
-                and self._on_kernels(x) and _ordinary(self.weight, self.bias) and x.shape[-1:] == (self.hidden_size,)):
+                and self._on_kernels(x) and type(self.weight) in _ORDINARY and type(self.bias) in _ORDINARY
+                and x.shape[-1:] == (self.hidden_size,)):
             r, y, *_ = _LayerNormResidualEager.apply(x, self.weight, self.bias, self.eps, self.activation_bits == 8)
             return y, r
         return self(x), x

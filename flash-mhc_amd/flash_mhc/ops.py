@@ -36,6 +36,7 @@ from __future__ import annotations
 
 import functools
 import os
+import types
 from contextlib import contextmanager
 
 import torch
@@ -443,11 +444,16 @@ def _fused_post_res_backward_cuda(grad_out, x_streams, layer_output, H_merged, h
 # Forward-mode differentiation, which the kernels do not have.
 
 
+# Whether a forward-mode level is entered: its number is a private name of the
+# module's (without it, every tensor is asked).
+if not hasattr(_forward_ad, "_current_level"):
+    _forward_ad = types.SimpleNamespace(unpack_dual=_forward_ad.unpack_dual, _current_level=0)
+
+
 def refuse_tangents(*tensors) -> None:
     """Raise if one of tensors is a dual tensor.  An autograd Function does so by
     itself; a kernel launched outside of one would drop the tangent."""
-    # (The level is a private name: without it, every tensor is asked.)
-    if getattr(_forward_ad, "_current_level", 0) < 0 or torch.compiler.is_compiling():
+    if _forward_ad._current_level < 0 or torch.compiler.is_compiling():
         return
     for t in tensors:
         if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
@@ -514,7 +520,8 @@ def differentiable_once(backward):
 
     @functools.wraps(backward)
     def once(ctx, *grads):
-        refuse_tangents(*grads)
+        if _forward_ad._current_level >= 0:
+            refuse_tangents(*grads)
         if not torch.is_grad_enabled():  # an ordinary backward
             return backward(ctx, *grads)
         with torch.no_grad():

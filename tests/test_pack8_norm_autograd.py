@@ -604,14 +604,19 @@ def test_wrapped_parameters(opdev, monkeypatch, bits):
         assert OPS.layer_norm.default in _Held.seen or OPS.layer_norm_pack8.default in _Held.seen
 
 
-def test_launcher_refuses_parameters_without_memory(monkeypatch):
+def test_launchers_refuse_parameters_without_memory(monkeypatch):
+    from flash_mhc import _abi
     from flash_mhc import kernels as K
 
     monkeypatch.setattr(K, "_device_of", lambda t: t.device)
-    x, w = rnd((5, 48), 1), rnd((48,), 2)
+    monkeypatch.setattr(_abi, "stream_of", lambda t: None)
+    monkeypatch.setattr(K, "_launch", lambda *args: pytest.fail("launched"))
+    x, w, stat = rnd((5, 48), 1), rnd((48,), 2), torch.ones(5)
     for weight, bias in ((_Held(w), None), (w, _Held(w))):
         with pytest.raises(TypeError, match="wrapper"):
             K.layer_norm_fwd(x, weight, bias, 1e-5)
+    with pytest.raises(TypeError, match="wrapper"):
+        K.layer_norm_bwd(x, x, None, None, stat, stat, _Held(w), F32)
 
 
 # ---------------------------------------------------------------------------
