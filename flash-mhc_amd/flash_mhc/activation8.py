@@ -39,9 +39,9 @@ from .ops import (
     _mhc_pre_map_cuda,
     _mhc_pre_map_fake,
     _params,
+    backward_op,
     differentiable_once,
     graph_link,
-    register_no_autograd,
     without_tangents,
 )
 
@@ -159,7 +159,7 @@ for _op in ("fused_post_res_pack8_traced", "fused_post_res_pack8"):
 
 
 @torch.library.impl(_lib, "fused_post_res_backward_pack8", "CUDA")
-@without_tangents
+@backward_op
 def _fused_post_res_backward_pack8_cuda(grad_out, x_codes, x_scales, lo_codes, lo_scales, H_merged, h_post):
     _check_n4(x_codes, "flash_mhc::fused_post_res_backward_pack8 supports n=4 only")
     return _k.k4_bwd_pack8(grad_out.contiguous(), x_codes.contiguous(), x_scales.contiguous(), lo_codes.contiguous(),
@@ -167,7 +167,7 @@ def _fused_post_res_backward_pack8_cuda(grad_out, x_codes, x_scales, lo_codes, l
 
 
 @torch.library.impl(_lib, "fused_rmsnorm_project_bwd_pack8", "CUDA")
-@without_tangents
+@backward_op
 def _fused_rmsnorm_project_bwd_pack8_cuda(grad_out, x_codes, x_scales, W, proj_out, inv_rms):
     _check_n4(x_codes, "flash_mhc::fused_rmsnorm_project_bwd_pack8 supports n=4 only")
     return _k.k1_bwd_pack8(grad_out.contiguous(), x_codes.contiguous(), x_scales.contiguous(),
@@ -187,7 +187,7 @@ def _mhc_pre_map_pack8_cuda(x_streams, W, alpha_pre, alpha_post, alpha_res, bias
 
 
 @torch.library.impl(_lib, "mhc_pre_map_backward_pack8", "CUDA")
-@without_tangents
+@backward_op
 def _mhc_pre_map_backward_pack8_cuda(grad_layer_input, grad_H_merged, grad_h_post, grad_h_pre, grad_proj, grad_x_sink,
                                      x_codes, x_scales, W, alpha_pre, alpha_post, alpha_res, bias, perm_mat, h_pre,
                                      proj, inv_rms):
@@ -330,10 +330,6 @@ def _mhc_post_res_pack8_backward(ctx, grad_out, _gc, _gs):
 
 torch.library.register_autograd("flash_mhc::mhc_post_res_pack8", _mhc_post_res_pack8_backward,
                                 setup_context=_setup_mhc_post_res)
-
-
-for _op in ("fused_post_res_backward_pack8", "fused_rmsnorm_project_bwd_pack8", "mhc_pre_map_backward_pack8"):
-    register_no_autograd(_op)
 
 
 def _stream_of(t) -> int:

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from . import kernels as _k
 from .activation8 import _packed_like
 from .block import _plain_eager
-from .ops import _forward_ad, differentiable_once, refuse_tangents, register_no_autograd, without_tangents
+from .ops import _forward_ad, backward_op, differentiable_once, refuse_tangents, without_tangents
 
 _lib = torch.library.Library("flash_mhc", "FRAGMENT")
 
@@ -75,7 +75,7 @@ def _layer_norm_pack8_cuda(x, weight, bias, eps):
 
 
 @torch.library.impl(_lib, "layer_norm_backward", "CUDA")
-@without_tangents
+@backward_op
 def _layer_norm_backward_cuda(grad_y, x, x_codes, x_scales, mean, rstd, weight, param_dtype, need_weight, need_bias):
     gx, gw, gb = _k.layer_norm_bwd(grad_y.contiguous(), _dense(x), _dense(x_codes), _dense(x_scales),
                                    mean.contiguous(), rstd.contiguous(), _dense(weight), param_dtype, need_weight,
@@ -116,7 +116,6 @@ def _backward(ctx, grad_y, *_rest):
 
 torch.library.register_autograd("flash_mhc::layer_norm", _backward, setup_context=_setup)
 torch.library.register_autograd("flash_mhc::layer_norm_pack8", _backward, setup_context=_setup)
-register_no_autograd("layer_norm_backward")
 
 
 # The two eager Functions' backward.

@@ -533,15 +533,25 @@ def differentiable_once(backward):
     return once
 
 
-def register_no_autograd(op: str) -> None:
-    """A backward op called by itself, with inputs that require grad: its outputs
-    raise where they are differentiated (without a formula, torch only warns and
-    takes them as constants)."""
+def backward_op(fn):
+    """fn(*args), a device implementation of a backward op.  Called by itself with
+    inputs that require grad, its outputs raise where they are differentiated
+    (torch's fallback for an op without a formula only warns and takes them as
+    constants; a registered formula costs every call a pass through Python)."""
 
-    def backward(ctx, *_grads):
-        raise RuntimeError(f"flash_mhc::{op} is a backward pass, which is once_differentiable: it has no derivative")
+    @functools.wraps(fn)
+    def call(*args):
+        refuse_tangents(*args)
+        if not torch.is_grad_enabled():
+            return fn(*args)
+        links = [t for t in args if isinstance(t, torch.Tensor) and t.requires_grad]
+        if not links:
+            return fn(*args)
+        with torch.no_grad():
+            out = fn(*args)
+        return _Once.apply(len(links), *links, *out)
 
-    torch.library.register_autograd(f"flash_mhc::{op}", backward)
+    return call
 
 
 # ---------------------------------------------------------------------------

@@ -120,7 +120,9 @@ def registered():
     lib = torch.library.Library("flash_mhc", "IMPL")
     try:
         for name, fn in REGISTERED.items():
-            lib.impl(name, fn if name == "pack8" else ops.without_tangents(fn), "CPU")
+            if name != "pack8":
+                fn = ops.backward_op(fn) if "backward" in name or "bwd" in name else ops.without_tangents(fn)
+            lib.impl(name, fn, "CPU")
         yield
     finally:
         lib._destroy()
