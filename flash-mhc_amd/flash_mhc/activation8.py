@@ -258,8 +258,8 @@ class _FusedPostResEager(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_streams, layer_output, H_merged, h_post):
         outs = _fused_post_res_pack8_cuda(x_streams, layer_output, H_merged, h_post)
-        link = H_merged.new_empty(0)  # a last output, kept for differentiable_once
-        ctx.save_for_backward(*outs[1:], H_merged, h_post, link)
+        link = h_post.detach()  # h_post as a last output, for differentiable_once
+        ctx.save_for_backward(*outs[1:], H_merged, link)
         ctx.mark_non_differentiable(*outs[1:])
         ctx.set_materialize_grads(False)
         return (*outs, link)
@@ -269,7 +269,7 @@ class _FusedPostResEager(torch.autograd.Function):
     def backward(ctx, grad_out, *_codes):
         if grad_out is None:
             return None, None, None, None
-        *codes, H_merged, h_post, _link = ctx.saved_tensors
+        *codes, H_merged, h_post = ctx.saved_tensors
         return _k.k4_bwd_pack8_saved(grad_out.contiguous(), *codes, _coeff(H_merged), _coeff(h_post))
 
 
@@ -413,8 +413,8 @@ class _PostResEager(torch.autograd.Function):
         ctx.residual = residual is not None
         kept.post = weakref.ref(ctx)
         kept.stream = _stream_of(out)
-        link = H_merged.new_empty(0)  # a second output, kept for differentiable_once
-        ctx.save_for_backward(*codes, H_merged, h_post, link)
+        link = h_post.detach()  # h_post as a second output, for differentiable_once
+        ctx.save_for_backward(*codes, H_merged, link)
         ctx.set_materialize_grads(False)
         return out, link
 
@@ -423,7 +423,7 @@ class _PostResEager(torch.autograd.Function):
     def backward(ctx, grad_out, _link):
         if grad_out is None:
             return (None,) * 7
-        *codes, H_merged, h_post, _link = ctx.saved_tensors
+        *codes, H_merged, h_post = ctx.saved_tensors
         # Not where no pre-map's backward will take them (frozen streams and coefficients).
         _x, x_sink, _lo, H, hp, _kept, _res = ctx.needs_input_grad
         if x_sink or H or hp:
