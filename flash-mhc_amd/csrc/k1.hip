@@ -647,8 +647,10 @@ struct BwdFrag {
 // consecutive k) are exactly the A operand of v_mfma_f32_16x16x16_bf16 with
 // the contraction over tokens, so tile m of dW^T is
 //   D (16 k x 16 d) += x[tokens, k_slice + 8 * i + m]^T (A) * G[tokens, 16 h + j] (B)
-// with G = bf16(go * inv_rms).  G reaches the B layout through a 1 KiB
-// wave-private LDS tile.  Each wave writes its fp32 partial dW for its slice;
+// with G = bf16(go * inv_rms): the reference's grad_W rounds there, and x's codes
+// and values are bf16 operands as they are.  For normal inputs grad_W is off by
+// 0.0024 of its norm, with an unrounded G by 0.0017 (its own rounding to bf16).
+// G reaches the B layout through a 1 KiB wave-private LDS tile.  Each wave writes its fp32 partial dW for its slice;
 // k1_dw_reduce sums the partials of all runs in a fixed order.
 //
 // With EPI = true (the pre-map backward) the store also adds the K3 term of
@@ -1258,9 +1260,10 @@ constexpr int kBwdDwNTB = 64;
 // kernels that read x in 8 bits, whose buffers are smaller but whose VALU work
 // (4 more operations per two elements) one wave per SIMD does not hide: two
 // buffers and two waves T = 16384, C = 4096 172 us, three and one 193, four 202.
-// At two waves it is bound by the memory's mix of reads and twice as many
-// written bytes (805 MB, 4.7 TB/s; the VALU is issued 45% of the time): a third
-// buffer beside two waves 174, loads and stores without a branch 177.
+// (Both kernels, here and below; k1_bwd_mfma is 164 of the 172.)  At two waves it
+// is bound by the memory's mix of reads and twice as many written bytes (0.85 GB
+// with grad_W's partial sums in 164 us, 5.2 TB/s; the VALU is issued 45% of the
+// time): a third buffer beside two waves 174, loads and stores without a branch 177.
 constexpr int kBwdBufs = 3;
 constexpr int kBwdEpiBufs = 2;
 constexpr int kBwdDwMinNTB = 4;

@@ -6,7 +6,8 @@ of their bf16 bytes: groups of 32 columns share a power of two, an element is a
 signed code times it (the format is defined in ``include/flash_mhc_hip.h``), off
 by at most a 128th of the group's power of two (a 64th at its top).  The forward
 is computed from the exact tensors; the backward reads the codes and gives the
-bits that the bf16 backward gives on the unpacked tensors.
+bits that the bf16 backward gives on the unpacked tensors (K1's backward by
+itself up to the order of fp32 sums where C % 8 != 0).
 
   pack8, unpack8                    a tensor (..., C) to codes and scales and back
   fused_post_res_pack8              fused_post_res that keeps its inputs packed

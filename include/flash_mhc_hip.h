@@ -286,7 +286,8 @@ int fmhc_k4_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const int8
 /* fmhc_k1_bwd from packed streams: x_codes (T, n, C), x_scales (T, n, G), W
  * (32, n C), grad_x (T, n, C), grad_W (32, n C); values as fmhc_k1_bwd gives
  * them for the unpacked x up to the order of fp32 sums (the same bits where
- * C % 8 == 0).  `workspace`: at least fmhc_k1_bwd_pack8_workspace_bytes(T, C)
+ * C % 8 == 0), with fmhc_k1_bwd's rounding of go * inv_rms to bf16 in grad_W.
+ * `workspace`: at least fmhc_k1_bwd_pack8_workspace_bytes(T, C)
  * bytes, 16-byte aligned (may be NULL where that is 0). */
 int fmhc_k1_bwd_pack8(const int8_t* x_codes, const uint8_t* x_scales, const uint16_t* W,
                       const uint16_t* grad_out, const uint16_t* proj_out, const float* inv_rms,
