@@ -509,6 +509,16 @@ def graph_link(*tensors):
         return _Link.apply(*tensors)
 
 
+class _Unpacked:
+    """ctx with its saved tensors unpacked: under torch.utils.checkpoint they can be only once."""
+
+    def __init__(self, ctx):
+        self._ctx, self.saved_tensors = ctx, ctx.saved_tensors
+
+    def __getattr__(self, name):
+        return getattr(self._ctx, name)
+
+
 def differentiable_once(backward):
     """backward(ctx, *grads) of an autograd Function or a registered op whose
     gradients have no derivative.  They depend on what the forward kept whether or
@@ -524,6 +534,7 @@ def differentiable_once(backward):
             refuse_tangents(*grads)
         if not torch.is_grad_enabled():  # an ordinary backward
             return backward(ctx, *grads)
+        ctx = _Unpacked(ctx)
         with torch.no_grad():
             out = backward(ctx, *grads)
         links = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]

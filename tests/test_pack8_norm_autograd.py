@@ -149,6 +149,23 @@ def test_gradients_with_a_graph_have_the_same_values(dev):
     torch.autograd.grad(gp.sum(), p)
 
 
+def test_once_under_checkpoint(dev):
+    """Recomputed tensors can be unpacked once: a graph of the gradients has the same values there."""
+    from torch.utils.checkpoint import checkpoint
+
+    blk = cpu.make_block(64, pre_norm=True).to(dev)
+    x, g = rnd((6, 4, 64), 3, dtype=BF16).to(dev), rnd((6, 4, 64), 4, dtype=BF16).to(dev)
+    results = []
+    for graph in (False, True):
+        xs = _grad(x.clone())
+        out = checkpoint(blk._forward_triton, xs, use_reentrant=False)
+        results.append(torch.autograd.grad(out, [xs, *blk.parameters()], g, create_graph=graph))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        results[1][0].float().sum().backward()
+
+
 # The same through the registered ops: called by name, under a dispatch mode, with
 # tensor subclasses.
 
