@@ -296,7 +296,7 @@ def _check_version(x, version) -> None:
 def _setup_pre_map(ctx, inputs, output):
     x, *params = inputs
     _li, _H, _hq, h_pre, proj, inv_rms, _sink, codes, scales = output
-    codes._streams_version = _version(x)  # for mhc_post_res_pack8, also while a graph is traced
+    codes._streams = id(x), _version(x)  # for mhc_post_res_pack8, also while a graph is traced
     ctx.save_for_backward(codes, scales, *params, h_pre, proj, inv_rms)
     ctx.set_materialize_grads(False)
 
@@ -313,9 +313,10 @@ torch.library.register_autograd("flash_mhc::mhc_pre_map_pack8", _mhc_pre_map_pac
 
 def _setup_mhc_post_res(ctx, inputs, output):
     x, x_sink, codes, scales, lo, H_merged, h_post = inputs
-    # (Codes from elsewhere, or from another compiled graph, have no version.)
-    if hasattr(codes, "_streams_version"):
-        _check_version(x, codes._streams_version)
+    # (Codes from elsewhere, or from another compiled graph, have no version; a copy of the streams has its own.)
+    packed, version = getattr(codes, "_streams", (None, None))
+    if packed == id(x):
+        _check_version(x, version)
     _out, lo_codes, lo_scales = output
     ctx.save_for_backward(codes, scales, lo_codes, lo_scales, H_merged, h_post, graph_link(x_sink, lo))
     ctx.set_materialize_grads(False)

@@ -365,6 +365,18 @@ def test_block_ops_refuse_changed_streams(op_route, route, how):
         torch.autograd.grad(blk_out.sum(), blk.W_all.weight)
 
 
+def test_post_res_op_takes_copies_of_the_streams(opdev):
+    """By name: the codes with an equal tensor that has a history of its own."""
+    x, *params, perm = premap_args(opdev)
+    x.add_(1)
+    li, H, hq, *_o, sink, codes, scales = OPS.mhc_pre_map_pack8(_grad(x), *params, perm)
+    want = OPS.mhc_post_res_pack8(x, sink, codes, scales, li, H, hq)[0]
+    got = OPS.mhc_post_res_pack8(x.detach().clone(), sink, codes, scales, li, H, hq)[0]
+    assert torch.equal(got, want)
+    for a, b in zip(*(torch.autograd.grad(t.float().sum(), [x, H], retain_graph=True) for t in (got, want))):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("breaks", [False, True])
 @pytest.mark.parametrize("route", ROUTES)
 def test_block_ops_take_streams_changed_before(op_route, route, breaks):
