@@ -1,0 +1,55 @@
+// Kernels of the RMS norm and of rows in 8 bits (rms_norm.hip has the entry points
+// and the formulas) for one storage type; compiled once per type
+// (rms_norm_{f32,bf16,f16}.hip).
+#pragma once
+
+#include "elems.h"
+
+namespace fmhc {
+
+struct RmsFwdArgs {
+  const void* x;
+  const void* r;   // added to x first; may be null
+  const void* w;   // may be null (1)
+  bool w_f32;      // w in fp32, otherwise in x's type
+  bool norm;       // false: the rows are packed as they are (no r, no w)
+  void* y;         // or null: codes
+  int8_t* codes;   // rows of ld_codes bytes
+  float* scales;
+  int64_t ld_codes;
+  void* sum;       // x + r, with r
+  float* rstd;     // may be null
+  int64_t T;
+  int C;
+  float eps;
+};
+
+struct RmsBwdArgs {
+  const void* gy;
+  const void* x;       // the sum where the forward had r
+  const float* rstd;
+  const void* w;       // may be null
+  bool w_f32;          // w and gw
+  const void* gi;      // a gradient of x from elsewhere, added to gx; may be null
+  void* gx;
+  float* partial;      // null: no gw
+  void* gw;
+  int64_t T;
+  int C;
+};
+
+// Defined per storage type; the sizes are checked and T > 0.
+template <int DT>
+int rms_fwd_run(const RmsFwdArgs& a, hipStream_t s);
+template <int DT>
+int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s);
+
+// Workgroups of the backward, each of which leaves a sum of every column, at most.
+constexpr int64_t kRmsParts = 512;
+// Columns of a workgroup's sums.
+inline int64_t rms_cols(int64_t C) { return (C + 7) / 8 * 8; }
+
+// A row's largest magnitude counts as at least this where the row is packed.
+constexpr float kRowLeast = 7.888609052210118e-31f;  // 2^-100
+
+}  // namespace fmhc

@@ -56,6 +56,12 @@ SIGNATURES: dict[str, list] = {
     "fmhc_layer_norm_fwd": [_P] * 8 + [_INT, _INT, _I64, _I64, _F32, _P],
     "fmhc_layer_norm_bwd": [_P] * 12 + [_I64, _INT, _INT, _I64, _I64, _P],
     "fmhc_layer_norm_bwd_workspace_bytes": [_I64, _I64],
+    "fmhc_rms_norm_fwd": [_P] * 6 + [_INT, _INT, _I64, _I64, _F32, _P],
+    "fmhc_rms_norm_bwd": [_P] * 8 + [_I64, _INT, _INT, _I64, _I64, _P],
+    "fmhc_rms_norm_bwd_workspace_bytes": [_I64, _I64],
+    "fmhc_pack8_rows": [_P, _INT, _P, _P, _I64, _I64, _I64, _P],
+    "fmhc_rms_norm_pack8_rows": [_P] * 6 + [_INT, _INT, _I64, _I64, _I64, _F32, _P],
+    "fmhc_linear8": [_P, _I64, _P, _P, _I64] + [_P] * 4 + [_INT, _INT, _I64, _I64, _I64, _P],
     "fmhc_error_string": [ctypes.c_int],
     "fmhc_abi_version": [],
 }
@@ -68,9 +74,10 @@ RESTYPES = {
     "fmhc_premap_bwd_workspace_bytes": ctypes.c_int64,
     "fmhc_k1_bwd_pack8_workspace_bytes": ctypes.c_int64,
     "fmhc_layer_norm_bwd_workspace_bytes": ctypes.c_int64,
+    "fmhc_rms_norm_bwd_workspace_bytes": ctypes.c_int64,
 }
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -36,6 +36,7 @@ from torch.utils.checkpoint import checkpoint as _checkpoint
 
 from . import activation8 as _a8
 from . import ops as _ops
+from . import rows8 as _r8
 
 
 def build_permutation_matrices(n: int) -> tuple[torch.Tensor, int]:
@@ -111,11 +112,14 @@ class MHCLiteBlock(nn.Module):
             the tensors.  The layer must not change x_streams in place: that
             raises, except where torch.compile breaks the graph in the layer,
             which leaves it unnoticed (16 bits raise in the backward there).
-        pre_norm: give the block a layer norm ``norm`` of the layer's input, and
+        pre_norm: give the block a norm ``norm`` of the layer's input, and
             the residual around it: the layer maps u to F, the block uses
-            u + F(norm(u)).  Off by default (the layer contains both, as in
-            the reference).  With activation_bits=8 the norm keeps 8-bit codes
-            too.
+            u + F(norm(u)).  True or "layer" is a layer norm, "rms" an RMS norm.
+            Off by default (the layer contains both, as in the reference).  With
+            activation_bits=8 the layer norm keeps 8-bit codes too (the RMS norm
+            keeps its input).  Without a graph (inference) a layer that is a
+            ``Linear8`` takes the norm's rows in 8 bits and adds the residual
+            itself.
         norm_eps: the norm's epsilon.
     """
 
@@ -128,7 +132,7 @@ class MHCLiteBlock(nn.Module):
         activation_checkpointing: bool = False,
         rmsnorm_weight: bool = False,
         activation_bits: int = 16,
-        pre_norm: bool = False,
+        pre_norm: bool | str = False,
         norm_eps: float = 1e-5,
     ) -> None:
         super().__init__()
@@ -157,7 +161,13 @@ class MHCLiteBlock(nn.Module):
             self.rms_weight = nn.Parameter(torch.ones(self.nC))
         else:
             self.rms_weight = None
-        if pre_norm:
+        if pre_norm not in (False, True, "layer", "rms"):
+            raise ValueError(f'pre_norm must be False, True, "layer" or "rms", got {pre_norm!r}')
+        if pre_norm == "rms":
+            from .norm import RMSNorm
+
+            self.norm = RMSNorm(hidden_size, eps=norm_eps)
+        elif pre_norm:
             from .norm import LayerNorm
 
             self.norm = LayerNorm(hidden_size, eps=norm_eps, activation_bits=activation_bits)
@@ -179,11 +189,29 @@ class MHCLiteBlock(nn.Module):
         otherwise there is no residual (None)."""
         if self.norm is None:
             return self.layer(layer_input, **kwargs), None
+        if type(self.layer) is _r8.Linear8 and not kwargs and not torch.is_grad_enabled():
+            layer_output = self._layer_in_codes(layer_input)
+            if layer_output is not None:
+                return layer_output, None
         # (Of its class: a wrapper that passes attributes on is another module.)
         if getattr(type(self.norm), "with_residual", None) is None:
             return self.layer(self.norm(layer_input), **kwargs), layer_input
         normed, residual = self.norm.with_residual(layer_input)
         return self.layer(normed, **kwargs), residual
+
+    def _layer_in_codes(self, u: torch.Tensor):
+        """u + F(norm(u)) with F a Linear8: the norm leaves its rows in 8 bits, the product
+        adds u; None where a call of the layer does more."""
+        from .norm import RMSNorm, hooked
+
+        layer, norm = self.layer, self.norm
+        if not layer.on_kernels(u) or layer.out_features != u.shape[-1] or hooked(layer, _r8.Linear8):
+            return None
+        if type(norm) is RMSNorm and norm._on_kernels(u) and not hooked(norm, RMSNorm):
+            codes, scales = norm.packed(u)
+        else:
+            codes, scales = _r8.pack8_rows(norm(u))
+        return layer.product(codes, scales, u.dtype, residual=u)
 
     def _apply_layer(self, layer_input: torch.Tensor, kwargs) -> torch.Tensor:
         """The layer, with pre_norm around it: u + F(norm(u))."""

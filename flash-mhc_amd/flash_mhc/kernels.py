@@ -25,6 +25,9 @@ Without a counterpart there:
                              K4's forward that keeps its inputs in 8 bits, and
                              the backward passes that read them
   layer_norm_fwd, layer_norm_bwd
+  rms_norm_fwd, rms_norm_bwd
+  pack8_rows, rms_norm_pack8_rows, linear8
+                             rows in 8 bits with a scale each, and their product
 """
 
 from __future__ import annotations
@@ -838,3 +841,171 @@ def _layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, n
             _ptr_or_none(gw), _ptr_or_none(gb), _ptr_or_none(ws), ws_bytes, code, DTYPES[param_dtype], T, C,
             _abi.stream_of(grad_y))
     return gx, gw, gb
+
+
+# ---------------------------------------------------------------------------
+# RMS norm
+
+
+def _sum_like(x, residual, dev):
+    """The tensor for x + residual (None without a residual)."""
+    if residual is None:
+        return None
+    _require(residual, "residual", x.dtype, x.shape, dev)
+    return torch.empty_like(x)
+
+
+def rms_norm_fwd(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, eps: float,
+                 stats: bool = True):
+    """(y, sum, rstd) of x (..., C): y in x's dtype, sum = x + residual (None without
+    one), rstd (...,) fp32 (None without stats)."""
+    dev = _device_of(x)
+    code = _dtype_code(x.dtype, "x")
+    T, C = _rows(x, "x")
+    pdt = _norm_params(weight, None, x.dtype, C, dev)
+    total = _sum_like(x, residual, dev)
+    y = torch.empty_like(x)
+    rstd = x.new_empty(x.shape[:-1], dtype=_F32) if stats else None
+    _launch("rms_norm_fwd", dev, _abi.load().fmhc_rms_norm_fwd, x.data_ptr(), _ptr_or_none(residual),
+            _param_ptr(weight), y.data_ptr(), _ptr_or_none(total), _ptr_or_none(rstd), code, DTYPES[pdt], T, C, eps,
+            _abi.stream_of(x))
+    return y, total, rstd
+
+
+def rms_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None,
+                 param_dtype: torch.dtype, need_weight: bool = True, grad_x_in: torch.Tensor | None = None):
+    """(grad_x, grad_weight) of rms_norm_fwd, x its x or its sum; grad_weight is in
+    param_dtype, None where not needed.  grad_x_in: a gradient of x from elsewhere,
+    added to grad_x."""
+    dev = _device_of(grad_y)
+    _dtype_code(grad_y.dtype, "grad_y")
+    C = _rows(grad_y, "grad_y")[1]
+    _require(x, "x", grad_y.dtype, grad_y.shape, dev)
+    _require(rstd, "rstd", _F32, grad_y.shape[:-1], dev)
+    if param_dtype is not _F32 and param_dtype is not grad_y.dtype:
+        raise TypeError(f"param_dtype must be float32 or grad_y's dtype {grad_y.dtype}, got {param_dtype}")
+    if weight is not None:
+        _require(weight, "weight", param_dtype, (C,), dev)
+    if grad_x_in is not None:
+        _require(grad_x_in, "grad_x_in", grad_y.dtype, grad_y.shape, dev)
+    return rms_norm_bwd_saved(grad_y, x, rstd, weight, param_dtype, need_weight, grad_x_in)
+
+
+def rms_norm_bwd_saved(grad_y, x, rstd, weight, param_dtype, need_weight, grad_x_in=None):
+    """rms_norm_bwd for operands that need no checks: what rms_norm_fwd took and gave,
+    and autograd's gradients, contiguous."""
+    C = grad_y.shape[-1]
+    T = grad_y.numel() // C
+    dev = grad_y.device
+    gx = torch.empty_like(grad_y)
+    gw = grad_y.new_empty((C,), dtype=param_dtype) if need_weight else None
+    lib = _abi.load()
+    ws_bytes = lib.fmhc_rms_norm_bwd_workspace_bytes(T, C) if need_weight else 0
+    ws = _workspace(ws_bytes, dev)
+    _launch("rms_norm_bwd", dev, lib.fmhc_rms_norm_bwd, grad_y.data_ptr(), x.data_ptr(), rstd.data_ptr(),
+            _param_ptr(weight), _ptr_or_none(grad_x_in), gx.data_ptr(), _ptr_or_none(gw), _ptr_or_none(ws), ws_bytes,
+            DTYPES[grad_y.dtype], DTYPES[param_dtype], T, C, _abi.stream_of(grad_y))
+    return gx, gw
+
+
+# ---------------------------------------------------------------------------
+# Rows in 8 bits (the format: include/flash_mhc_hip.h)
+
+ROW_PITCH = 16  # rows of codes begin at multiples of this many bytes
+MOST_PITCH = 1 << 22
+MOST_K = (1 << 17) - 1  # the integer sums stay in 32 bits
+
+
+def row_pitch(C: int) -> int:
+    return (C + ROW_PITCH - 1) // ROW_PITCH * ROW_PITCH
+
+
+def empty_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Unwritten (codes, scales) for a contiguous x (..., C): codes in rows of row_pitch(C) bytes."""
+    shape = x.shape
+    C = shape[-1]
+    codes = x.new_empty((*shape[:-1], row_pitch(C)), dtype=torch.int8)
+    return codes if C % ROW_PITCH == 0 else codes[..., :C], x.new_empty(shape[:-1], dtype=_F32)
+
+
+def pack8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """codes (..., C) int8 and scales (...,) fp32 of the rows of x (..., C)."""
+    dev = _device_of(x)
+    code = _dtype_code(x.dtype, "x")
+    rows, C = _rows(x, "x")
+    codes, scales = empty_rows(x)
+    _launch("pack8_rows", dev, _abi.load().fmhc_pack8_rows, x.data_ptr(), code, codes.data_ptr(), scales.data_ptr(),
+            rows, C, row_pitch(C), _abi.stream_of(x))
+    return codes, scales
+
+
+def rms_norm_pack8_rows(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, eps: float):
+    """(codes, scales, sum): rms_norm_fwd's y in 8 bits."""
+    dev = _device_of(x)
+    code = _dtype_code(x.dtype, "x")
+    T, C = _rows(x, "x")
+    pdt = _norm_params(weight, None, x.dtype, C, dev)
+    total = _sum_like(x, residual, dev)
+    codes, scales = empty_rows(x)
+    _launch("rms_norm_pack8_rows", dev, _abi.load().fmhc_rms_norm_pack8_rows, x.data_ptr(), _ptr_or_none(residual),
+            _param_ptr(weight), codes.data_ptr(), scales.data_ptr(), _ptr_or_none(total), code, DTYPES[pdt], T, C,
+            row_pitch(C), eps, _abi.stream_of(x))
+    return codes, scales, total
+
+
+def _code_rows(codes: torch.Tensor, name: str, dev) -> tuple[torch.Tensor, int, int]:
+    """(codes, rows, bytes between rows) of codes (..., K) as fmhc_linear8 takes them: as they
+    are, or a copy in rows of row_pitch(K) bytes."""
+    if not isinstance(codes, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if codes.dtype is not torch.int8:
+        raise TypeError(f"{name} must be {torch.int8}, got {codes.dtype}")
+    if codes.device != dev:
+        raise ValueError(f"{name} is on {codes.device}, expected {dev}")
+    shape = codes.shape
+    if len(shape) == 0 or not 1 <= shape[-1] <= MOST_K:
+        raise ValueError(f"{name} must have shape (..., K) with 1 <= K <= {MOST_K}, got {tuple(shape)}")
+    K = shape[-1]
+    rows = codes.numel() // K
+    if K % ROW_PITCH == 0 and codes.is_contiguous() and codes.data_ptr() % ROW_PITCH == 0:
+        return codes, rows, K
+    pitch = row_pitch(K)
+    flat = codes.reshape(rows, K)
+    ld = flat.stride(0) if rows > 1 else pitch
+    if (rows > 0 and flat.stride(1) == 1 and pitch <= ld <= MOST_PITCH and ld % ROW_PITCH == 0
+            and flat.data_ptr() % ROW_PITCH == 0
+            and flat.storage_offset() + (rows - 1) * ld + pitch <= flat.untyped_storage().nbytes()):
+        return flat, rows, ld
+    copy = flat.new_empty((rows, pitch))
+    copy[:, :K].copy_(flat)
+    return copy, rows, pitch
+
+
+def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tensor, weight_scales: torch.Tensor,
+            bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+            dtype: torch.dtype = _BF16) -> torch.Tensor:
+    """out (..., N) in dtype, of codes (..., K), scales (...,), weight_codes (N, K) and
+    weight_scales (N,); bias (N,) in fp32 or dtype, residual (..., N) in dtype."""
+    dev = _device_of(codes)
+    code = _dtype_code(dtype, "dtype")
+    lead = codes.shape[:-1]
+    x, T, ldx = _code_rows(codes, "codes", dev)
+    if weight_codes.dim() != 2 or weight_codes.shape[1] != codes.shape[-1] or weight_codes.shape[0] < 1:
+        raise ValueError(f"weight_codes must have shape (N, {codes.shape[-1]}) with N >= 1, got "
+                         f"{tuple(weight_codes.shape)}")
+    w, N, ldw = _code_rows(weight_codes, "weight_codes", dev)
+    _require(scales, "scales", _F32, lead, dev)
+    _require(weight_scales, "weight_scales", _F32, (N,), dev)
+    bias_code = 0
+    if bias is not None:
+        if bias.dtype is not _F32 and bias.dtype is not dtype:
+            raise TypeError(f"bias must be float32 or dtype {dtype}, got {bias.dtype}")
+        _require(bias, "bias", bias.dtype, (N,), dev)
+        bias_code = DTYPES[bias.dtype]
+    if residual is not None:
+        _require(residual, "residual", dtype, (*lead, N), dev)
+    out = codes.new_empty((*lead, N), dtype=dtype)
+    _launch("linear8", dev, _abi.load().fmhc_linear8, x.data_ptr(), ldx, scales.data_ptr(), w.data_ptr(), ldw,
+            weight_scales.data_ptr(), _ptr_or_none(bias), _ptr_or_none(residual), out.data_ptr(), code, bias_code, T, N,
+            codes.shape[-1], _abi.stream_of(codes))
+    return out

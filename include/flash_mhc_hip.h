@@ -39,15 +39,15 @@ extern "C" {
 #define FMHC_ERR_SCRATCH_LIMIT 2    /* fmhc_premap_fwd_noalloc: shape needs more than its scratch */
 #define FMHC_ERR_HIP_BASE 1000      /* + hipError_t from the launch */
 
-#define FMHC_ABI_VERSION 8
+#define FMHC_ABI_VERSION 9
 
 /* Storage dtype of the block parameters K2 reads (alpha_pre, alpha_post,
  * alpha_res, bias, perm: all five the same) and of their gradients. */
 #define FMHC_PARAM_F32 0
 #define FMHC_PARAM_BF16 1
 
-/* Storage dtype of the tensors that fmhc_pack8 / fmhc_unpack8 and the layer
- * norm take. */
+/* Storage dtype of the tensors that fmhc_pack8 / fmhc_unpack8, the norms and the
+ * functions of rows in 8 bits take. */
 #define FMHC_DTYPE_F32 0
 #define FMHC_DTYPE_BF16 1
 #define FMHC_DTYPE_F16 2
@@ -335,6 +335,57 @@ int fmhc_layer_norm_bwd(const void* grad_y, const void* x, const int8_t* x_codes
                         void* grad_bias, void* workspace, int64_t workspace_bytes, int dtype,
                         int param_dtype, int64_t T, int64_t C, void* stream);
 int64_t fmhc_layer_norm_bwd_workspace_bytes(int64_t T, int64_t C);
+
+/* ---- RMS norm --------------------------------------------------------------
+ * No counterpart in the reference.  x, residual, sum, y (T, C) in `dtype`; weight
+ * (C,) in `param_dtype`, which is FMHC_DTYPE_F32 or `dtype`, or NULL (1); the
+ * statistic and sums in fp32, every output rounded once.
+ *   sum[t,c] = x[t,c] + residual[t,c], rounded   (both NULL: s is x, otherwise sum)
+ *   rstd[t]  = rsqrt(sum_c s[t,c]^2 / C + eps)
+ *   y[t,c]   = s[t,c] rstd[t] weight[c]
+ * rstd (T,) may be NULL.  No output may overlap an input. */
+int fmhc_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* sum,
+                      float* rstd, int dtype, int param_dtype, int64_t T, int64_t C, float eps,
+                      void* stream);
+/* Backward, with x the forward's x, or its sum, h = x rstd and g = grad_y weight:
+ *   grad_x[t,c]    = rstd[t] (g[t,c] - h[t,c] sum_c g h / C) + grad_x_in[t,c]
+ *   grad_weight[c] = sum_t grad_y[t,c] h[t,c]
+ * grad_x is also residual's gradient.  grad_x_in (may be NULL, not grad_x): a
+ * gradient of x from elsewhere (sum's).  grad_weight, in param_dtype, may be NULL;
+ * with it `workspace` has at least fmhc_rms_norm_bwd_workspace_bytes(T, C) bytes,
+ * 16-byte aligned.  Sums are added in a fixed order. */
+int fmhc_rms_norm_bwd(const void* grad_y, const void* x, const float* rstd, const void* weight,
+                      const void* grad_x_in, void* grad_x, void* grad_weight, void* workspace,
+                      int64_t workspace_bytes, int dtype, int param_dtype, int64_t T, int64_t C,
+                      void* stream);
+int64_t fmhc_rms_norm_bwd_workspace_bytes(int64_t T, int64_t C);
+
+/* ---- Rows in 8 bits --------------------------------------------------------
+ * No counterpart in the reference.  A row v of C columns as int8 codes with one
+ * fp32 scale (a token's activations, an output channel's weights):
+ *   top = max(max_c |v[c]|, 2^-100),  scale = top / 127
+ *   code[c] = round_half_even(v[c] 127 / top)      (in fp32)
+ * which stand for code * scale.  A row that holds an Inf or NaN has scale NaN and
+ * codes 0.  Rows of codes begin ld_codes (>= C) bytes apart; what lies between them
+ * is left as it is. */
+int fmhc_pack8_rows(const void* x, int dtype, int8_t* codes, float* scales, int64_t rows, int64_t C,
+                    int64_t ld_codes, void* stream);
+/* The rows y of fmhc_rms_norm_fwd, before their rounding to `dtype`, as codes (T, C)
+ * and scales (T,); sum as there. */
+int fmhc_rms_norm_pack8_rows(const void* x, const void* residual, const void* weight, int8_t* codes,
+                             float* scales, void* sum, int dtype, int param_dtype, int64_t T,
+                             int64_t C, int64_t ld_codes, float eps, void* stream);
+/* Their product:
+ *   out[t,n] = (sum_k x[t,k] w[n,k]) x_scales[t] w_scales[n] + bias[n] + residual[t,n]
+ * x (T, K) and w (N, K) are codes, any int8 values, in rows ldx and ldw bytes apart:
+ * multiples of 16, at most 2^22, from a 16-byte aligned address, and every row, the
+ * last one too, can be read to the next multiple of 16 bytes (what is there does not
+ * matter).  The sum is exact; K < 2^17.  out and residual (may be NULL) are (T, N)
+ * in `dtype`, contiguous; bias (N,), in bias_dtype, FMHC_DTYPE_F32 or `dtype`, may be
+ * NULL.  out is rounded once; it may not overlap an input. */
+int fmhc_linear8(const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, int64_t ldw,
+                 const float* w_scales, const void* bias, const void* residual, void* out, int dtype,
+                 int bias_dtype, int64_t T, int64_t N, int64_t K, void* stream);
 
 /* Human-readable text for a status code.  Never returns NULL.
  * No counterpart in the reference (Triton raises Python exceptions). */
