@@ -27,127 +27,525 @@ struct L8Args {
   int N, K;
 };
 
-constexpr int kStepK = 128;      // bytes of a row per step: two matrix instructions' k
-constexpr int kChunk = 16;       // bytes that a lane moves
+constexpr int kChunk = 16;  // bytes that a lane moves
+constexpr int kXcds = 8;
+constexpr int kCus = 256;
 
-using Lds = __attribute__((address_space(3))) int8_t;
-
-// (The host's pass has no type for a buffer's descriptor.)
-#if defined(__HIP_DEVICE_COMPILE__)
-// A tile's rows, `rows` of them in the tensor, read to a whole chunk past the row's K columns;
-// reads past the last one give zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t l8_rows(const int8_t* p, int64_t ld, int rows, int K) {
-  const int bytes = static_cast<int>((rows - 1) * ld) + (K + kChunk - 1) / kChunk * kChunk;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p), 0, bytes, 0x00027000);
-}
-#endif
+// A kernel's bounds: a row is read to the next whole chunk.
+__host__ __device__ __forceinline__ int l8_row_bytes(int K) { return (K + kChunk - 1) / kChunk * kChunk; }
 
 // Bits of a dword that hold columns below n (of its four).
 __device__ __forceinline__ int l8_mask(int n) { return n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1; }
 
-// BT tokens x BC channels by WT x WC waves, each of which has MT x MC fragments of 16 x 16.
-template <int DT, int BT, int BC, int WT, int WC>
-__global__ __launch_bounds__(64 * WT * WC) void l8_tile_kernel(const L8Args a) {
+// What scales a product and is added to it, for eight channels from c on (those past N as the last one).
+template <int DT>
+struct L8Channels {
+  float s[8], b[8];
+  __device__ __forceinline__ L8Channels(const L8Args& a, int c) {
+    using S = typename Elems<DT>::S;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int n = c + e < a.N ? c + e : a.N - 1;
+      s[e] = a.ws[n];
+      b[e] = 0.f;
+      if (a.bias)
+        b[e] = a.bias_f32 ? static_cast<const float*>(a.bias)[n] : Elems<DT>::load(static_cast<const S*>(a.bias) + n);
+    }
+  }
+};
+
+// Eight elements of the residual as loaded.
+template <int DT>
+struct L8Raw {
+  u32x4 a;
+  __device__ __forceinline__ void load(const typename Elems<DT>::S* p) { a = ld16(p); }
+  __device__ __forceinline__ void add_to(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == FMHC_DTYPE_BF16) {
+        v[2 * i] += bf_lo(a[i]);
+        v[2 * i + 1] += bf_hi(a[i]);
+      } else {
+        v[2 * i] += Elems<DT>::widen(a[i] & 0xffffu);
+        v[2 * i + 1] += Elems<DT>::widen(a[i] >> 16);
+      }
+    }
+  }
+};
+template <>
+struct L8Raw<FMHC_DTYPE_F32> {
+  u32x4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = ld16(p);
+    b = ld16(p + 4);
+  }
+  __device__ __forceinline__ void add_to(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] += __uint_as_float(a[i]);
+      v[4 + i] += __uint_as_float(b[i]);
+    }
+  }
+};
+
+// Products of a token with eight channels, scaled, and the bias.
+template <int DT>
+__device__ __forceinline__ void l8_scale(const int (&acc)[8], const L8Channels<DT>& ch, float xs, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(static_cast<float>(acc[e]) * xs, ch.s[e], ch.b[e]);
+}
+
+// What a wave's lanes have written to LDS is there for its other lanes, and what they have read may be
+// written over (in order by themselves; the compiler has to know).
+__device__ __forceinline__ void l8_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of tokens x channels through LDS.
+
+// Waits until N vector memory instructions of the wave are under way at most.
+template <int N>
+__device__ __forceinline__ void l8_wait_vm() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+}
+
+// BT tokens x BC channels per workgroup, WT x WC waves, steps of BK columns.
+template <int kBT, int kBC, int kWT, int kWC, int kBK>
+struct L8Tile {
+  static constexpr int BT = kBT, BC = kBC, WT = kWT, WC = kWC, BK = kBK;
+  static constexpr int THREADS = kWave * WT * WC;
+  static constexpr int LDS = 2 * (BT + BC) * BK;
+};
+
+// How a launch's workgroups walk the tiles: each XCD (workgroup id mod 8) has a run of them, in which
+// eight token tiles take turns before the channel tile moves on, so that an XCD's L2 holds what its
+// CUs read at a time.
+struct L8Walk {
+  int tiles, tiles_t, tiles_c;
+  __device__ __forceinline__ int first(int id) const { return id / kXcds; }
+  __device__ __forceinline__ int run(int id) const {  // tiles of this workgroup's XCD
+    return tiles / kXcds + (id % kXcds < tiles % kXcds ? 1 : 0);
+  }
+  __device__ __forceinline__ int step(int id, int groups) const {  // workgroups of this XCD
+    return groups / kXcds + (id % kXcds < groups % kXcds ? 1 : 0);
+  }
+  __device__ __forceinline__ void at(int id, int pos, int& t, int& c) const {
+    const int xcd = id % kXcds, rest = tiles % kXcds;
+    const int n = xcd * (tiles / kXcds) + (xcd < rest ? xcd : rest) + pos;
+    constexpr int kGroup = 8;
+    const int per = kGroup * tiles_c, g = n / per, in = n % per;
+    const int rows = tiles_t - g * kGroup < kGroup ? tiles_t - g * kGroup : kGroup;
+    t = __builtin_amdgcn_readfirstlane(g * kGroup + in % rows);
+    c = __builtin_amdgcn_readfirstlane(in / rows);
+  }
+};
+
+// Loads go from memory to LDS without registers (rows of BK bytes, 16 bytes a lane), a step and a part
+// ahead of the products, fragments from LDS to registers one part of 64 columns ahead.  The loads run on
+// into the workgroup's next tile while this one's results are stored.
+template <int DT, typename Tile>
+__global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args a, const L8Walk walk) {
+// (The host's pass has no type for a buffer's descriptor.)
 #if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int BT = Tile::BT, BC = Tile::BC, WT = Tile::WT, WC = Tile::WC, BK = Tile::BK;
   constexpr int WAVES = WT * WC, MT = BT / WT / 16, MC = BC / WC / 16;
-  constexpr int LT = BT / 8 / WAVES, LC = BC / 8 / WAVES;  // loads of eight rows per wave and step
-  __shared__ __align__(16) int8_t xl[2][BT * kStepK];
-  __shared__ __align__(16) int8_t wl[2][BC * kStepK];
+  constexpr int RPL = kWave * kChunk / BK;                     // rows per load of a wave
+  constexpr int LT = BT / RPL / WAVES, LC = BC / RPL / WAVES;  // loads per wave and step
+  constexpr int PARTS = BK / 64;                               // of a step: one instruction's columns
+  static_assert(LT >= 1 && LC >= 1 && MT >= 1 && MC >= 2 && MC % 2 == 0 && PARTS % 2 == 0);
+  __shared__ __align__(16) int8_t x0[BT * BK];
+  __shared__ __align__(16) int8_t x1[BT * BK];
+  __shared__ __align__(16) int8_t w0[BC * BK];
+  __shared__ __align__(16) int8_t w1[BC * BK];
+  __shared__ __align__(16) int turn[WAVES][16 * 16 * MC];
+  using Lds = __attribute__((address_space(3))) int8_t;
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int64_t t0 = static_cast<int64_t>(blockIdx.y) * BT;
-  const int c0 = static_cast<int>(blockIdx.x) * BC;
-  const int rows_t = static_cast<int>(a.T - t0 < BT ? a.T - t0 : BT), rows_c = a.N - c0 < BC ? a.N - c0 : BC;
-  const auto xr = l8_rows(a.x + t0 * a.ldx, a.ldx, rows_t, a.K);
-  const auto wr = l8_rows(a.w + c0 * a.ldw, a.ldw, rows_c, a.K);
+  const int id = static_cast<int>(blockIdx.x), run = walk.run(id), stride = walk.step(id, static_cast<int>(gridDim.x));
+  // Two steps, one per buffer, at a time.
+  const int bytes = l8_row_bytes(a.K), steps = (a.K + 2 * BK - 1) / (2 * BK) * 2;
 
-  // A row's chunk j lies at j ^ (row & 7): eight rows' same chunks in eight places.
-  const int row0 = 8 * wave + (lane >> 3), chunk = (lane & 7) ^ (lane >> 3);
+  // What is loaded next: rows from xp and wp on, xn and wn bytes of which can be read.  Reads past a
+  // tile's last row give zeros, and so do those past the last tile.
+  int xn = 0, wn = 0;
+  const int8_t *xp = a.x, *wp = a.w;
+  auto tile_rows = [&](int pos) __attribute__((always_inline)) {
+    int t, c;
+    walk.at(id, pos < run ? pos : 0, t, c);
+    const int64_t t0 = static_cast<int64_t>(t) * BT, c0 = static_cast<int64_t>(c) * BC;
+    const int rt = static_cast<int>(a.T - t0 < BT ? a.T - t0 : BT), rc = static_cast<int>(a.N - c0 < BC ? a.N - c0 : BC);
+    xp = a.x + t0 * a.ldx;
+    wp = a.w + c0 * a.ldw;
+    xn = pos < run ? (rt - 1) * static_cast<int>(a.ldx) + bytes : 0;
+    wn = pos < run ? (rc - 1) * static_cast<int>(a.ldw) + bytes : 0;
+  };
+  auto next_step = [&]() __attribute__((always_inline)) {
+    xp += BK;
+    wp += BK;
+    xn = xn > BK ? xn - BK : 0;
+    wn = wn > BK ? wn - BK : 0;
+  };
+  // A row's chunk j lies at j ^ (row & 7): 16 rows' same chunks spread over the banks.
+  const int lrow = lane / (BK / kChunk), lchunk = lane % (BK / kChunk) ^ (RPL * wave + lrow & 7);
   int xo[LT], wo[LC];
 #pragma unroll
-  for (int j = 0; j < LT; ++j) xo[j] = (row0 + 8 * WAVES * j) * static_cast<int>(a.ldx) + chunk * kChunk;
+  for (int j = 0; j < LT; ++j) xo[j] = (lrow + RPL * (wave + WAVES * j)) * static_cast<int>(a.ldx) + lchunk * kChunk;
 #pragma unroll
-  for (int j = 0; j < LC; ++j) wo[j] = (row0 + 8 * WAVES * j) * static_cast<int>(a.ldw) + chunk * kChunk;
-  auto load = [&](int buf) {
+  for (int j = 0; j < LC; ++j) wo[j] = (lrow + RPL * (wave + WAVES * j)) * static_cast<int>(a.ldw) + lchunk * kChunk;
+  // Loads j0 .. j1 of a step: x's first, then w's.
+  auto load = [&](int8_t* xb, int8_t* wb, int j0, int j1) __attribute__((always_inline)) {
+    const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp), 0, xn, 0x00027000);
+    const auto wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp), 0, wn, 0x00027000);
 #pragma unroll
-    for (int j = 0; j < LT; ++j) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (Lds*)(xl[buf] + (wave + WAVES * j) * 8 * kStepK), 16, xo[j], 0, 0, 0);
-      xo[j] += kStepK;
-    }
-#pragma unroll
-    for (int j = 0; j < LC; ++j) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (Lds*)(wl[buf] + (wave + WAVES * j) * 8 * kStepK), 16, wo[j], 0, 0, 0);
-      wo[j] += kStepK;
+    for (int j = j0; j < j1; ++j) {
+      int8_t* to = (j < LT ? xb : wb) + (wave + WAVES * (j < LT ? j : j - LT)) * RPL * BK;
+      if (j < LT)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (Lds*)to, kChunk, xo[j], 0, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (Lds*)to, kChunk, wo[j - LT], 0, 0, 0);
     }
   };
 
   const int wt = wave / WC * (BT / WT), wc = wave % WC * (BC / WC);
+  const int fr = lane & 15, fk = lane >> 4;
+  auto at = [&](int part) __attribute__((always_inline)) { return fr * BK + ((fk + 4 * part) ^ (fr & 7)) * kChunk; };
+  // AHEAD fragments of x are in registers at a time.
+  constexpr int AHEAD = MT < 4 ? MT : 4;
+  i32x4 acc[MT][MC], xf[AHEAD], wf[2][MC];
+  auto read_w = [&](const int8_t* wb, int part, int q, int j) __attribute__((always_inline)) {
+    wf[q][j] = *reinterpret_cast<const i32x4*>(wb + (wc + 16 * j) * BK + at(part));
+  };
+  auto read_x = [&](const int8_t* xb, int part, int i) __attribute__((always_inline)) {
+    xf[i % AHEAD] = *reinterpret_cast<const i32x4*>(xb + (wt + 16 * i) * BK + at(part));
+  };
+  // A wave's own loads have landed and its reads are done; then all waves'.
+  auto sync = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step with only `left` < BK columns: the others of x are set to zero (w's may be anything).
+  auto cut = [&](int8_t* xb, int left) __attribute__((always_inline)) {
+    if (left >= BK) return;
+    for (int i = static_cast<int>(threadIdx.x); i < BT * BK / kChunk; i += Tile::THREADS) {
+      const int row = i / (BK / kChunk), n = left - (i % (BK / kChunk) ^ (row & 7)) * kChunk;
+      if (n >= kChunk) continue;
+      auto* p = reinterpret_cast<i32x4*>(xb + i * kChunk);
+      i32x4 v = *p;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] &= l8_mask(n - 4 * d);
+      *p = v;
+    }
+    sync();
+  };
+
+  // A buffer's parts.  Where the last one reads on into the other buffer every wave has its fragments of
+  // this buffer and the other buffer's loads have landed (`left` columns of it are x's); then this buffer
+  // is free.
+  auto buffer = [&](int8_t* xb, int8_t* wb, int8_t* xnext, const int8_t* wnext, int left) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const bool last = p == PARTS - 1;
+      // For each fragment of x its products, with a read of the next part's w and loads between them, then
+      // the read that takes its place; in this order.
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int k = i - (MT - AHEAD);  // of the next part's first fragments
+        if (last && k == 0) {
+          sync();
+          cut(xnext, left);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        constexpr int NL = (LT + LC + AHEAD - 1) / AHEAD;
+#pragma unroll
+        for (int j = 0; j < MC; ++j) {
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[p & 1][j], xf[i % AHEAD], acc[i][j], 0, 0, 0);
+          if (j == MC / 2 - 1 && k >= 0) {
+#pragma unroll
+            for (int n = k; n < MC; n += AHEAD) read_w(last ? wnext : wb, last ? 0 : p + 1, (p + 1) & 1, n);
+            if (last) load(xb, wb, k * NL < LT + LC ? k * NL : LT + LC, (k + 1) * NL < LT + LC ? (k + 1) * NL : LT + LC);
+          }
+        }
+        if (k >= 0)
+          read_x(last ? xnext : xb, last ? 0 : p + 1, k);
+        else
+          read_x(xb, p, i + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  int pos = walk.first(id);
+  tile_rows(pos);
+  load(x0, w0, 0, LT + LC);
+  sync();
+  cut(x0, a.K);
+  next_step();
+  load(x1, w1, 0, LT + LC);
+#pragma unroll
+  for (int j = 0; j < MC; ++j) read_w(w0, 0, 0, j);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) read_x(x0, 0, i);
+  for (; pos < run; pos += stride) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < MC; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    for (int s = 0; s < steps; s += 2) {
+      // Two steps ahead, or the next tile's first two.
+      const int ahead = s + 2 < steps ? s + 2 : 0;
+      if (ahead > 0)
+        next_step();
+      else
+        tile_rows(pos + stride);
+      buffer(x0, w0, x1, w1, a.K - (s + 1) * BK);
+      next_step();
+      buffer(x1, w1, x0, w0, a.K - ahead * BK);
+    }
+    // A lane has four channels of a token in each fragment; through LDS it gets eight of two tokens
+    // (or of more, where the wave has fewer channels), so that stores fill lines.
+    int t, c;
+    walk.at(id, pos, t, c);
+    constexpr int CHANNELS = 16 * MC, LPR = CHANNELS / 8, ROWS = kWave / LPR;  // lanes per token, tokens at a time
+    constexpr int TURNS = 16 / ROWS;                                           // token groups of a fragment
+    using S = typename Elems<DT>::S;
+    int ln = lane;  // (not to be kept in registers over the loop above)
+    asm volatile("" : "+v"(ln));
+    const int64_t t0 = static_cast<int64_t>(t) * BT + wt, left_t = a.T - t0;
+    const int c0 = c * BC + wc, col = ln % LPR * 8, row = ln / LPR;
+    L8Channels<DT> ch(a, c0 + col);
+    // (Waited for here, also where no token of the lane's is stored: not in the loop above.)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(ch.s[e]), "+v"(ch.b[e]));
+    int* own = turn[wave];
+    auto put = [&](int i) __attribute__((always_inline)) {
+      const int er = ln & 15, ek = ln >> 4;
+      l8_wave_sync();
+#pragma unroll
+      for (int j = 0; j < MC; ++j)
+        *reinterpret_cast<i32x4*>(own + er * CHANNELS + ((4 * j + ek) ^ (er & (4 * MC - 1))) * 4) = acc[i][j];
+      l8_wave_sync();
+    };
+    auto take = [&](int r, int (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<i32x4*>(v + 4 * h) =
+            *reinterpret_cast<const i32x4*>(own + r * CHANNELS + ((col / 4 + h) ^ (r & (4 * MC - 1))) * 4);
+    };
+    const float* xs0 = a.xs + t0;
+    auto* out0 = static_cast<S*>(a.out) + t0 * a.N + c0;
+    const auto* res0 = static_cast<const S*>(a.res) + t0 * a.N + c0;
+    const uint32_t at0 = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.N) + static_cast<uint32_t>(col);
+    // A whole tile: the tokens' scales and the residual are loaded before stores that their arrival would
+    // otherwise wait for.
+    auto whole = [&](auto with) __attribute__((always_inline)) {
+      constexpr bool RES = decltype(with)::value;
+      asm volatile("" ::: "memory");  // (its loads are its own: none is under way where it is not taken)
+      const int64_t by = static_cast<int64_t>(ROWS) * a.N;
+      float xs[2][TURNS];
+      L8Raw<DT> r[2][RES ? TURNS : 1];
+      auto fetch = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+          xs[i & 1][u] = (xs0 + 16 * i + ROWS * u)[static_cast<uint32_t>(row)];
+          if constexpr (RES) r[i & 1][u].load(res0 + (TURNS * i + u) * by + at0);
+        }
+      };
+      fetch(0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (i + 1 < MT) fetch(i + 1);
+        put(i);
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+          int q[8];
+          float v[8];
+          take(row + ROWS * u, q);
+          l8_scale<DT>(q, ch, xs[i & 1][u], v);
+          if constexpr (RES) r[i & 1][u].add_to(v);
+          Elems<DT>::template store8<false>(out0 + (TURNS * i + u) * by + at0, v);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // Every load has arrived, only the last stores may be under way (which the compiler does not see
+      // where the paths meet; it would wait in the loop above).
+      constexpr int last = (MT > 1 ? 2 : 1) * TURNS * (DT == FMHC_DTYPE_F32 ? 2 : 1);
+      l8_wait_vm<(last < 63 ? last : 63)>();
+    };
+    if (left_t >= BT - wt && c0 + BC - wc <= a.N) {
+      a.res ? whole(std::true_type{}) : whole(std::false_type{});
+    } else {
+      // One channel of a token at a time, what is inside.
+      static_assert(kWave % CHANNELS == 0 || CHANNELS % kWave == 0);
+      constexpr int EACH = kWave / CHANNELS > 1 ? kWave / CHANNELS : 1;  // tokens at a time
+      const int e = ln % CHANNELS;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        put(i);
+        if (c0 + e < a.N) {
+          float bias = 0.f;
+          if (a.bias)
+            bias = a.bias_f32 ? static_cast<const float*>(a.bias)[c0 + e]
+                              : Elems<DT>::load(static_cast<const S*>(a.bias) + c0 + e);
+#pragma unroll 1
+          for (int r = ln / CHANNELS; r < 16 && 16 * i + r < left_t; r += EACH) {
+            const int q = own[r * CHANNELS + (((e >> 2) ^ (r & (4 * MC - 1))) << 2 | (e & 3))];
+            float v = __builtin_fmaf(static_cast<float>(q) * xs0[16 * i + r], a.ws[c0 + e], bias);
+            const int64_t o = static_cast<int64_t>(16 * i + r) * a.N + e;
+            if (a.res) v += Elems<DT>::load(res0 + o);
+            Elems<DT>::store(out0 + o, v);
+          }
+        }
+      }
+      l8_wait_vm<0>();
+    }
+  }
+#endif
+}
+
+template <int DT, typename Tile>
+void l8_tile_launch(const L8Args& a, hipStream_t s) {
+  const int64_t tt = (a.T + Tile::BT - 1) / Tile::BT, tc = (a.N + Tile::BC - 1) / Tile::BC, tiles = tt * tc;
+  constexpr int per_cu = kLdsPerCu / (Tile::LDS + Tile::THREADS / kWave * 16 * Tile::BC / Tile::WC * 4);
+  const int64_t most = static_cast<int64_t>(kCus) * (per_cu > 4 ? 4 : per_cu);
+  const L8Walk walk{static_cast<int>(tiles), static_cast<int>(tt), static_cast<int>(tc)};
+  l8_tile_kernel<DT, Tile><<<dim3(static_cast<unsigned>(tiles < most ? tiles : most)), Tile::THREADS, 0, s>>>(a, walk);
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens: the weight's bytes, read once per 16 MT tokens.
+
+// A workgroup has 16 MC channels and 16 MT tokens; its waves share K, each a run of columns, straight
+// from memory to registers, UNROLL loads of a row under way at a time, and their sums meet in LDS.
+template <int kMT, int kMC, int kWaves, int kUnroll>
+struct L8Few {
+  static constexpr int MT = kMT, MC = kMC, WAVES = kWaves, UNROLL = kUnroll;
+};
+
+template <int DT, typename Few>
+__global__ __launch_bounds__(kWave * Few::WAVES) void l8_few_kernel(const L8Args a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int MT = Few::MT, MC = Few::MC, WAVES = Few::WAVES, U = Few::UNROLL;
+  __shared__ __align__(16) i32x4 sums[WAVES][MT * MC][kWave];
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int c0 = static_cast<int>(blockIdx.x) * 16 * MC;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  const int chunks = (a.K + 63) / 64, each = (chunks + WAVES - 1) / WAVES;
+  const int first = wave * each, last = first + each < chunks ? first + each : chunks;
+  // Rows past the last one are read as the last one, columns past K's last whole chunk as that chunk.
+  const int8_t *xp[MT], *wp[MC];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t t = t0 + 16 * i + (lane & 15);
+    xp[i] = a.x + (t < a.T ? t : a.T - 1) * a.ldx;
+  }
+#pragma unroll
+  for (int j = 0; j < MC; ++j) {
+    const int c = c0 + 16 * j + (lane & 15);
+    wp[j] = a.w + static_cast<int64_t>(c < a.N ? c : a.N - 1) * a.ldw;
+  }
+  const int end = l8_row_bytes(a.K) - kChunk, k0 = (lane >> 4) * kChunk;
   i32x4 acc[MT][MC];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < MC; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-
-  const int steps = (a.K + kStepK - 1) / kStepK;
-  load(0);
-  for (int k = 0; k < steps; ++k) {
-    __syncthreads();
-    if (k + 1 < steps) load((k + 1) & 1);
-    const int8_t* xb = xl[k & 1];
-    const int8_t* wb = wl[k & 1];
-    const int left = a.K - k * kStepK;
+  for (int s = first; s < last; s += U) {
+    i32x4 xf[U][MT], wf[U][MC];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = (lane >> 4) + 4 * h;
-      const int at = (lane & 15) * kStepK + ((c ^ (lane & 7)) * kChunk);
-      i32x4 xf[MT], wf[MC];
+    for (int u = 0; u < U; ++u) {
+      const int at = 64 * (s + u) + k0, k = at < end ? at : end;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        xf[i] = *reinterpret_cast<const i32x4*>(xb + (wt + 16 * i) * kStepK + at);
-        if (left < kStepK) {
+      for (int j = 0; j < MC; ++j) wf[u][j] = *reinterpret_cast<const i32x4*>(wp[j] + k);
 #pragma unroll
-          for (int d = 0; d < 4; ++d) xf[i][d] &= l8_mask(left - c * kChunk - 4 * d);
+      for (int i = 0; i < MT; ++i) xf[u][i] = *reinterpret_cast<const i32x4*>(xp[i] + k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= last) break;
+      const int left = a.K - 64 * (s + u);  // (x's columns from K on count as zero)
+      if (left < 64) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int m = l8_mask(left - k0 - 4 * d);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xf[u][i][d] &= m;
         }
       }
 #pragma unroll
-      for (int j = 0; j < MC; ++j) wf[j] = *reinterpret_cast<const i32x4*>(wb + (wc + 16 * j) * kStepK + at);
-#pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < MC; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < MC; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][j], xf[u][i], acc[i][j], 0, 0, 0);
     }
   }
-
-  // A lane has four channels of a token in each fragment.
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < MC; ++j) sums[wave][i * MC + j][lane] = acc[i][j];
+  __syncthreads();
   using S = typename Elems<DT>::S;
-  auto* out = static_cast<S*>(a.out);
-  const auto* res = static_cast<const S*>(a.res);
+  constexpr int CHANNELS = 16 * MC;
+  for (int o = static_cast<int>(threadIdx.x); o < 16 * MT * CHANNELS; o += kWave * WAVES) {
+    const int e = o % CHANNELS, r = o / CHANNELS, c = c0 + e;
+    const int64_t t = t0 + r;
+    if (c >= a.N || t >= a.T) continue;
+    const int* p = reinterpret_cast<const int*>(&sums[0][(r >> 4) * MC + (e >> 4)][(e >> 2 & 3) * 16 + (r & 15)]) + (e & 3);
+    int v = p[0];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t t = t0 + wt + 16 * i + (lane & 15);
-    if (t >= a.T) continue;
-    const float xs = a.xs[t];
-#pragma unroll
-    for (int j = 0; j < MC; ++j) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = c0 + wc + 16 * j + (lane >> 4) * 4 + e;
-        if (c >= a.N) continue;
-        float b = 0.f;
-        if (a.bias) b = a.bias_f32 ? static_cast<const float*>(a.bias)[c] : Elems<DT>::load(static_cast<const S*>(a.bias) + c);
-        float v = __builtin_fmaf(static_cast<float>(acc[i][j][e]) * xs, a.ws[c], b);
-        if (res) v += Elems<DT>::load(res + t * a.N + c);
-        Elems<DT>::store(out + t * a.N + c, v);
-      }
-    }
+    for (int k = 1; k < WAVES; ++k) v += p[k * MT * MC * kWave * 4];
+    float b = 0.f;
+    if (a.bias) b = a.bias_f32 ? static_cast<const float*>(a.bias)[c] : Elems<DT>::load(static_cast<const S*>(a.bias) + c);
+    float y = __builtin_fmaf(static_cast<float>(v) * a.xs[t], a.ws[c], b);
+    if (a.res) y += Elems<DT>::load(static_cast<const S*>(a.res) + t * a.N + c);
+    Elems<DT>::store(static_cast<S*>(a.out) + t * a.N + c, y);
   }
 #endif
 }
 
+template <int DT, typename Few>
+void l8_few_launch(const L8Args& a, hipStream_t s) {
+  const dim3 grid(blocks_for(a.N, 16 * Few::MC), blocks_for(a.T, 16 * Few::MT));
+  l8_few_kernel<DT, Few><<<grid, kWave * Few::WAVES, 0, s>>>(a);
+}
+
+// The shortest of the tile kernels for `tiles` tiles of theirs, in hundredths of a round of 256 x 256 tiles,
+// one per CU (63 us at K = 4096): of 128 x 128 and 64 x 64 two fit on a CU, and one there is not twice as
+// fast (37 and 27 us, 17 and 13).
+struct L8Cost {
+  int tile, per_cu, round, one_each;
+  int64_t of(int64_t T, int64_t N) const {
+    const int64_t tiles = ((T + tile - 1) / tile) * ((N + tile - 1) / tile), slots = int64_t{kCus} * per_cu;
+    return tiles <= kCus ? one_each : (tiles + slots - 1) / slots * round;
+  }
+};
+constexpr L8Cost kL8Cost256{256, 1, 100, 100}, kL8Cost128{128, 2, 56, 43}, kL8Cost64{64, 2, 25, 21};
+
+// Few tokens go without LDS: up to 16 per workgroup where every workgroup has a CU of its own (us, against
+// 32 tokens and against 64 x 64 tiles: T = 64, N = 1024, K = 4096 5.8, 7.6, 9.6; T = 1, N = K = 4096 4.9, 5.3,
+// 12.3), 32 up to 32 tokens (T = 32, N = K = 4096 8.1; 16 9.5, tiles 15.1; T = 64 13.3 against 13.0 of tiles).
 template <int DT>
 int l8_run(const L8Args& a, hipStream_t s) {
-  const dim3 grid(blocks_for(a.N, 128), blocks_for(a.T, 128));
-  l8_tile_kernel<DT, 128, 128, 2, 2><<<grid, 256, 0, s>>>(a);
+  const int64_t channels = (a.N + 15) / 16;
+  if (a.T <= 16 || (a.T + 15) / 16 * channels <= kCus) {
+    l8_few_launch<DT, L8Few<1, 1, 8, 2>>(a, s);
+  } else if (a.T <= 32) {
+    l8_few_launch<DT, L8Few<2, 1, 8, 2>>(a, s);
+  } else {
+    const int64_t large = kL8Cost256.of(a.T, a.N), medium = kL8Cost128.of(a.T, a.N), small = kL8Cost64.of(a.T, a.N);
+    if (large <= medium && large <= small)
+      l8_tile_launch<DT, L8Tile<256, 256, 2, 4, 128>>(a, s);
+    else if (medium <= small)
+      l8_tile_launch<DT, L8Tile<128, 128, 2, 2, 128>>(a, s);
+    else
+      l8_tile_launch<DT, L8Tile<64, 64, 2, 2, 256>>(a, s);
+  }
   return launch_status();
 }
 
@@ -164,7 +562,7 @@ extern "C" int fmhc_linear8(const int8_t* x, int64_t ldx, const float* x_scales,
                             const float* w_scales, const void* bias, const void* residual, void* out, int dtype,
                             int bias_dtype, int64_t T, int64_t N, int64_t K, void* stream) {
   using namespace fmhc;
-  if (T < 0 || N <= 0 || K <= 0 || K >= (1 << 17) || N > (int64_t{1} << 30) || T > (int64_t{1} << 60) / N ||
+  if (T < 0 || N <= 0 || K <= 0 || K >= (1 << 17) || N >= (1 << 22) || T >= (int64_t{1} << 31) || T > (int64_t{1} << 40) / N ||
       (bias_dtype != FMHC_DTYPE_F32 && bias_dtype != dtype))
     return FMHC_ERR_INVALID_ARGUMENT;
   if (dtype != FMHC_DTYPE_F32 && dtype != FMHC_DTYPE_BF16 && dtype != FMHC_DTYPE_F16) return FMHC_ERR_INVALID_ARGUMENT;

@@ -57,7 +57,8 @@ COMMON_FLAGS = [
 # loop-carried weight-gradient accumulators in VGPRs and copies them to and
 # from AGPRs around every MFMA, which doubles the kernel's register footprint.
 SOURCE_FLAGS = {"k1.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-                "premap_resident.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+                "premap_resident.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "linear8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 # Evidence builds of the same library, selected at compile time.  k1_valu: the
 # K1 forward and backward-dx contractions as fp32 FMAs on the VALU instead of
