@@ -23,6 +23,7 @@ struct L8Args {
   bool bias_f32;     // bias in fp32, otherwise in out's type
   const void* res;   // may be null
   void* out;
+  bool lines;        // rows of out begin at multiples of 16 bytes
   int64_t T;
   int N, K;
 };
@@ -58,7 +59,10 @@ struct L8Channels {
 template <int DT>
 struct L8Raw {
   u32x4 a;
-  __device__ __forceinline__ void load(const typename Elems<DT>::S* p) { a = ld16(p); }
+  template <bool NT>
+  __device__ __forceinline__ void load(const typename Elems<DT>::S* p) {
+    a = NT ? ld16_stream(p) : ld16(p);
+  }
   __device__ __forceinline__ void add_to(float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -75,6 +79,7 @@ struct L8Raw {
 template <>
 struct L8Raw<FMHC_DTYPE_F32> {
   u32x4 a, b;
+  template <bool NT>
   __device__ __forceinline__ void load(const float* p) {
     a = ld16(p);
     b = ld16(p + 4);
@@ -343,9 +348,13 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     const auto* res0 = static_cast<const S*>(a.res) + t0 * a.N + c0;
     const uint32_t at0 = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.N) + static_cast<uint32_t>(col);
     // A whole tile: the tokens' scales and the residual are loaded before stores that their arrival would
-    // otherwise wait for.
-    auto whole = [&](auto with) __attribute__((always_inline)) {
-      constexpr bool RES = decltype(with)::value;
+    // otherwise wait for.  Rows that begin at 16 bytes are stored, and the residual's loaded, with the
+    // nontemporal hint: neither is read again here, and what the tiles read stays cached (with / without, us:
+    // T = 65536, N = K = 1024 80 / 96, with a residual 99 / 106; T = 16384, N = K = 4096 235 / 245; the
+    // residual's loads alone 120 / 127 for a norm and its product at T = 65536).  Other rows share lines with
+    // their neighbours' stores, which are to meet in the cache.
+    auto whole = [&](auto with, auto lines) __attribute__((always_inline)) {
+      constexpr bool RES = decltype(with)::value, LINES = decltype(lines)::value;
       asm volatile("" ::: "memory");  // (its loads are its own: none is under way where it is not taken)
       const int64_t by = static_cast<int64_t>(ROWS) * a.N;
       float xs[2][TURNS];
@@ -354,7 +363,7 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
           xs[i & 1][u] = (xs0 + 16 * i + ROWS * u)[static_cast<uint32_t>(row)];
-          if constexpr (RES) r[i & 1][u].load(res0 + (TURNS * i + u) * by + at0);
+          if constexpr (RES) r[i & 1][u].template load<LINES>(res0 + (TURNS * i + u) * by + at0);
         }
       };
       fetch(0);
@@ -369,7 +378,7 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
           take(row + ROWS * u, q);
           l8_scale<DT>(q, ch, xs[i & 1][u], v);
           if constexpr (RES) r[i & 1][u].add_to(v);
-          Elems<DT>::template store8<false>(out0 + (TURNS * i + u) * by + at0, v);
+          Elems<DT>::template store8<LINES>(out0 + (TURNS * i + u) * by + at0, v);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -379,7 +388,10 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
       l8_wait_vm<(last < 63 ? last : 63)>();
     };
     if (left_t >= BT - wt && c0 + BC - wc <= a.N) {
-      a.res ? whole(std::true_type{}) : whole(std::false_type{});
+      if (a.lines)
+        a.res ? whole(std::true_type{}, std::true_type{}) : whole(std::false_type{}, std::true_type{});
+      else
+        a.res ? whole(std::true_type{}, std::false_type{}) : whole(std::false_type{}, std::false_type{});
     } else {
       // One channel of a token at a time, what is inside.
       static_assert(kWave % CHANNELS == 0 || CHANNELS % kWave == 0);
@@ -568,7 +580,7 @@ extern "C" int fmhc_linear8(const int8_t* x, int64_t ldx, const float* x_scales,
   if (dtype != FMHC_DTYPE_F32 && dtype != FMHC_DTYPE_BF16 && dtype != FMHC_DTYPE_F16) return FMHC_ERR_INVALID_ARGUMENT;
   if (T == 0) return FMHC_OK;
   if (bad_rows(x, ldx, K) || bad_rows(w, ldw, K) || !x_scales || !w_scales || !out) return FMHC_ERR_INVALID_ARGUMENT;
-  const L8Args a{x, ldx, x_scales, w, ldw, w_scales, bias, bias_dtype == FMHC_DTYPE_F32, residual, out, T,
-                 static_cast<int>(N), static_cast<int>(K)};
+  const L8Args a{x, ldx, x_scales, w, ldw, w_scales, bias, bias_dtype == FMHC_DTYPE_F32, residual, out,
+                 aligned16(out) && N % 8 == 0, T, static_cast<int>(N), static_cast<int>(K)};
   return with_dtype(dtype, [&](auto dt) { return l8_run<decltype(dt)::value>(a, static_cast<hipStream_t>(stream)); });
 }
