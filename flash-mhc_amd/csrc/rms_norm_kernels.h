@@ -515,28 +515,34 @@ int rms_fwd_run(const RmsFwdArgs& a, hipStream_t s) {
   const auto* r = static_cast<const S*>(a.r);
   auto* y = static_cast<S*>(a.y);
   auto* sum = static_cast<S*>(a.sum);
-  const bool nt = ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(x) && aligned16(r) && aligned16(y) &&
-                  aligned16(sum) && (reinterpret_cast<uintptr_t>(a.codes) & 7u) == 0 && a.ld_codes % 8 == 0;
+  // Packed rows carry no nontemporal hint: their codes are multiplied next, and the row may be that
+  // product's residual (pack and product with the hint / without, us: T = 65536, C = 1024 with the norm and
+  // the residual 136 / 120, T = 8192, C = 2048 47 / 44).
+  const bool nt = y && ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(x) && aligned16(r) && aligned16(y) &&
+                  aligned16(sum);
   const bool held = with_ln_walk<(DT == FMHC_DTYPE_F32 ? 3 : 5)>(a.T, a.C, [&](auto walk) {
     constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, BLOCK = ln_fwd_block<LPT>();
     auto launch = [&](auto ntc, auto add, auto out) {
       auto* kernel = &rms_fwd_kernel<DT, LPT, R, decltype(ntc)::value, decltype(add)::value, decltype(out)::value>;
-      // Workgroups as the layer norm's forward has them (ln_fwd_run).
-      const int64_t want = (a.T + BLOCK / LPT - 1) / (BLOCK / LPT);
-      const int64_t deep = LPT <= kWave ? want / 4 : 0, fit = ((int64_t{1} << 32) - 1) / BLOCK;
-      const int64_t many = deep > 256 * 8 ? deep : 256 * 8, most = many < fit ? many : fit;
+      // Eight workgroups per CU, and from there one row per slot where there is a residual, two otherwise
+      // (eight per CU / two rows / one, us, T = 65536, C = 2048: with a residual 183 / 176 / 172, without 95 /
+      // 86 / 88, packed 75 / 73 / 78 and with a residual 177 / 171 / 164; T = 262144, C = 1024 423 / 365 / 354
+      // and 200 / 172 / 171; T = 8192, C = 8192 100 / 98 / 94 and 49 / 48 / 48).  A launch has fewer than 2^32
+      // threads; the workgroups walk the rest of the rows.
+      const int64_t want = (a.T + BLOCK / LPT - 1) / (BLOCK / LPT), fit = ((int64_t{1} << 32) - 1) / BLOCK;
+      const int64_t some = r ? want : want / 2, many = some > 256 * 8 ? some : 256 * 8, most = many < fit ? many : fit;
       kernel<<<dim3(static_cast<unsigned>(want < most ? want : most)), BLOCK, 0, s>>>(
           x, r, a.w, a.w_f32, y, a.codes, a.scales, a.ld_codes, sum, a.rstd, a.T, a.C, a.eps);
     };
     using std::integral_constant;
-    auto pick = [&](auto ntc) {
-      constexpr integral_constant<int, kRmsY> as_y;
-      constexpr integral_constant<int, kRmsCodes> as_codes;
-      if (!a.norm) launch(ntc, std::false_type{}, integral_constant<int, kRmsRows>{});
-      else if (y) r ? launch(ntc, std::true_type{}, as_y) : launch(ntc, std::false_type{}, as_y);
-      else r ? launch(ntc, std::true_type{}, as_codes) : launch(ntc, std::false_type{}, as_codes);
-    };
-    nt ? pick(std::true_type{}) : pick(std::false_type{});
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    constexpr integral_constant<int, kRmsY> as_y;
+    constexpr integral_constant<int, kRmsCodes> as_codes;
+    if (!a.norm) launch(no, no, integral_constant<int, kRmsRows>{});
+    else if (!y) r ? launch(no, yes, as_codes) : launch(no, no, as_codes);
+    else if (nt) r ? launch(yes, yes, as_y) : launch(yes, no, as_y);
+    else r ? launch(no, yes, as_y) : launch(no, no, as_y);
   });
   if (!held) {
     const int64_t most = 16384;
