@@ -924,8 +924,10 @@ def empty_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Unwritten (codes, scales) for a contiguous x (..., C): codes in rows of row_pitch(C) bytes."""
     shape = x.shape
     C = shape[-1]
-    codes = x.new_empty((*shape[:-1], row_pitch(C)), dtype=torch.int8)
-    return codes if C % ROW_PITCH == 0 else codes[..., :C], x.new_empty(shape[:-1], dtype=_F32)
+    scales = x.new_empty(shape[:-1], dtype=_F32)
+    if C % ROW_PITCH == 0:
+        return torch.empty_like(x, dtype=torch.int8), scales
+    return x.new_empty((*shape[:-1], row_pitch(C)), dtype=torch.int8)[..., :C], scales
 
 
 def pack8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -958,11 +960,11 @@ def _code_rows(codes: torch.Tensor, name: str, dev) -> tuple[torch.Tensor, int, 
     are, or a copy in rows of row_pitch(K) bytes."""
     if not isinstance(codes, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    shape = codes.shape
     if codes.dtype is not torch.int8:
         raise TypeError(f"{name} must be {torch.int8}, got {codes.dtype}")
     if codes.device != dev:
         raise ValueError(f"{name} is on {codes.device}, expected {dev}")
-    shape = codes.shape
     if len(shape) == 0 or not 1 <= shape[-1] <= MOST_K:
         raise ValueError(f"{name} must have shape (..., K) with 1 <= K <= {MOST_K}, got {tuple(shape)}")
     K = shape[-1]

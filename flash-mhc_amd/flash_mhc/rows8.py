@@ -108,12 +108,13 @@ def _direct(x, *tensors) -> bool:
     no graph is recorded (the ops' backward raises)."""
     if not _block._plain_eager(x):
         return False
-    ordinary = True
-    for t in tensors:
-        ordinary = ordinary and (t is None or type(t) is torch.Tensor or type(t) is nn.Parameter)
-    if not ordinary or torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad
-                                                                           for t in tensors)):
+    graph = torch.is_grad_enabled()
+    if graph and x.requires_grad:
         return False
+    for t in tensors:
+        if t is not None and ((type(t) is not torch.Tensor and type(t) is not nn.Parameter)
+                              or (graph and t.requires_grad)):
+            return False
     if _forward_ad._current_level >= 0:
         refuse_tangents(x, *tensors)
     return True
