@@ -60,15 +60,19 @@ struct RmsStats {
   }
 };
 
-// A packed row's scale and the factor of its codes, from its largest magnitude: code =
-// round_half_even(v 127 / top), scale = top / 127.  Inf or NaN in the row: scale NaN, codes 0.
+// A packed row's scale and the factor of its codes, from the bits of its largest magnitude
+// before rstd: code = round_half_even(v 127 / top), scale = top / 127.  Inf or NaN in the row:
+// scale NaN, codes 0.  A magnitude below the normal numbers has too few bits for a scale where
+// rstd is large (eps near 0): such a row counts as zero.
 struct RowScale {
   float scale, to_code;
   uint32_t keep;
 };
-__device__ __forceinline__ RowScale row_scale(float top, bool finite) {
-  top = fmaxf(top, kRowLeast);
-  return RowScale{finite ? top / 127.f : __uint_as_float(0x7fc00000u), finite ? 127.f / top : 0.f, finite ? ~0u : 0u};
+__device__ __forceinline__ RowScale row_scale(uint32_t m, float rstd) {
+  float top = __uint_as_float(m) * rstd;
+  const bool finite = top < __builtin_inff(), some = finite && m >= 0x00800000u;
+  top = some ? fmaxf(top, kRowLeast) : kRowLeast;
+  return RowScale{finite ? top / 127.f : __uint_as_float(0x7fc00000u), some ? 127.f / top : 0.f, some ? ~0u : 0u};
 }
 
 // v 127 / top is rounded, so that half the largest magnitude (a common value in 16 bits) is 63.5
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(ln_fwd_block<LPT>()) void rms_fwd_kernel(
     stats(s, m);
     if constexpr (OUT != kRmsRows) rstd = rsqrtf(s * n_inv + eps);
     RowScale rs;
-    if constexpr (OUT != kRmsY) rs = row_scale(__uint_as_float(m) * rstd, m < 0x7f800000u && rstd < __builtin_inff());
+    if constexpr (OUT != kRmsY) rs = row_scale(m, rstd);
     if (t < T) {
 #pragma unroll
       for (int k = 0; k < R; ++k) {
@@ -367,7 +371,7 @@ __global__ __launch_bounds__(ln_any_block<N>()) void rms_fwd_any(
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < BLOCK / kWave; ++i) m = redm[i] > m ? redm[i] : m;
-      rs = row_scale(__uint_as_float(m) * rstd, m < 0x7f800000u && rstd < __builtin_inff());
+      rs = row_scale(m, rstd);
     }
     for (int i = lane; N * i < C; i += BLOCK) {
       const LnPlace p = ln_any_place<N>(i, C);

@@ -371,7 +371,8 @@ int64_t fmhc_rms_norm_bwd_workspace_bytes(int64_t T, int64_t C);
 int fmhc_pack8_rows(const void* x, int dtype, int8_t* codes, float* scales, int64_t rows, int64_t C,
                     int64_t ld_codes, void* stream);
 /* The rows y of fmhc_rms_norm_fwd, before their rounding to `dtype`, as codes (T, C)
- * and scales (T,); sum as there. */
+ * and scales (T,); sum as there.  A row whose s weight overflows fp32 has scale NaN,
+ * one in which every |s weight| is below 2^-126 counts as zero. */
 int fmhc_rms_norm_pack8_rows(const void* x, const void* residual, const void* weight, int8_t* codes,
                              float* scales, void* sum, int dtype, int param_dtype, int64_t T,
                              int64_t C, int64_t ld_codes, float eps, void* stream);
@@ -382,7 +383,8 @@ int fmhc_rms_norm_pack8_rows(const void* x, const void* residual, const void* we
  * last one too, can be read to the next multiple of 16 bytes (what is there does not
  * matter).  The sum is exact; K < 2^17.  out and residual (may be NULL) are (T, N)
  * in `dtype`, contiguous; bias (N,), in bias_dtype, FMHC_DTYPE_F32 or `dtype`, may be
- * NULL.  out is rounded once; it may not overlap an input. */
+ * NULL.  out is rounded once; it may not overlap an input.  T < 2^31, N < 2^22 and
+ * T N <= 2^40. */
 int fmhc_linear8(const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, int64_t ldw,
                  const float* w_scales, const void* bias, const void* residual, void* out, int dtype,
                  int bias_dtype, int64_t T, int64_t N, int64_t K, void* stream);

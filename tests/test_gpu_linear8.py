@@ -104,6 +104,22 @@ def test_norm_rows_without_weight_and_with_bad_rows():
     assert float(scales[5]) == float(torch.tensor(2.0 ** -100) / 127)
 
 
+@pytest.mark.parametrize("C", [5, 40, 1024, 20000])
+def test_norm_rows_at_the_ends_of_fp32(C):
+    """Products with the weight past fp32's range and below its normal numbers, at eps = 0."""
+    x = torch.ones(4, C, device=DEV) * torch.tensor([2.0 ** 60, 2.0 ** -63, 1.0, 0.0], device=DEV)[:, None]
+    for e, bad in ((70, [0, 3]), (-70, [3])):  # 2^130 and 2^-133 (0 / 0 in the last row)
+        codes, scales = flash_mhc.rms_norm_pack8_rows(x, torch.full((C,), 2.0 ** e, device=DEV), 0.0)
+        assert bool(torch.isnan(scales[bad]).all()) and int(codes[bad].abs().max()) == 0
+        # (The scale is off by the statistic's roundings: C / C, rsqrt, and its own two.)
+        # From C = 256 on the first row's sum of squares is 2^120 C >= 2^128, past fp32: rstd and the norm are 0.
+        zero = C >= 256
+        for row in ([2] if e > 0 or zero else [0, 2]):
+            assert abs(float(scales[row]) * 127 / 2.0 ** e - 1) <= 2.0 ** -21 and int(codes[row].min()) == 127
+        for row in ([] if e > 0 else [0, 1] if zero else [1]):
+            assert float(scales[row]) == float(torch.tensor(2.0 ** -100) / 127) and int(codes[row].abs().max()) == 0
+
+
 def test_norm_rows_in_fp32_are_the_norms_rows():
     """fp32 rows are packed from the values that rms_norm returns: the same codes but for the
     scale's last bits."""
