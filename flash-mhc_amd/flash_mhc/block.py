@@ -161,7 +161,7 @@ class MHCLiteBlock(nn.Module):
             self.rms_weight = nn.Parameter(torch.ones(self.nC))
         else:
             self.rms_weight = None
-        if pre_norm not in (False, True, "layer", "rms"):
+        if isinstance(pre_norm, str) and pre_norm not in ("layer", "rms"):
             raise ValueError(f'pre_norm must be False, True, "layer" or "rms", got {pre_norm!r}')
         if pre_norm == "rms":
             from .norm import RMSNorm

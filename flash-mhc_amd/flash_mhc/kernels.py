@@ -914,6 +914,7 @@ def rms_norm_bwd_saved(grad_y, x, rstd, weight, param_dtype, need_weight, grad_x
 ROW_PITCH = 16  # rows of codes begin at multiples of this many bytes
 MOST_PITCH = 1 << 22
 MOST_K = (1 << 17) - 1  # the integer sums stay in 32 bits
+MOST_N = (1 << 22) - 1
 
 
 def row_pitch(C: int) -> int:
@@ -992,8 +993,8 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
     code = _dtype_code(dtype, "dtype")
     lead = codes.shape[:-1]
     x, T, ldx = _code_rows(codes, "codes", dev)
-    if weight_codes.dim() != 2 or weight_codes.shape[1] != codes.shape[-1] or weight_codes.shape[0] < 1:
-        raise ValueError(f"weight_codes must have shape (N, {codes.shape[-1]}) with N >= 1, got "
+    if weight_codes.dim() != 2 or weight_codes.shape[1] != codes.shape[-1] or not 1 <= weight_codes.shape[0] <= MOST_N:
+        raise ValueError(f"weight_codes must have shape (N, {codes.shape[-1]}) with 1 <= N <= {MOST_N}, got "
                          f"{tuple(weight_codes.shape)}")
     w, N, ldw = _code_rows(weight_codes, "weight_codes", dev)
     _require(scales, "scales", _F32, lead, dev)

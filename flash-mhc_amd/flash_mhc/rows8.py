@@ -138,7 +138,10 @@ def pack8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def rms_norm_pack8_rows(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
                         residual: torch.Tensor | None = None):
     """(codes, scales) of rms_norm(x, weight, eps), taken from its fp32 values; with a
-    residual (codes, scales, sum) of rms_norm(x, weight, eps, residual).  No gradient."""
+    residual (codes, scales, sum) of rms_norm(x, weight, eps, residual).  No gradient.
+
+    (A row has scale NaN where its product with weight overflows fp32, and counts as zero where
+    all of it is below 2^-126.)"""
     if _direct(x, weight, residual):
         out = _k.rms_norm_pack8_rows(x.contiguous(), _dense(residual), _dense(weight), eps)
         return out[:2] if residual is None else out
@@ -157,7 +160,7 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
 
         (codes @ weight_codes^T) * scales[..., None] * weight_scales + bias + residual
 
-    codes (..., K) and weight_codes (N, K) int8 with K < 2^17, scales (...,) and
+    codes (..., K) and weight_codes (N, K) int8 with K < 2^17 and N < 2^22, scales (...,) and
     weight_scales (N,) fp32 (pack8_rows of a token's row and of a weight's), bias (N,)
     fp32 or of dtype, residual (..., N) of dtype.  The sum of integers is exact.  No
     gradient."""
@@ -193,9 +196,9 @@ class Linear8(nn.Module):
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None) -> None:
         super().__init__()
-        if not 1 <= in_features <= _k.MOST_K or out_features < 1:
-            raise ValueError(f"Linear8 takes in_features from 1 to {_k.MOST_K} and out_features from 1, got "
-                             f"{in_features} and {out_features}")
+        if not 1 <= in_features <= _k.MOST_K or not 1 <= out_features <= _k.MOST_N:
+            raise ValueError(f"Linear8 takes in_features from 1 to {_k.MOST_K} and out_features from 1 to {_k.MOST_N}, "
+                             f"got {in_features} and {out_features}")
         self.in_features = in_features
         self.out_features = out_features
         # Rows at the kernels' pitch; the columns past in_features are zero.

@@ -139,6 +139,9 @@ def test_refusals():
         flash_mhc.Linear8(8, 4)(torch.zeros(3, 9))
     with pytest.raises(ValueError, match="pre_norm must be"):
         flash_mhc.MHCLiteBlock(4, 8, torch.nn.Linear(8, 8), pre_norm="group")
+    assert flash_mhc.MHCLiteBlock(4, 8, torch.nn.Linear(8, 8), pre_norm=None).norm is None
+    with pytest.raises(ValueError, match="out_features"):
+        flash_mhc.Linear8(4, 1 << 22)
 
 
 def _meta(shape, dtype=BF16):
@@ -168,6 +171,7 @@ def test_launchers_name_what_is_wrong(monkeypatch):
                         ("weight_codes must be torch.int8", (q, s, _meta((5, 16), torch.uint8), ws)),
                         (r"weight_codes must have shape \(N, 16\)", (q, s, _meta((5, 17), i8), ws)),
                         (r"weight_codes must have shape \(N, 16\)", (q, s, _meta((0, 16), i8), ws)),
+                        ("1 <= N", (q, s, _meta((1 << 22, 16), i8), ws)),
                         ("scales must have shape", (q, _meta((3,), F32), w, ws)),
                         ("scales must be torch.float32", (q, _meta((2,)), w, ws)),
                         ("weight_scales must have shape", (q, s, w, _meta((4,), F32))),
