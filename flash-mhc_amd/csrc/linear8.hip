@@ -117,12 +117,12 @@ __device__ __forceinline__ void l8_wait_vm() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
 }
 
-// BT tokens x BC channels per workgroup, WT x WC waves, steps of BK columns.
-template <int kBT, int kBC, int kWT, int kWC, int kBK>
+// BT tokens x BC channels per workgroup, WT x WC waves, steps of BK columns, NB (2 or 4) of them in LDS.
+template <int kBT, int kBC, int kWT, int kWC, int kNB>
 struct L8Tile {
-  static constexpr int BT = kBT, BC = kBC, WT = kWT, WC = kWC, BK = kBK;
+  static constexpr int BT = kBT, BC = kBC, WT = kWT, WC = kWC, BK = 128, NB = kNB;
   static constexpr int THREADS = kWave * WT * WC;
-  static constexpr int LDS = 2 * (BT + BC) * BK;
+  static constexpr int LDS = NB * (BT + BC) * BK;
 };
 
 // How a launch's workgroups walk the tiles: each XCD (workgroup id mod 8) has a run of them, in which
@@ -148,30 +148,36 @@ struct L8Walk {
   }
 };
 
-// Loads go from memory to LDS without registers (rows of BK bytes, 16 bytes a lane), a step and a part
-// ahead of the products, fragments from LDS to registers one part of 64 columns ahead.  The loads run on
+// Loads go from memory to LDS without registers (rows of BK bytes, 16 bytes a lane), NB - 1 steps and a
+// part ahead of the products, fragments from LDS to registers one part of 64 columns ahead.  The loads run on
 // into the workgroup's next tile while this one's results are stored.
 template <int DT, typename Tile>
 __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args a, const L8Walk walk) {
 // (The host's pass has no type for a buffer's descriptor.)
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int BT = Tile::BT, BC = Tile::BC, WT = Tile::WT, WC = Tile::WC, BK = Tile::BK;
+  constexpr int BT = Tile::BT, BC = Tile::BC, WT = Tile::WT, WC = Tile::WC, BK = Tile::BK, NB = Tile::NB;
   constexpr int WAVES = WT * WC, MT = BT / WT / 16, MC = BC / WC / 16;
   constexpr int RPL = kWave * kChunk / BK;                     // rows per load of a wave
   constexpr int LT = BT / RPL / WAVES, LC = BC / RPL / WAVES;  // loads per wave and step
   constexpr int PARTS = BK / 64;                               // of a step: one instruction's columns
-  static_assert(LT >= 1 && LC >= 1 && MT >= 1 && MC >= 2 && MC % 2 == 0 && PARTS % 2 == 0);
+  static_assert((NB == 2 || NB == 4) && LT >= 1 && LC >= 1 && MT >= 1 && MC >= 2 && MC % 2 == 0 && PARTS % 2 == 0);
+  // (Arrays of their own: in one array the compiler would wait for all loads before each read.)
+  constexpr bool FOUR = NB == 4;
   __shared__ __align__(16) int8_t x0[BT * BK];
   __shared__ __align__(16) int8_t x1[BT * BK];
+  __shared__ __align__(16) int8_t x2[FOUR ? BT * BK : 16];
+  __shared__ __align__(16) int8_t x3[FOUR ? BT * BK : 16];
   __shared__ __align__(16) int8_t w0[BC * BK];
   __shared__ __align__(16) int8_t w1[BC * BK];
+  __shared__ __align__(16) int8_t w2[FOUR ? BC * BK : 16];
+  __shared__ __align__(16) int8_t w3[FOUR ? BC * BK : 16];
   __shared__ __align__(16) int turn[WAVES][16 * 16 * MC];
   using Lds = __attribute__((address_space(3))) int8_t;
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int id = static_cast<int>(blockIdx.x), run = walk.run(id), stride = walk.step(id, static_cast<int>(gridDim.x));
-  // Two steps, one per buffer, at a time.
-  const int bytes = l8_row_bytes(a.K), steps = (a.K + 2 * BK - 1) / (2 * BK) * 2;
+  // NB steps, one per buffer, at a time.
+  const int bytes = l8_row_bytes(a.K), steps = (a.K + NB * BK - 1) / (NB * BK) * NB;
 
   // What is loaded next: rows from xp and wp on, xn and wn bytes of which can be read.  Reads past a
   // tile's last row give zeros, and so do those past the last tile.
@@ -202,8 +208,9 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
   for (int j = 0; j < LC; ++j) wo[j] = (lrow + RPL * (wave + WAVES * j)) * static_cast<int>(a.ldw) + lchunk * kChunk;
   // Loads j0 .. j1 of a step: x's first, then w's.
   auto load = [&](int8_t* xb, int8_t* wb, int j0, int j1) __attribute__((always_inline)) {
-    const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp), 0, xn, 0x00027000);
-    const auto wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp), 0, wn, 0x00027000);
+    // (Uniform as they are; the compiler is told, or it loops over the lanes.)
+    const auto xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(xp), 0, __builtin_amdgcn_readfirstlane(xn), 0x00027000);
+    const auto wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wp), 0, __builtin_amdgcn_readfirstlane(wn), 0x00027000);
 #pragma unroll
     for (int j = j0; j < j1; ++j) {
       int8_t* to = (j < LT ? xb : wb) + (wave + WAVES * (j < LT ? j : j - LT)) * RPL * BK;
@@ -226,11 +233,13 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
   auto read_x = [&](const int8_t* xb, int part, int i) __attribute__((always_inline)) {
     xf[i % AHEAD] = *reinterpret_cast<const i32x4*>(xb + (wt + 16 * i) * BK + at(part));
   };
-  // A wave's own loads have landed and its reads are done; then all waves'.
+  // A wave's own loads for the next step have landed, those for the NB - 2 after it may be under way, and its
+  // reads are done; then all waves'.
   auto sync = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    constexpr int N = (NB - 2) * (LT + LC);
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);  // vmcnt(N) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -289,10 +298,17 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
   int pos = walk.first(id);
   tile_rows(pos);
   load(x0, w0, 0, LT + LC);
+  l8_wait_vm<0>();
   sync();
   cut(x0, a.K);
   next_step();
   load(x1, w1, 0, LT + LC);
+  if constexpr (FOUR) {
+    next_step();
+    load(x2, w2, 0, LT + LC);
+    next_step();
+    load(x3, w3, 0, LT + LC);
+  }
 #pragma unroll
   for (int j = 0; j < MC; ++j) read_w(w0, 0, 0, j);
 #pragma unroll
@@ -302,16 +318,24 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < MC; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    for (int s = 0; s < steps; s += 2) {
-      // Two steps ahead, or the next tile's first two.
-      const int ahead = s + 2 < steps ? s + 2 : 0;
+    for (int s = 0; s < steps; s += NB) {
+      // NB steps ahead, or the next tile's first NB.
+      const int ahead = s + NB < steps ? s + NB : 0;
       if (ahead > 0)
         next_step();
       else
         tile_rows(pos + stride);
       buffer(x0, w0, x1, w1, a.K - (s + 1) * BK);
       next_step();
-      buffer(x1, w1, x0, w0, a.K - ahead * BK);
+      if constexpr (FOUR) {
+        buffer(x1, w1, x2, w2, a.K - (s + 2) * BK);
+        next_step();
+        buffer(x2, w2, x3, w3, a.K - (s + 3) * BK);
+        next_step();
+        buffer(x3, w3, x0, w0, a.K - ahead * BK);
+      } else {
+        buffer(x1, w1, x0, w0, a.K - ahead * BK);
+      }
     }
     // A lane has four channels of a token in each fragment; through LDS it gets eight of two tokens
     // (or of more, where the wave has fewer channels), so that stores fill lines.
@@ -347,14 +371,19 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     auto* out0 = static_cast<S*>(a.out) + t0 * a.N + c0;
     const auto* res0 = static_cast<const S*>(a.res) + t0 * a.N + c0;
     const uint32_t at0 = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.N) + static_cast<uint32_t>(col);
-    // A whole tile: the tokens' scales and the residual are loaded before stores that their arrival would
-    // otherwise wait for.  Rows that begin at 16 bytes are stored, and the residual's loaded, with the
-    // nontemporal hint: neither is read again here, and what the tiles read stays cached (with / without, us:
-    // T = 65536, N = K = 1024 80 / 96, with a residual 99 / 106; T = 16384, N = K = 4096 235 / 245; the
-    // residual's loads alone 120 / 127 for a norm and its product at T = 65536).  Other rows share lines with
-    // their neighbours' stores, which are to meet in the cache.
-    auto whole = [&](auto with, auto lines) __attribute__((always_inline)) {
-      constexpr bool RES = decltype(with)::value, LINES = decltype(lines)::value;
+    // What is inside: tokens of the wave, channels of the lane.
+    constexpr int most_t = 16 * MT;
+    const int tokens = static_cast<int>(left_t < most_t ? left_t : most_t);
+    const int mine = a.N - c0 - col < 8 ? a.N - c0 - col : 8;
+    // The tokens' scales and the residual are loaded before stores that their arrival would otherwise wait
+    // for.  Rows that begin at 16 bytes are stored, and the residual's loaded, with the nontemporal hint:
+    // neither is read again here, and what the tiles read stays cached (with / without, us: T = 65536,
+    // N = K = 1024 80 / 96, with a residual 99 / 106; T = 16384, N = K = 4096 235 / 245; the residual's loads
+    // alone 120 / 127 for a norm and its product at T = 65536).  Other rows share lines with their neighbours'
+    // stores, which are to meet in the cache.  At the edges (EDGE) tokens past the last one are read as the
+    // last one, and only what is inside is stored.
+    auto finish = [&](auto with, auto lines, auto edge) __attribute__((always_inline)) {
+      constexpr bool RES = decltype(with)::value, LINES = decltype(lines)::value, EDGE = decltype(edge)::value;
       asm volatile("" ::: "memory");  // (its loads are its own: none is under way where it is not taken)
       const int64_t by = static_cast<int64_t>(ROWS) * a.N;
       float xs[2][TURNS];
@@ -362,13 +391,22 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
       auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
-          xs[i & 1][u] = (xs0 + 16 * i + ROWS * u)[static_cast<uint32_t>(row)];
-          if constexpr (RES) r[i & 1][u].template load<LINES>(res0 + (TURNS * i + u) * by + at0);
+          if constexpr (EDGE) {
+            const int t = 16 * i + ROWS * u + row, tc = t < tokens ? t : tokens - 1;
+            xs[i & 1][u] = xs0[tc];
+            if constexpr (RES) {
+              if (mine == 8) r[i & 1][u].template load<false>(res0 + static_cast<int64_t>(tc) * a.N + col);
+            }
+          } else {
+            xs[i & 1][u] = (xs0 + 16 * i + ROWS * u)[static_cast<uint32_t>(row)];
+            if constexpr (RES) r[i & 1][u].template load<LINES>(res0 + (TURNS * i + u) * by + at0);
+          }
         }
       };
       fetch(0);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
+        if (EDGE && 16 * i >= tokens) continue;
         if (i + 1 < MT) fetch(i + 1);
         put(i);
 #pragma unroll
@@ -377,46 +415,40 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
           float v[8];
           take(row + ROWS * u, q);
           l8_scale<DT>(q, ch, xs[i & 1][u], v);
-          if constexpr (RES) r[i & 1][u].add_to(v);
-          Elems<DT>::template store8<LINES>(out0 + (TURNS * i + u) * by + at0, v);
+          if constexpr (EDGE) {
+            if (16 * i + ROWS * u + row >= tokens) continue;
+            const int64_t o = (TURNS * i + u) * by + at0;
+            if (mine == 8) {
+              if constexpr (RES) r[i & 1][u].add_to(v);
+              Elems<DT>::template store8<false>(out0 + o, v);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 7; ++e) {
+                if (e >= mine) continue;
+                if constexpr (RES) v[e] += Elems<DT>::load(res0 + o + e);
+                Elems<DT>::store(out0 + o + e, v[e]);
+              }
+            }
+          } else {
+            if constexpr (RES) r[i & 1][u].add_to(v);
+            Elems<DT>::template store8<LINES>(out0 + (TURNS * i + u) * by + at0, v);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
       // Every load has arrived, only the last stores may be under way (which the compiler does not see
       // where the paths meet; it would wait in the loop above).
-      constexpr int last = (MT > 1 ? 2 : 1) * TURNS * (DT == FMHC_DTYPE_F32 ? 2 : 1);
+      constexpr int last = EDGE ? 0 : (MT > 1 ? 2 : 1) * TURNS * (DT == FMHC_DTYPE_F32 ? 2 : 1);
       l8_wait_vm<(last < 63 ? last : 63)>();
     };
-    if (left_t >= BT - wt && c0 + BC - wc <= a.N) {
-      if (a.lines)
-        a.res ? whole(std::true_type{}, std::true_type{}) : whole(std::false_type{}, std::true_type{});
-      else
-        a.res ? whole(std::true_type{}, std::false_type{}) : whole(std::false_type{}, std::false_type{});
-    } else {
-      // One channel of a token at a time, what is inside.
-      static_assert(kWave % CHANNELS == 0 || CHANNELS % kWave == 0);
-      constexpr int EACH = kWave / CHANNELS > 1 ? kWave / CHANNELS : 1;  // tokens at a time
-      const int e = ln % CHANNELS;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        put(i);
-        if (c0 + e < a.N) {
-          float bias = 0.f;
-          if (a.bias)
-            bias = a.bias_f32 ? static_cast<const float*>(a.bias)[c0 + e]
-                              : Elems<DT>::load(static_cast<const S*>(a.bias) + c0 + e);
-#pragma unroll 1
-          for (int r = ln / CHANNELS; r < 16 && 16 * i + r < left_t; r += EACH) {
-            const int q = own[r * CHANNELS + (((e >> 2) ^ (r & (4 * MC - 1))) << 2 | (e & 3))];
-            float v = __builtin_fmaf(static_cast<float>(q) * xs0[16 * i + r], a.ws[c0 + e], bias);
-            const int64_t o = static_cast<int64_t>(16 * i + r) * a.N + e;
-            if (a.res) v += Elems<DT>::load(res0 + o);
-            Elems<DT>::store(out0 + o, v);
-          }
-        }
-      }
-      l8_wait_vm<0>();
-    }
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    if (left_t < most_t || c0 + CHANNELS > a.N)
+      a.res ? finish(yes, no, yes) : finish(no, no, yes);
+    else if (a.lines)
+      a.res ? finish(yes, yes, no) : finish(no, yes, no);
+    else
+      a.res ? finish(yes, no, no) : finish(no, no, no);
   }
 #endif
 }
@@ -527,36 +559,44 @@ void l8_few_launch(const L8Args& a, hipStream_t s) {
   l8_few_kernel<DT, Few><<<grid, kWave * Few::WAVES, 0, s>>>(a);
 }
 
-// The shortest of the tile kernels for `tiles` tiles of theirs, in hundredths of a round of 256 x 256 tiles,
-// one per CU (63 us at K = 4096): of 128 x 128 and 64 x 64 two fit on a CU, and one there is not twice as
-// fast (37 and 27 us, 17 and 13).
+// The shortest of the tile kernels for the tiles that a product has of each, in hundredths of a round of
+// 256 x 256 tiles, one per CU (52 us at K = 4096; 43 where there is one round).  Two of the others share a CU
+// (a round of 512: 128 x 128 32 us, 64 x 64 13), or have one each (21 and 10).
 struct L8Cost {
   int tile, per_cu, round, one_each;
+  int64_t tiles(int64_t T, int64_t N) const { return ((T + tile - 1) / tile) * ((N + tile - 1) / tile); }
   int64_t of(int64_t T, int64_t N) const {
-    const int64_t tiles = ((T + tile - 1) / tile) * ((N + tile - 1) / tile), slots = int64_t{kCus} * per_cu;
-    return tiles <= kCus ? one_each : (tiles + slots - 1) / slots * round;
+    const int64_t n = tiles(T, N), slots = int64_t{kCus} * per_cu;
+    return n <= kCus ? one_each : (n + slots - 1) / slots * round;
   }
 };
-constexpr L8Cost kL8Cost256{256, 1, 100, 100}, kL8Cost128{128, 2, 56, 43}, kL8Cost64{64, 2, 25, 21};
+constexpr L8Cost kL8Cost256{256, 1, 100, 83}, kL8Cost128{128, 2, 62, 40}, kL8Cost64{64, 2, 25, 19};
 
-// Few tokens go without LDS: up to 16 per workgroup where every workgroup has a CU of its own (us, against
-// 32 tokens and against 64 x 64 tiles: T = 64, N = 1024, K = 4096 5.8, 7.6, 9.6; T = 1, N = K = 4096 4.9, 5.3,
-// 12.3), 32 up to 32 tokens (T = 32, N = K = 4096 8.1; 16 9.5, tiles 15.1; T = 64 13.3 against 13.0 of tiles).
+// Without LDS where every workgroup has a CU of its own, 16 tokens each, else 32 (us, against 64 x 64 tiles:
+// T = 1, N = K = 4096 5.0, 9.1; T = 64, N = 1024, K = 4096 5.8, 8.2; T = 32, N = K = 4096 8.0, 9.0, 16 tokens
+// 9.5), and up to 8 tokens also where two workgroups share one (N = K = 8192: T = 1 12.7, 14.6, T = 8 14.1,
+// 14.5, T = 16 16.7, 14.6).  Beyond that tiles read the operands less often (T = 64, N = K = 4096 9.3, 32
+// tokens 13.4; T = 1, N = 11008, K = 4096 9.6, 10.2).
 template <int DT>
 int l8_run(const L8Args& a, hipStream_t s) {
   const int64_t channels = (a.N + 15) / 16;
-  if (a.T <= 16 || (a.T + 15) / 16 * channels <= kCus) {
+  if ((a.T + 15) / 16 * channels <= (a.T <= 8 ? 2 : 1) * kCus) {
     l8_few_launch<DT, L8Few<1, 1, 8, 2>>(a, s);
-  } else if (a.T <= 32) {
+  } else if ((a.T + 31) / 32 * channels <= kCus) {
     l8_few_launch<DT, L8Few<2, 1, 8, 2>>(a, s);
   } else {
     const int64_t large = kL8Cost256.of(a.T, a.N), medium = kL8Cost128.of(a.T, a.N), small = kL8Cost64.of(a.T, a.N);
+    // Four steps in LDS where a tile has its CU alone, two where two tiles share it (128 x 128, four and two,
+    // us at N = K = 4096: T = 1024 20.8, 25.8; T = 2048 37.6, 33.3); four in 64 x 64, two of which fit
+    // (with two steps of 256 columns T = 128 9.4, 12.9).
     if (large <= medium && large <= small)
-      l8_tile_launch<DT, L8Tile<256, 256, 2, 4, 128>>(a, s);
-    else if (medium <= small)
-      l8_tile_launch<DT, L8Tile<128, 128, 2, 2, 128>>(a, s);
+      l8_tile_launch<DT, L8Tile<256, 256, 2, 4, 2>>(a, s);
+    else if (small < medium)
+      l8_tile_launch<DT, L8Tile<64, 64, 2, 2, 4>>(a, s);
+    else if (kL8Cost128.tiles(a.T, a.N) <= kCus)
+      l8_tile_launch<DT, L8Tile<128, 128, 2, 2, 4>>(a, s);
     else
-      l8_tile_launch<DT, L8Tile<64, 64, 2, 2, 256>>(a, s);
+      l8_tile_launch<DT, L8Tile<128, 128, 2, 2, 2>>(a, s);
   }
   return launch_status();
 }

@@ -223,6 +223,31 @@ def test_many(T, N, K):
     verify(T, N, K, bias=F32, residual=True)
 
 
+# Sizes at which each of the product's kernels is taken: rows in lines, rows off them, and edges.
+KINDS = [(8, 8000), (40, 2000), (192, 2560), (201, 2561), (1024, 2560), (1030, 2603), (1030, 2600), (2048, 4096),
+         (2049, 4097), (8192, 2048), (8190, 2041), (8190, 2040)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,N", KINDS)
+def test_kinds(T, N, dtype):
+    for residual in (False, True):
+        verify(T, N, 200, dtype, F32, residual)
+
+
+@pytest.mark.parametrize("K", [1, 64, 127, 128, 129, 256, 257, 500, 512, 513, 640, 769, 1024, 1300])
+def test_lengths(K):
+    """Ends inside and at a step, and numbers of steps on both sides of what lies in LDS."""
+    for T, N in ((8, 8000), (40, 2000), (192, 1111), (1030, 2600), (2049, 4097), (8190, 2048)):
+        x, xs, w, ws = operands(T, N, K)
+        out = flash_mhc.linear8(x, xs, w, ws, dtype=F32)
+        pick = torch.tensor([0, 1, T // 2, T - 7, T - 2, T - 1], device=DEV)
+        check(f"{T} {N} {K}", out[pick], *R.linear8(x[pick], xs[pick], w, ws))
+        # All of it against the same rows in another order, which lie in other tiles.
+        turned = flash_mhc.linear8(x.flip(0), xs.flip(0), w, ws, dtype=F32)
+        assert torch.equal(turned.flip(0), out)
+
+
 @pytest.mark.parametrize("T", [1, 40, 300])
 def test_exact_sums(T):
     """The largest codes over the longest rows: the integer sum stays exact."""
