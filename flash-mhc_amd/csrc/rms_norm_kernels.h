@@ -3,7 +3,12 @@
 // Rows lie over lanes as the layer norm's do (layer_norm_kernels.h): LPT lanes hold
 // a row, R groups of 8 columns each, from its loads to its stores, a lane keeps the
 // same columns for every row of its workgroup, and the next row's loads are issued
-// before the current row is computed.
+// before the current row is computed.  One pass: the sum of squares needs no mean,
+// and a packed row's maximum is that of |s w|, whose product with rstd is the norm's.
+// Bound by HBM, in bf16: T = 65536, C = 2048 with a residual (8 bytes an element) the
+// forward takes 172 us (6.2 TB/s), the backward 167 + 4.8 for the weight's sums (6.4);
+// without one 88 and 129; T = 65536, C = 1024 in 8 bits 34 (3 bytes an element, 5.9
+// TB/s).  One row of 4096: 2.5 us, a launch's latency.
 #pragma once
 
 #include "layer_norm_kernels.h"
@@ -198,7 +203,7 @@ __global__ __launch_bounds__(ln_fwd_block<LPT>()) void rms_fwd_kernel(
   }
 }
 
-// partial (may be null): this workgroup's sums of grad_w, ln_cols(C) of them.
+// partial (may be null): this workgroup's sums of grad_w, rms_cols(C) of them.
 template <int DT, int LPT, int R, bool NT, bool GI>
 __global__ __launch_bounds__(kLnBwdBlock) void rms_bwd_kernel(
     const typename Elems<DT>::S* __restrict__ gy, const typename Elems<DT>::S* __restrict__ x,
@@ -579,7 +584,10 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s) {
   const bool held = with_ln_walk<3>(a.T, a.C, [&](auto walk) {
     constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, SLOTS = kLnBwdBlock / LPT;
     const int64_t want = (a.T + SLOTS - 1) / SLOTS;
-    const int64_t most = R == 1 ? kRmsParts : kRmsParts / 2;
+    // Two workgroups per CU where a lane has one group and no second gradient, otherwise one (one / two,
+    // us: T = 65536, C = 512 36.5 / 33.2, with a second gradient 43.5 / 45.9; C = 2048 128.6 / 132.4 and
+    // 167.5 / 167.5; T = 16384, C = 1024 18.8 / 18.5 and 23.4 / 25.1; T = 262144, C = 1024 280 / 295).
+    const int64_t most = R == 1 && !gi ? kRmsParts : kRmsParts / 2;
     parts = want < most ? want : most;
     auto launch = [&](auto ntc, auto add) {
       rms_bwd_kernel<DT, LPT, R, decltype(ntc)::value, decltype(add)::value>
