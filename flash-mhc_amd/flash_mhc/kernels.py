@@ -922,12 +922,12 @@ def row_pitch(C: int) -> int:
 
 
 def empty_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Unwritten (codes, scales) for a contiguous x (..., C): codes in rows of row_pitch(C) bytes."""
+    """Unwritten (codes, scales) for x (..., C): codes in rows of row_pitch(C) bytes."""
     shape = x.shape
     C = shape[-1]
     scales = x.new_empty(shape[:-1], dtype=_F32)
     if C % ROW_PITCH == 0:
-        return torch.empty_like(x, dtype=torch.int8), scales
+        return torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format), scales
     return x.new_empty((*shape[:-1], row_pitch(C)), dtype=torch.int8)[..., :C], scales
 
 

@@ -219,6 +219,9 @@ def test_fakes():
         for out in (OPS.pack8_rows(x), OPS.rms_norm_pack8_rows(x, w, 1e-6), OPS.add_rms_norm_pack8_rows(x, r, w, 1e-6)):
             assert out[0].shape == x.shape and out[0].dtype is torch.int8 and out[0].stride() == (144, 48, 1)
             assert out[1].shape == (7, 3) and out[1].dtype is F32
+        turned = torch.empty(48, 5, dtype=BF16).t()  # what comes back is dense by rows
+        assert OPS.pack8_rows(turned)[0].stride() == (48, 1) and OPS.rms_norm(turned, None, 1e-6)[0].stride() == (48, 1)
+        assert OPS.add_rms_norm_pack8_rows(turned, turned, None, 1e-6)[0].stride() == (48, 1)
         q, s = OPS.pack8_rows(x)
         o = OPS.linear8(q, s, torch.empty(9, 40, dtype=torch.int8), torch.empty(9), None, None, torch.float16)
         assert o.shape == (7, 3, 9) and o.dtype is torch.float16
