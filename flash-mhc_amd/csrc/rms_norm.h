@@ -48,6 +48,14 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s);
 constexpr int64_t kRmsParts = 512;
 // Columns of a workgroup's sums.
 inline int64_t rms_cols(int64_t C) { return (C + 7) / 8 * 8; }
+// Rows that registers hold, and the partial sums at most of others, whose columns are cut into workgroups
+// of 256 N: four workgroups per CU in all.
+constexpr int64_t kRmsHeld = 16384;
+inline int64_t rms_any_parts(int64_t T, int64_t C) {
+  const int64_t each = C < 8 ? 256 : 256 * 8, blocks = (C + each - 1) / each;
+  const int64_t share = 1024 / blocks > 1 ? 1024 / blocks : 1, limit = share < kRmsParts ? share : kRmsParts;
+  return T < limit ? T : limit;
+}
 
 // A row's largest magnitude counts as at least this where the row is packed.
 constexpr float kRowLeast = 7.888609052210118e-31f;  // 2^-100

@@ -25,7 +25,8 @@ __global__ __launch_bounds__(256) void rms_zero_kernel(uint16_t* __restrict__ p,
 }
 
 int64_t rms_workspace(int64_t T, int64_t C) {
-  return (T < kRmsParts ? T : kRmsParts) * rms_cols(C) * static_cast<int64_t>(sizeof(float));
+  const int64_t parts = C > kRmsHeld ? rms_any_parts(T, C) : T < kRmsParts ? T : kRmsParts;
+  return parts * rms_cols(C) * static_cast<int64_t>(sizeof(float));
 }
 
 bool bad_sizes(int64_t T, int64_t C) {

@@ -605,9 +605,9 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s) {
           gy, x, a.rstd, a.w, a.w_f32, gi, gx, a.T, a.C);
       if (!a.partial) return;
       // Four workgroups per CU: each writes sums of all its columns.
+      static_assert(kLnColumnsBlock == 256);
       const unsigned blocks = blocks_for(a.C, kLnColumnsBlock * N);
-      const int64_t share = 1024 / blocks > 1 ? 1024 / blocks : 1, limit = share < kRmsParts ? share : kRmsParts;
-      parts = a.T < limit ? a.T : limit;
+      parts = rms_any_parts(a.T, a.C);
       rms_columns_any<DT, N><<<dim3(blocks, static_cast<unsigned>(parts)), kLnColumnsBlock, 0, s>>>(
           gy, x, a.rstd, a.partial, a.T, a.C);
     };

@@ -878,8 +878,8 @@ def rms_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weig
     param_dtype, None where not needed.  grad_x_in: a gradient of x from elsewhere,
     added to grad_x."""
     dev = _device_of(grad_y)
-    _dtype_code(grad_y.dtype, "grad_y")
-    C = _rows(grad_y, "grad_y")[1]
+    code = _dtype_code(grad_y.dtype, "grad_y")
+    T, C = _rows(grad_y, "grad_y")
     _require(x, "x", grad_y.dtype, grad_y.shape, dev)
     _require(rstd, "rstd", _F32, grad_y.shape[:-1], dev)
     if param_dtype is not _F32 and param_dtype is not grad_y.dtype:
@@ -888,15 +888,6 @@ def rms_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weig
         _require(weight, "weight", param_dtype, (C,), dev)
     if grad_x_in is not None:
         _require(grad_x_in, "grad_x_in", grad_y.dtype, grad_y.shape, dev)
-    return rms_norm_bwd_saved(grad_y, x, rstd, weight, param_dtype, need_weight, grad_x_in)
-
-
-def rms_norm_bwd_saved(grad_y, x, rstd, weight, param_dtype, need_weight, grad_x_in=None):
-    """rms_norm_bwd for operands that need no checks: what rms_norm_fwd took and gave,
-    and autograd's gradients, contiguous."""
-    C = grad_y.shape[-1]
-    T = grad_y.numel() // C
-    dev = grad_y.device
     gx = torch.empty_like(grad_y)
     gw = grad_y.new_empty((C,), dtype=param_dtype) if need_weight else None
     lib = _abi.load()
@@ -904,7 +895,7 @@ def rms_norm_bwd_saved(grad_y, x, rstd, weight, param_dtype, need_weight, grad_x
     ws = _workspace(ws_bytes, dev)
     _launch("rms_norm_bwd", dev, lib.fmhc_rms_norm_bwd, grad_y.data_ptr(), x.data_ptr(), rstd.data_ptr(),
             _param_ptr(weight), _ptr_or_none(grad_x_in), gx.data_ptr(), _ptr_or_none(gw), _ptr_or_none(ws), ws_bytes,
-            DTYPES[grad_y.dtype], DTYPES[param_dtype], T, C, _abi.stream_of(grad_y))
+            code, DTYPES[param_dtype], T, C, _abi.stream_of(grad_y))
     return gx, gw
 
 

@@ -363,9 +363,10 @@ torch.library.register_autograd("flash_mhc::add_rms_norm", _rms_backward, setup_
 
 @differentiable_once
 def _rms_eager_gradients(ctx, grad_y, grad_x):
-    x, rstd, weight = ctx.saved_tensors
-    return _k.rms_norm_bwd_saved(grad_y.contiguous(), x, rstd, weight, _param_dtype(weight, None),
-                                 weight is not None and ctx.needs_input_grad[ctx.weight_at], _dense(grad_x))
+    x, rstd, weight = ctx.saved_tensors  # (hooks for saved tensors may have given them other strides)
+    return _k.rms_norm_bwd(grad_y.contiguous(), x.contiguous(), rstd.contiguous(), _dense(weight),
+                           _param_dtype(weight, None),
+                           weight is not None and ctx.needs_input_grad[ctx.weight_at], _dense(grad_x))
 
 
 def _rms_eager_backward(ctx, grad_y, grad_x):

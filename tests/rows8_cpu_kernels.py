@@ -77,7 +77,7 @@ def eager(monkeypatch):
         monkeypatch.setattr(module, "_plain_eager", lambda x: True)
     monkeypatch.setattr(norm.RMSNorm, "_on_kernels", lambda self, x: True)
     monkeypatch.setattr(rows8.Linear8, "on_kernels", lambda self, x: True)
-    for name, fn in (("rms_norm_fwd", rms_norm_fwd), ("rms_norm_bwd_saved", rms_norm_bwd), ("pack8_rows", pack8_rows),
+    for name, fn in (("rms_norm_fwd", rms_norm_fwd), ("rms_norm_bwd", rms_norm_bwd), ("pack8_rows", pack8_rows),
                      ("rms_norm_pack8_rows", rms_norm_pack8_rows), ("linear8", linear8)):
         monkeypatch.setattr(kernels, name, fn)
 

@@ -395,6 +395,26 @@ def test_block(T, C, norm):
         assert torch.equal(out, torch.ops.flash_mhc.fused_post_res(x, lo, H, hq))
 
 
+@pytest.mark.parametrize("kw", [{"activation_bits": 8}, {"activation_checkpointing": True}, {"triton_fused": False}])
+def test_block_with_its_options(kw):
+    """What concerns the backward changes no inference; the plain formulation rounds the layer's input elsewhere."""
+    blk, x = _block(256), rnd((30, 4, 256), 5).to(DEV)
+    other = flash_mhc.MHCLiteBlock(4, 256, blk.layer, pre_norm="rms", **kw).to(DEV).to(BF16).eval()
+    other.load_state_dict(blk.state_dict())
+    with torch.no_grad():
+        want, got = blk(x), other(x)
+    if kw.get("triton_fused", True):
+        assert torch.equal(got, want)
+    else:
+        assert float((got.float() - want.float()).norm()) <= 2.0 ** -6 * float(want.float().norm())
+
+
+def test_strided_rows_compiled():
+    x = rows(40, 264).t().contiguous().t()
+    f = lambda x: flash_mhc.linear8(*flash_mhc.pack8_rows(x), *flash_mhc.rms_norm_pack8_rows(x), dtype=F32)
+    assert torch.equal(torch.compile(f, fullgraph=True)(x), f(x))
+
+
 def test_block_with_hooks():
     """A hooked layer or norm is called: the same up to the rounding of what passes between."""
     blk = _block(256)

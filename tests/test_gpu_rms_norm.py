@@ -334,3 +334,40 @@ def test_nothing_beside_the_outputs():
         for buf, part in bufs:
             assert float((buf[:32] - 7).abs().sum() + (buf[32 + part.numel():] - 7).abs().sum()) == 0
         assert bool((ws[n:] == 77).all())
+
+
+def test_hooks_for_saved_tensors():
+    """Saved tensors that went through the host, lie elsewhere or have other strides."""
+    x, r, w, gy, gs = inputs(20, 264, pdt=F32)
+    leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+    norm = lambda: flash_mhc.rms_norm(leaves[0], leaves[2], EPS, residual=leaves[1])
+    want = torch.autograd.grad(norm(), leaves, [gy, gs])
+    for unpack in (lambda t: t.to(DEV), lambda t: torch.stack([t, t], -1)[..., 0].to(DEV)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+            out = norm()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, [gy, gs]), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):  # left on the host
+        out = norm()
+    with pytest.raises(ValueError, match="expected cuda"):
+        torch.autograd.grad(out, leaves, [gy, gs])
+
+
+def test_compiled():
+    """Traced and compiled, forward and backward: the eager call's bits."""
+    x, r, w, gy, gs = inputs(33, 520)
+    leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+
+    def both(x, r, w):
+        y, s = flash_mhc.rms_norm(x, w, EPS, residual=r)
+        return y, s, flash_mhc.rms_norm(s, None, EPS)
+
+    fast = torch.compile(both, fullgraph=True)
+    want, got = both(*leaves), fast(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    want, got = (torch.autograd.grad(list(out), leaves, [gy, gs, gy]) for out in (want, got))
+    # The sum's two gradients are added by autograd, in bf16 or in the compiler's kernels: one rounding apart.
+    for a, b in zip(want, got):
+        assert float((a.float() - b.float()).norm()) <= 2.0 ** -8 * float(a.float().norm())
+    strided = [t.t().contiguous().t() for t in (x, r)]
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(both(*strided, w), fast(*strided, w)))

@@ -107,6 +107,10 @@ def test_entry_points_take_empty_batches():
     assert L.fmhc_rms_norm_pack8_rows(*[None] * 6, 1, 0, 0, 8, 16, 1e-6, None) == 0
     assert _linear8(T=0, x=None, out=None)(L) == 0
     assert L.fmhc_rms_norm_bwd_workspace_bytes(0, 8) == 0 and L.fmhc_rms_norm_bwd_workspace_bytes(3, 9) == 3 * 16 * 4
+    # Partial sums of 512 rows at most, of very long rows fewer.
+    ws = L.fmhc_rms_norm_bwd_workspace_bytes
+    assert ws(1 << 20, 2048) == 512 * 2048 * 4 == ws(512, 2048) and ws(1 << 20, 5) == 512 * 8 * 4
+    assert ws(1 << 20, 1 << 28) == 4 << 28 and ws(1 << 20, 20000) == 102 * 20000 * 4
 
 
 def test_refusals():
@@ -400,6 +404,20 @@ def test_with_residual(eager):
         torch.testing.assert_close(p, q)
     norm.register_forward_hook(lambda *args: None)
     assert norm.with_residual(a)[1] is a
+
+
+def test_saved_tensors_are_checked(eager, monkeypatch):
+    """What a hook for saved tensors gives back goes through the launcher's checks, on its way to a GPU."""
+    seen = []
+    bwd = cpu.rms_norm_bwd
+    monkeypatch.setattr(K, "rms_norm_bwd", lambda *a: (seen.append([t.is_contiguous() for t in a[:4]]), bwd(*a))[1])
+    x, w, g = _grad(rnd((6, 5), 1)), _grad(rnd((5,), 2)), rnd((6, 5), 3)
+    want = torch.autograd.grad(flash_mhc.rms_norm(x, w), [x, w], g)
+    spread = lambda t: torch.stack([t, t], -1)[..., 0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), spread):
+        y = flash_mhc.rms_norm(x, w)
+    got = torch.autograd.grad(y, [x, w], g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and seen[-1] == [True] * 4
 
 
 def test_dual_tensors_are_refused(route):
