@@ -847,6 +847,17 @@ def _layer_norm_bwd(grad_y, x, codes, scales, mean, rstd, weight, param_dtype, n
 # RMS norm
 
 
+def _live_ptr(t: torch.Tensor | None, name: str):
+    """The address of a tensor that is added; None, which the kernels take as nothing to add, only for None
+    or where there are no elements."""
+    if t is None:
+        return None
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise TypeError(f"{name} has no memory that the kernels can read")
+    return p
+
+
 def _sum_like(x, residual, dev):
     """The tensor for x + residual (None without a residual)."""
     if residual is None:
@@ -866,7 +877,7 @@ def rms_norm_fwd(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
     total = _sum_like(x, residual, dev)
     y = torch.empty_like(x)
     rstd = x.new_empty(x.shape[:-1], dtype=_F32) if stats else None
-    _launch("rms_norm_fwd", dev, _abi.load().fmhc_rms_norm_fwd, x.data_ptr(), _ptr_or_none(residual),
+    _launch("rms_norm_fwd", dev, _abi.load().fmhc_rms_norm_fwd, x.data_ptr(), _live_ptr(residual, "residual"),
             _param_ptr(weight), y.data_ptr(), _ptr_or_none(total), _ptr_or_none(rstd), code, DTYPES[pdt], T, C, eps,
             _abi.stream_of(x))
     return y, total, rstd
@@ -894,8 +905,8 @@ def rms_norm_bwd(grad_y: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weig
     ws_bytes = lib.fmhc_rms_norm_bwd_workspace_bytes(T, C) if need_weight else 0
     ws = _workspace(ws_bytes, dev)
     _launch("rms_norm_bwd", dev, lib.fmhc_rms_norm_bwd, grad_y.data_ptr(), x.data_ptr(), rstd.data_ptr(),
-            _param_ptr(weight), _ptr_or_none(grad_x_in), gx.data_ptr(), _ptr_or_none(gw), _ptr_or_none(ws), ws_bytes,
-            code, DTYPES[param_dtype], T, C, _abi.stream_of(grad_y))
+            _param_ptr(weight), _live_ptr(grad_x_in, "grad_x_in"), gx.data_ptr(), _ptr_or_none(gw), _ptr_or_none(ws),
+            ws_bytes, code, DTYPES[param_dtype], T, C, _abi.stream_of(grad_y))
     return gx, gw
 
 
@@ -941,7 +952,7 @@ def rms_norm_pack8_rows(x: torch.Tensor, residual: torch.Tensor | None, weight: 
     pdt = _norm_params(weight, None, x.dtype, C, dev)
     total = _sum_like(x, residual, dev)
     codes, scales = empty_rows(x)
-    _launch("rms_norm_pack8_rows", dev, _abi.load().fmhc_rms_norm_pack8_rows, x.data_ptr(), _ptr_or_none(residual),
+    _launch("rms_norm_pack8_rows", dev, _abi.load().fmhc_rms_norm_pack8_rows, x.data_ptr(), _live_ptr(residual, "residual"),
             _param_ptr(weight), codes.data_ptr(), scales.data_ptr(), _ptr_or_none(total), code, DTYPES[pdt], T, C,
             row_pitch(C), eps, _abi.stream_of(x))
     return codes, scales, total
@@ -1000,6 +1011,6 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
         _require(residual, "residual", dtype, (*lead, N), dev)
     out = codes.new_empty((*lead, N), dtype=dtype)
     _launch("linear8", dev, _abi.load().fmhc_linear8, x.data_ptr(), ldx, scales.data_ptr(), w.data_ptr(), ldw,
-            weight_scales.data_ptr(), _ptr_or_none(bias), _ptr_or_none(residual), out.data_ptr(), code, bias_code, T, N,
+            weight_scales.data_ptr(), _live_ptr(bias, "bias"), _live_ptr(residual, "residual"), out.data_ptr(), code, bias_code, T, N,
             codes.shape[-1], _abi.stream_of(codes))
     return out

@@ -146,6 +146,24 @@ def test_strided_and_leading_dims():
     assert torch.equal(codes.reshape(24, 104), packed[0]) and torch.equal(scales.reshape(24), packed[1])
 
 
+def test_one_row_without_a_batch():
+    x, w = rows(1, 100)[0], rnd((7, 100), 3, dtype=F32).to(DEV)
+    q, s = flash_mhc.pack8_rows(x)
+    wq, ws = flash_mhc.pack8_rows(w)
+    assert q.shape == (100,) and s.shape == ()
+    out = flash_mhc.linear8(q, s, wq, ws, residual=x[:7].contiguous())
+    assert out.shape == (7,)
+    check("row", out, *R.linear8(q[None], s[None], wq, ws, None, x[None, :7]))
+    n, sn = flash_mhc.rms_norm_pack8_rows(x)
+    R.check_rows(n[None], sn[None], *R.rms_fwd(x[None], None, EPS))
+    y, total = flash_mhc.rms_norm(x, residual=x)
+    assert torch.equal(total, x + x)
+    check("norm", y, *(t[0] for t in R.rms_fwd(total[None], None, EPS)))
+    with torch.no_grad():
+        layer = flash_mhc.Linear8.from_linear(torch.nn.Linear(100, 7).to(DEV))
+        assert layer(x).shape == (7,) and layer(x.expand(2, 3, 100)).shape == (2, 3, 7)
+
+
 def test_rows_leave_what_is_between():
     """The bytes between rows, and before and behind the codes, stay as they were."""
     lib = _abi.load()

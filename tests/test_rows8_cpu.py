@@ -189,6 +189,23 @@ def test_launchers_name_what_is_wrong(monkeypatch):
             K.linear8(*args)
 
 
+def test_operands_without_memory_are_not_left_out(monkeypatch):
+    """A null address stands for no bias, residual or second gradient in the kernels' entry points."""
+    monkeypatch.setattr(K, "_device_of", lambda t: t.device)
+    monkeypatch.setattr(K, "_launch", lambda what, dev, fn, *a: None)
+    monkeypatch.setattr(_abi, "stream_of", lambda t: 0)
+    x, w, stat = _meta((2, 16)), _meta((16,)), _meta((2,), F32)
+    q, wq, ws = _meta((2, 16), torch.int8), _meta((5, 16), torch.int8), _meta((5,), F32)
+    for call in (lambda: K.rms_norm_fwd(x, x, None, 1e-6), lambda: K.rms_norm_fwd(x, None, w, 1e-6),
+                 lambda: K.rms_norm_pack8_rows(x, x, None, 1e-6), lambda: K.rms_norm_bwd(x, x, stat, None, F32, False, x),
+                 lambda: K.linear8(q, stat, wq, ws, _meta((5,))), lambda: K.linear8(q, stat, wq, ws, None, _meta((2, 5)))):
+        with pytest.raises(TypeError, match="memory that the kernels can read"):
+            call()
+    for call in (lambda: K.rms_norm_fwd(x, None, None, 1e-6), lambda: K.linear8(q, stat, wq, ws),
+                 lambda: K.linear8(q[:0], stat[:0], wq, ws, None, _meta((0, 5)))):
+        call()
+
+
 def test_codes_are_copied_only_where_rows_are_off():
     def rows(t):
         out, n, ld = K._code_rows(t, "codes", t.device)
