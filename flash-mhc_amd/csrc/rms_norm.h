@@ -32,8 +32,8 @@ struct RmsBwdArgs {
   bool w_f32;          // w and gw
   const void* gi;      // a gradient of x from elsewhere, added to gx; may be null
   void* gx;
-  float* partial;      // null: no gw
-  void* gw;
+  float* partial;      // null: no gw, or few rows (rms_few)
+  void* gw;            // may be null
   int64_t T;
   int C;
 };
@@ -56,6 +56,12 @@ inline int64_t rms_any_parts(int64_t T, int64_t C) {
   const int64_t share = 1024 / blocks > 1 ? 1024 / blocks : 1, limit = share < kRmsParts ? share : kRmsParts;
   return T < limit ? T : limit;
 }
+
+// Whether grad_w of these rows is summed by workgroups of the backward's own launch, which read the rows
+// again, instead of by partial sums and a second launch (one launch / two, us, bf16: T = 16 C = 1024 3.1 / 6.0,
+// T = 512 3.5 / 6.4 and C = 4096 5.4 / 10.0, T = 1024 C = 1024 4.5 / 7.3, C = 2560 12.6 / 10.0, T = 2048 C = 1024
+// 10.5 / 8.2).
+inline bool rms_few(int64_t T, int64_t C) { return C >= 8 && C <= kRmsHeld && T <= (C <= 1024 ? 1024 : 512); }
 
 // A row's largest magnitude counts as at least this where the row is packed.
 constexpr float kRowLeast = 7.888609052210118e-31f;  // 2^-100

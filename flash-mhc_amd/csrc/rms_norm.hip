@@ -9,8 +9,9 @@
 //             grad_w = sum_t gy h
 //
 // Everything is fp32 but the stored tensors, each rounded once; r's gradient is
-// x's.  The workgroups' sums of grad_w are added by a second kernel in a fixed
-// order (no atomics: deterministic).  The kernels are in rms_norm_kernels.h.
+// x's.  grad_w of many rows is added from the workgroups' sums by a second kernel,
+// that of few rows by workgroups of their own; in a fixed order (no atomics:
+// deterministic).  The kernels are in rms_norm_kernels.h.
 #include "rms_norm.h"
 
 namespace fmhc {
@@ -25,6 +26,7 @@ __global__ __launch_bounds__(256) void rms_zero_kernel(uint16_t* __restrict__ p,
 }
 
 int64_t rms_workspace(int64_t T, int64_t C) {
+  if (rms_few(T, C)) return 0;
   const int64_t parts = C > kRmsHeld ? rms_any_parts(T, C) : T < kRmsParts ? T : kRmsParts;
   return parts * rms_cols(C) * static_cast<int64_t>(sizeof(float));
 }
@@ -112,9 +114,9 @@ extern "C" int fmhc_rms_norm_bwd(const void* grad_y, const void* x, const float*
     return launch_status();
   }
   if (!grad_y || !x || !rstd || !grad_x || (grad_x_in && grad_x_in == grad_x)) return FMHC_ERR_INVALID_ARGUMENT;
-  if (grad_weight && (!workspace || workspace_bytes < rms_workspace(T, C) || !aligned16(workspace)))
-    return FMHC_ERR_INVALID_ARGUMENT;
+  const int64_t need = grad_weight ? rms_workspace(T, C) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FMHC_ERR_INVALID_ARGUMENT;
   const RmsBwdArgs a{grad_y, x, rstd, weight, f32, grad_x_in, grad_x,
-                     grad_weight ? static_cast<float*>(workspace) : nullptr, grad_weight, T, static_cast<int>(C)};
+                     need > 0 ? static_cast<float*>(workspace) : nullptr, grad_weight, T, static_cast<int>(C)};
   return with_dtype(dtype, [&](auto dt) { return rms_bwd_run<decltype(dt)::value>(a, s); });
 }

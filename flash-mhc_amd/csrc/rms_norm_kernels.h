@@ -203,15 +203,68 @@ __global__ __launch_bounds__(ln_fwd_block<LPT>()) void rms_fwd_kernel(
   }
 }
 
-// partial (may be null): this workgroup's sums of grad_w, rms_cols(C) of them.
+// grad_w of kRmsColumns columns from `group` kRmsColumns on, from all rows: it needs no row's sum.
+constexpr int kRmsColumns = 64;
+constexpr int kRmsPitch = kLnBwdBlock + 4;
+template <int DT>
+__device__ __forceinline__ void rms_columns(const typename Elems<DT>::S* __restrict__ gy,
+                                            const typename Elems<DT>::S* __restrict__ x,
+                                            const float* __restrict__ rstd_in, bool w_f32, void* __restrict__ gw,
+                                            float* acc, int group, int64_t T, int C) {
+  constexpr int BLOCK = kLnBwdBlock, VECS = kRmsColumns / 8, SLOTS = BLOCK / VECS;
+  const int own = static_cast<int>(threadIdx.x) % VECS, slot = static_cast<int>(threadIdx.x) / VECS;
+  const LnPlace p = ln_place(group * VECS + own, C);
+  float dw[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dw[e] = 0.f;
+#pragma unroll 4
+  for (int64_t t = slot; t < T; t += SLOTS) {
+    float q[8], h[8];
+    ln_unpack<DT>(ln_load<DT, false>(gy + t * C + p.c), q);
+    ln_unpack<DT>(ln_load<DT, false>(x + t * C + p.c), h);
+    const float rstd = rstd_in[t];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[e] = __builtin_fmaf(q[e], h[e] * rstd, dw[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e * kRmsPitch + threadIdx.x] = dw[e];
+  __syncthreads();
+  // A column's slots: eight threads add eight each, one adds their sums.
+  constexpr int SHARE = SLOTS / 8;
+  const int c = static_cast<int>(threadIdx.x) % kRmsColumns, part = static_cast<int>(threadIdx.x) / kRmsColumns;
+  const float* src = acc + c % 8 * kRmsPitch + c / 8;
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < SHARE; ++k) s += src[(part * SHARE + k) * VECS];
+  __syncthreads();
+  acc[part * kRmsColumns + c] = s;
+  __syncthreads();
+  if (part != 0) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += acc[k * kRmsColumns + c];
+  const LnPlace at = ln_place(group * VECS + c / 8, C);
+  if (c % 8 < at.skip) return;
+  const int64_t n = at.c + c % 8;
+  if (w_f32)
+    static_cast<float*>(gw)[n] = s;
+  else
+    Elems<DT>::store(static_cast<typename Elems<DT>::S*>(gw) + n, s);
+}
+
+// partial (may be null): this workgroup's sums of grad_w, rms_cols(C) of them.  The first col_groups
+// workgroups take columns of grad_w instead of rows (then partial is null).
 template <int DT, int LPT, int R, bool NT, bool GI>
 __global__ __launch_bounds__(kLnBwdBlock) void rms_bwd_kernel(
     const typename Elems<DT>::S* __restrict__ gy, const typename Elems<DT>::S* __restrict__ x,
     const float* __restrict__ rstd_in, const void* __restrict__ wp, bool w_f32,
     const typename Elems<DT>::S* __restrict__ gi, typename Elems<DT>::S* __restrict__ gx, float* __restrict__ partial,
-    int64_t T, int C) {
+    void* __restrict__ gw, int col_groups, int64_t T, int C) {
   constexpr int BLOCK = kLnBwdBlock, SLOTS = BLOCK / LPT;
   __shared__ float red[2][BLOCK / kWave][1];
+  __shared__ float acc[8 * kRmsPitch];
+  if (static_cast<int>(blockIdx.x) < col_groups)
+    return rms_columns<DT>(gy, x, rstd_in, w_f32, gw, acc, static_cast<int>(blockIdx.x), T, C);
+  const int64_t group = static_cast<int>(blockIdx.x) - col_groups, groups = static_cast<int>(gridDim.x) - col_groups;
   LnSums<LPT, BLOCK, 1> row_sum{red};
   const int sub = static_cast<int>(threadIdx.x) % LPT, slot = static_cast<int>(threadIdx.x) / LPT;
   const float n_inv = 1.f / static_cast<float>(C);
@@ -226,8 +279,8 @@ __global__ __launch_bounds__(kLnBwdBlock) void rms_bwd_kernel(
     for (int e = 0; e < 8; ++e) dw[k][e] = 0.f;
   }
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * SLOTS;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * SLOTS;
+  const int64_t step = groups * SLOTS;
+  const int64_t first = group * SLOTS;
   LnRaw<DT> rg[R], rx[R], ri[GI ? R : 1];
   float rstd_n;
   auto load = [&](int64_t tt) {
@@ -308,18 +361,16 @@ __global__ __launch_bounds__(kLnBwdBlock) void rms_bwd_kernel(
   }
   if (!partial) return;
   // The workgroup's rows: the threads that hold the same columns, in slot order.
-  constexpr int kPitch = BLOCK + 4;
-  __shared__ float acc[8 * kPitch];
   float* dst = partial + static_cast<int64_t>(blockIdx.x) * ((C + 7) / 8 * 8);
 #pragma unroll
   for (int k = 0; k < R; ++k) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e * kPitch + threadIdx.x] = dw[k][e];
+    for (int e = 0; e < 8; ++e) acc[e * kRmsPitch + threadIdx.x] = dw[k][e];
     __syncthreads();
     for (int i = static_cast<int>(threadIdx.x); i < 8 * LPT; i += BLOCK) {
       const int own = i / 8, e = i % 8;
-      const float* src = acc + e * kPitch + own;
+      const float* src = acc + e * kRmsPitch + own;
       float v = src[0];
 #pragma unroll
       for (int sl = 1; sl < SLOTS; ++sl) v += src[sl * LPT];
@@ -589,10 +640,11 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s) {
     // 167.5 / 167.5; T = 16384, C = 1024 18.8 / 18.5 and 23.4 / 25.1; T = 262144, C = 1024 280 / 295).
     const int64_t most = R == 1 && !gi ? kRmsParts : kRmsParts / 2;
     parts = want < most ? want : most;
+    const unsigned columns = a.gw && !a.partial ? blocks_for(a.C, kRmsColumns) : 0;
     auto launch = [&](auto ntc, auto add) {
       rms_bwd_kernel<DT, LPT, R, decltype(ntc)::value, decltype(add)::value>
-          <<<dim3(static_cast<unsigned>(parts)), kLnBwdBlock, 0, s>>>(gy, x, a.rstd, a.w, a.w_f32, gi, gx, a.partial,
-                                                                      a.T, a.C);
+          <<<dim3(static_cast<unsigned>(parts) + columns), kLnBwdBlock, 0, s>>>(
+              gy, x, a.rstd, a.w, a.w_f32, gi, gx, a.partial, a.gw, static_cast<int>(columns), a.T, a.C);
     };
     auto pick = [&](auto ntc) { gi ? launch(ntc, std::true_type{}) : launch(ntc, std::false_type{}); };
     nt ? pick(std::true_type{}) : pick(std::false_type{});

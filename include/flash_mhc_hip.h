@@ -352,8 +352,9 @@ int fmhc_rms_norm_fwd(const void* x, const void* residual, const void* weight, v
  *   grad_weight[c] = sum_t grad_y[t,c] h[t,c]
  * grad_x is also residual's gradient.  grad_x_in (may be NULL, not grad_x): a
  * gradient of x from elsewhere (sum's).  grad_weight, in param_dtype, may be NULL;
- * with it `workspace` has at least fmhc_rms_norm_bwd_workspace_bytes(T, C) bytes,
- * 16-byte aligned.  Sums are added in a fixed order. */
+ * with it `workspace` has at least fmhc_rms_norm_bwd_workspace_bytes(T, C) bytes
+ * (none for few rows: it may be NULL then), 16-byte aligned.  Sums are added in a
+ * fixed order. */
 int fmhc_rms_norm_bwd(const void* grad_y, const void* x, const float* rstd, const void* weight,
                       const void* grad_x_in, void* grad_x, void* grad_weight, void* workspace,
                       int64_t workspace_bytes, int dtype, int param_dtype, int64_t T, int64_t C,

@@ -85,6 +85,14 @@ def test_many_rows(T, C):
     verify(*inputs(T, C, BF16, F32))
 
 
+@pytest.mark.parametrize("dtype,pdt", [(BF16, F32), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("T,C", [(511, 12), (512, 1032), (513, 1025), (1024, 9), (1024, 1024), (1025, 777), (1100, 8),
+                                 (600, 2048), (700, 4099), (530, 16384), (515, 16390)])
+def test_weight_gradient(T, C, dtype, pdt):
+    """Sums of the weight's gradient on both sides of where they take a second launch."""
+    verify(*inputs(T, C, dtype, pdt, residual=bool(C % 2)))
+
+
 @pytest.mark.parametrize("C", [3, 24, 520, 20000])
 def test_without_weight(C):
     for residual in (False, True):

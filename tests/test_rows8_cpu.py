@@ -61,9 +61,10 @@ def _linear8(**changes):
         lambda L: L.fmhc_rms_norm_bwd(F, None, *[F] * 3, None, *[F] * 2, 1 << 40, 1, 0, 2, 8, None),  # no x
         lambda L: L.fmhc_rms_norm_bwd(F, F, None, F, None, *[F] * 3, 1 << 40, 1, 0, 2, 8, None),  # no rstd
         lambda L: L.fmhc_rms_norm_bwd(*[F] * 8, 1 << 40, 1, 0, 2, 8, None),  # grad_x_in is grad_x
-        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, *[F] * 3, 8, 1, 0, 2, 8, None),  # workspace too small
-        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, F, F, None, 1 << 40, 1, 0, 2, 8, None),
-        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, F, F, F + 8, 1 << 40, 1, 0, 2, 8, None),  # off 16 bytes
+        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, *[F] * 3, 8, 1, 0, 2000, 8, None),  # workspace too small
+        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, F, F, None, 1 << 40, 1, 0, 2000, 8, None),
+        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, F, F, F + 8, 1 << 40, 1, 0, 2000, 8, None),  # off 16 bytes
+        lambda L: L.fmhc_rms_norm_bwd(*[F] * 4, None, F, F, None, 0, 1, 0, 2, 5, None),
         lambda L: L.fmhc_pack8_rows(F, 3, F, F, 2, 8, 16, None),
         lambda L: L.fmhc_pack8_rows(F, 1, F, F, 2, 8, 7, None),  # rows overlap
         lambda L: L.fmhc_pack8_rows(F, 1, F, F, 1 << 30, 8, 1 << 40, None),
@@ -106,10 +107,11 @@ def test_entry_points_take_empty_batches():
     assert L.fmhc_pack8_rows(None, 1, None, None, 0, 8, 16, None) == 0
     assert L.fmhc_rms_norm_pack8_rows(*[None] * 6, 1, 0, 0, 8, 16, 1e-6, None) == 0
     assert _linear8(T=0, x=None, out=None)(L) == 0
-    assert L.fmhc_rms_norm_bwd_workspace_bytes(0, 8) == 0 and L.fmhc_rms_norm_bwd_workspace_bytes(3, 9) == 3 * 16 * 4
-    # Partial sums of 512 rows at most, of very long rows fewer.
+    assert L.fmhc_rms_norm_bwd_workspace_bytes(0, 8) == 0 and L.fmhc_rms_norm_bwd_workspace_bytes(3, 5) == 3 * 8 * 4
+    # Partial sums of 512 rows at most, of very long rows fewer, none for few rows.
     ws = L.fmhc_rms_norm_bwd_workspace_bytes
-    assert ws(1 << 20, 2048) == 512 * 2048 * 4 == ws(512, 2048) and ws(1 << 20, 5) == 512 * 8 * 4
+    assert ws(1 << 20, 2048) == 512 * 2048 * 4 == ws(513, 2048) and ws(1 << 20, 5) == 512 * 8 * 4
+    assert ws(512, 2048) == ws(1024, 1024) == ws(1, 8) == 0 and ws(1025, 1024) == 512 * 1024 * 4
     assert ws(1 << 20, 1 << 28) == 4 << 28 and ws(1 << 20, 20000) == 102 * 20000 * 4
 
 
