@@ -958,26 +958,25 @@ def rms_norm_pack8_rows(x: torch.Tensor, residual: torch.Tensor | None, weight: 
     return codes, scales, total
 
 
-def _code_rows(codes: torch.Tensor, name: str, dev) -> tuple[torch.Tensor, int, int]:
-    """(codes, rows, bytes between rows) of codes (..., K) as fmhc_linear8 takes them: as they
-    are, or a copy in rows of row_pitch(K) bytes."""
+def _code_rows(codes: torch.Tensor, name: str, dev, shape) -> tuple[torch.Tensor, int, int]:
+    """(codes, rows, bytes between rows) of codes of shape (..., K) as fmhc_linear8 takes them: as
+    they are, or a copy in rows of row_pitch(K) bytes."""
     if not isinstance(codes, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    shape = codes.shape
     if codes.dtype is not torch.int8:
         raise TypeError(f"{name} must be {torch.int8}, got {codes.dtype}")
     if codes.device != dev:
         raise ValueError(f"{name} is on {codes.device}, expected {dev}")
-    if len(shape) == 0 or not 1 <= shape[-1] <= MOST_K:
-        raise ValueError(f"{name} must have shape (..., K) with 1 <= K <= {MOST_K}, got {tuple(shape)}")
     K = shape[-1]
     rows = codes.numel() // K
     if K % ROW_PITCH == 0 and codes.is_contiguous() and codes.data_ptr() % ROW_PITCH == 0:
         return codes, rows, K
     pitch = row_pitch(K)
-    flat = codes.reshape(rows, K)
-    ld = flat.stride(0) if rows > 1 else pitch
-    if (rows > 0 and flat.stride(1) == 1 and pitch <= ld <= MOST_PITCH and ld % ROW_PITCH == 0
+    flat = codes if len(shape) == 2 else codes.reshape(rows, K)
+    ld, one = flat.stride()
+    if rows <= 1:
+        ld = pitch
+    if (rows > 0 and one == 1 and pitch <= ld <= MOST_PITCH and ld % ROW_PITCH == 0
             and flat.data_ptr() % ROW_PITCH == 0
             and flat.storage_offset() + (rows - 1) * ld + pitch <= flat.untyped_storage().nbytes()):
         return flat, rows, ld
@@ -993,12 +992,14 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
     weight_scales (N,); bias (N,) in fp32 or dtype, residual (..., N) in dtype."""
     dev = _device_of(codes)
     code = _dtype_code(dtype, "dtype")
-    lead = codes.shape[:-1]
-    x, T, ldx = _code_rows(codes, "codes", dev)
-    if weight_codes.dim() != 2 or weight_codes.shape[1] != codes.shape[-1] or not 1 <= weight_codes.shape[0] <= MOST_N:
-        raise ValueError(f"weight_codes must have shape (N, {codes.shape[-1]}) with 1 <= N <= {MOST_N}, got "
-                         f"{tuple(weight_codes.shape)}")
-    w, N, ldw = _code_rows(weight_codes, "weight_codes", dev)
+    shape, wshape = codes.shape, weight_codes.shape
+    if len(shape) == 0 or not 1 <= shape[-1] <= MOST_K:
+        raise ValueError(f"codes must have shape (..., K) with 1 <= K <= {MOST_K}, got {tuple(shape)}")
+    K, lead = shape[-1], shape[:-1]
+    if len(wshape) != 2 or wshape[1] != K or not 1 <= wshape[0] <= MOST_N:
+        raise ValueError(f"weight_codes must have shape (N, {K}) with 1 <= N <= {MOST_N}, got {tuple(wshape)}")
+    x, T, ldx = _code_rows(codes, "codes", dev, shape)
+    w, N, ldw = _code_rows(weight_codes, "weight_codes", dev, wshape)
     _require(scales, "scales", _F32, lead, dev)
     _require(weight_scales, "weight_scales", _F32, (N,), dev)
     bias_code = 0
@@ -1009,8 +1010,8 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
         bias_code = DTYPES[bias.dtype]
     if residual is not None:
         _require(residual, "residual", dtype, (*lead, N), dev)
-    out = codes.new_empty((*lead, N), dtype=dtype)
+    out = codes.new_empty((*lead, N), dtype=dtype) if residual is None else torch.empty_like(residual)
     _launch("linear8", dev, _abi.load().fmhc_linear8, x.data_ptr(), ldx, scales.data_ptr(), w.data_ptr(), ldw,
-            weight_scales.data_ptr(), _live_ptr(bias, "bias"), _live_ptr(residual, "residual"), out.data_ptr(), code, bias_code, T, N,
-            codes.shape[-1], _abi.stream_of(codes))
+            weight_scales.data_ptr(), _live_ptr(bias, "bias"), _live_ptr(residual, "residual"), out.data_ptr(), code, bias_code, T, N, K,
+            _abi.stream_of(codes))
     return out

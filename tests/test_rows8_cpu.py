@@ -210,7 +210,7 @@ def test_operands_without_memory_are_not_left_out(monkeypatch):
 
 def test_codes_are_copied_only_where_rows_are_off():
     def rows(t):
-        out, n, ld = K._code_rows(t, "codes", t.device)
+        out, n, ld = K._code_rows(t, "codes", t.device, t.shape)
         assert n == t.numel() // t.shape[-1] and ld % 16 == 0 and out.data_ptr() % 16 == 0
         # What the kernel may read lies inside the storage.
         end = out.data_ptr() - out.untyped_storage().data_ptr() + (n - 1) * ld + K.row_pitch(t.shape[-1])
