@@ -427,6 +427,20 @@ def test_block_with_its_options(kw):
         assert float((got.float() - want.float()).norm()) <= 2.0 ** -6 * float(want.float().norm())
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_block_in_other_types(dtype):
+    """Where the streams take the plain formulation, the layer is the same two calls."""
+    blk = _block(264).to(dtype)
+    u = rnd((21, 264), 5, dtype=dtype).to(DEV)
+    with torch.no_grad():
+        q, s = flash_mhc.rms_norm_pack8_rows(u, blk.norm.weight, blk.norm.eps)
+        layer = blk.layer
+        want = flash_mhc.linear8(q, s, layer.weight_codes[:, :264], layer.weight_scales, layer.bias, residual=u, dtype=dtype)
+        assert layer.weight_scales.dtype is F32 and want.dtype is dtype
+        assert torch.equal(blk._apply_layer(u, {}), want)
+        assert bool(torch.isfinite(blk(rnd((21, 4, 264), 6, dtype=dtype).to(DEV))).all())
+
+
 def test_strided_rows_compiled():
     x = rows(40, 264).t().contiguous().t()
     f = lambda x: flash_mhc.linear8(*flash_mhc.pack8_rows(x), *flash_mhc.rms_norm_pack8_rows(x), dtype=F32)
