@@ -171,14 +171,17 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
 
 
 def _plain_rows(x):
-    """pack8_rows in PyTorch operations."""
+    """pack8_rows in PyTorch operations: the same codes and scales."""
     v = x.float()
     top = v.abs().amax(-1)
     bad = ~torch.isfinite(top)
     top = top.clamp(min=2.0 ** -100)
-    codes = (v * (127.0 / top).unsqueeze(-1)).round()
+    # (Divisions of tensors: those by or of a Python number may be products with a rounded reciprocal, which
+    # moves half a row's largest magnitude, 63.5, off its tie.)
+    most = torch.full_like(top, 127.0)
+    codes = (v * (most / top).unsqueeze(-1)).round()
     codes = torch.where(bad.unsqueeze(-1), torch.zeros_like(codes), codes)
-    return codes.to(torch.int8), torch.where(bad, torch.full_like(top, float("nan")), top / 127.0)
+    return codes.to(torch.int8), torch.where(bad, torch.full_like(top, float("nan")), top / most)
 
 
 class Linear8(nn.Module):

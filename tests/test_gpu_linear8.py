@@ -381,6 +381,15 @@ def test_layer_is_the_product_of_its_rows():
         check("layer", y, *R.linear8(q, s, wq, ws, lin.bias.detach()))
 
 
+def test_layer_in_64_bits_packs_the_same_rows():
+    """Off the kernels the layer packs its rows as they do."""
+    for dtype in (BF16, F16, F32):
+        x = rows(200, 1000, dtype)
+        q, s = flash_mhc.rows8._plain_rows(x.double())
+        want = flash_mhc.pack8_rows(x)
+        assert torch.equal(q, want[0]) and torch.equal(s, want[1])
+
+
 def _block(C, norm="rms", bias=True, seed=0):
     torch.manual_seed(seed)
     lin = torch.nn.Linear(C, C, bias=bias)

@@ -13,7 +13,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 import flash_mhc
 import rows8_cpu_kernels as cpu
-from flash_mhc import _abi
+from flash_mhc import _abi, rows8
 from flash_mhc import kernels as K
 from oracle import rows8_oracle as R
 
@@ -319,6 +319,19 @@ def test_linear8_module(K_, bias):
     bad[0, 0, 3] = float("inf")
     out = layer(bad)
     assert bool(torch.isnan(out[0, 0]).all()) and torch.equal(out[1:], layer(x)[1:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, F32])
+def test_plain_rows_are_the_formats(dtype):
+    """16-bit rows hold half their largest magnitude often: 63.5, which goes to the even 64."""
+    x = rnd((512, 1024), 1, dtype=dtype)
+    x[0, :4] = torch.tensor([1.7, 0.85, -0.85, 0.425])
+    x[0, 4:] = 0
+    for rows in (x, x.double()):
+        q, s = rows8._plain_rows(rows)
+        want = R.pack_rows(x)
+        assert torch.equal(q, want[0]) and torch.equal(s, want[1])
+    assert q[0, :3].tolist() == [127, 64, -64]
 
 
 def test_block_on_the_cpu():
