@@ -10,7 +10,7 @@ times the two rows' scales:
   linear8               codes times an 8-bit weight, with bias and residual
   Linear8               the module, made from an ``nn.Linear``
 
-They serve inference: the backward of each raises.  ``MHCLiteBlock(pre_norm="rms")``
+They serve inference: the backward of each raises, on any device.  ``MHCLiteBlock(pre_norm="rms")``
 around a ``Linear8`` runs rms_norm_pack8_rows and linear8 with the block's residual.
 
 Codes of rows whose length is no multiple of 16 lie at the next multiple's pitch, so
@@ -184,11 +184,26 @@ def _plain_rows(x):
     return codes.to(torch.int8), torch.where(bad, torch.full_like(top, float("nan")), top / most)
 
 
+class _PlainLinear8(torch.autograd.Function):
+    """Linear8's plain formula where a graph is recorded: its backward raises."""
+
+    @staticmethod
+    def forward(layer, x, weight_scales, bias):
+        return layer._plain(x)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    backward = staticmethod(_no_gradient("linear8"))
+
+
 class Linear8(nn.Module):
     """A linear layer with an 8-bit weight, for inference: x (..., in_features) to
     (..., out_features) in x's dtype (bf16, fp16 or fp32), with x packed by rows in the
     call.  Tensors that are not on a GPU go through the same formulas in PyTorch
-    operations.  The scales stay fp32 where the module is cast.
+    operations, and neither have a gradient.  The scales stay fp32 where the module is
+    cast.
 
     Args:
         in_features, out_features: K and N.
@@ -253,6 +268,13 @@ class Linear8(nn.Module):
             raise ValueError(f"expected x of shape (..., {self.in_features}), got {tuple(x.shape)}")
         if self.on_kernels(x):
             return self.product(*pack8_rows(x), x.dtype)
+        kept = x, self.weight_scales, self.bias
+        refuse_tangents(*kept)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in kept):
+            return _PlainLinear8.apply(self, *kept)
+        return self._plain(x)
+
+    def _plain(self, x: torch.Tensor) -> torch.Tensor:
         codes, scales = _plain_rows(x)
         # In 64 bits the products of codes and their sums are exact.
         out = F.linear(codes.double(), self._weight().double()).float() * scales.unsqueeze(-1) * self.weight_scales

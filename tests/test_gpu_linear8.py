@@ -390,6 +390,16 @@ def test_layer_in_64_bits_packs_the_same_rows():
         assert torch.equal(q, want[0]) and torch.equal(s, want[1])
 
 
+def test_layer_in_64_bits_has_no_gradient():
+    layer = flash_mhc.Linear8.from_linear(torch.nn.Linear(100, 7)).to(DEV)
+    x = rows(5, 100, F32)
+    for leaf in (x.double().requires_grad_(True), x.clone().requires_grad_(True)):
+        out = layer(leaf)
+        assert out.requires_grad
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            out.sum().backward()
+
+
 def _block(C, norm="rms", bias=True, seed=0):
     torch.manual_seed(seed)
     lin = torch.nn.Linear(C, C, bias=bias)

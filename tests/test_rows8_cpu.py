@@ -488,6 +488,33 @@ def test_eight_bit_operators_have_no_gradient(monkeypatch):
             assert not flash_mhc.Linear8.from_linear(torch.nn.Linear(48, 7))(x).requires_grad
 
 
+def test_linear8_off_the_kernels_has_no_gradient():
+    """The plain formula's codes are constants and its scales are not: a part of a gradient, which it does not give."""
+    layer = flash_mhc.Linear8.from_linear(torch.nn.Linear(48, 48))
+    x = rnd((5, 48), 1)
+    blocks = [flash_mhc.MHCLiteBlock(4, 48, layer, pre_norm=norm, **kw)
+              for norm in ("rms", "layer", False) for kw in ({}, {"activation_checkpointing": True})]
+    streams = _grad(rnd((5, 4, 48), 2))
+    scaled = copy.deepcopy(layer)
+    scaled.weight_scales.requires_grad_(True)
+    for f in (lambda: layer(_grad(x.clone())).sum().backward(), lambda: layer(_grad(x.double())).sum().backward(),
+              lambda: torch.compile(layer, backend="aot_eager")(_grad(x.clone())).sum().backward(),
+              lambda: torch.func.grad(lambda t: layer(t).sum())(x), lambda: scaled(x).sum().backward(),
+              *(lambda blk=blk: blk(streams).sum().backward() for blk in blocks)):
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            f()
+    with fwAD.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="dual tensor"):
+        layer(fwAD.make_dual(x, x))
+    with pytest.raises(NotImplementedError, match="dual tensor"):
+        torch.func.jvp(layer, (x,), (x,))
+    with torch.no_grad():
+        want = layer(x)
+        assert not layer(_grad(x.clone())).requires_grad
+    out = layer(_grad(x.clone()))
+    assert out.requires_grad and torch.equal(out, want) and not layer(x).requires_grad
+    assert torch.equal(torch.func.vmap(layer)(x.view(5, 1, 48)).view(5, 48), want)
+
+
 def test_opcheck():
     with cpu.registered():
         x, r, w = _grad(rnd((5, 40), 1)), _grad(rnd((5, 40), 2)), _grad(rnd((40,), 3))
