@@ -251,8 +251,9 @@ class Linear8(nn.Module):
         return self.weight_codes if self.weight_codes.shape[1] == K else self.weight_codes[:, :K]
 
     def _bias(self, dtype: torch.dtype):
+        # (Of another type, in fp32: 16 bits of one type may not hold what 16 of another do.)
         b = self.bias
-        return b if b is None or b.dtype is dtype or b.dtype is torch.float32 else b.to(dtype)
+        return b if b is None or b.dtype is dtype else b.float()
 
     def on_kernels(self, x: torch.Tensor) -> bool:
         return x.is_cuda and x.dtype in _k.DTYPES

@@ -400,6 +400,28 @@ def test_layer_in_64_bits_has_no_gradient():
             out.sum().backward()
 
 
+@pytest.mark.parametrize("T", [3, 40, 700])
+@pytest.mark.parametrize("dtype,kept", [(F16, BF16), (BF16, F16), (BF16, torch.float64), (F32, BF16)])
+def test_bias_of_another_type(T, dtype, kept):
+    """A bias is added in its own bits, before the one rounding: 99840 in bf16 is past fp16's range, and the sum is not."""
+    x = rnd((T, 500), 1, dtype=dtype).to(DEV)
+    x[:, 0] = 50
+    w = rnd((300, 500), 2, 0.04, dtype=F32)
+    w[:, 0] = -1000
+    lin = torch.nn.Linear(500, 300).to(kept)
+    with torch.no_grad():
+        lin.weight.copy_(w)
+        lin.bias.copy_(rnd((300,), 3, 1.0, 1000.0, F32))
+        if kept is BF16:
+            lin.bias[::3] = 99840
+        layer = flash_mhc.Linear8.from_linear(lin).to(DEV)
+        assert layer.bias.dtype is kept
+        y = layer(x)
+    wq, ws = R.pack_rows(lin.weight.detach().float())
+    check("layer", y, *R.linear8(*R.pack_rows(x), wq, ws, lin.bias.detach().float()))
+    assert bool(torch.isfinite(y).all())
+
+
 def _block(C, norm="rms", bias=True, seed=0):
     torch.manual_seed(seed)
     lin = torch.nn.Linear(C, C, bias=bias)

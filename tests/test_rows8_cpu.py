@@ -566,6 +566,17 @@ def test_block_calls_what_is_put_around_its_norm_and_layer(monkeypatch):
             out.sum().backward()
 
 
+@pytest.mark.parametrize("dtype,kept", [(torch.float16, BF16), (BF16, torch.float16), (BF16, torch.float64),
+                                        (torch.float16, F32), (F32, BF16), (BF16, BF16)])
+def test_bias_of_another_type(dtype, kept):
+    """The bias is added as it is: neither cut to the output's bits nor past its range before the sum."""
+    layer = flash_mhc.Linear8.from_linear(torch.nn.Linear(40, 4).to(kept))
+    layer.bias.copy_(torch.tensor([65000.0, 1.0 + 2.0 ** -7, 2.0 ** -12 * 1.25, 99840.0], dtype=torch.float64))
+    b = layer._bias(dtype)
+    assert torch.equal(b.double(), layer.bias.float().double()) and b.dtype in (dtype, F32)
+    assert layer._bias(layer.bias.dtype) is layer.bias
+
+
 def test_block_of_another_width(eager):
     """A layer that is no map of (T, C) to itself is left to the ordinary path and its error."""
     blk = cpu.make_block(32, layer=flash_mhc.Linear8(32, 16), dtype=F32)
