@@ -3,7 +3,8 @@
 //   out[t, n] = round(sum_k x[t, k] w[n, k] * x_scale[t] * w_scale[n] + bias[n] + residual[t, n])
 //
 // The sum is of integers and exact: |code| <= 128 and K < 2^17 keep it below 2^31.
-// It is widened to fp32 (one rounding), scaled, and the output rounded once.
+// It is widened to fp32 (one rounding), scaled, and the output rounded once.  A token's scale past 2^96
+// multiplies last (l8_value), so that only a product that is itself past fp32's range becomes infinite.
 //
 // Many tokens are bound by the matrix cores at the clock that the power limit leaves them: T = 16384,
 // N = K = 4096 takes 209 us, 2.63 POP/s (PyTorch's integer product 269 us), where instructions that only
@@ -99,11 +100,26 @@ struct L8Raw<FMHC_DTYPE_F32> {
   }
 };
 
-// Products of a token with eight channels, scaled, and the bias.
-template <int DT>
+// Token scales up to this one multiply a sum (at most 2^31) within fp32's range.  Past it the channel's scale
+// multiplies first: then what is on the way passes the range only where the result does.  (Scales of packed
+// rows are 2^-107 or more: no product on the way is subnormal where they are.)
+constexpr float kL8Large = 0x1p96f;
+
+__device__ __forceinline__ float l8_value(int acc, float xs, float ws, float b) {
+  const bool last = fabsf(xs) > kL8Large;
+  return __builtin_fmaf(static_cast<float>(acc) * (last ? ws : xs), last ? xs : ws, b);
+}
+
+// Products of a token with eight channels, scaled, and the bias; ANY: the token's scale may be past kL8Large.
+template <int DT, bool ANY>
 __device__ __forceinline__ void l8_scale(const int (&acc)[8], const L8Channels<DT>& ch, float xs, float (&v)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(static_cast<float>(acc[e]) * xs, ch.s[e], ch.b[e]);
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (ANY)
+      v[e] = l8_value(acc[e], xs, ch.s[e], ch.b[e]);
+    else
+      v[e] = __builtin_fmaf(static_cast<float>(acc[e]) * xs, ch.s[e], ch.b[e]);
+  }
 }
 
 // What a wave's lanes have written to LDS is there for its other lanes, and what they have read may be
@@ -361,6 +377,15 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     const int64_t t0 = static_cast<int64_t>(t) * BT + wt, left_t = a.T - t0;
     const int c0 = c * BC + wc, col = ln % LPR * 8, row = ln / LPR;
     L8Channels<DT> ch(a, c0 + col);
+    // What is inside: tokens of the wave, channels of the lane.
+    constexpr int most_t = 16 * MT;
+    const int tokens = static_cast<int>(left_t < most_t ? left_t : most_t);
+    const int mine = a.N - c0 - col < 8 ? a.N - c0 - col : 8;
+    const float* xs0 = a.xs + t0;
+    float xs_most = 0.f;
+#pragma unroll
+    for (int k = 0; k < most_t; k += kWave) xs_most = fmaxf(xs_most, fabsf(xs0[k + ln < tokens ? k + ln : tokens - 1]));
+    const bool large = __builtin_amdgcn_ballot_w64(xs_most > kL8Large) != 0;
     // (Waited for here, also where no token of the lane's is stored: not in the loop above.)
 #pragma unroll
     for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(ch.s[e]), "+v"(ch.b[e]));
@@ -379,21 +404,18 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
         *reinterpret_cast<i32x4*>(v + 4 * h) =
             *reinterpret_cast<const i32x4*>(own + r * CHANNELS + ((col / 4 + h) ^ (r & (4 * MC - 1))) * 4);
     };
-    const float* xs0 = a.xs + t0;
     auto* out0 = static_cast<S*>(a.out) + t0 * a.N + c0;
     const auto* res0 = static_cast<const S*>(a.res) + t0 * a.N + c0;
     const uint32_t at0 = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.N) + static_cast<uint32_t>(col);
-    // What is inside: tokens of the wave, channels of the lane.
-    constexpr int most_t = 16 * MT;
-    const int tokens = static_cast<int>(left_t < most_t ? left_t : most_t);
-    const int mine = a.N - c0 - col < 8 ? a.N - c0 - col : 8;
     // The tokens' scales and the residual are loaded before stores that their arrival would otherwise wait
     // for.  Rows that begin at 16 bytes are stored, and the residual's loaded, with the nontemporal hint:
     // neither is read again here, and what the tiles read stays cached (with / without, us: T = 65536,
     // N = K = 1024 80 / 96, with a residual 99 / 106; T = 16384, N = K = 4096 235 / 245; the residual's loads
     // alone 120 / 127 for a norm and its product at T = 65536).  Other rows share lines with their neighbours'
     // stores, which are to meet in the cache.  At the edges (EDGE) tokens past the last one are read as the
-    // last one, and only what is inside is stored.
+    // last one, and only what is inside is stored.  Tokens with scales past kL8Large take that form too: to
+    // look at the scales costs up to 1%, to choose for each element in every form 2% (T = 65536, N = K = 1024
+    // 71.8 -> 72.2 and 74.1 us, T = 16384, N = K = 4096 212.5 -> 214.1 and 215.5).
     auto finish = [&](auto with, auto lines, auto edge) __attribute__((always_inline)) {
       constexpr bool RES = decltype(with)::value, LINES = decltype(lines)::value, EDGE = decltype(edge)::value;
       asm volatile("" ::: "memory");  // (its loads are its own: none is under way where it is not taken)
@@ -426,7 +448,7 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
           int q[8];
           float v[8];
           take(row + ROWS * u, q);
-          l8_scale<DT>(q, ch, xs[i & 1][u], v);
+          l8_scale<DT, EDGE>(q, ch, xs[i & 1][u], v);
           if constexpr (EDGE) {
             if (16 * i + ROWS * u + row >= tokens) continue;
             const int64_t o = (TURNS * i + u) * by + at0;
@@ -455,7 +477,7 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     };
     constexpr std::true_type yes;
     constexpr std::false_type no;
-    if (left_t < most_t || c0 + CHANNELS > a.N)
+    if (large || left_t < most_t || c0 + CHANNELS > a.N)
       a.res ? finish(yes, no, yes) : finish(no, no, yes);
     else if (a.lines)
       a.res ? finish(yes, yes, no) : finish(no, yes, no);
@@ -558,7 +580,7 @@ __global__ __launch_bounds__(kWave * Few::WAVES) void l8_few_kernel(const L8Args
     for (int k = 1; k < WAVES; ++k) v += p[k * MT * MC * kWave * 4];
     float b = 0.f;
     if (a.bias) b = a.bias_f32 ? static_cast<const float*>(a.bias)[c] : Elems<DT>::load(static_cast<const S*>(a.bias) + c);
-    float y = __builtin_fmaf(static_cast<float>(v) * a.xs[t], a.ws[c], b);
+    float y = l8_value(v, a.xs[t], a.ws[c], b);
     if (a.res) y += Elems<DT>::load(static_cast<const S*>(a.res) + t * a.N + c);
     Elems<DT>::store(static_cast<S*>(a.out) + t * a.N + c, y);
   }

@@ -162,8 +162,8 @@ def linear8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tenso
 
     codes (..., K) and weight_codes (N, K) int8 with K < 2^17 and N < 2^22, scales (...,) and
     weight_scales (N,) fp32 (pack8_rows of a token's row and of a weight's), bias (N,)
-    fp32 or of dtype, residual (..., N) of dtype.  The sum of integers is exact.  No
-    gradient."""
+    fp32 or of dtype, residual (..., N) of dtype.  The sum of integers is exact, and the
+    product overflows only where it is itself past fp32's range.  No gradient."""
     if _direct(codes, scales, weight_codes, weight_scales, bias, residual):
         return _k.linear8(codes, scales.contiguous(), weight_codes, weight_scales.contiguous(), _dense(bias),
                           _dense(residual), dtype)
@@ -182,6 +182,9 @@ def _plain_rows(x):
     codes = (v * (most / top).unsqueeze(-1)).round()
     codes = torch.where(bad.unsqueeze(-1), torch.zeros_like(codes), codes)
     return codes.to(torch.int8), torch.where(bad, torch.full_like(top, float("nan")), top / most)
+
+
+_LARGE = 2.0 ** 96  # times a sum of products, at most 2^31, within fp32's range
 
 
 class _PlainLinear8(torch.autograd.Function):
@@ -278,7 +281,11 @@ class Linear8(nn.Module):
     def _plain(self, x: torch.Tensor) -> torch.Tensor:
         codes, scales = _plain_rows(x)
         # In 64 bits the products of codes and their sums are exact.
-        out = F.linear(codes.double(), self._weight().double()).float() * scales.unsqueeze(-1) * self.weight_scales
+        out = F.linear(codes.double(), self._weight().double()).float()
+        # (As the kernels: a token's large scale multiplies last, lest the product on the way pass fp32's range.)
+        scales = scales.unsqueeze(-1)
+        last = scales.abs() > _LARGE
+        out = out * torch.where(last, self.weight_scales, scales) * torch.where(last, scales, self.weight_scales)
         return (out if self.bias is None else out + self.bias.float()).to(x.dtype)
 
     def extra_repr(self) -> str:

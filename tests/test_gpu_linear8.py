@@ -279,6 +279,57 @@ def test_exact_sums(T):
         assert bool((out[:, n].double() == float(torch.tensor(v).to(F32))).all())
 
 
+def check_range(name, out, value, error):
+    """check, where a value that rounds past the type's largest is Inf: from half a step above it on, which is
+    65504 + 16 in fp16 (steps of 32 from 2^15 on), max + max eps / (2 - eps) / 2 in general."""
+    info = torch.finfo(out.dtype)
+    half = info.max * info.eps / (2 - info.eps) / 2
+    past = value.abs() >= info.max + half + error
+    o = out.detach().to("cpu", torch.float64)
+    assert torch.equal(o[past], torch.sign(value[past]) * float("inf"))
+    assert not bool(((value.abs() - info.max - half).abs() < error).any())  # none that may be either
+    check(name, out.cpu().masked_fill(past, 0), value.masked_fill(past, 0), error)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,N", [(1, 4096), (8, 8000), (40, 2000), (192, 2560), (201, 2561), (1030, 2600), (2048, 4096),
+                                 (2049, 4097), (8192, 2048), (8190, 2041)])
+def test_scales_at_the_ends_of_fp32(T, N, dtype):
+    """A sum times its larger scale is past fp32's range, times both it is not; in all, some or one of the rows."""
+    x, xs, w, ws = operands(T, N, 200)
+    w[N // 2] = 0
+    small, large = 1e-35, 1e36 / 0.02
+    for mine, other, n in ((xs, ws, T), (ws, xs, N)):
+        for which in (slice(None), slice(None, None, 3), slice(n - 1, n)):
+            a, b = mine.clone(), other * small
+            a[which] *= large
+            pair = (a, b) if mine is xs else (b, a)
+            for residual in (None, rnd((T, N), 5, 100.0, dtype=dtype).to(DEV)):
+                out = flash_mhc.linear8(x, pair[0], w, pair[1], residual=residual, dtype=dtype)
+                check_range(f"{T} {N}", out, *R.linear8(x, pair[0], w, pair[1], None, residual))
+    # On both sides of where the order changes, and rows that are NaN.
+    a = xs * 0 + 2.0 ** 96
+    a[::2] = 2.0 ** 96 * (1 + 2.0 ** -23)
+    a[T // 2] = float("nan")
+    out = flash_mhc.linear8(x, a, w, ws * 1e-30, dtype=dtype)
+    ok = [t for t in range(T) if t != T // 2]
+    check_range("threshold", out[ok], *R.linear8(x[ok], a[ok], w, ws * 1e-30))
+    assert bool(torch.isnan(out[T // 2]).all())
+
+
+@pytest.mark.parametrize("T", [2, 40, 700])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_layer_of_huge_rows(T, dtype):
+    lin = torch.nn.Linear(4096, 300, bias=False)
+    torch.nn.init.constant_(lin.weight, 0.01)
+    layer = flash_mhc.Linear8.from_linear(lin).to(DEV)
+    x = torch.full((T, 4096), 1e33, device=DEV, dtype=dtype)
+    with torch.no_grad():
+        y = layer(x)
+    check("layer", y, *R.linear8(*R.pack_rows(x), *R.pack_rows(lin.weight.detach())))
+    assert bool(torch.isfinite(y).all())
+
+
 def test_strides():
     """Codes at any strides: rows off 16 bytes, transposed, broadcast, spread, at a buffer's end."""
     T, N, K = 37, 50, 100

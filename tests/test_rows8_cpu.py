@@ -577,6 +577,20 @@ def test_bias_of_another_type(dtype, kept):
     assert layer._bias(layer.bias.dtype) is layer.bias
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("x,w", [(1e33, 0.01), (1e38, 1e-6), (1e-6, 1e33), (-1e35, 1e-4), (1e-25, 1e38)])
+def test_products_past_the_range_on_the_way(x, w, dtype):
+    """4096 products of codes 127 times a large scale are past fp32; times the small one too they are not."""
+    lin = torch.nn.Linear(4096, 3, bias=False)
+    torch.nn.init.constant_(lin.weight, w)
+    layer = flash_mhc.Linear8.from_linear(lin)
+    out = layer(torch.full((2, 4096), x, dtype=F32).to(dtype))
+    q, s = R.pack_rows(torch.full((2, 4096), x, dtype=F32).to(dtype))
+    want, err = R.linear8(q, s, layer.weight_codes, layer.weight_scales)
+    assert bool(torch.isfinite(out).all())
+    assert bool(((out.double() - want).abs() <= err + want.abs() * torch.finfo(dtype).eps / 2).all())
+
+
 def test_block_of_another_width(eager):
     """A layer that is no map of (T, C) to itself is left to the ordinary path and its error."""
     blk = cpu.make_block(32, layer=flash_mhc.Linear8(32, 16), dtype=F32)
