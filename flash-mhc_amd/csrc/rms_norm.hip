@@ -116,6 +116,8 @@ extern "C" int fmhc_rms_norm_bwd(const void* grad_y, const void* x, const float*
   if (!grad_y || !x || !rstd || !grad_x || (grad_x_in && grad_x_in == grad_x)) return FMHC_ERR_INVALID_ARGUMENT;
   const int64_t need = grad_weight ? rms_workspace(T, C) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return FMHC_ERR_INVALID_ARGUMENT;
+  // (grad_w's workgroups read grad_y and x while others store grad_x, or after it.)
+  if (grad_x == grad_y || grad_x == x) return FMHC_ERR_INVALID_ARGUMENT;
   const RmsBwdArgs a{grad_y, x, rstd, weight, f32, grad_x_in, grad_x,
                      need > 0 ? static_cast<float*>(workspace) : nullptr, grad_weight, T, static_cast<int>(C)};
   return with_dtype(dtype, [&](auto dt) { return rms_bwd_run<decltype(dt)::value>(a, s); });

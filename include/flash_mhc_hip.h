@@ -350,8 +350,9 @@ int fmhc_rms_norm_fwd(const void* x, const void* residual, const void* weight, v
 /* Backward, with x the forward's x, or its sum, h = x rstd and g = grad_y weight:
  *   grad_x[t,c]    = rstd[t] (g[t,c] - h[t,c] sum_c g h / C) + grad_x_in[t,c]
  *   grad_weight[c] = sum_t grad_y[t,c] h[t,c]
- * grad_x is also residual's gradient.  grad_x_in (may be NULL, not grad_x): a
- * gradient of x from elsewhere (sum's).  grad_weight, in param_dtype, may be NULL;
+ * grad_x is also residual's gradient.  grad_x_in (may be NULL): a gradient of x from
+ * elsewhere (sum's).  No output may overlap an input (grad_x as grad_y, x or grad_x_in
+ * is refused).  grad_weight, in param_dtype, may be NULL;
  * with it `workspace` has at least fmhc_rms_norm_bwd_workspace_bytes(T, C) bytes
  * (none for few rows: it may be NULL then), 16-byte aligned.  Sums are added in a
  * fixed order. */

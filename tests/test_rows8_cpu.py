@@ -101,6 +101,18 @@ def test_entry_points_refuse(call):
     assert call(_abi.load()) == 1
 
 
+@pytest.mark.parametrize("T,C", [(4, 1024), (4, 5), (3, 20000), (2000, 1024)])
+@pytest.mark.parametrize("same", ["grad_y", "x", "grad_x_in"])
+def test_rms_backward_refuses_grad_x_over_its_inputs(same, T, C):
+    """grad_weight's workgroups read the inputs while grad_x is stored, or afterwards."""
+    L = _abi.load()
+    at = dict(grad_y=F, x=2 * F, grad_x_in=None)
+    gx = 4 * F
+    at[same] = gx
+    assert L.fmhc_rms_norm_bwd(at["grad_y"], at["x"], 3 * F, None, at["grad_x_in"], gx, 5 * F, 6 * F, 1 << 40, 1, 0, T, C,
+                               None) == 1
+
+
 def test_entry_points_take_empty_batches():
     L = _abi.load()
     assert L.fmhc_rms_norm_fwd(*[None] * 6, 1, 0, 0, 8, 1e-6, None) == 0
