@@ -57,6 +57,11 @@ inline int64_t rms_any_parts(int64_t T, int64_t C) {
   return T < limit ? T : limit;
 }
 
+// Sums of every column that a backward leaves at most: what the workspace holds and the launches keep to.
+inline int64_t rms_parts(int64_t T, int64_t C) {
+  return C > kRmsHeld ? rms_any_parts(T, C) : T < kRmsParts ? T : kRmsParts;
+}
+
 // Whether grad_w of these rows is summed by workgroups of the backward's own launch, which read the rows
 // again, instead of by partial sums and a second launch (one launch / two, us, bf16: T = 16 C = 1024 3.1 / 6.0,
 // T = 512 3.5 / 6.4 and C = 4096 5.4 / 10.0, T = 1024 C = 1024 4.5 / 7.3, C = 2560 12.6 / 10.0, T = 2048 C = 1024

@@ -27,8 +27,7 @@ __global__ __launch_bounds__(256) void rms_zero_kernel(uint16_t* __restrict__ p,
 
 int64_t rms_workspace(int64_t T, int64_t C) {
   if (rms_few(T, C)) return 0;
-  const int64_t parts = C > kRmsHeld ? rms_any_parts(T, C) : T < kRmsParts ? T : kRmsParts;
-  return parts * rms_cols(C) * static_cast<int64_t>(sizeof(float));
+  return rms_parts(T, C) * rms_cols(C) * static_cast<int64_t>(sizeof(float));
 }
 
 bool bad_sizes(int64_t T, int64_t C) {

@@ -631,6 +631,7 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s) {
   const auto* gi = static_cast<const S*>(a.gi);
   auto* gx = static_cast<S*>(a.gx);
   int64_t parts = 0;
+  static_assert(ln_most_rounds<3, 512>() * 512 * 8 == kRmsHeld);  // with_ln_walk's widest rows
   const bool nt = ln_hint<DT>(a.T, a.C) && a.C % 8 == 0 && aligned16(gy) && aligned16(x) && aligned16(gx) && aligned16(gi);
   const bool held = with_ln_walk<3>(a.T, a.C, [&](auto walk) {
     constexpr int LPT = decltype(walk)::LPT, R = decltype(walk)::R, SLOTS = kLnBwdBlock / LPT;
@@ -638,8 +639,9 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s) {
     // Two workgroups per CU where a lane has one group and no second gradient, otherwise one (one / two,
     // us: T = 65536, C = 512 36.5 / 33.2, with a second gradient 43.5 / 45.9; C = 2048 128.6 / 132.4 and
     // 167.5 / 167.5; T = 16384, C = 1024 18.8 / 18.5 and 23.4 / 25.1; T = 262144, C = 1024 280 / 295).
-    const int64_t most = R == 1 && !gi ? kRmsParts : kRmsParts / 2;
+    const int64_t most = R == 1 && !gi ? kRmsParts : kRmsParts / 2, room = rms_parts(a.T, a.C);
     parts = want < most ? want : most;
+    parts = parts < room ? parts : room;
     const unsigned columns = a.gw && !a.partial ? blocks_for(a.C, kRmsColumns) : 0;
     auto launch = [&](auto ntc, auto add) {
       rms_bwd_kernel<DT, LPT, R, decltype(ntc)::value, decltype(add)::value>
@@ -659,7 +661,7 @@ int rms_bwd_run(const RmsBwdArgs& a, hipStream_t s) {
       // Four workgroups per CU: each writes sums of all its columns.
       static_assert(kLnColumnsBlock == 256);
       const unsigned blocks = blocks_for(a.C, kLnColumnsBlock * N);
-      parts = rms_any_parts(a.T, a.C);
+      parts = rms_parts(a.T, a.C);
       rms_columns_any<DT, N><<<dim3(blocks, static_cast<unsigned>(parts)), kLnColumnsBlock, 0, s>>>(
           gy, x, a.rstd, a.partial, a.T, a.C);
     };

@@ -344,6 +344,27 @@ def test_nothing_beside_the_outputs():
         assert bool((ws[n:] == 77).all())
 
 
+@pytest.mark.parametrize("T,C", [(513, 2048), (600, 16384), (515, 16390), (1025, 1024), (2000, 5), (5000, 32),
+                                 (9000, 64), (4097, 520), (1100, 4096)])
+def test_partial_sums_stay_in_the_workspace(T, C):
+    """The workspace that the query names is enough, with a second gradient and without: what follows it stays."""
+    lib = _abi.load()
+    x, r, w, gy, gs = inputs(T, C, BF16, F32)
+    n = lib.fmhc_rms_norm_bwd_workspace_bytes(T, C)
+    assert n > 0
+    rstd = (x.float().square().mean(-1) + EPS).rsqrt()
+    for gi in (None, gs):
+        ws = torch.full((n + 4096,), 77, device=DEV, dtype=torch.uint8)
+        gx, gw = torch.empty_like(x), torch.empty_like(w)
+        assert lib.fmhc_rms_norm_bwd(gy.data_ptr(), x.data_ptr(), rstd.data_ptr(), w.data_ptr(),
+                                     None if gi is None else gi.data_ptr(), gx.data_ptr(), gw.data_ptr(), ws.data_ptr(),
+                                     n, 1, 0, T, C, _abi.stream_of(x)) == 0
+        assert bool((ws[n:] == 77).all())
+        want = R.rms_bwd(gy, x, w, EPS, gi)
+        check("grad_x", gx, *want["x"])
+        check("grad_w", gw, *want["w"])
+
+
 def test_hooks_for_saved_tensors():
     """Saved tensors that went through the host, lie elsewhere or have other strides."""
     x, r, w, gy, gs = inputs(20, 264, pdt=F32)
