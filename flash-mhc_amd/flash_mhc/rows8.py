@@ -270,6 +270,8 @@ class Linear8(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() == 0 or x.shape[-1] != self.in_features:
             raise ValueError(f"expected x of shape (..., {self.in_features}), got {tuple(x.shape)}")
+        if not x.is_floating_point():
+            raise TypeError(f"expected x of a floating-point type, got {x.dtype}")
         if self.on_kernels(x):
             return self.product(*pack8_rows(x), x.dtype)
         kept = x, self.weight_scales, self.bias

@@ -500,6 +500,14 @@ def test_eight_bit_operators_have_no_gradient(monkeypatch):
             assert not flash_mhc.Linear8.from_linear(torch.nn.Linear(48, 7))(x).requires_grad
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int8, torch.bool, torch.complex64])
+def test_linear8_refuses_rows_of_other_types(dtype):
+    """Their outputs would be cut to whole numbers, or to a real part."""
+    layer = flash_mhc.Linear8.from_linear(torch.nn.Linear(48, 7))
+    with pytest.raises(TypeError, match="floating-point"):
+        layer(torch.ones(5, 48, dtype=dtype))
+
+
 def test_linear8_off_the_kernels_has_no_gradient():
     """The plain formula's codes are constants and its scales are not: a part of a gradient, which it does not give."""
     layer = flash_mhc.Linear8.from_linear(torch.nn.Linear(48, 48))
