@@ -7,10 +7,10 @@
 // multiplies last (l8_value), so that only a product that is itself past fp32's range becomes infinite.
 //
 // Many tokens are bound by the matrix cores at the clock that the power limit leaves them: T = 16384,
-// N = K = 4096 takes 209 us, 2.63 POP/s (PyTorch's integer product 269 us), where instructions that only
-// read LDS reach 3.1 to 3.4 POP/s.  At K = 1024 the tiles' results take as long as their products' last
-// third (T = 65536, N = 1024 71 us, 1.9 POP/s; with a residual 95).  Few tokens are bound by latency: T = 1,
-// N = K = 4096 5 us for 16.8 MB of weight.
+// N = K = 4096 takes 209 to 218 us by card, 2.5 to 2.6 POP/s (PyTorch's integer product 269 us), where
+// instructions that only read LDS reach 3.1 to 3.4 POP/s.  At K = 1024 the tiles' results take as long as their
+// products' last third (T = 65536, N = 1024 72 to 73 us, 1.9 POP/s; with a residual 92 to 93).  Few tokens are
+// bound by latency: T = 1, N = K = 4096 5.2 us for 16.8 MB of weight.
 #include "elems.h"
 
 namespace fmhc {
@@ -171,7 +171,7 @@ struct L8Walk {
 };
 
 // A wave has up to 128 x 64 of a tile: 12 reads of LDS for 32 instructions, accumulators in half of its
-// registers.  Measured and slower (POP/s at T = N = K = 8192, against 2.41): 128 x 128 per wave with four
+// registers.  Measured in turn with the kernel as it was then, and slower (POP/s at T = N = K = 8192, against 2.41): 128 x 128 per wave with four
 // waves 2.0 to 2.16, instructions of 32 x 32 x 32 2.25, four steps of 64 columns 2.28; two workgroups of
 // 128 x 256 in steps of 64 on a CU, so that one stores while the other multiplies, 79 -> 84 us at T = 65536,
 // N = K = 1024 and 214 -> 260 at T = 16384, N = K = 4096.
@@ -409,13 +409,13 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     const uint32_t at0 = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.N) + static_cast<uint32_t>(col);
     // The tokens' scales and the residual are loaded before stores that their arrival would otherwise wait
     // for.  Rows that begin at 16 bytes are stored, and the residual's loaded, with the nontemporal hint:
-    // neither is read again here, and what the tiles read stays cached (with / without, us: T = 65536,
-    // N = K = 1024 80 / 96, with a residual 99 / 106; T = 16384, N = K = 4096 235 / 245; the residual's loads
-    // alone 120 / 127 for a norm and its product at T = 65536).  Other rows share lines with their neighbours'
+    // neither is read again here, and what the tiles read stays cached (with / without, us, bf16: T = 65536,
+    // N = 1024, K = 512 50 / 64, K = 1024 73 / 89, with a residual 93 / 102, the hint for its loads alone 93 /
+    // 102; T = 16384, N = K = 4096 218 / 224).  Other rows share lines with their neighbours'
     // stores, which are to meet in the cache.  At the edges (EDGE) tokens past the last one are read as the
     // last one, and only what is inside is stored.  Tokens with scales past kL8Large take that form too: to
-    // look at the scales costs up to 1%, to choose for each element in every form 2% (T = 65536, N = K = 1024
-    // 71.8 -> 72.2 and 74.1 us, T = 16384, N = K = 4096 212.5 -> 214.1 and 215.5).
+    // look at the scales costs up to 1% (T = 65536, N = K = 1024 71.8 -> 72.2 us, T = 16384, N = K = 4096 212.5
+    // -> 214.1), to choose for each element in every form 2% (72.3 -> 74.1 and 210.8 -> 213.8).
     auto finish = [&](auto with, auto lines, auto edge) __attribute__((always_inline)) {
       constexpr bool RES = decltype(with)::value, LINES = decltype(lines)::value, EDGE = decltype(edge)::value;
       asm volatile("" ::: "memory");  // (its loads are its own: none is under way where it is not taken)
@@ -594,7 +594,8 @@ void l8_few_launch(const L8Args& a, hipStream_t s) {
 }
 
 // The shortest of the tile kernels for the tiles that a product has of each, in hundredths of a round of
-// 256 x 256 tiles, one per CU (52 us at K = 4096; 43 where there is one round).  Two of the others share a CU
+// 256 x 256 tiles, one per CU (52 us at K = 4096, bf16 without a residual, where all of this was measured; 43
+// where there is one round).  Two of the others share a CU
 // (a round of 512: 128 x 128 32 us, 64 x 64 13), or have one each (21 and 10).
 struct L8Cost {
   int tile, per_cu, round, one_each;

@@ -7,8 +7,8 @@
 // and a packed row's maximum is that of |s w|, whose product with rstd is the norm's.
 // Bound by HBM, in bf16: T = 65536, C = 2048 with a residual (8 bytes an element) the
 // forward takes 172 us (6.2 TB/s), the backward 167 + 4.8 for the weight's sums (6.4);
-// without one 88 and 129; T = 65536, C = 1024 in 8 bits 34 (3 bytes an element, 5.9
-// TB/s).  One row of 4096: 2.5 us, a launch's latency.
+// without one 88 and 129; T = 65536, C = 1024 in 8 bits 34 to 36 (3 bytes an element,
+// 5.6 to 5.9 TB/s).  One row of 4096: 2.5 us, a launch's latency.
 #pragma once
 
 #include "layer_norm_kernels.h"
