@@ -171,10 +171,10 @@ struct L8Walk {
 };
 
 // A wave has up to 128 x 64 of a tile: 12 reads of LDS for 32 instructions, accumulators in half of its
-// registers.  Measured in turn with the kernel as it was then, and slower (POP/s at T = N = K = 8192, against 2.41): 128 x 128 per wave with four
-// waves 2.0 to 2.16, instructions of 32 x 32 x 32 2.25, four steps of 64 columns 2.28; two workgroups of
-// 128 x 256 in steps of 64 on a CU, so that one stores while the other multiplies, 79 -> 84 us at T = 65536,
-// N = K = 1024 and 214 -> 260 at T = 16384, N = K = 4096.
+// registers.  Measured in turn with the kernel as it was then, and slower (POP/s at T = N = K = 8192, against
+// 2.41): 128 x 128 per wave with four waves 2.0 to 2.16, instructions of 32 x 32 x 32 2.25, four steps of 64
+// columns 2.28; two workgroups of 128 x 256 in steps of 64 on a CU, so that one stores while the other
+// multiplies, 79 -> 84 us at T = 65536, N = K = 1024 and 214 -> 260 at T = 16384, N = K = 4096.
 //
 // Loads go from memory to LDS without registers (rows of BK bytes, 16 bytes a lane), NB - 1 steps and a
 // part ahead of the products, fragments from LDS to registers one part of 64 columns ahead.  The loads run on
@@ -411,11 +411,11 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void l8_tile_kernel(const L8Args 
     // for.  Rows that begin at 16 bytes are stored, and the residual's loaded, with the nontemporal hint:
     // neither is read again here, and what the tiles read stays cached (with / without, us, bf16: T = 65536,
     // N = 1024, K = 512 50 / 64, K = 1024 73 / 89, with a residual 93 / 102, the hint for its loads alone 93 /
-    // 102; T = 16384, N = K = 4096 218 / 224).  Other rows share lines with their neighbours'
-    // stores, which are to meet in the cache.  At the edges (EDGE) tokens past the last one are read as the
-    // last one, and only what is inside is stored.  Tokens with scales past kL8Large take that form too: to
-    // look at the scales costs up to 1% (T = 65536, N = K = 1024 71.8 -> 72.2 us, T = 16384, N = K = 4096 212.5
-    // -> 214.1), to choose for each element in every form 2% (72.3 -> 74.1 and 210.8 -> 213.8).
+    // 102; T = 16384, N = K = 4096 218 / 224).  Other rows share lines with their neighbours' stores, which are
+    // to meet in the cache.  At the edges (EDGE) tokens past the last one are read as the last one, and only what
+    // is inside is stored.  Tokens with scales past kL8Large take that form too: to look at the scales costs up
+    // to 1% (T = 65536, N = K = 1024 71.8 -> 72.2 us, T = 16384, N = K = 4096 212.5 -> 214.1), to choose for each
+    // element in every form 2% (72.3 -> 74.1 and 210.8 -> 213.8).
     auto finish = [&](auto with, auto lines, auto edge) __attribute__((always_inline)) {
       constexpr bool RES = decltype(with)::value, LINES = decltype(lines)::value, EDGE = decltype(edge)::value;
       asm volatile("" ::: "memory");  // (its loads are its own: none is under way where it is not taken)
@@ -595,8 +595,8 @@ void l8_few_launch(const L8Args& a, hipStream_t s) {
 
 // The shortest of the tile kernels for the tiles that a product has of each, in hundredths of a round of
 // 256 x 256 tiles, one per CU (52 us at K = 4096, bf16 without a residual, where all of this was measured; 43
-// where there is one round).  Two of the others share a CU
-// (a round of 512: 128 x 128 32 us, 64 x 64 13), or have one each (21 and 10).
+// where there is one round).  Two of the others share a CU (a round of 512: 128 x 128 32 us, 64 x 64 13), or have
+// one each (21 and 10).
 struct L8Cost {
   int tile, per_cu, round, one_each;
   int64_t tiles(int64_t T, int64_t N) const { return ((T + tile - 1) / tile) * ((N + tile - 1) / tile); }

@@ -205,7 +205,7 @@ class Linear8(nn.Module):
     """A linear layer with an 8-bit weight, for inference: x (..., in_features) to
     (..., out_features) in x's dtype (bf16, fp16 or fp32), with x packed by rows in the
     call.  Tensors that are not on a GPU go through the same formulas in PyTorch
-    operations, and neither have a gradient.  The scales stay fp32 where the module is
+    operations; neither form has a gradient.  The scales stay fp32 where the module is
     cast.
 
     Args:

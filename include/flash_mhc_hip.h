@@ -383,9 +383,9 @@ int fmhc_rms_norm_pack8_rows(const void* x, const void* residual, const void* we
  * x (T, K) and w (N, K) are codes, any int8 values, in rows ldx and ldw bytes apart:
  * multiples of 16, at most 2^22, from a 16-byte aligned address, and every row, the
  * last one too, can be read to the next multiple of 16 bytes (what is there does not
- * matter).  The sum is exact; K < 2^17.  Its product with the scales, in whichever
- * order, overflows only where it is itself past fp32's range.  out and residual (may be NULL) are (T, N)
- * in `dtype`, contiguous; bias (N,), in bias_dtype, FMHC_DTYPE_F32 or `dtype`, may be
+ * matter).  The sum is exact; K < 2^17.  Its product with the scales overflows only
+ * where it is itself past fp32's range.  out and residual (may be NULL) are (T, N) in
+ * `dtype`, contiguous; bias (N,), in bias_dtype, FMHC_DTYPE_F32 or `dtype`, may be
  * NULL.  out is rounded once; it may not overlap an input.  T < 2^31, N < 2^22 and
  * T N <= 2^40. */
 int fmhc_linear8(const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, int64_t ldw,

@@ -317,6 +317,21 @@ def test_scales_at_the_ends_of_fp32(T, N, dtype):
     assert bool(torch.isnan(out[T // 2]).all())
 
 
+def test_large_scales_among_many_tiles():
+    """Workgroups with several tiles, of which some hold tokens with large scales: before, between and behind others."""
+    T, N, K = 66000, 1024, 264
+    x, xs, w, ws = operands(T, N, K)
+    ws = ws * 1e-35
+    want = flash_mhc.linear8(x, xs, w, ws, dtype=F32)
+    large = torch.tensor([3, 255, 256, 9000, 30000, 30001, 65535, 65999], device=DEV)
+    xs[large] *= 1e36 / 0.02
+    out = flash_mhc.linear8(x, xs, w, ws, dtype=F32)
+    check("large", out[large], *R.linear8(x[large], xs[large], w, ws))
+    rest = torch.ones(T, dtype=torch.bool, device=DEV)
+    rest[large] = False
+    assert torch.equal(out[rest], want[rest])
+
+
 @pytest.mark.parametrize("T", [2, 40, 700])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_layer_of_huge_rows(T, dtype):
